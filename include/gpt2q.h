@@ -254,6 +254,124 @@ int gpt2q_bwd_gelu(int device, const float* x_pre, const float* dy, int n, float
 int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float* v, const float* dy, int t, int hd,
                          int stride, float* dq, float* dk, float* dv);
 
+/* ---- Operators on device memory: a paged key/value cache and token log probabilities ----
+ *
+ * Like gpt2q_argmax_noalloc these take device pointers and a cudaStream_t (NULL = the legacy
+ * default stream), allocate nothing and do not synchronise, so they may be captured into a CUDA
+ * graph. They launch on the current device, which has to own the memory and the stream. Calls that
+ * share no output and no workspace may run at the same time. Errors found on the host are reported
+ * by gpt2q_last_error(NULL); nothing is launched then. No counterpart in the reference, whose cache
+ * is one [n_ctx][d] buffer per layer (gpu.rs:128-134). */
+#define GPT2Q_F32 0
+#define GPT2Q_F16 1
+#define GPT2Q_BF16 2
+
+/* One layer's paged cache. Keys and values lie in two pools of n_pages pages with the same strides
+ * (in elements): the entry of token slot o in page p for kv head h starts at
+ * p * page_stride + h * head_stride + o * token_stride and holds head_dim elements. The pools' base
+ * addresses and all strides are multiples of 16 bytes; head_dim is a multiple of 8, at most 256.
+ * Entries must not overlap. */
+typedef struct gpt2q_paged_kv {
+    void* k;
+    void* v;
+    int32_t dtype; /* GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16 */
+    int32_t n_pages;
+    int32_t page_size; /* token slots of a page, any number >= 1 */
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t reserved; /* 0 */
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t token_stride;
+} gpt2q_paged_kv;
+
+/* Rows of page ids: row r's token at position p lies in page table[r * ld + p / page_size], slot
+ * p % page_size. Entries past a row's last used page are never read. */
+typedef struct gpt2q_page_table {
+    const int32_t* ids; /* device */
+    int32_t n_rows;
+    int32_t width; /* pages a row can name */
+    int64_t ld;    /* row stride, >= width */
+} gpt2q_page_table;
+
+/* Position rotation over the first `dim` elements of a head: pair i is turned by
+ * position * 2 pi * turns[i]. Pairs are (i, i + dim/2), or (2i, 2i + 1) when interleaved != 0. */
+typedef struct gpt2q_rotary {
+    int32_t dim;
+    int32_t interleaved;
+    double turns[128];
+} gpt2q_rotary;
+
+/* turns[i] = base^(-2i/dim) / (2 pi). dim even, 2..256; a caller may write other turns afterwards. */
+int gpt2q_rotary_init(gpt2q_rotary* rot, int dim, int interleaved, double base);
+
+/* A device tensor [token][head][head_dim] with unit stride over head_dim; strides in elements. */
+typedef struct gpt2q_heads {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} gpt2q_heads;
+
+/* Bits of the optional device status word (int32, OR-ed into, never cleared). */
+#define GPT2Q_STATUS_PAGE 1     /* a page id outside [0, n_pages) was needed */
+#define GPT2Q_STATUS_POSITION 2 /* a position or length past the table's width */
+#define GPT2Q_STATUS_ROW 4      /* a table row outside [0, n_rows) */
+
+/* Appends n_tokens keys and values (both or neither of k->data and v->data) to the cache. Token i
+ * belongs to table row d_seq[i] (d_seq NULL: row i) and position d_pos[i]. Keys are rotated when
+ * `rot` is given, rounded once to the cache's type; with `q` and `q_out` the token's n_q_heads
+ * queries are rotated into q_out too (q_out may be q). k, v, q and q_out are of type `dtype`, the
+ * cache's or GPT2Q_F32. A token with d_pos[i] < 0 is padding: nothing of it is written to the
+ * cache and its queries are copied unrotated. A token whose page, position or row is out of range
+ * is not written either and sets its bit in d_status (may be NULL). No two tokens of a call may
+ * name the same cache entry. */
+int gpt2q_paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                       const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads,
+                       int n_tokens, const int32_t* d_pos, const int32_t* d_seq, const gpt2q_rotary* rot,
+                       int32_t* d_status, void* stream);
+
+/* Attention of one new token per table row over that row's cached entries:
+ * out[r][h] = sum_j softmax_j(scale * q[r][h] . K[j][h / (n_heads / n_kv_heads)]) V[j], j over the
+ * last `window` of the positions 0..d_lens[r]-1 (window 0: all of them). q and out are of type
+ * `dtype`, the cache's or GPT2Q_F32; data and strides multiples of 16 bytes. d_lse (may be NULL),
+ * [n_rows][n_heads] fp32, receives the natural logarithm of each row's sum of exp. A row of length
+ * <= 0 gives zeros and -inf. A row that needs a page id out of range, or whose length exceeds the
+ * table, gives NaN and sets its bit in d_status (may be NULL). Scores, the running maximum and sum
+ * and the output are accumulated in fp32; results do not depend on the order in which blocks run.
+ * d_work: gpt2q_paged_attention_workspace(kv, n_heads) bytes of device memory, 16-byte aligned,
+ * that no other call running at the same time uses; its content does not matter. */
+uint64_t gpt2q_paged_attention_workspace(const gpt2q_paged_kv* kv, int n_heads);
+int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                          const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
+                          int window, float* d_lse, int32_t* d_status, void* d_work, void* stream);
+
+/* Log probabilities of given tokens under softmax(logits / temperature), per row of n_rows rows of
+ * `vocab` logits (type `dtype`, row stride ld >= vocab elements, any alignment of that type):
+ *   d_lp[r]       log probability of targets[r] (int32, or int64 when targets_i64 != 0). A negative
+ *                 target gives 0, one >= vocab NaN.
+ *   d_entropy[r]  -sum p ln p
+ *   d_stats[r][3] the largest logit, ln sum exp((logit - largest) / temperature), the entropy: what
+ *                 gpt2q_logprobs_grad takes
+ *   d_top_ids[r][top], d_top_lp[r][top]  the `top` likeliest tokens (0 <= top <= min(vocab,
+ *                 GPT2Q_TOP_MAX)) in falling order, equal logits by rising index, and their log
+ *                 probabilities
+ * Each output may be NULL (targets, too, when d_lp is). A logit of -inf has probability 0. A row of
+ * nothing but -inf gives log probabilities of -inf and entropy 0. A row with NaN or +inf gives NaN;
+ * among alternatives NaN ranks as -inf. Sums are fp32 in a fixed order. */
+#define GPT2Q_TOP_MAX 64
+int gpt2q_logprobs(const void* d_logits, int dtype, int64_t ld, int n_rows, int vocab, float temperature,
+                   const void* d_targets, int targets_i64, int top, float* d_lp, float* d_entropy, float* d_stats,
+                   int32_t* d_top_ids, float* d_top_lp, void* stream);
+
+/* Its gradient: d_dlogits[r][j] = (d_lp[r] ([j == target] - p_j) - d_ent[r] p_j (ln p_j + H)) / temperature,
+ * the sum of both outputs' gradients for the incoming gradients d_lp and d_ent (fp32 [n_rows]; either may be
+ * NULL, then its term is left out). d_stats are the forward's. d_dlogits has the logits' type and row stride
+ * ld_out >= vocab; it may be d_logits itself (ld_out == ld), otherwise the two must not overlap. Elements past
+ * vocab are left as they are. A row of negative target has no d_lp term; a row of nothing but -inf gets zeros. */
+int gpt2q_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int n_rows, int vocab, float temperature,
+                        const void* d_targets, int targets_i64, const float* d_stats, const float* d_lp,
+                        const float* d_ent, void* d_dlogits, int64_t ld_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,13 @@ pub const GPT2Q_ENCCL: c_int = -4;
 pub const GPT2Q_ETIMEOUT: c_int = -5;
 pub const GPT2Q_EUNSUP: c_int = -6;
 pub const GPT2Q_NOALLOC_MAX_ROWS: c_int = 1024;
+pub const GPT2Q_F32: c_int = 0;
+pub const GPT2Q_F16: c_int = 1;
+pub const GPT2Q_BF16: c_int = 2;
+pub const GPT2Q_STATUS_PAGE: c_int = 1;
+pub const GPT2Q_STATUS_POSITION: c_int = 2;
+pub const GPT2Q_STATUS_ROW: c_int = 4;
+pub const GPT2Q_TOP_MAX: c_int = 64;
 
 #[repr(C)]
 pub struct gpt2q_handle {
@@ -44,6 +51,51 @@ pub struct gpt2q_tensor_desc {
     pub shape: [i64; 2],
     pub data: *const c_void,
     pub len: u64,
+}
+
+/// One layer's paged cache (device pools, strides in elements).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct gpt2q_paged_kv {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: i32,
+    pub n_pages: i32,
+    pub page_size: i32,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub reserved: i32,
+    pub page_stride: i64,
+    pub head_stride: i64,
+    pub token_stride: i64,
+}
+
+/// Rows of page ids on the device.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct gpt2q_page_table {
+    pub ids: *const i32,
+    pub n_rows: i32,
+    pub width: i32,
+    pub ld: i64,
+}
+
+/// Position rotation, filled by `gpt2q_rotary_init`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct gpt2q_rotary {
+    pub dim: i32,
+    pub interleaved: i32,
+    pub turns: [f64; 128],
+}
+
+/// A device tensor [token][head][head_dim], strides in elements.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct gpt2q_heads {
+    pub data: *mut c_void,
+    pub token_stride: i64,
+    pub head_stride: i64,
 }
 
 extern "C" {
@@ -95,4 +147,22 @@ extern "C" {
     pub fn gpt2q_bwd_attn_train(device: c_int, q: *const f32, k: *const f32, v: *const f32, dy: *const f32,
                                 t: c_int, hd: c_int, stride: c_int, dq: *mut f32, dk: *mut f32,
                                 dv: *mut f32) -> c_int;
+    pub fn gpt2q_rotary_init(rot: *mut gpt2q_rotary, dim: c_int, interleaved: c_int, base: f64) -> c_int;
+    pub fn gpt2q_paged_append(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, k: *const gpt2q_heads,
+                              v: *const gpt2q_heads, q: *const gpt2q_heads, q_out: *const gpt2q_heads, dtype: c_int,
+                              n_q_heads: c_int, n_tokens: c_int, d_pos: *const i32, d_seq: *const i32,
+                              rot: *const gpt2q_rotary, d_status: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn gpt2q_paged_attention_workspace(kv: *const gpt2q_paged_kv, n_heads: c_int) -> u64;
+    pub fn gpt2q_paged_attention(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, d_lens: *const i32,
+                                 q: *const gpt2q_heads, out: *const gpt2q_heads, dtype: c_int, n_heads: c_int,
+                                 scale: f32, window: c_int, d_lse: *mut f32, d_status: *mut i32, d_work: *mut c_void,
+                                 stream: *mut c_void) -> c_int;
+    pub fn gpt2q_logprobs(d_logits: *const c_void, dtype: c_int, ld: i64, n_rows: c_int, vocab: c_int, temperature: f32,
+                          d_targets: *const c_void, targets_i64: c_int, top: c_int, d_lp: *mut f32,
+                          d_entropy: *mut f32, d_stats: *mut f32, d_top_ids: *mut i32, d_top_lp: *mut f32,
+                          stream: *mut c_void) -> c_int;
+    pub fn gpt2q_logprobs_grad(d_logits: *const c_void, dtype: c_int, ld: i64, n_rows: c_int, vocab: c_int,
+                               temperature: f32, d_targets: *const c_void, targets_i64: c_int, d_stats: *const f32,
+                               d_lp: *const f32, d_ent: *const f32, d_dlogits: *mut c_void, ld_out: i64,
+                               stream: *mut c_void) -> c_int;
 }

@@ -25,6 +25,8 @@ EXPORTS = [
     "gpt2q_create_from_smt", "gpt2q_smt_inspect", "gpt2q_blake3",
     "gpt2q_trunk_input_grad", "gpt2q_bwd_lin_input_grad", "gpt2q_bwd_ln_backward", "gpt2q_bwd_gelu",
     "gpt2q_bwd_attn_train",
+    "gpt2q_rotary_init", "gpt2q_paged_append", "gpt2q_paged_attention", "gpt2q_paged_attention_workspace",
+    "gpt2q_logprobs", "gpt2q_logprobs_grad",
 ]
 
 
@@ -37,6 +39,24 @@ class Config(C.Structure):
 class TensorDesc(C.Structure):
     _fields_ = [("name", C.c_char_p), ("atom", C.c_char_p), ("ndim", C.c_int32),
                 ("shape", C.c_int64 * 2), ("data", C.c_void_p), ("len", C.c_uint64)]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("n_rows", C.c_int32), ("width", C.c_int32), ("ld", C.c_int64)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("dim", C.c_int32), ("interleaved", C.c_int32), ("turns", C.c_double * 128)]
+
+
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 class Gpt2qError(RuntimeError):
@@ -134,6 +154,20 @@ def load(path: str | None = None):
     lib.gpt2q_bwd_attn_train.argtypes = [C.c_int, _f32p, _f32p, _f32p, _f32p, C.c_int, C.c_int, C.c_int, _f32p,
                                          _f32p, _f32p]
     lib.gpt2q_bwd_attn_train.restype = C.c_int
+    # structures are passed by address (C.byref)
+    vp, ci = C.c_void_p, C.c_int
+    lib.gpt2q_rotary_init.argtypes = [vp, ci, ci, C.c_double]
+    lib.gpt2q_rotary_init.restype = ci
+    lib.gpt2q_paged_append.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp]
+    lib.gpt2q_paged_append.restype = ci
+    lib.gpt2q_paged_attention_workspace.argtypes = [vp, ci]
+    lib.gpt2q_paged_attention_workspace.restype = C.c_uint64
+    lib.gpt2q_paged_attention.argtypes = [vp, vp, vp, vp, vp, ci, ci, C.c_float, ci, vp, vp, vp, vp]
+    lib.gpt2q_paged_attention.restype = ci
+    lib.gpt2q_logprobs.argtypes = [vp, ci, C.c_int64, ci, ci, C.c_float, vp, ci, ci, vp, vp, vp, vp, vp, vp]
+    lib.gpt2q_logprobs.restype = ci
+    lib.gpt2q_logprobs_grad.argtypes = [vp, ci, C.c_int64, ci, ci, C.c_float, vp, ci, vp, vp, vp, vp, C.c_int64, vp]
+    lib.gpt2q_logprobs_grad.restype = ci
     for fn in (lib.gpt2q_quantize_q8, lib.gpt2q_quantize_q4):
         fn.argtypes = [_f32p, C.c_size_t, C.POINTER(C.c_uint8)]
         fn.restype = C.c_int

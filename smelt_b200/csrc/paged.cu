@@ -1,0 +1,484 @@
+// Paged key/value cache (gpt2q_paged_append, gpt2q_paged_attention): gpt2q.h states the layout.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <type_traits>
+#include <utility>
+
+#include "gpt2q.h"
+#include "paged.h"
+#include "tcgen05.cuh"
+
+namespace gpt2q {
+void set_global_error(const std::string& msg);  // runtime.cu
+bool pdl_enabled();                             // kernels.cu
+}  // namespace gpt2q
+
+using namespace gpt2q;
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+// Programmatic dependent launch, as in kernels.cu: every kernel here waits (pdl_wait) before it
+// reads or writes anything, so only its launch overlaps the previous kernel.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+// V consecutive elements; V = 8 moves 16-byte vectors (the address is a multiple of 16 bytes).
+template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float* f) {
+    if constexpr (V == 8) {
+        constexpr int N = sizeof(T) * 8 / 16;
+        union {
+            uint4 u[N];
+            T t[8];
+        } r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(r.t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = to_f(p[i]);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float* f) {
+    if constexpr (V == 8) {
+        constexpr int N = sizeof(T) * 8 / 16;
+        union {
+            uint4 u[N];
+            T t[8];
+        } r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.t[i] = from_f<T>(f[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = r.u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = from_f<T>(f[i]);
+    }
+}
+
+// ------------------------------------------------------------------ append
+struct AppendParams {
+    const void *k, *v, *q;
+    void* qo;
+    long long k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, qo_ts, qo_hs;  // elements
+    void *kc, *vc;
+    long long c_ps, c_hs, c_ts;
+    int page, n_pages, n_tokens, n_q, n_kv, dim, rot, interleaved;
+    const int *pos, *seq, *table;
+    int pos0, n_rows, width;
+    long long ld;
+    int* status;
+    int unit_shift, groups;  // threads of a token: groups * 2^unit_shift
+    double turns[128];
+};
+
+// A unit is two chunks of V consecutive elements, the (a, b) of V rotated pairs or 2 V elements that
+// are only copied; a head has dim / (2 V) of them. A thread takes one unit index of one token and
+// walks over the token's heads (queries, keys, values), `groups` threads sharing a unit index, so
+// that the sines and cosines of its V pairs are computed once per thread. The angle is the
+// fractional part of position * turns, formed in fp64 (fp32 would lose 2^-24 * position turns:
+// 0.4 rad at a position of a million), then sincospif in fp32.
+template <class TI, class TC, int V>
+__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ AppendParams p) {
+    tc::pdl_trigger();
+    tc::pdl_wait();
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int u = (int)(id & ((1 << p.unit_shift) - 1));
+    const long long rest = id >> p.unit_shift;
+    const int g = (int)(rest % p.groups);
+    const long long ti = rest / p.groups;
+    if (ti >= p.n_tokens || u * 2 * V >= p.dim) return;
+    const int pos = p.pos ? __ldcg(p.pos + ti) : p.pos0 + (int)ti;
+    const int row = p.pos ? (p.seq ? __ldcg(p.seq + ti) : (int)ti) : 0;
+    long long at = -1;  // the token's entry in a pool, before the head
+    int why = 0;
+    if (pos >= 0) {
+        const int pg = pos / p.page;
+        if (row < 0 || row >= p.n_rows) {
+            why = GPT2Q_STATUS_ROW;
+        } else if (pg >= p.width) {
+            why = GPT2Q_STATUS_POSITION;
+        } else {
+            const int id_ = __ldcg(p.table + (long long)row * p.ld + pg);
+            if (id_ < 0 || id_ >= p.n_pages)
+                why = GPT2Q_STATUS_PAGE;
+            else
+                at = (long long)id_ * p.c_ps + (long long)(pos - pg * p.page) * p.c_ts;
+        }
+        if (why && p.status && u == 0 && g == 0) atomicOr(p.status, why);
+    }
+    const bool turned = u * 2 * V < p.rot;
+    const bool halves = turned && !p.interleaved;
+    const int ca = halves ? u * V : u * 2 * V;
+    const int cb = halves ? p.rot / 2 + u * V : ca + V;
+    const bool turn = turned && pos >= 0;
+    float cs[V], sn[V];
+    if (turn) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            double t = (double)pos * p.turns[u * V + e];
+            t -= rint(t);
+            sincospif((float)(2.0 * t), &sn[e], &cs[e]);
+        }
+    }
+    const int heads = p.n_q + 2 * p.n_kv;
+    for (int h = g; h < heads; h += p.groups) {
+        const bool is_q = h < p.n_q;
+        const bool is_v = h >= p.n_q + p.n_kv;
+        if (!is_q && at < 0) continue;
+        const int hk = is_q ? h : is_v ? h - p.n_q - p.n_kv : h - p.n_q;
+        const TI* src = is_q ? static_cast<const TI*>(p.q) + ti * p.q_ts + hk * p.q_hs
+                             : is_v ? static_cast<const TI*>(p.v) + ti * p.v_ts + hk * p.v_hs
+                                    : static_cast<const TI*>(p.k) + ti * p.k_ts + hk * p.k_hs;
+        const int oa = is_v ? u * 2 * V : ca, ob = is_v ? oa + V : cb;
+        float a[V], b[V];
+        load_vec<TI, V>(src + oa, a);
+        load_vec<TI, V>(src + ob, b);
+        if (turn && !is_v) {
+            if (halves || V == 1) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float x = a[e], y = b[e];
+                    a[e] = x * cs[e] - y * sn[e];
+                    b[e] = y * cs[e] + x * sn[e];
+                }
+            } else {  // pairs (2i, 2i + 1): the first V / 2 in a, the rest in b
+#pragma unroll
+                for (int e = 0; e + 1 < V; e += 2) {
+                    float x = a[e], y = a[e + 1];
+                    a[e] = x * cs[e / 2] - y * sn[e / 2];
+                    a[e + 1] = y * cs[e / 2] + x * sn[e / 2];
+                    x = b[e], y = b[e + 1];
+                    b[e] = x * cs[V / 2 + e / 2] - y * sn[V / 2 + e / 2];
+                    b[e + 1] = y * cs[V / 2 + e / 2] + x * sn[V / 2 + e / 2];
+                }
+            }
+        }
+        if (is_q) {
+            TI* dst = static_cast<TI*>(p.qo) + ti * p.qo_ts + hk * p.qo_hs;
+            store_vec<TI, V>(dst + oa, a);
+            store_vec<TI, V>(dst + ob, b);
+        } else {
+            TC* dst = static_cast<TC*>(is_v ? p.vc : p.kc) + at + hk * p.c_hs;
+            store_vec<TC, V>(dst + oa, a);
+            store_vec<TC, V>(dst + ob, b);
+        }
+    }
+}
+
+template <class TI, class TC>
+cudaError_t launch_append(const AppendParams& p, bool vec, unsigned blocks, cudaStream_t st) {
+    return vec ? launch_pdl(k_paged_append<TI, TC, 8>, dim3(blocks), dim3(256), 0, st, p)
+               : launch_pdl(k_paged_append<TI, TC, 1>, dim3(blocks), dim3(256), 0, st, p);
+}
+
+// ------------------------------------------------------------------ attention of one token
+struct AttnParams {
+    const void *k, *v;
+    long long c_ps, c_hs, c_ts;  // elements
+    int page, n_pages;
+    const void* q;
+    void* out;
+    long long q_ts, q_hs, o_ts, o_hs;
+    HiLo hl;
+    float* lse;
+    const int *table, *lens;
+    long long ld;
+    int n_rows, n_heads, n_kv, group, dim, window;
+    int cap;  // the longest length a row of the table can hold
+    float scale;
+    int* status;
+};
+
+// One block per (row, head); its warps take keys in turn, lanes the head's dims, each warp with its
+// own running maximum and sum.
+template <class TC, class TI>
+__global__ void __launch_bounds__(128) k_paged_attn_simple(const AttnParams p) {
+    __shared__ float sm[4], sl[4];
+    __shared__ float so[4][256];
+    tc::pdl_trigger();
+    tc::pdl_wait();
+    const int head = blockIdx.x, row = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int len = __ldcg(p.lens + row);
+    const bool over = len > p.cap;
+    if (over) len = p.cap;
+    const int begin = p.window > 0 ? max(0, len - p.window) : 0;
+    const TI* q = static_cast<const TI*>(p.q) + row * p.q_ts + head * p.q_hs;
+    float qv[8], o[8];
+    int bad = over ? GPT2Q_STATUS_POSITION : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        qv[i] = d < p.dim && len > 0 ? to_f(q[d]) * p.scale : 0.f;
+        o[i] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int j = begin + warp; j < len; j += 4) {
+        const int id = __ldcg(p.table + row * p.ld + j / p.page);
+        if (id < 0 || id >= p.n_pages) {
+            bad |= GPT2Q_STATUS_PAGE;
+            continue;
+        }
+        const long long at = id * p.c_ps + (j % p.page) * p.c_ts + (head / p.group) * p.c_hs;
+        const TC* k = static_cast<const TC*>(p.k) + at;
+        const TC* v = static_cast<const TC*>(p.v) + at;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = lane + 32 * i;
+            if (d < p.dim) s = fmaf(qv[i], to_f(k[d]), s);
+        }
+#pragma unroll
+        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+        const float mn = fmaxf(m, s);
+        const float ms = mn == -INFINITY ? 0.f : mn;
+        const float al = expf(m - ms), e = expf(s - ms);
+        l = l * al + e;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = lane + 32 * i;
+            if (d < p.dim) o[i] = o[i] * al + e * to_f(v[d]);
+        }
+    }
+    if (bad) {
+        l = NAN;
+        if (p.status && lane == 0) atomicOr(p.status, bad);
+    }
+    if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) so[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    float M = -INFINITY, L = 0.f;
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w]);
+    const float ms = M == -INFINITY ? 0.f : M;
+    for (int w = 0; w < 4; ++w) L += sl[w] * expf(sm[w] - ms);
+    TI* out = static_cast<TI*>(p.out) + row * p.o_ts + head * p.o_hs;
+    for (int d = threadIdx.x; d < p.dim; d += 128) {
+        float r = 0.f;
+        for (int w = 0; w < 4; ++w) r += so[w][d] * expf(sm[w] - ms);
+        r = L == 0.f ? 0.f : r / L;
+        if (p.out) out[d] = from_f<TI>(r);
+        if (p.hl.hi) {
+            const __half h = __float2half_rn(r);
+            const long long at = (long long)row * p.hl.ld + head * p.dim + d;
+            p.hl.hi[at] = h;
+            p.hl.lo[at] = __float2half_rn(r - __half2float(h));
+        }
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[(long long)row * p.n_heads + head] = ms + logf(L);
+}
+
+template <class TC, class TI>
+cudaError_t launch_attn(const AttnParams& p, void*, cudaStream_t st) {
+    return launch_pdl(k_paged_attn_simple<TC, TI>, dim3(p.n_heads, p.n_rows), dim3(128), 0, st, p);
+}
+
+// ------------------------------------------------------------------ checks
+int size_of(int dtype) { return dtype == GPT2Q_F32 ? 4 : 2; }
+
+bool aligned16(const void* p, int64_t a, int64_t b, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
+}
+
+int refuse(std::string* why, const char* msg) {
+    *why = msg;
+    return GPT2Q_EARG;
+}
+
+int check_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, std::string* why) {
+    if (!kv || !kv->k || !kv->v) return refuse(why, "null cache");
+    if (kv->dtype < GPT2Q_F32 || kv->dtype > GPT2Q_BF16) return refuse(why, "unknown cache dtype");
+    if (dtype != kv->dtype && dtype != GPT2Q_F32) return refuse(why, "dtype must be the cache's or GPT2Q_F32");
+    if (kv->n_pages < 1 || kv->page_size < 1 || kv->n_kv_heads < 1) return refuse(why, "n_pages, page_size and n_kv_heads must be >= 1");
+    if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8)
+        return refuse(why, "head_dim must be a multiple of 8 in [8, 256]");
+    if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0) return refuse(why, "negative cache stride");
+    const int sz = size_of(kv->dtype);
+    if (!aligned16(kv->k, kv->page_stride, kv->head_stride, sz) || !aligned16(kv->v, kv->token_stride, 0, sz))
+        return refuse(why, "the cache's addresses and strides must be multiples of 16 bytes");
+    if (!t || !t->ids || t->n_rows < 0 || t->width < 1 || t->ld < t->width)
+        return refuse(why, "null page table, or bad n_rows / width / ld");
+    return GPT2Q_OK;
+}
+
+}  // namespace
+
+int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                        const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads,
+                        int n_tokens, const int32_t* d_pos, int pos0, const int32_t* d_seq, const gpt2q_rotary* rot,
+                        int32_t* d_status, cudaStream_t st, std::string* why) {
+    const int rc = check_cache(kv, table, dtype, why);
+    if (rc) return rc;
+    if (n_tokens < 0) return refuse(why, "n_tokens < 0");
+    if (n_tokens == 0) return GPT2Q_OK;
+    if (!k || !k->data || !v || !v->data) return refuse(why, "null k or v");
+    if ((q && q->data) != (q_out && q_out->data)) return refuse(why, "q and q_out come together");
+    const bool with_q = q && q->data;
+    if (with_q && n_q_heads < 1) return refuse(why, "n_q_heads must be >= 1");
+    if (!d_pos && (d_seq || table->n_rows < 1 || pos0 < 0)) return refuse(why, "null d_pos");
+    if (d_pos && !d_seq && n_tokens > table->n_rows) return refuse(why, "more tokens than table rows, and no d_seq");
+    if (rot && (rot->dim < 2 || rot->dim % 2 || rot->dim > kv->head_dim))
+        return refuse(why, "the rotary dim must be even and at most head_dim");
+    const int sz = size_of(dtype);
+    AppendParams p{};
+    p.k = k->data, p.k_ts = k->token_stride, p.k_hs = k->head_stride;
+    p.v = v->data, p.v_ts = v->token_stride, p.v_hs = v->head_stride;
+    bool vec = kv->head_dim % 16 == 0 && (!rot || rot->dim % 16 == 0) && aligned16(p.k, p.k_ts, p.k_hs, sz) &&
+               aligned16(p.v, p.v_ts, p.v_hs, sz);
+    if (with_q) {
+        p.q = q->data, p.q_ts = q->token_stride, p.q_hs = q->head_stride;
+        p.qo = q_out->data, p.qo_ts = q_out->token_stride, p.qo_hs = q_out->head_stride;
+        p.n_q = n_q_heads;
+        vec = vec && aligned16(p.q, p.q_ts, p.q_hs, sz) && aligned16(p.qo, p.qo_ts, p.qo_hs, sz);
+    }
+    p.kc = kv->k, p.vc = kv->v;
+    p.c_ps = kv->page_stride, p.c_hs = kv->head_stride, p.c_ts = kv->token_stride;
+    p.page = kv->page_size, p.n_pages = kv->n_pages, p.n_tokens = n_tokens, p.n_kv = kv->n_kv_heads, p.dim = kv->head_dim;
+    p.pos = d_pos, p.pos0 = pos0, p.seq = d_seq, p.table = table->ids, p.n_rows = table->n_rows, p.width = table->width;
+    p.ld = table->ld, p.status = d_status;
+    if (rot) {
+        p.rot = rot->dim, p.interleaved = rot->interleaved != 0;
+        for (int i = 0; i < rot->dim / 2; ++i) p.turns[i] = rot->turns[i];
+    }
+    const int units = kv->head_dim / (vec ? 16 : 2);
+    while ((1 << p.unit_shift) < units) ++p.unit_shift;
+    // heads a thread walks over: one while the call has fewer threads than the GPU holds, so that a
+    // decode step is one round of loads; up to 8 in a large call, where the angles' arithmetic
+    // would otherwise be repeated for every head
+    const long long heads = (long long)p.n_q + 2LL * p.n_kv;
+    const long long threads = ((long long)n_tokens << p.unit_shift) * heads;
+    const long long walk = std::clamp<long long>(threads / (148 * 2048), 1, 8);
+    p.groups = (int)((heads + walk - 1) / walk);
+    const long long blocks = ((((long long)n_tokens * p.groups) << p.unit_shift) + 255) / 256;
+    if (heads > INT32_MAX / 2 || blocks > INT32_MAX) return refuse(why, "too many tokens in one call");
+    cudaError_t e;
+    const unsigned nb = (unsigned)blocks;
+    if (kv->dtype == GPT2Q_F32)
+        e = launch_append<float, float>(p, vec, nb, st);
+    else if (kv->dtype == GPT2Q_F16)
+        e = dtype == GPT2Q_F32 ? launch_append<float, __half>(p, vec, nb, st) : launch_append<__half, __half>(p, vec, nb, st);
+    else
+        e = dtype == GPT2Q_F32 ? launch_append<float, bf16>(p, vec, nb, st) : launch_append<bf16, bf16>(p, vec, nb, st);
+    if (e != cudaSuccess) {
+        *why = cudaGetErrorString(e);
+        return GPT2Q_ECUDA;
+    }
+    return GPT2Q_OK;
+}
+
+int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                           const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
+                           int window, float* d_lse, int32_t* d_status, void* d_work, const HiLo& hl, cudaStream_t st,
+                           std::string* why) {
+    const int rc = check_cache(kv, table, dtype, why);
+    if (rc) return rc;
+    if (table->n_rows == 0) return GPT2Q_OK;
+    if (!d_lens || !q || !q->data || !out || (!out->data && !hl.hi)) return refuse(why, "null d_lens, q or out");
+    if (n_heads < 1 || n_heads % kv->n_kv_heads) return refuse(why, "n_heads must be a multiple of n_kv_heads");
+    if (!std::isfinite(scale)) return refuse(why, "scale must be finite");
+    if (window < 0) return refuse(why, "window < 0");
+    if (!d_work || reinterpret_cast<uintptr_t>(d_work) % 16) return refuse(why, "null or unaligned d_work");
+    const int sz = size_of(dtype);
+    if (!aligned16(q->data, q->token_stride, q->head_stride, sz) ||
+        !aligned16(out->data, out->token_stride, out->head_stride, sz))
+        return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
+    AttnParams p{};
+    p.k = kv->k, p.v = kv->v, p.c_ps = kv->page_stride, p.c_hs = kv->head_stride, p.c_ts = kv->token_stride;
+    p.page = kv->page_size, p.n_pages = kv->n_pages;
+    p.q = q->data, p.q_ts = q->token_stride, p.q_hs = q->head_stride;
+    p.out = out->data, p.o_ts = out->token_stride, p.o_hs = out->head_stride, p.hl = hl, p.lse = d_lse;
+    p.table = table->ids, p.lens = d_lens, p.ld = table->ld, p.n_rows = table->n_rows;
+    p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX);
+    p.n_heads = n_heads, p.n_kv = kv->n_kv_heads, p.group = n_heads / kv->n_kv_heads, p.dim = kv->head_dim;
+    p.window = window, p.scale = scale, p.status = d_status;
+    cudaError_t e;
+    if (kv->dtype == GPT2Q_F32)
+        e = launch_attn<float, float>(p, d_work, st);
+    else if (kv->dtype == GPT2Q_F16)
+        e = dtype == GPT2Q_F32 ? launch_attn<__half, float>(p, d_work, st) : launch_attn<__half, __half>(p, d_work, st);
+    else
+        e = dtype == GPT2Q_F32 ? launch_attn<bf16, float>(p, d_work, st) : launch_attn<bf16, bf16>(p, d_work, st);
+    if (e != cudaSuccess) {
+        *why = cudaGetErrorString(e);
+        return GPT2Q_ECUDA;
+    }
+    return GPT2Q_OK;
+}
+
+// =================================================================== C-ABI
+extern "C" int gpt2q_rotary_init(gpt2q_rotary* rot, int dim, int interleaved, double base) {
+    if (!rot || dim < 2 || dim % 2 || dim > 256 || !(base > 0.0) || !std::isfinite(base)) {
+        set_global_error("gpt2q_rotary_init: null rot, dim not even in [2, 256], or base not positive");
+        return GPT2Q_EARG;
+    }
+    rot->dim = dim;
+    rot->interleaved = interleaved != 0;
+    for (int i = 0; i < 128; ++i)
+        rot->turns[i] = i < dim / 2 ? std::pow(base, -2.0 * i / dim) / (2.0 * 3.14159265358979323846) : 0.0;
+    return GPT2Q_OK;
+}
+
+extern "C" int gpt2q_paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                                  const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype,
+                                  int n_q_heads, int n_tokens, const int32_t* d_pos, const int32_t* d_seq,
+                                  const gpt2q_rotary* rot, int32_t* d_status, void* stream) {
+    std::string why;
+    int rc;
+    if (!d_pos && n_tokens > 0)
+        rc = refuse(&why, "null d_pos");
+    else
+        rc = paged_append(kv, table, k, v, q, q_out, dtype, n_q_heads, n_tokens, d_pos, 0, d_seq, rot, d_status,
+                          static_cast<cudaStream_t>(stream), &why);
+    if (rc) set_global_error("gpt2q_paged_append: " + why);
+    return rc;
+}
+
+extern "C" uint64_t gpt2q_paged_attention_workspace(const gpt2q_paged_kv* kv, int n_heads) {
+    return kv && n_heads > 0 ? 16 : 0;
+}
+
+extern "C" int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                                     const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
+                                     int window, float* d_lse, int32_t* d_status, void* d_work, void* stream) {
+    std::string why;
+    const int rc = paged_attention(kv, table, d_lens, q, out, dtype, n_heads, scale, window, d_lse, d_status, d_work,
+                                   HiLo{}, static_cast<cudaStream_t>(stream), &why);
+    if (rc) set_global_error("gpt2q_paged_attention: " + why);
+    return rc;
+}

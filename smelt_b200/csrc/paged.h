@@ -1,0 +1,31 @@
+// Paged key/value cache: append with position rotation, and attention of one new token per row.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include "gpt2q.h"
+
+namespace gpt2q {
+
+// fp16 hi/lo copies of the attention's fp32 output (x = hi + lo), which the tensor-core linears
+// read; row stride ld. Null when not wanted.
+struct HiLo {
+    __half* hi = nullptr;
+    __half* lo = nullptr;
+    int ld = 0;
+};
+
+// The checks and launches behind gpt2q_paged_append / gpt2q_paged_attention; `why` receives the
+// message of a failed call. Return GPT2Q_* codes. In paged_append a null d_pos means positions
+// pos0, pos0 + 1, ... of table row 0.
+int paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k, const gpt2q_heads* v,
+                 const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads, int n_tokens,
+                 const int32_t* d_pos, int pos0, const int32_t* d_seq, const gpt2q_rotary* rot, int32_t* d_status,
+                 cudaStream_t st, std::string* why);
+int paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                    const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale, int window,
+                    float* d_lse, int32_t* d_status, void* d_work, const HiLo& hl, cudaStream_t st, std::string* why);
+
+}  // namespace gpt2q
