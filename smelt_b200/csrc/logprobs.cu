@@ -1,55 +1,20 @@
 // Log probabilities of given tokens, entropy and top alternatives (gpt2q_logprobs), and their
 // gradient (gpt2q_logprobs_grad): gpt2q.h states the definitions.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
-#include <utility>
 
+#include "device_op.cuh"
 #include "gpt2q.h"
-#include "tcgen05.cuh"
 
 namespace gpt2q {
 void set_global_error(const std::string& msg);  // runtime.cu
-bool pdl_enabled();                             // kernels.cu
-}  // namespace gpt2q
+}
 
 using namespace gpt2q;
 
 namespace {
-
-using bf16 = __nv_bfloat16;
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
-template <class T>
-__device__ __forceinline__ T from_f(float x);
-template <>
-__device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
 
 struct LpParams {
     const void* x;
@@ -213,11 +178,11 @@ extern "C" int gpt2q_logprobs(const void* d_logits, int dtype, int64_t ld, int n
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (dtype == GPT2Q_F32)
-        e = launch_pdl(k_logprobs_simple<float>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_simple<float>, dim3(n_rows), dim3(256), 0, st, p);
     else if (dtype == GPT2Q_F16)
-        e = launch_pdl(k_logprobs_simple<__half>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_simple<__half>, dim3(n_rows), dim3(256), 0, st, p);
     else
-        e = launch_pdl(k_logprobs_simple<bf16>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_simple<bf16>, dim3(n_rows), dim3(256), 0, st, p);
     if (e != cudaSuccess) {
         set_global_error(std::string(who) + ": " + cudaGetErrorString(e));
         return GPT2Q_ECUDA;
@@ -242,11 +207,11 @@ extern "C" int gpt2q_logprobs_grad(const void* d_logits, int dtype, int64_t ld, 
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (dtype == GPT2Q_F32)
-        e = launch_pdl(k_logprobs_grad_simple<float>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_grad_simple<float>, dim3(n_rows), dim3(256), 0, st, p);
     else if (dtype == GPT2Q_F16)
-        e = launch_pdl(k_logprobs_grad_simple<__half>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_grad_simple<__half>, dim3(n_rows), dim3(256), 0, st, p);
     else
-        e = launch_pdl(k_logprobs_grad_simple<bf16>, dim3(n_rows), dim3(256), 0, st, p);
+        e = launch_dependent(k_logprobs_grad_simple<bf16>, dim3(n_rows), dim3(256), 0, st, p);
     if (e != cudaSuccess) {
         set_global_error(std::string(who) + ": " + cudaGetErrorString(e));
         return GPT2Q_ECUDA;

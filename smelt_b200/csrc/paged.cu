@@ -1,94 +1,20 @@
 // Paged key/value cache (gpt2q_paged_append, gpt2q_paged_attention): gpt2q.h states the layout.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
-#include <type_traits>
-#include <utility>
 
+#include "device_op.cuh"
 #include "gpt2q.h"
 #include "paged.h"
-#include "tcgen05.cuh"
 
 namespace gpt2q {
 void set_global_error(const std::string& msg);  // runtime.cu
-bool pdl_enabled();                             // kernels.cu
-}  // namespace gpt2q
+}
 
 using namespace gpt2q;
 
 namespace {
-
-using bf16 = __nv_bfloat16;
-
-// Programmatic dependent launch, as in kernels.cu: every kernel here waits (pdl_wait) before it
-// reads or writes anything, so only its launch overlaps the previous kernel.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
-template <class T>
-__device__ __forceinline__ T from_f(float x);
-template <>
-__device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
-
-// V consecutive elements; V = 8 moves 16-byte vectors (the address is a multiple of 16 bytes).
-template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float* f) {
-    if constexpr (V == 8) {
-        constexpr int N = sizeof(T) * 8 / 16;
-        union {
-            uint4 u[N];
-            T t[8];
-        } r;
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f(r.t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = to_f(p[i]);
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float* f) {
-    if constexpr (V == 8) {
-        constexpr int N = sizeof(T) * 8 / 16;
-        union {
-            uint4 u[N];
-            T t[8];
-        } r;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.t[i] = from_f<T>(f[i]);
-#pragma unroll
-        for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = r.u[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = from_f<T>(f[i]);
-    }
-}
 
 // ------------------------------------------------------------------ append
 struct AppendParams {
@@ -202,111 +128,8 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
 
 template <class TI, class TC>
 cudaError_t launch_append(const AppendParams& p, bool vec, unsigned blocks, cudaStream_t st) {
-    return vec ? launch_pdl(k_paged_append<TI, TC, 8>, dim3(blocks), dim3(256), 0, st, p)
-               : launch_pdl(k_paged_append<TI, TC, 1>, dim3(blocks), dim3(256), 0, st, p);
-}
-
-// ------------------------------------------------------------------ attention of one token
-struct AttnParams {
-    const void *k, *v;
-    long long c_ps, c_hs, c_ts;  // elements
-    int page, n_pages;
-    const void* q;
-    void* out;
-    long long q_ts, q_hs, o_ts, o_hs;
-    HiLo hl;
-    float* lse;
-    const int *table, *lens;
-    long long ld;
-    int n_rows, n_heads, n_kv, group, dim, window;
-    int cap;  // the longest length a row of the table can hold
-    float scale;
-    int* status;
-};
-
-// One block per (row, head); its warps take keys in turn, lanes the head's dims, each warp with its
-// own running maximum and sum.
-template <class TC, class TI>
-__global__ void __launch_bounds__(128) k_paged_attn_simple(const AttnParams p) {
-    __shared__ float sm[4], sl[4];
-    __shared__ float so[4][256];
-    tc::pdl_trigger();
-    tc::pdl_wait();
-    const int head = blockIdx.x, row = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int len = __ldcg(p.lens + row);
-    const bool over = len > p.cap;
-    if (over) len = p.cap;
-    const int begin = p.window > 0 ? max(0, len - p.window) : 0;
-    const TI* q = static_cast<const TI*>(p.q) + row * p.q_ts + head * p.q_hs;
-    float qv[8], o[8];
-    int bad = over ? GPT2Q_STATUS_POSITION : 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        qv[i] = d < p.dim && len > 0 ? to_f(q[d]) * p.scale : 0.f;
-        o[i] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int j = begin + warp; j < len; j += 4) {
-        const int id = __ldcg(p.table + row * p.ld + j / p.page);
-        if (id < 0 || id >= p.n_pages) {
-            bad |= GPT2Q_STATUS_PAGE;
-            continue;
-        }
-        const long long at = id * p.c_ps + (j % p.page) * p.c_ts + (head / p.group) * p.c_hs;
-        const TC* k = static_cast<const TC*>(p.k) + at;
-        const TC* v = static_cast<const TC*>(p.v) + at;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d < p.dim) s = fmaf(qv[i], to_f(k[d]), s);
-        }
-#pragma unroll
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        const float mn = fmaxf(m, s);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        const float al = expf(m - ms), e = expf(s - ms);
-        l = l * al + e;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d < p.dim) o[i] = o[i] * al + e * to_f(v[d]);
-        }
-    }
-    if (bad) {
-        l = NAN;
-        if (p.status && lane == 0) atomicOr(p.status, bad);
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) so[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w]);
-    const float ms = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < 4; ++w) L += sl[w] * expf(sm[w] - ms);
-    TI* out = static_cast<TI*>(p.out) + row * p.o_ts + head * p.o_hs;
-    for (int d = threadIdx.x; d < p.dim; d += 128) {
-        float r = 0.f;
-        for (int w = 0; w < 4; ++w) r += so[w][d] * expf(sm[w] - ms);
-        r = L == 0.f ? 0.f : r / L;
-        if (p.out) out[d] = from_f<TI>(r);
-        if (p.hl.hi) {
-            const __half h = __float2half_rn(r);
-            const long long at = (long long)row * p.hl.ld + head * p.dim + d;
-            p.hl.hi[at] = h;
-            p.hl.lo[at] = __float2half_rn(r - __half2float(h));
-        }
-    }
-    if (p.lse && threadIdx.x == 0) p.lse[(long long)row * p.n_heads + head] = ms + logf(L);
-}
-
-template <class TC, class TI>
-cudaError_t launch_attn(const AttnParams& p, void*, cudaStream_t st) {
-    return launch_pdl(k_paged_attn_simple<TC, TI>, dim3(p.n_heads, p.n_rows), dim3(128), 0, st, p);
+    return vec ? launch_dependent(k_paged_append<TI, TC, 8>, dim3(blocks), dim3(256), 0, st, p)
+               : launch_dependent(k_paged_append<TI, TC, 1>, dim3(blocks), dim3(256), 0, st, p);
 }
 
 // ------------------------------------------------------------------ checks
@@ -418,22 +241,16 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     if (!aligned16(q->data, q->token_stride, q->head_stride, sz) ||
         !aligned16(out->data, out->token_stride, out->head_stride, sz))
         return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
-    AttnParams p{};
+    PagedAttn p{};
     p.k = kv->k, p.v = kv->v, p.c_ps = kv->page_stride, p.c_hs = kv->head_stride, p.c_ts = kv->token_stride;
     p.page = kv->page_size, p.n_pages = kv->n_pages;
     p.q = q->data, p.q_ts = q->token_stride, p.q_hs = q->head_stride;
     p.out = out->data, p.o_ts = out->token_stride, p.o_hs = out->head_stride, p.hl = hl, p.lse = d_lse;
     p.table = table->ids, p.lens = d_lens, p.ld = table->ld, p.n_rows = table->n_rows;
-    p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX);
+    p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX - 64);
     p.n_heads = n_heads, p.n_kv = kv->n_kv_heads, p.group = n_heads / kv->n_kv_heads, p.dim = kv->head_dim;
     p.window = window, p.scale = scale, p.status = d_status;
-    cudaError_t e;
-    if (kv->dtype == GPT2Q_F32)
-        e = launch_attn<float, float>(p, d_work, st);
-    else if (kv->dtype == GPT2Q_F16)
-        e = dtype == GPT2Q_F32 ? launch_attn<__half, float>(p, d_work, st) : launch_attn<__half, __half>(p, d_work, st);
-    else
-        e = dtype == GPT2Q_F32 ? launch_attn<bf16, float>(p, d_work, st) : launch_attn<bf16, bf16>(p, d_work, st);
+    const cudaError_t e = launch_paged_attn(p, kv->dtype, dtype, d_work, st);
     if (e != cudaSuccess) {
         *why = cudaGetErrorString(e);
         return GPT2Q_ECUDA;
@@ -470,7 +287,8 @@ extern "C" int gpt2q_paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_tab
 }
 
 extern "C" uint64_t gpt2q_paged_attention_workspace(const gpt2q_paged_kv* kv, int n_heads) {
-    return kv && n_heads > 0 ? 16 : 0;
+    if (!kv || n_heads < 1 || kv->n_kv_heads < 1 || kv->head_dim < 8 || kv->head_dim > 256) return 0;
+    return paged_attn_workspace(kv->head_dim, (n_heads + kv->n_kv_heads - 1) / kv->n_kv_heads);
 }
 
 extern "C" int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,

@@ -17,6 +17,33 @@ struct HiLo {
     int ld = 0;
 };
 
+// One attention call, checked (paged.cu); the fields after `status` are set by launch_paged_attn.
+struct PagedAttn {
+    const void *k, *v;
+    long long c_ps, c_hs, c_ts;  // elements
+    int page, n_pages;
+    const void* q;
+    void* out;
+    long long q_ts, q_hs, o_ts, o_hs;  // elements
+    HiLo hl;
+    float* lse;
+    const int *table, *lens;
+    long long ld;
+    int n_rows, n_heads, n_kv, group, dim, window;
+    int cap;  // the longest length a row of the table can hold
+    float scale;
+    int* status;
+    int page_shift;  // page = 1 << page_shift, or -1
+    // a kv head's `group` query heads are taken in blocks_per_kv blocks of up to heads_per_block
+    int blocks_per_kv, n_vh, heads_per_block;
+    int warp_bytes;  // shared memory of a warp
+    int4* meta;
+    float *warp_part, *block_part;
+    float2* block_ml;
+};
+uint64_t paged_attn_workspace(int dim, int group);
+cudaError_t launch_paged_attn(PagedAttn p, int cache_dtype, int dtype, void* work, cudaStream_t st);
+
 // The checks and launches behind gpt2q_paged_append / gpt2q_paged_attention; `why` receives the
 // message of a failed call. Return GPT2Q_* codes. In paged_append a null d_pos means positions
 // pos0, pos0 + 1, ... of table row 0.
