@@ -153,6 +153,8 @@ int check_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, 
         return refuse(why, "head_dim must be a multiple of 8 in [8, 256]");
     if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0) return refuse(why, "negative cache stride");
     const int sz = size_of(kv->dtype);
+    if (std::max({kv->page_stride, kv->head_stride, kv->token_stride}) > (int64_t)UINT32_MAX * 16 / sz)
+        return refuse(why, "cache stride past 64 GB");
     if (!aligned16(kv->k, kv->page_stride, kv->head_stride, sz) || !aligned16(kv->v, kv->token_stride, 0, sz))
         return refuse(why, "the cache's addresses and strides must be multiples of 16 bytes");
     if (!t || !t->ids || t->n_rows < 0 || t->width < 1 || t->ld < t->width)
@@ -242,7 +244,10 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
         !aligned16(out->data, out->token_stride, out->head_stride, sz))
         return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
     PagedAttn p{};
-    p.k = kv->k, p.v = kv->v, p.c_ps = kv->page_stride, p.c_hs = kv->head_stride, p.c_ts = kv->token_stride;
+    p.k = kv->k, p.v = kv->v;
+    const int csz = size_of(kv->dtype);
+    p.ps16 = (uint32_t)(kv->page_stride * csz / 16), p.hs16 = (uint32_t)(kv->head_stride * csz / 16);
+    p.ts16 = (uint32_t)(kv->token_stride * csz / 16);
     p.page = kv->page_size, p.n_pages = kv->n_pages;
     p.q = q->data, p.q_ts = q->token_stride, p.q_hs = q->head_stride;
     p.out = out->data, p.o_ts = out->token_stride, p.o_hs = out->head_stride, p.hl = hl, p.lse = d_lse;

@@ -20,7 +20,7 @@ struct HiLo {
 // One attention call, checked (paged.cu); the fields after `status` are set by launch_paged_attn.
 struct PagedAttn {
     const void *k, *v;
-    long long c_ps, c_hs, c_ts;  // elements
+    uint32_t ps16, hs16, ts16;  // strides in units of 16 bytes
     int page, n_pages;
     const void* q;
     void* out;
@@ -34,6 +34,7 @@ struct PagedAttn {
     float scale;
     int* status;
     int page_shift;  // page = 1 << page_shift, or -1
+    int grouped;     // a page holds whole groups of keys
     // a kv head's `group` query heads are taken in blocks_per_kv blocks of up to heads_per_block
     int blocks_per_kv, n_vh, heads_per_block;
     int warp_bytes;  // shared memory of a warp

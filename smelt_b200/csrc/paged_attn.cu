@@ -48,6 +48,8 @@ struct Cfg {
     // keys of a tile: 8 KB of keys and values (16 KB at 256 dims)
     static constexpr int TK = F32 ? (HD == 64 ? 16 : 8) : (HD == 64 ? 32 : 16);
     static constexpr int LPK = 32 / TK;  // lanes per key (fp32 cache)
+    static constexpr int GR = TK < 16 ? TK : 16, NG = TK / GR;  // keys of one page lookup where pages allow it
+    static constexpr int ITS = TK * CHP / 32, RPI = 32 / CHP > 0 ? 32 / CHP : 1;  // copies of a tile, rows of one copy
     static constexpr int STAGE = 2 * TK * ROWB;
     static constexpr int HS = HD + 4;  // floats of a partial result's row
     // 16-bit pieces of the query and of the weights. Queries of the cache's type are exact in one;
@@ -79,7 +81,8 @@ __device__ __forceinline__ void enter(const PagedAttn& p, Walk& w, int row) {
     w.over = len > p.cap;
     w.end = w.over ? p.cap : len;
     w.start = p.window > 0 && w.end > p.window ? w.end - p.window : 0;
-    w.nt = w.end > 0 ? (w.end - w.start + C::TK - 1) / C::TK : 0;
+    // tiles begin at multiples of TK, so that a group of GR keys lies in one page
+    w.nt = w.end > 0 ? (w.end + C::TK - 1) / C::TK - w.start / C::TK : 0;
 }
 
 template <class C>
@@ -256,24 +259,38 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
         }
         w.vh = (int)(rem / w.nt);
         w.j = (int)(rem - (long long)w.vh * w.nt);
-        Walk L = w;  // of the next tile to load; its pages are looked up when the tile before it is loaded
-
-        const int kr = lane & (TK - 1);  // the key of a tile this lane looks up
-        int page = -1, slot = 0;
-        auto look = [&]() {
-            const int key = L.start + L.j * TK + kr;
-            page = -1;
-            slot = 0;
-            if (key < L.end) {
-                const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
-                slot = key - pg * p.page;
-                page = __ldcg(p.table + (long long)L.row * p.ld + pg);
-                if ((unsigned)page >= (unsigned)p.n_pages) page = -2;
+        // L is the next tile to load, N the one after it, whose pages are on their way
+        Walk L = w, N;
+        const int kr = lane & (TK - 1);
+        const bool grouped = p.grouped != 0;
+        int page[C::NG], npage[C::NG];
+        // page ids of a tile: of every group of GR keys (the same load in all lanes) where a page is
+        // a multiple of GR, else of the lane's own key, in element 0
+        auto look = [&](const Walk& t, int* out) {
+            const int k0 = (t.start / TK + t.j) * TK;
+            const int* ids = p.table + (long long)t.row * p.ld;
+            if (grouped) {
+#pragma unroll
+                for (int g = 0; g < C::NG; ++g) {
+                    const int key = k0 + g * C::GR;
+                    out[g] = key < t.end && key + C::GR > t.start
+                                 ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page))
+                                 : 0;
+                }
+            } else {
+                const int key = k0 + kr;
+                out[0] = key < t.end && key >= t.start ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page)) : 0;
             }
         };
-        look();
-        int loaded = 0, qload = -1;   // tiles and queries put into the rings
-        uint32_t badmask = 0;         // stages with a page id out of range
+        look(L, page);
+        int loaded = 0, qload = -1;  // tiles and queries put into the rings
+        uint32_t badmask = 0;        // stages with a page id out of range
+        if (n > 1) {
+            N = L;
+            advance<C>(p, N);
+            look(N, npage);
+        }
+        const int lr = lane / C::CHP, lc = lane % C::CHP;  // the lane's row and chunk of a copy
         auto issue = [&](int stage) {
             const int kvh = L.vh / p.blocks_per_kv;
             if (loaded == 0 || L.j == 0) {
@@ -288,27 +305,72 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         cp16(q32 + qload * hv * qrow + i * 16, q + (there ? h * p.q_hs * (int)sizeof(TI) + c * 16 : 0), there);
                 }
             }
-            long long at = -1;
-            if (page >= 0)
-                at = ((long long)page * p.c_ps + (long long)slot * p.c_ts + (long long)kvh * p.c_hs) * (int)sizeof(TC);
-            const bool bad = __any_sync(0xffffffffu, page == -2);
-            badmask = (badmask & ~(1u << stage)) | ((bad ? 1u : 0u) << stage);
+            const int k0 = (L.start / TK + L.j) * TK;
             const uint32_t dst = ring32 + stage * C::STAGE;
+            const unsigned long long hoff = (unsigned long long)kvh * p.hs16 * 16;
+            const long long vk = static_cast<const char*>(p.v) - static_cast<const char*>(p.k);
+            bool bad = false;
+            if (grouped) {
+                const int lo = L.start - k0, hi = L.end - k0;  // rows lo <= r < hi are wanted
+                const unsigned long long step = (unsigned long long)p.ts16 * 16 * C::RPI;
+                const char* src = nullptr;
 #pragma unroll
-            for (int it = 0; it < TK * C::CHP / 32; ++it) {
-                const int idx = it * 32 + lane, r = idx / C::CHP, c = idx % C::CHP;
-                const long long o = __shfl_sync(0xffffffffu, at, r);
-                if (c < nch) {
+                for (int it = 0; it < C::ITS; ++it) {
+                    const int r0 = C::CHP > 32 ? it * 32 / C::CHP : it * C::RPI;
+                    const int r = r0 + (C::CHP > 32 ? 0 : lr), c = C::CHP > 32 ? (it * 32 + lane) % C::CHP : lc;
+                    if (r0 % C::GR == 0 && (C::CHP <= 32 || it * 32 % C::CHP == 0)) {
+                        const int id = page[r0 / C::GR];
+                        const bool ok = (unsigned)id < (unsigned)p.n_pages;
+                        bad |= !ok;
+                        const int key = k0 + r0;
+                        const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
+                        src = static_cast<const char*>(p.k) + hoff +
+                              ((unsigned long long)(unsigned)(ok ? id : 0) * p.ps16 +
+                               (unsigned long long)(unsigned)(slot + (C::CHP > 32 ? 0 : lr)) * p.ts16) * 16 +
+                              (C::CHP > 32 ? 0 : lc * 16);
+                    }
                     const int swz = C::F32 ? (r * C::LPK) & 7 : r & 7;
                     const uint32_t d = dst + r * C::ROWB + ((c ^ swz) * 16);
-                    const long long s = o >= 0 ? o + c * 16 : 0;
-                    cp16(d, static_cast<const char*>(p.k) + s, o >= 0);
-                    cp16(d + TK * C::ROWB, static_cast<const char*>(p.v) + s, o >= 0);
+                    const bool there = r >= lo && r < hi;
+                    if (c < nch) {
+                        const char* at = src + (C::CHP > 32 ? c * 16 : 0);
+                        cp16(d, at, there);
+                        cp16(d + TK * C::ROWB, at + vk, there);
+                    }
+                    if (C::CHP <= 32 || (it + 1) * 32 % C::CHP == 0) src += step;
+                }
+            } else {
+                const int key = k0 + kr;
+                long long at = -1;
+                if (key < L.end && key >= L.start) {
+                    const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
+                    if ((unsigned)page[0] < (unsigned)p.n_pages)
+                        at = (long long)(hoff + ((unsigned long long)(unsigned)page[0] * p.ps16 +
+                                                 (unsigned long long)(unsigned)(key - pg * p.page) * p.ts16) * 16);
+                    else
+                        bad = true;
+                }
+#pragma unroll
+                for (int it = 0; it < C::ITS; ++it) {
+                    const int idx = it * 32 + lane, r = idx / C::CHP, c = idx % C::CHP;
+                    const long long o = __shfl_sync(0xffffffffu, at, r);
+                    if (c < nch) {
+                        const int swz = C::F32 ? (r * C::LPK) & 7 : r & 7;
+                        const uint32_t d = dst + r * C::ROWB + ((c ^ swz) * 16);
+                        const char* src = static_cast<const char*>(p.k) + (o >= 0 ? o + c * 16 : 0);
+                        cp16(d, src, o >= 0);
+                        cp16(d + TK * C::ROWB, src + vk, o >= 0);
+                    }
                 }
             }
-            if (++loaded < n) {
-                advance<C>(p, L);
-                look();
+            badmask = (badmask & ~(1u << stage)) | ((__any_sync(0xffffffffu, bad) ? 1u : 0u) << stage);
+            ++loaded;
+            L = N;
+#pragma unroll
+            for (int g = 0; g < C::NG; ++g) page[g] = npage[g];
+            if (loaded + 1 < n) {
+                advance<C>(p, N);
+                look(N, npage);
             }
         };
 
@@ -387,7 +449,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                 }
             }
             if ((badmask >> stage) & 1u) bad |= GPT2Q_STATUS_PAGE;
-            const int rem_keys = w.end - (w.start + w.j * TK);
+            const int k0 = (w.start / TK + w.j) * TK, klo = w.start - k0, khi = w.end - k0;
+            const bool cut = klo > 0 || khi < TK;  // some of the tile's keys are not the row's
             const uint32_t kt = ring32 + stage * C::STAGE, vt = kt + TK * C::ROWB;
 
             if constexpr (!C::F32) {
@@ -401,17 +464,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         for (int z = 0; z < 4; ++z) s[x][y][0][z] = s[x][y][1][z] = 0.f;
 #pragma unroll
                 for (int k = 0; k < C::KD; ++k) {
-                    if (k * 16 < p.dim) {
 #pragma unroll
-                        for (int x = 0; x < MT; ++x) {
-                            const int r = x * 16 + (lane & 15), c = 2 * k + (lane >> 4);
-                            uint32_t af[4];
-                            ldsm4(af, kt + r * C::ROWB + ((c ^ (r & 7)) * 16));
+                    for (int x = 0; x < MT; ++x) {
+                        const int r = x * 16 + (lane & 15), c = 2 * k + (lane >> 4);
+                        uint32_t af[4];
+                        ldsm4(af, kt + r * C::ROWB + ((c ^ (r & 7)) * 16));
 #pragma unroll
-                            for (int y = 0; y < NT; ++y)
+                        for (int y = 0; y < NT; ++y)
 #pragma unroll
-                                for (int t = 0; t < C::SQ; ++t) mma16816<TC>(s[x][y][k & 1], af, qf[t][y][k][0], qf[t][y][k][1]);
-                        }
+                            for (int t = 0; t < C::SQ; ++t) mma16816<TC>(s[x][y][k & 1], af, qf[t][y][k][0], qf[t][y][k][1]);
                     }
                 }
                 bool moved = false;
@@ -426,7 +487,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
 #pragma unroll
                             for (int z = c; z < 4; z += 2) {
                                 float v = (s[x][y][0][z] + s[x][y][1][z]) * fac[2 * y + c];
-                                if (x * 16 + (lane >> 2) + (z >> 1) * 8 >= rem_keys) v = -INFINITY;
+                                const int r = x * 16 + (lane >> 2) + (z >> 1) * 8;
+                                if (cut && (r < klo || r >= khi)) v = -INFINITY;
                                 s[x][y][0][z] = v;
                                 mx = fmaxf(mx, v);
                             }
@@ -471,17 +533,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         }
 #pragma unroll
                 for (int d = 0; d < C::KD; ++d) {
-                    if (d * 16 < p.dim) {
 #pragma unroll
-                        for (int x = 0; x < MT; ++x) {
-                            const int r = x * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, c = 2 * d + ((lane >> 3) & 1);
-                            uint32_t af[4];
-                            ldsm4t(af, vt + r * C::ROWB + ((c ^ (r & 7)) * 16));
+                    for (int x = 0; x < MT; ++x) {
+                        const int r = x * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, c = 2 * d + ((lane >> 3) & 1);
+                        uint32_t af[4];
+                        ldsm4t(af, vt + r * C::ROWB + ((c ^ (r & 7)) * 16));
 #pragma unroll
-                            for (int y = 0; y < NT; ++y)
+                        for (int y = 0; y < NT; ++y)
 #pragma unroll
-                                for (int t = 0; t < C::sp(); ++t) mma16816<TC>(O[d][y], af, pf[t][x][y][0], pf[t][x][y][1]);
-                        }
+                            for (int t = 0; t < C::sp(); ++t) mma16816<TC>(O[d][y], af, pf[t][x][y][0], pf[t][x][y][1]);
                     }
                 }
             } else {
@@ -511,7 +571,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     float v = s[h];
 #pragma unroll
                     for (int o = 1; o < C::LPK; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    v = key < rem_keys ? v * sl2 : -INFINITY;
+                    v = key >= klo && key < khi ? v * sl2 : -INFINITY;
                     float mx = v;
 #pragma unroll
                     for (int o = C::LPK; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -781,11 +841,12 @@ cudaError_t launch(PagedAttn p, cudaStream_t st) {
     p.heads_per_block = std::min(p.group, C::HB);
     size_t wb = STAGES * C::STAGE + (size_t)STAGES * p.heads_per_block * C::HD * sizeof(typename C::TI);
     if (C::F32) wb += (size_t)C::TK * C::HB * 4;
+    p.grouped = p.page % C::GR == 0;
     p.warp_bytes = (int)((wb + 127) / 128 * 128);
     const int nw = (int)std::min<size_t>(MAX_WARPS, SMEM_LIMIT / p.warp_bytes);
     // no more blocks than the longest rows the table can hold would fill
     const long long longest = p.window > 0 ? std::min(p.window, p.cap) : p.cap;
-    const long long tiles = (longest + C::TK - 1) / C::TK * p.n_vh;
+    const long long tiles = ((longest + C::TK - 1) / C::TK + (p.window > 0 ? 1 : 0)) * p.n_vh;
     const long long want = tiles > MAX_CTAS * 8LL ? MAX_CTAS : (tiles * p.n_rows + nw - 1) / nw;
     const int grid = (int)std::clamp<long long>(want, 1, MAX_CTAS);
     int dev = 0;

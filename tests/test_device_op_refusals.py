@@ -59,7 +59,7 @@ CACHES = [
     (dict(head_dim=0), "head_dim"), (dict(head_dim=12), "head_dim"), (dict(head_dim=264), "head_dim"),
     (dict(k=A + 8), "16 bytes"), (dict(v=A + 2), "16 bytes"), (dict(token_stride=68), "16 bytes"),
     (dict(head_stride=1), "16 bytes"), (dict(page_stride=2044), "16 bytes"), (dict(page_stride=-2048), "negative"),
-    (dict(dtype=2), "dtype must be"),
+    (dict(dtype=2), "dtype must be"), (dict(page_stride=1 << 36), "64 GB"),
 ]
 
 
