@@ -20,7 +20,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;  // of the gradient
 constexpr int CANDIDATES = 2048;
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp; results under 2^-126 are 0
@@ -105,6 +105,40 @@ __device__ __forceinline__ void unpack(const uint4& u, float2* f) {  // VE / 2 p
     }
 }
 
+// VE / 2 pairs rounded to a vector
+template <class T>
+__device__ __forceinline__ uint4 packed(const float2* f) {
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, bf16>::value) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[i].x, f[i].y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(f[i].x, f[i].y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// the largest of a vector's elements that are numbers (-inf or NaN where none is)
+template <class T>
+__device__ __forceinline__ float largest(const uint4& u) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+        using T2 = std::conditional_t<std::is_same<T, bf16>::value, __nv_bfloat162, __half2>;
+        const T2* h = reinterpret_cast<const T2*>(&u);
+        const T2 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(to_f(a.x), to_f(a.y));
+    }
+}
+
 struct LpParams {
     const void* x;
     long long ld;
@@ -140,25 +174,37 @@ __device__ __forceinline__ unsigned long long maxu(unsigned long long a, unsigne
 struct Sums {
     float m, s, t;
 };
-__device__ __forceinline__ Sums merge(const Sums& a, const Sums& b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    const float r = m == -INFINITY ? 0.f : m;
+// The sums of all lanes' parts, in every lane: brought to the largest m, then added as a tree.
+__device__ __forceinline__ Sums join(const Sums& a, float c) {
+    Sums r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r.m) : "f"(a.m));
     // a part without mass has z = -inf; the clamp keeps 0 * z at 0
-    const float za = fmaxf((a.m - r) * c, -2000.f), zb = fmaxf((b.m - r) * c, -2000.f);
-    const float wa = ex2(za), wb = ex2(zb);
-    return Sums{m, a.s * wa + b.s * wb, wa * (a.t + za * a.s) + wb * (b.t + zb * b.s)};
+    const float z = fmaxf((a.m - (r.m == -INFINITY ? 0.f : r.m)) * c, -2000.f), w = ex2(z);
+    r.s = a.s * w;
+    r.t = w * fmaf(z, a.s, a.t);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
+    }
+    return r;
 }
 
+template <int THREADS>
 struct LpShared {
     Sums warp[THREADS / 32];
-    Sums part;                                   // this block's, read by the cluster's first block
-    unsigned long long group[THREADS / 2];       // best of every group of threads
-    unsigned long long top[GPT2Q_TOP_MAX];       // this block's alternatives, in order
+    Sums part[8];                          // of every block of the cluster (first block)
+    unsigned long long group[THREADS];     // best of every group of threads
+    unsigned long long every[128];         // those of the whole cluster
     unsigned long long threshold;
     unsigned long long best[THREADS / 32];
-    int n_scan, n_cand;
-    short scan[THREADS];
-    unsigned long long cand[CANDIDATES];
+    unsigned long long top[GPT2Q_TOP_MAX];  // the alternatives, in order (first block)
+    int n_cand;
+    unsigned long long cand[CANDIDATES];   // (first block)
+};
+struct LpSharedSums {  // without alternatives
+    Sums warp[8];
+    Sums part[8];
 };
 
 // One pass over the logits. A cluster of `parts` blocks shares a row (one where there are rows
@@ -166,15 +212,18 @@ struct LpShared {
 // time: the batch's largest logit first, so that the running sums are rescaled at most once per
 // batch, then the exponentials.
 //
-// Alternatives need no second pass: the k-th best of the groups' best logits (a group is 2 to 8
-// threads) is reached by k elements at least, so only elements from there on matter, and only
-// threads whose own best reaches it can hold any. Those threads' elements, a small part of the
-// row, are read once more from L2, and what passes (a few dozen) is ranked by counting. Rows that
-// put more than CANDIDATES elements above the threshold take one round of search per alternative.
-template <class T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) k_logprobs(const __grid_constant__ LpParams p) {
+// Alternatives need no second pass. Each thread keeps its best logit, the vector that holds it and
+// the best of its other vectors. The k-th best of the bests of 64 or 128 groups of threads is
+// reached by at least k elements, so only elements from there on matter: those lie in the best
+// vectors of the threads that reach it (a few more than k), and in other vectors only of threads
+// whose second best reaches it (a few). These are read once more, and what passes is ranked by
+// counting. Rereading every vector of the first kind of thread, which needs no second best, cost 42
+// thousand cycles a row in a call of 4096 rows, as the row had left L2 by then. Rows that put more
+// than CANDIDATES elements above the threshold take one round of search per alternative.
+template <class T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __grid_constant__ LpParams p) {
     constexpr int VE = Row<T>::VE, U = 32 / VE;  // vectors of a batch
-    __shared__ LpShared sh;
+    __shared__ std::conditional_t<TOP, LpShared<THREADS>, LpSharedSums> sh;
     namespace cg = cooperative_groups;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
@@ -185,132 +234,169 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(const __grid_constant__
     const int share = (row.vectors + p.parts - 1) / p.parts;
     const int v0 = share * part, v1 = min(v0 + share, row.vectors);
     const float c = p.inv_t * LOG2E;
-    const bool leader = part == 0 && tid == 0;
     long long target = -1;
     float xt = 0.f;
-    if (leader && p.lp) {
+    if (part == 0 && tid == 0 && p.lp) {
         target = target_of(p.targets, p.i64, r);
         if (target >= 0 && target < p.vocab) xt = to_f(x[target]);
     }
 
-    float m = -INFINITY;
+    float m = -INFINITY, second = -INFINITY;
     float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
-    int at = v0 + tid;  // the vector that holds this thread's best logit first
+    int at = v0 + tid;  // the first vector that holds this thread's best logit
+    // a batch whose vectors all lie inside the row takes no checks of its own
+    const int in0 = row.shift ? 1 : 0, in1 = min(v1, (p.vocab + row.shift) / VE);
+    const uint4* vec = reinterpret_cast<const uint4*>(x - row.shift);
+    auto sums = [&](const uint4& raw, float2 nm, float2 cc) {
+        float2 f[VE / 2];
+        unpack<T>(raw, f);
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+            const float2 z = mul2(add2(f[i], nm), cc);
+            const float2 e = make_float2(ex2(z.x), ex2(z.y));
+            s = add2(s, e);
+            t = fma2(e, make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f)), t);
+        }
+    };
     for (int v = v0 + tid; v < v1; v += U * THREADS) {
         uint4 raw[U];
+        const bool inside = v >= in0 && v + (U - 1) * THREADS < in1;
+        if (inside) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vu = v + u * THREADS;
-            raw[u] = vu < v1 ? row.load(vu) : nothing<T>();
+            for (int u = 0; u < U; ++u) raw[u] = __ldcg(vec + v + u * THREADS);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = v + u * THREADS < v1 ? row.load(v + u * THREADS) : nothing<T>();
         }
-        float bm = -INFINITY;
+        float bm = m;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float2 f[VE / 2];
-            unpack<T>(raw[u], f);
-#pragma unroll
-            for (int i = 0; i < VE / 2; ++i) bm = fmaxf(bm, fmaxf(f[i].x, f[i].y));
+            const float um = largest<T>(raw[u]);
+            if constexpr (TOP) {
+                // the first vector counts as the best until a larger one comes
+                if (u > 0 || v != v0 + tid) second = fmaxf(second, fminf(bm, um));
+                if (um > bm) at = v + u * THREADS;
+            }
+            bm = fmaxf(bm, um);
         }
         if (bm > m) {
             const float z = fmaxf((m - bm) * c, -2000.f), w = ex2(z);
             t = make_float2(w * fmaf(z, s.x, t.x), w * fmaf(z, s.y, t.y));
             s = make_float2(w * s.x, w * s.y);
             m = bm;
-            if constexpr (TOP) {
-#pragma unroll
-                for (int u = U - 1; u >= 0; --u) {
-                    float2 f[VE / 2];
-                    unpack<T>(raw[u], f);
-                    float um = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < VE / 2; ++i) um = fmaxf(um, fmaxf(f[i].x, f[i].y));
-                    if (um == bm) at = v + u * THREADS;
-                }
-            }
         }
         const float ref = m == -INFINITY ? 0.f : m;
         const float2 nm = make_float2(-ref, -ref), cc = make_float2(c, c);
+        if (inside) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float2 f[VE / 2];
-            unpack<T>(raw[u], f);
+            for (int u = 0; u < U; ++u) sums(raw[u], nm, cc);
+        } else {
 #pragma unroll
-            for (int i = 0; i < VE / 2; ++i) {
-                const float2 z = mul2(add2(f[i], nm), cc);
-                const float2 e = make_float2(ex2(z.x), ex2(z.y));
-                s = add2(s, e);
-                t = fma2(e, make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f)), t);
-            }
+            for (int u = 0; u < U; ++u)
+                if (v + u * THREADS < v1) sums(raw[u], nm, cc);
         }
     }
-    const float mine = m;
-    Sums a{m, s.x + s.y, t.x + t.y};
+    if constexpr (TOP) {
+        // at most the key of the thread's best element: its value, and its vector's last index
+        const int groups = (p.top <= 20 ? 64 : 128) / p.parts, g = THREADS / groups;
+        unsigned long long key = v0 + tid < v1 ? rank_key(m, row.first(at) + VE - 1) : (unsigned)blockIdx.x * THREADS + tid;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                     __shfl_xor_sync(0xffffffffu, a.t, o)};
-        a = (lane & o) ? merge(b, a, c) : merge(a, b, c);  // the same order in both lanes
+        for (int o = 1; o < 32; o <<= 1)
+            if (o < g) key = maxu(key, __shfl_xor_sync(0xffffffffu, key, o));
+        if (tid % g == 0) sh.group[tid / g] = key;
+        if (tid == 0) sh.n_cand = 0, sh.threshold = 0;
     }
+    const Sums none{-INFINITY, 0.f, 0.f};
+    Sums a = join(Sums{m, s.x + s.y, t.x + t.y}, c);
     if (lane == 0) sh.warp[warp] = a;
-    if (tid == 0) sh.n_scan = 0, sh.n_cand = 0, sh.threshold = 0;
+    auto* first = p.parts > 1 ? cg::this_cluster().map_shared_rank(&sh, 0) : &sh;
 
     if constexpr (TOP) {
-        const int K = p.top;
-        const bool any = v0 + tid < v1;
-        // at most the thread's best element's key: its value, and the last index of its vector
-        unsigned long long key = any ? rank_key(mine, row.first(at) + VE - 1) : 0;
-        const int g = K <= 20 ? 8 : K <= 40 ? 4 : 2;
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1)
-            if (o < g) key = maxu(key, __shfl_xor_sync(0xffffffffu, key, o));
-        if (lane % g == 0) sh.group[tid / g] = key;
+        const int groups = (p.top <= 20 ? 64 : 128) / p.parts;
+        const int total = groups * p.parts;
+        const unsigned long long* keys = sh.group;
+        if (p.parts > 1) {
+            cg::this_cluster().sync();
+            if (tid < total) sh.every[tid] = cg::this_cluster().map_shared_rank(&sh, tid / groups)->group[tid % groups];
+            keys = sh.every;
+        }
         __syncthreads();
-        const int G = THREADS / g;
-        if (tid < G) {
-            const unsigned long long k0 = sh.group[tid];
+        // the `top`-th of the groups' keys, which are all different (the keys of groups without a
+        // vector, below 2^32, pass for no threshold); four or fewer threads count for a key
+        {
+            const int share_n = THREADS / total, k = tid / share_n, i0 = tid % share_n;
+            const unsigned long long k0 = keys[k];
             int above = 0;
-            for (int i = 0; i < G; ++i) above += sh.group[i] > k0 || (sh.group[i] == k0 && i < tid);
-            if (above == K - 1) sh.threshold = k0;  // 0 where fewer than K groups hold anything
+#pragma unroll 8
+            for (int i = i0; i < total; i += share_n) above += keys[i] > k0;
+            for (int o = 1; o < share_n; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+            if (above == p.top - 1 && i0 == 0) sh.threshold = k0 >> 32 ? k0 : 0;
         }
         __syncthreads();
         const unsigned long long thr = sh.threshold;
-        // the thread's best possible key: its value at the first index of its vector
-        if (any && rank_key(mine, max(0, row.first(at))) >= thr) sh.scan[atomicAdd(&sh.n_scan, 1)] = (short)tid;
-        __syncthreads();
-        const int per = (v1 - v0 + THREADS - 1) / THREADS;
-        for (int i = tid; i < sh.n_scan * per; i += THREADS) {
-            const int v = v0 + sh.scan[i / per] + (i % per) * THREADS;
-            if (v < v1) {
-                float2 f[VE / 2];
-                unpack<T>(row.load(v), f);
-                const int e = row.first(v);
+        const float least = thr ? key_value(thr) : -INFINITY;
+        auto take = [&](const uint4& raw, int v) {
+            float2 f[VE / 2];
+            unpack<T>(raw, f);
+            const int e = row.first(v);
 #pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    const float y = j & 1 ? f[j / 2].y : f[j / 2].x;
-                    const unsigned long long k = rank_key(y, e + j);
-                    if (k >= thr && e + j >= 0 && e + j < p.vocab) {
-                        const int n = atomicAdd(&sh.n_cand, 1);
-                        if (n < CANDIDATES) sh.cand[n] = k;
-                    }
+            for (int j = 0; j < VE; ++j) {
+                const float y = j & 1 ? f[j / 2].y : f[j / 2].x;
+                if (y < least || e + j < 0 || e + j >= p.vocab) continue;
+                const unsigned long long k = rank_key(y, e + j);
+                if (k >= thr) {
+                    const int n = atomicAdd(&first->n_cand, 1);
+                    if (n < CANDIDATES) first->cand[n] = k;
                 }
             }
+        };
+        // the best keys possible: of the best element, and of the other vectors' best
+        const int other = at == v0 + tid ? at + THREADS : v0 + tid;
+        const bool every = other < v1 && second >= least && rank_key(second, max(0, row.first(other))) >= thr;
+        if (!every && v0 + tid < v1 && m >= least && rank_key(m, max(0, row.first(at))) >= thr) take(row.load(at), at);
+        for (unsigned todo = __ballot_sync(0xffffffffu, every); todo; todo &= todo - 1) {
+            // the warp rereads all vectors of one of its threads, four loads at a time
+            const int v2 = v0 + warp * 32 + __ffs(todo) - 1;
+            for (int v = v2 + lane * THREADS; v < v1; v += 4 * 32 * THREADS) {
+                uint4 raw[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) raw[q] = v + q * 32 * THREADS < v1 ? row.load(v + q * 32 * THREADS) : nothing<T>();
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (v + q * 32 * THREADS < v1) take(raw[q], v + q * 32 * THREADS);
+            }
         }
-        if (tid < GPT2Q_TOP_MAX) sh.top[tid] = 0;
+    } else {
         __syncthreads();
+    }
+    if (warp == 0) {
+        a = join(lane < THREADS / 32 ? sh.warp[lane] : none, c);
+        if (lane == 0) first->part[part] = a;
+    }
+    if (p.parts > 1)
+        cg::this_cluster().sync();  // after it only the first block's shared memory is used
+    else
+        __syncthreads();
+    if (part != 0) return;
+    if (warp == 0) {
+        a = join(lane < p.parts ? sh.part[lane] : none, c);
+        if (lane == 0) sh.warp[0] = a;
+    }
+    if constexpr (TOP) {
         const int n = sh.n_cand;
         if (n <= CANDIDATES) {
             for (int i = tid; i < n; i += THREADS) {
                 const unsigned long long k = sh.cand[i];
                 int above = 0;
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
-                if (above < K) sh.top[above] = k;
+                if (above < p.top) sh.top[above] = k;
             }
         } else {
             unsigned long long last = ~0ull;
-            for (int q = 0; q < K && last; ++q) {
+            for (int q = 0; q < p.top; ++q) {
                 unsigned long long best = 0;
-                const int e1 = min(p.vocab, row.first(v1));
-                for (int e = max(0, row.first(v0)) + tid; e < e1; e += THREADS) {
+                for (int e = tid; e < p.vocab; e += THREADS) {
                     const unsigned long long k = rank_key(to_f(x[e]), e);
                     if (k < last) best = maxu(best, k);
                 }
@@ -326,36 +412,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(const __grid_constant__
         }
     }
     __syncthreads();
-    if (tid == 0) {
-        a = sh.warp[0];
-        for (int w = 1; w < THREADS / 32; ++w) a = merge(a, sh.warp[w], c);
-        sh.part = a;
-    }
-    if (p.parts > 1) {
-        cg::this_cluster().sync();
-        if (part == 0) {
-            if (tid == 0) {
-                for (int q = 1; q < p.parts; ++q) a = merge(a, cg::this_cluster().map_shared_rank(&sh, q)->part, c);
-                sh.part = a;
-            }
-            if constexpr (TOP) {
-                for (int i = tid; i < p.parts * p.top; i += THREADS)
-                    sh.cand[i] = cg::this_cluster().map_shared_rank(&sh, i / p.top)->top[i % p.top];
-                __syncthreads();
-                const int n = p.parts * p.top;
-                for (int i = tid; i < n; i += THREADS) {
-                    const unsigned long long k = sh.cand[i];  // 0: the block has fewer elements than that
-                    int above = 0;
-                    for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
-                    if (k && above < p.top) sh.top[above] = k;
-                }
-            }
-        }
-        cg::this_cluster().sync();  // no block leaves while its shared memory may be read
-    }
-    if (part != 0) return;
-    __syncthreads();
-    a = sh.part;
+    a = sh.warp[0];
     const bool empty = a.m == -INFINITY && a.s == 0.f;
     const float ls = empty ? -INFINITY : logf(a.s);
     auto lp_of = [&](float v) { return empty ? -INFINITY : (v - a.m) * p.inv_t - ls; };
@@ -374,26 +431,39 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(const __grid_constant__
     }
 }
 
-template <class T>
-cudaError_t launch_logprobs(LpParams p, cudaStream_t st) {
-    // blocks per row: enough for eight per SM in all, as long as every thread has a batch
-    const int batches = (p.vocab + 32 * THREADS - 1) / (32 * THREADS);
-    p.parts = 1;
-    while (p.parts < 8 && p.parts < batches && (long long)p.rows * p.parts < 148 * 8) p.parts *= 2;
+template <class T, int THREADS>
+cudaError_t launch_logprobs_by(LpParams p, cudaStream_t st) {
     if ((long long)p.rows * p.parts > INT32_MAX) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.rows * p.parts);
     cfg.blockDim = dim3(THREADS);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = p.parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = p.parts;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return p.top ? cudaLaunchKernelEx(&cfg, k_logprobs<T, true>, p) : cudaLaunchKernelEx(&cfg, k_logprobs<T, false>, p);
+    cfg.numAttrs = p.parts > 1 ? 2 : 1;
+    return p.top ? cudaLaunchKernelEx(&cfg, k_logprobs<T, true, THREADS>, p)
+                 : cudaLaunchKernelEx(&cfg, k_logprobs<T, false, THREADS>, p);
+}
+
+template <class T>
+cudaError_t launch_logprobs(LpParams p, cudaStream_t st) {
+    // Blocks per row: as many as still run at the same time (four of 256 threads per SM), while a
+    // thread has a batch. 256 rows of 128000 bf16, 20 alternatives: 29.6, 21.4, 25.3 and 35.0 us with
+    // 1, 2, 4 and 8 blocks per row; one row: 15.8, 11.1, 7.7, 6.6 us.
+    const int batches = (p.vocab + 32 * 256 - 1) / (32 * 256);
+    p.parts = 1;
+    while (p.parts < 8 && p.parts < batches && (long long)p.rows * p.parts * 2 <= 148 * 4) p.parts *= 2;
+    // With more rows than run at once, eight blocks of 128 threads per SM overlap one row's end with
+    // other rows' loads better than four of 256 (2000 rows of 50257 bf16: 44 and 46 us, with 20
+    // alternatives 62 and 66), but for many alternatives, whose ranking is shared by the threads (64 of
+    // 4096 fp32 rows: 228 and 190 us).
+    if (p.rows > 148 * 4 && p.top <= 20) return launch_logprobs_by<T, 128>(p, st);
+    return launch_logprobs_by<T, 256>(p, st);
 }
 
 struct GradParams {
@@ -466,11 +536,12 @@ __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant
     const float m = __ldcg(p.stats + 3LL * r), ls = __ldcg(p.stats + 3LL * r + 1), h = __ldcg(p.stats + 3LL * r + 2);
     float g = p.d_lp ? __ldcg(p.d_lp + r) : 0.f;
     const float ge = p.d_ent ? __ldcg(p.d_ent + r) : 0.f;
-    long long target = -1;
+    int target = -1;
     if (p.d_lp) {
-        target = target_of(p.targets, p.i64, r);
-        if (target < 0) g = 0.f;
-        if (target >= p.vocab) g = NAN;
+        const long long t = target_of(p.targets, p.i64, r);
+        target = t >= 0 && t < p.vocab ? (int)t : -1;
+        if (t < 0) g = 0.f;
+        if (t >= p.vocab) g = NAN;
     }
     const bool empty = m == -INFINITY && ls == -INFINITY;
     const float A = -p.inv_t * (g + ge * h), B = -p.inv_t * ge * LN2, hit = p.inv_t * g;
@@ -481,23 +552,28 @@ __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant
         if (vu >= out.vectors) break;
         float2 f[VE / 2];
         unpack<T>(raw[u], f);
-        union {
-            uint4 u4;
-            T t[VE];
-        } o;
 #pragma unroll
         for (int i = 0; i < VE / 2; ++i) {
             const float2 z = fma2(add2(f[i], make_float2(-m, -m)), make_float2(c, c), make_float2(l2, l2));
             const float2 q = make_float2(ex2(z.x), ex2(z.y));
             // log2 p of a masked element is -inf; the clamp keeps its 0 * log2 p at 0
             const float2 k = fma2(make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f)), make_float2(B, B), make_float2(A, A));
-            float2 d = mul2(q, k);
-            if (target == e + 2 * i) d.x += hit;
-            if (target == e + 2 * i + 1) d.y += hit;
-            if (empty) d = make_float2(0.f, 0.f);
-            o.t[2 * i] = from_f<T>(d.x);
-            o.t[2 * i + 1] = from_f<T>(d.y);
+            f[i] = mul2(q, k);
         }
+        if (target >= e && target < e + VE) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (target == e + i) (i & 1 ? f[i / 2].y : f[i / 2].x) += hit;
+        }
+        if (empty) {
+#pragma unroll
+            for (int i = 0; i < VE / 2; ++i) f[i] = make_float2(0.f, 0.f);
+        }
+        union {
+            uint4 u4;
+            T t[VE];
+        } o;
+        o.u4 = packed<T>(f);
         if (e >= 0 && e + VE <= p.vocab) {
             *reinterpret_cast<uint4*>(dx + e) = o.u4;
         } else {
