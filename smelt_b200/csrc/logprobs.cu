@@ -477,65 +477,47 @@ struct GradParams {
     const float *stats, *d_lp, *d_ent;
 };
 
-// 16 bytes from byte `by` (a multiple of the element's size, under 16) of the 32 bytes (a, b).
+// 16 bytes from byte `by` (a multiple of the element's size, under 16) of the 32 bytes (a, b). `by`
+// is the same in all lanes of a row, so the branch is uniform.
 __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int by) {
-    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (by & 8) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-    }
-    if (by & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-    }
     const int bits = (by & 3) * 8;
-    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    switch (by >> 2) {
+        case 0:
+            return make_uint4(__funnelshift_r(a.x, a.y, bits), __funnelshift_r(a.y, a.z, bits),
+                              __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits));
+        case 1:
+            return make_uint4(__funnelshift_r(a.y, a.z, bits), __funnelshift_r(a.z, a.w, bits),
+                              __funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits));
+        case 2:
+            return make_uint4(__funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits),
+                              __funnelshift_r(b.x, b.y, bits), __funnelshift_r(b.y, b.z, bits));
+        default:
+            return make_uint4(__funnelshift_r(a.w, b.x, bits), __funnelshift_r(b.x, b.y, bits),
+                              __funnelshift_r(b.y, b.z, bits), __funnelshift_r(b.z, b.w, bits));
+    }
 }
 
-// One element in, one out: d_j = -p_j (A + B log2 p_j), the target's plus g / temperature. A block
-// takes four vectors per thread of one row. Vectors are the output's; where the input row lies
-// differently against the 16-byte boundaries, its 16 bytes are cut from two aligned vectors, the
-// second of which the neighbouring lane holds.
-template <class T>
+// One element in, one out: d_j = -p_j (A + B log2 p_j), the target's plus g / temperature; without an
+// entropy gradient (ENT false) B is 0. A block takes four vectors per thread of one row at a time. Vectors are
+// the output's; where the input row lies differently against the 16-byte boundaries, its 16 bytes are
+// cut from two aligned vectors, the second of which the neighbouring lane holds. Only warps at a
+// row's ends check where they are.
+template <class T, bool ENT>
 __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant__ GradParams p) {
     constexpr int VE = Row<T>::VE, U = 4;
     tc::pdl_trigger();
     tc::pdl_wait();
-    const int r = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
+    const int r = blockIdx.x / p.chunks, chunk = blockIdx.x - r * p.chunks;
     const Row<T> in(static_cast<const T*>(p.x) + (long long)r * p.ld, p.vocab);
     T* dx = static_cast<T*>(p.dx) + (long long)r * p.ldo;
     const Row<T> out(dx, p.vocab);
-    const int v = chunk * U * THREADS + threadIdx.x;
-    // element e of the output's vector is e + off of the input's, counted from its boundary
-    const int off = in.shift - out.shift;
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int vu = v + u * THREADS, e = out.first(vu);
-        if (off == 0) {
-            raw[u] = vu < out.vectors ? in.load(vu) : nothing<T>();
-        } else {
-            const int q = vu * VE + off, v0 = q >= 0 ? q / VE : -1;  // off > -VE
-            const int e0 = in.first(v0);
-            const uint4* src = reinterpret_cast<const uint4*>(in.x - in.shift) + v0;
-            uint4 a = nothing<T>(), b;
-            if (e0 >= 0 && e0 + VE <= p.vocab) a = __ldcg(src);
-            b.x = __shfl_down_sync(0xffffffffu, a.x, 1);
-            b.y = __shfl_down_sync(0xffffffffu, a.y, 1);
-            b.z = __shfl_down_sync(0xffffffffu, a.z, 1);
-            b.w = __shfl_down_sync(0xffffffffu, a.w, 1);
-            if (e0 >= 0 && e0 + 2 * VE <= p.vocab) {
-                if ((threadIdx.x & 31) == 31) b = __ldcg(src + 1);
-                raw[u] = shifted(a, b, (q - v0 * VE) * (int)sizeof(T));
-            } else {
-                raw[u] = vu < out.vectors ? in.edge(e) : nothing<T>();
-            }
-        }
-    }
-    const float m = __ldcg(p.stats + 3LL * r), ls = __ldcg(p.stats + 3LL * r + 1), h = __ldcg(p.stats + 3LL * r + 2);
+    const int lane = threadIdx.x & 31;
+    // the output's vector v begins `off` elements into the input's vector v + down
+    const int off = (in.shift - out.shift + VE) % VE, down = in.shift < out.shift ? -1 : 0;
+    const uint4* src0 = reinterpret_cast<const uint4*>(in.x - in.shift) + down + lane;
+    float m = __ldcg(p.stats + 3LL * r), ls = __ldcg(p.stats + 3LL * r + 1), h = __ldcg(p.stats + 3LL * r + 2);
     float g = p.d_lp ? __ldcg(p.d_lp + r) : 0.f;
-    const float ge = p.d_ent ? __ldcg(p.d_ent + r) : 0.f;
+    const float ge = ENT ? __ldcg(p.d_ent + r) : 0.f;
     int target = -1;
     if (p.d_lp) {
         const long long t = target_of(p.targets, p.i64, r);
@@ -543,43 +525,85 @@ __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant
         if (t < 0) g = 0.f;
         if (t >= p.vocab) g = NAN;
     }
-    const bool empty = m == -INFINITY && ls == -INFINITY;
-    const float A = -p.inv_t * (g + ge * h), B = -p.inv_t * ge * LN2, hit = p.inv_t * g;
+    float A = -p.inv_t * (g + ge * h), B = -p.inv_t * ge * LN2, hit = p.inv_t * g;
+    if (m == -INFINITY && ls == -INFINITY) m = 0.f, ls = INFINITY, A = B = hit = 0.f;  // a row of nothing but -inf: all zeros
     const float c = p.inv_t * LOG2E, l2 = -ls * LOG2E;
+    // a warp's U * 32 vectors lie side by side
+    for (int wv = chunk * U * THREADS + (threadIdx.x & ~31) * U; wv < out.vectors; wv += p.chunks * U * THREADS) {
+        const uint4* src = src0 + wv;
+        uint4 raw[U];
+        bool inner[U];  // all of the warp's vectors, and those they are cut from, are inside the row
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int vu = v + u * THREADS, e = out.first(vu);
-        if (vu >= out.vectors) break;
-        float2 f[VE / 2];
-        unpack<T>(raw[u], f);
-#pragma unroll
-        for (int i = 0; i < VE / 2; ++i) {
-            const float2 z = fma2(add2(f[i], make_float2(-m, -m)), make_float2(c, c), make_float2(l2, l2));
-            const float2 q = make_float2(ex2(z.x), ex2(z.y));
-            // log2 p of a masked element is -inf; the clamp keeps its 0 * log2 p at 0
-            const float2 k = fma2(make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f)), make_float2(B, B), make_float2(A, A));
-            f[i] = mul2(q, k);
+        for (int u = 0; u < U; ++u) {
+            const int w0 = wv + u * 32;
+            inner[u] = w0 >= 2 && (w0 + 34) * VE <= p.vocab;
+            if (inner[u])
+                raw[u] = __ldcg(src + u * 32);
+            else if (w0 < out.vectors)
+                raw[u] = in.edge(out.first(w0 + lane));
         }
-        if (target >= e && target < e + VE) {
+        if (off && inner[0]) {
+            // lane i's second vector is lane i + 1's, lane 31's that of lane 0 one step on; the last
+            // inner step's is loaded for it
+            int last = 0;
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-                if (target == e + i) (i & 1 ? f[i / 2].y : f[i / 2].x) += hit;
+            for (int u = 1; u < U; ++u) last += inner[u];
+            uint4 more = raw[0];
+            if (lane == 0) more = __ldcg(src + last * 32 + 32);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (!inner[u]) continue;
+                uint4 b = u + 1 < U && u < last ? raw[u + 1 < U ? u + 1 : u] : more;
+                if (lane != 0) b = raw[u];
+                b.x = __shfl_sync(0xffffffffu, b.x, (lane + 1) & 31);
+                b.y = __shfl_sync(0xffffffffu, b.y, (lane + 1) & 31);
+                b.z = __shfl_sync(0xffffffffu, b.z, (lane + 1) & 31);
+                b.w = __shfl_sync(0xffffffffu, b.w, (lane + 1) & 31);
+                raw[u] = shifted(raw[u], b, off * (int)sizeof(T));
+            }
+        } else if (off) {
+            // the row's beginning: its inner steps one by one
+#pragma unroll
+            for (int u = 1; u < U; ++u) {
+                if (!inner[u]) continue;
+                raw[u] = in.edge(out.first(wv + u * 32 + lane));
+            }
         }
-        if (empty) {
 #pragma unroll
-            for (int i = 0; i < VE / 2; ++i) f[i] = make_float2(0.f, 0.f);
-        }
-        union {
-            uint4 u4;
-            T t[VE];
-        } o;
-        o.u4 = packed<T>(f);
-        if (e >= 0 && e + VE <= p.vocab) {
-            *reinterpret_cast<uint4*>(dx + e) = o.u4;
-        } else {
+        for (int u = 0; u < U; ++u) {
+            const int v = wv + u * 32 + lane, e = out.first(v);
+            if (!inner[u] && v >= out.vectors) continue;
+            float2 f[VE / 2];
+            unpack<T>(raw[u], f);
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-                if (e + i >= 0 && e + i < p.vocab) dx[e + i] = o.t[i];
+            for (int i = 0; i < VE / 2; ++i) {
+                const float2 z = fma2(add2(f[i], make_float2(-m, -m)), make_float2(c, c), make_float2(l2, l2));
+                const float2 q = make_float2(ex2(z.x), ex2(z.y));
+                if constexpr (ENT) {
+                    // log2 p of a masked element is -inf; the clamp keeps its 0 * log2 p at 0
+                    const float2 k = make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f));
+                    f[i] = mul2(q, fma2(k, make_float2(B, B), make_float2(A, A)));
+                } else {
+                    f[i] = mul2(q, make_float2(A, A));
+                }
+            }
+            if ((unsigned)(target - e) < (unsigned)VE && target >= 0) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (target == e + i) (i & 1 ? f[i / 2].y : f[i / 2].x) += hit;
+            }
+            union {
+                uint4 u4;
+                T t[VE];
+            } o;
+            o.u4 = packed<T>(f);
+            if (inner[u] || (e >= 0 && e + VE <= p.vocab)) {
+                *reinterpret_cast<uint4*>(dx + e) = o.u4;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (e + i >= 0 && e + i < p.vocab) dx[e + i] = o.t[i];
+            }
         }
     }
 }
@@ -587,9 +611,15 @@ __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant
 template <class T>
 cudaError_t launch_grad(GradParams p, cudaStream_t st) {
     constexpr int per = 4 * THREADS * Row<T>::VE;
-    p.chunks = (p.vocab + Row<T>::VE - 1 + per - 1) / per;
+    // blocks per row: one batch of four vectors per thread each while the call has fewer blocks than
+    // run at once (five per SM), else as few as fill the GPU four times over, so that a thread's reading of the row's
+    // statistics and alignment serves many batches
+    const int most = (p.vocab + Row<T>::VE - 1 + per - 1) / per;
+    p.chunks = (int)std::clamp<long long>(148LL * 5 * 4 / p.rows, 1, most);
     if ((long long)p.rows * p.chunks > INT32_MAX) return cudaErrorInvalidConfiguration;
-    return launch_dependent(k_logprobs_grad<T>, dim3((unsigned)p.rows * p.chunks), dim3(THREADS), 0, st, p);
+    const dim3 grid((unsigned)p.rows * p.chunks);
+    return p.d_ent ? launch_dependent(k_logprobs_grad<T, true>, grid, dim3(THREADS), 0, st, p)
+                   : launch_dependent(k_logprobs_grad<T, false>, grid, dim3(THREADS), 0, st, p);
 }
 
 int refuse(const char* who, const char* msg) {
