@@ -316,6 +316,7 @@ typedef struct gpt2q_heads {
 #define GPT2Q_STATUS_PAGE 1     /* a page id outside [0, n_pages) was needed */
 #define GPT2Q_STATUS_POSITION 2 /* a position or length past the table's width */
 #define GPT2Q_STATUS_ROW 4      /* a table row outside [0, n_rows) */
+#define GPT2Q_STATUS_TIMEOUT 8  /* a bounded device-side wait gave up (results are NaN) */
 
 /* Appends n_tokens keys and values (both or neither of k->data and v->data) to the cache. Token i
  * belongs to table row d_seq[i] (d_seq NULL: row i) and position d_pos[i]. Keys are rotated when

@@ -20,6 +20,7 @@ pub const GPT2Q_BF16: c_int = 2;
 pub const GPT2Q_STATUS_PAGE: c_int = 1;
 pub const GPT2Q_STATUS_POSITION: c_int = 2;
 pub const GPT2Q_STATUS_ROW: c_int = 4;
+pub const GPT2Q_STATUS_TIMEOUT: c_int = 8;
 pub const GPT2Q_TOP_MAX: c_int = 64;
 
 #[repr(C)]

@@ -34,7 +34,7 @@ struct PagedAttn {
     float scale;
     int* status;
     int page_shift;  // page = 1 << page_shift, or -1
-    int grouped;     // a page holds whole groups of keys
+    int boxes;       // pieces of 128 bytes of a key
     // a kv head's `group` query heads are taken in blocks_per_kv blocks of up to heads_per_block
     int blocks_per_kv, n_vh, heads_per_block;
     int warp_bytes;  // shared memory of a warp

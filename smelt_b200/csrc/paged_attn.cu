@@ -11,9 +11,13 @@
 // inside the block, through shared memory, and then over the blocks in a second small kernel.
 // Nothing is accumulated with atomics, so results are the same on every run.
 //
-// A warp streams its tiles through a ring of three shared-memory stages of its own (cp.async, 16
-// bytes per lane; the page of every key is looked up one tile ahead), so warps never wait for each
-// other while they stream.
+// A warp streams its tiles through a ring of two shared-memory stages of its own, so warps never
+// wait for each other while they stream. Where a page is a multiple of 16 keys (8 for the short
+// tiles of an fp32 cache), one lane starts the tile's copies as TMA boxes of up to 16 keys x 128
+// bytes, swizzled; pages are looked up a tile ahead. Other page sizes are gathered key by key
+// with cp.async.
+#include <cuda.h>
+
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -29,8 +33,8 @@ using namespace gpt2q;
 
 namespace {
 
-constexpr int STAGES = 3;
-constexpr int MAX_WARPS = 8;
+constexpr int STAGES = 2;
+constexpr int MAX_WARPS = 12;
 constexpr int MAX_CTAS = 148;  // one per SM of a B200
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -46,10 +50,16 @@ struct Cfg {
     static constexpr int ROWB = HD * (int)sizeof(TC);
     static constexpr int CHP = ROWB / 16;  // 16-byte chunks of a row
     // keys of a tile: 8 KB of keys and values (16 KB at 256 dims)
-    static constexpr int TK = F32 ? (HD == 64 ? 16 : 8) : (HD == 64 ? 32 : 16);
-    static constexpr int LPK = 32 / TK;  // lanes per key (fp32 cache)
+    static constexpr int TK = F32 ? (HD == 256 ? 8 : 4096 / ROWB) : (HD == 256 ? 16 : 4096 / ROWB);
+    static __device__ constexpr int lpk() { return 32 / TK; }  // lanes per key (fp32 cache)
     static constexpr int GR = TK < 16 ? TK : 16, NG = TK / GR;  // keys of one page lookup where pages allow it
-    static constexpr int ITS = TK * CHP / 32, RPI = 32 / CHP > 0 ? 32 / CHP : 1;  // copies of a tile, rows of one copy
+    static constexpr int BOX = 128 / (int)sizeof(TC);  // dims of a TMA box
+    // a tile's rows are cut into pieces of 128 bytes, piece by piece one after the other; the 16-byte
+    // chunks of a piece are permuted by the row (the 128-byte swizzle), so that eight rows of one
+    // chunk lie in different banks
+    static __device__ __forceinline__ int at(int r, int c) {
+        return (c >> 3) * (TK * 128) + r * 128 + (((c ^ r) & 7) << 4);
+    }
     static constexpr int STAGE = 2 * TK * ROWB;
     static constexpr int HS = HD + 4;  // floats of a partial result's row
     // 16-bit pieces of the query and of the weights. Queries of the cache's type are exact in one;
@@ -58,13 +68,19 @@ struct Cfg {
     static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : HALF ? 2 : 3;
     static constexpr int sp() { return SQ == 1 ? 2 : SQ; }
     static constexpr int MT = TK / 16, NT = HB / 8, KD = HD / 16;
+    static __device__ constexpr int acc() { return MT * NT == 1 ? 2 : 1; }  // independent sums of a score tile
     // fp16 weights are held times 2^10, so that small ones stay normal numbers
     static constexpr float shift() { return HALF ? 10.f : 0.f; }
+    // rows whose queries are staged per warp: of the two tiles on their way and, where they are not held in
+    // registers, of the one worked on
+    static constexpr int QS = F32 ? 3 : 2;
+    // warps of a block, by the registers that queries and results take
+    static constexpr int WARPS = !F32 && SQ * NT * KD * 2 + NT * KD * 4 > 100 ? 8 : MAX_WARPS;
     static constexpr float UNSHIFT = HALF ? 1.f / 1024.f : 1.f;
 };
 
 struct Walk {
-    int row, vh, j, nt, start, end;
+    int row, kvh, hb, j, nt, start, end;  // hb: block of the kv head's query heads
     bool over;
 };
 
@@ -82,15 +98,17 @@ __device__ __forceinline__ void enter(const PagedAttn& p, Walk& w, int row) {
     w.end = w.over ? p.cap : len;
     w.start = p.window > 0 && w.end > p.window ? w.end - p.window : 0;
     // tiles begin at multiples of TK, so that a group of GR keys lies in one page
-    w.nt = w.end > 0 ? (w.end + C::TK - 1) / C::TK - w.start / C::TK : 0;
+    w.nt = w.end > 0 ? (int)((unsigned)(w.end + C::TK - 1) / C::TK - (unsigned)w.start / C::TK) : 0;
 }
 
 template <class C>
 __device__ __forceinline__ void advance(const PagedAttn& p, Walk& w) {
     if (++w.j < w.nt) return;
     w.j = 0;
-    if (++w.vh < p.n_vh) return;
-    w.vh = 0;
+    if (++w.hb < p.blocks_per_kv) return;
+    w.hb = 0;
+    if (++w.kvh < p.n_kv) return;
+    w.kvh = 0;
     do {
         enter<C>(p, w, w.row + 1);
     } while (w.nt == 0 && w.row < p.n_rows);
@@ -144,6 +162,12 @@ __device__ __forceinline__ uint32_t take_pair(float& a, float& b) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp; results under 2^-126 are 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -177,36 +201,50 @@ __device__ __forceinline__ void write1(const PagedAttn& p, int row, int head, in
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
 
-template <class C>
-__global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_constant__ PagedAttn p) {
+// ceil(a / b) and a / b of values that nearly always fit 32 bits (a 64-bit division is a hundred instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((unsigned long long)a | (unsigned long long)b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
+template <class C, bool TMA>
+__global__ void __launch_bounds__(C::WARPS * 32, 1)
+    k_paged_attn(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using TC = typename C::TC;
     using TI = typename C::TI;
     constexpr int HB = C::HB, HD = C::HD, TK = C::TK, NT = C::NT > 0 ? C::NT : 1, MT = C::MT > 0 ? C::MT : 1;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ long long cum[MAX_WARPS * 32 + 1];
     __shared__ long long wsum[MAX_WARPS];
     __shared__ Piece pieces[2 * MAX_WARPS];
+    __shared__ __align__(8) uint64_t full[MAX_WARPS][2 * STAGES];  // per stage: keys, values
     __shared__ float pm[2 * MAX_WARPS][HB], pl[2 * MAX_WARPS][HB];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x, nw = nthr >> 5;
     const int hv = p.heads_per_block;                    // heads a block's partial results hold
     const int qrow = HD * (int)sizeof(TI);               // bytes of a staged query
     unsigned char* ring = smem + (size_t)warp * p.warp_bytes;
     unsigned char* qring = ring + STAGES * C::STAGE;
-    float* pbuf = reinterpret_cast<float*>(qring + STAGES * hv * qrow);  // fp32 cache: the tile's weights
+    float* pbuf = reinterpret_cast<float*>(qring + C::QS * hv * qrow);  // fp32 cache: the tile's weights
     const uint32_t ring32 = tc::smem_u32(ring), q32 = tc::smem_u32(qring);
     const int nch = p.dim * (int)sizeof(TC) / 16, nqch = p.dim * (int)sizeof(TI) / 16;
 
     if (lane < 2) pieces[2 * warp + lane].nt = 0;
-    // dims past the head's own are zero in the ring and are never written again
-    if (nch < C::CHP)
-        for (int r = lane; r < STAGES * 2 * TK; r += 32)
-            for (int c = 0; c < C::CHP; ++c) {
-                const int rr = r % TK;
-                const int swz = C::F32 ? (rr * C::LPK) & 7 : rr & 7;
-                if (c >= nch) *reinterpret_cast<uint4*>(ring + r * C::ROWB + ((c ^ swz) * 16)) = make_uint4(0, 0, 0, 0);
+    if constexpr (TMA) {
+        if (lane == 0) {
+            for (int i = 0; i < 2 * STAGES; ++i) tc::mbar_init(&full[warp][i], 1);
+            tc::fence_mbar_init();
+            if (warp == 0) {
+                tc::prefetch_tmap(&kmap);
+                tc::prefetch_tmap(&vmap);
             }
+        }
+    } else if (nch < C::CHP) {
+        // dims past the head's own are zero in the ring and are never written again (TMA fills them)
+        for (int r = lane; r < STAGES * 2 * TK; r += 32)
+            for (int c = nch; c < C::CHP; ++c)
+                *reinterpret_cast<uint4*>(ring + r / TK * TK * C::ROWB + C::at(r % TK, c)) = make_uint4(0, 0, 0, 0);
+    }
     if (nch < C::CHP)
-        for (int i = lane; i < STAGES * hv * (qrow / 16); i += 32)
+        for (int i = lane; i < C::QS * hv * (qrow / 16); i += 32)
             if (i % (qrow / 16) >= nqch) *reinterpret_cast<uint4*>(qring + i * 16) = make_uint4(0, 0, 0, 0);
     tc::pdl_trigger();
     tc::pdl_wait();
@@ -235,9 +273,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
     }
     cum[tid] = before + inc - mine;
     __syncthreads();
-    const long long per = ((total + gridDim.x - 1) / gridDim.x + nw - 1) / nw * nw;
+    const long long wper = quotient(quotient(total + gridDim.x - 1, gridDim.x) + nw - 1, nw), per = wper * nw;
     const long long ca = per * blockIdx.x, cb = min(ca + per, total);
-    const long long a = ca + per / nw * warp, b = min(a + per / nw, cb);
+    const long long a = ca + wper * warp, b = min(a + wper, cb);
     const int n = (int)max(0LL, b - a);
 
     if (n > 0) {
@@ -257,90 +295,76 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
             rem -= (long long)w.nt * p.n_vh;
             enter<C>(p, w, ++row);
         }
-        w.vh = (int)(rem / w.nt);
-        w.j = (int)(rem - (long long)w.vh * w.nt);
-        // L is the next tile to load, N the one after it, whose pages are on their way
-        Walk L = w, N;
-        const int kr = lane & (TK - 1);
-        const bool grouped = p.grouped != 0;
-        int page[C::NG], npage[C::NG];
+        const int vh = (int)quotient(rem, w.nt);
+        w.j = (int)(rem - (long long)vh * w.nt);
+        w.kvh = vh / p.blocks_per_kv;
+        w.hb = vh - w.kvh * p.blocks_per_kv;
+        Walk L = w;  // the next tile to load; its pages are looked up when the tile before it is loaded
+        int page[C::NG];
         // page ids of a tile: of every group of GR keys (the same load in all lanes) where a page is
         // a multiple of GR, else of the lane's own key, in element 0
-        auto look = [&](const Walk& t, int* out) {
-            const int k0 = (t.start / TK + t.j) * TK;
-            const int* ids = p.table + (long long)t.row * p.ld;
-            if (grouped) {
+        auto look = [&]() {
+            const int k0 = ((unsigned)L.start / TK + L.j) * TK;
+            const int* ids = p.table + (long long)L.row * p.ld;
 #pragma unroll
-                for (int g = 0; g < C::NG; ++g) {
-                    const int key = k0 + g * C::GR;
-                    out[g] = key < t.end && key + C::GR > t.start
-                                 ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page))
-                                 : 0;
-                }
-            } else {
-                const int key = k0 + kr;
-                out[0] = key < t.end && key >= t.start ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page)) : 0;
+            for (int g = 0; g < C::NG; ++g) {
+                const int key = TMA ? k0 + g * C::GR : k0 + (lane & (TK - 1));
+                page[g] = key < L.end && key + (TMA ? C::GR : 1) > L.start
+                              ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page))
+                              : -1;
+                if (!TMA) break;
             }
         };
-        look(L, page);
-        int loaded = 0, qload = -1;  // tiles and queries put into the rings
-        uint32_t badmask = 0;        // stages with a page id out of range
-        if (n > 1) {
-            N = L;
-            advance<C>(p, N);
-            look(N, npage);
-        }
-        const int lr = lane / C::CHP, lc = lane % C::CHP;  // the lane's row and chunk of a copy
-        auto issue = [&](int stage) {
-            const int kvh = L.vh / p.blocks_per_kv;
-            if (loaded == 0 || L.j == 0) {
-                qload = qload + 1 == STAGES ? 0 : qload + 1;
-                const int h0 = (L.vh - kvh * p.blocks_per_kv) * HB;
+        look();
+        int qload = 0;         // where the last queries went
+        uint32_t badmask = 0;  // stages with a page id out of range
+        // Starts the copies of tile i's keys (and its row's queries) or values; values come second.
+        auto issue = [&](int i, auto values) {
+            constexpr bool V = decltype(values)::value;
+            const int stage = i % STAGES;
+            if (!V && (i == 0 || L.j == 0)) {
+                qload = qload + 1 == C::QS ? 0 : qload + 1;
+                const int h0 = L.hb * HB;
                 const char* q = static_cast<const char*>(p.q) +
-                                ((long long)L.row * p.q_ts + (long long)(kvh * p.group + h0) * p.q_hs) * (int)sizeof(TI);
-                for (int i = lane; i < hv * (qrow / 16); i += 32) {
-                    const int h = i / (qrow / 16), c = i - h * (qrow / 16);
+                                ((long long)L.row * p.q_ts + (long long)(L.kvh * p.group + h0) * p.q_hs) * (int)sizeof(TI);
+                for (int x = lane; x < hv * (qrow / 16); x += 32) {
+                    const int h = x / (qrow / 16), c = x - h * (qrow / 16);
                     const bool there = h0 + h < p.group;
                     if (c < nqch)
-                        cp16(q32 + qload * hv * qrow + i * 16, q + (there ? h * p.q_hs * (int)sizeof(TI) + c * 16 : 0), there);
+                        cp16(q32 + qload * hv * qrow + x * 16, q + (there ? h * p.q_hs * (int)sizeof(TI) + c * 16 : 0), there);
                 }
             }
-            const int k0 = (L.start / TK + L.j) * TK;
-            const uint32_t dst = ring32 + stage * C::STAGE;
-            const unsigned long long hoff = (unsigned long long)kvh * p.hs16 * 16;
-            const long long vk = static_cast<const char*>(p.v) - static_cast<const char*>(p.k);
+            const int k0 = ((unsigned)L.start / TK + L.j) * TK;
+            const uint32_t dst = ring32 + stage * C::STAGE + (V ? TK * C::ROWB : 0);
             bool bad = false;
-            if (grouped) {
-                const int lo = L.start - k0, hi = L.end - k0;  // rows lo <= r < hi are wanted
-                const unsigned long long step = (unsigned long long)p.ts16 * 16 * C::RPI;
-                const char* src = nullptr;
+            if constexpr (TMA) {
+                // groups of keys that the row has, and whose page is in the pool
+                int n_load = 0;
 #pragma unroll
-                for (int it = 0; it < C::ITS; ++it) {
-                    const int r0 = C::CHP > 32 ? it * 32 / C::CHP : it * C::RPI;
-                    const int r = r0 + (C::CHP > 32 ? 0 : lr), c = C::CHP > 32 ? (it * 32 + lane) % C::CHP : lc;
-                    if (r0 % C::GR == 0 && (C::CHP <= 32 || it * 32 % C::CHP == 0)) {
-                        const int id = page[r0 / C::GR];
-                        const bool ok = (unsigned)id < (unsigned)p.n_pages;
-                        bad |= !ok;
-                        const int key = k0 + r0;
+                for (int g = 0; g < C::NG; ++g) {
+                    const bool in = (unsigned)page[g] < (unsigned)p.n_pages;
+                    bad |= !in && k0 + g * C::GR < L.end && k0 + (g + 1) * C::GR > L.start;
+                    n_load += in;
+                }
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(&full[warp][2 * stage + V], n_load * p.boxes * C::GR * 128);
+                    const uint32_t bar = tc::smem_u32(&full[warp][2 * stage + V]);
+#pragma unroll
+                    for (int g = 0; g < C::NG; ++g) {
+                        if ((unsigned)page[g] >= (unsigned)p.n_pages) continue;
+                        const int key = k0 + g * C::GR;
                         const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
-                        src = static_cast<const char*>(p.k) + hoff +
-                              ((unsigned long long)(unsigned)(ok ? id : 0) * p.ps16 +
-                               (unsigned long long)(unsigned)(slot + (C::CHP > 32 ? 0 : lr)) * p.ts16) * 16 +
-                              (C::CHP > 32 ? 0 : lc * 16);
+#pragma unroll
+                        for (int x = 0; x < C::ROWB / 128; ++x) {
+                            if (x >= p.boxes) break;
+                            tma_load_4d(dst + x * (TK * 128) + g * (C::GR * 128), V ? &vmap : &kmap, x * C::BOX, slot, L.kvh, page[g], bar);
+                        }
                     }
-                    const int swz = C::F32 ? (r * C::LPK) & 7 : r & 7;
-                    const uint32_t d = dst + r * C::ROWB + ((c ^ swz) * 16);
-                    const bool there = r >= lo && r < hi;
-                    if (c < nch) {
-                        const char* at = src + (C::CHP > 32 ? c * 16 : 0);
-                        cp16(d, at, there);
-                        cp16(d + TK * C::ROWB, at + vk, there);
-                    }
-                    if (C::CHP <= 32 || (it + 1) * 32 % C::CHP == 0) src += step;
                 }
             } else {
-                const int key = k0 + kr;
+                const unsigned long long hoff = (unsigned long long)L.kvh * p.hs16 * 16;
+                const char* pool = static_cast<const char*>(V ? p.v : p.k);
+                const int key = k0 + (lane & (TK - 1));
                 long long at = -1;
                 if (key < L.end && key >= L.start) {
                     const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
@@ -351,26 +375,20 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         bad = true;
                 }
 #pragma unroll
-                for (int it = 0; it < C::ITS; ++it) {
+                for (int it = 0; it < TK * C::CHP / 32; ++it) {
                     const int idx = it * 32 + lane, r = idx / C::CHP, c = idx % C::CHP;
                     const long long o = __shfl_sync(0xffffffffu, at, r);
                     if (c < nch) {
-                        const int swz = C::F32 ? (r * C::LPK) & 7 : r & 7;
-                        const uint32_t d = dst + r * C::ROWB + ((c ^ swz) * 16);
-                        const char* src = static_cast<const char*>(p.k) + (o >= 0 ? o + c * 16 : 0);
-                        cp16(d, src, o >= 0);
-                        cp16(d + TK * C::ROWB, src + vk, o >= 0);
+                        const uint32_t d = dst + C::at(r, c);
+                        cp16(d, pool + (o >= 0 ? o + c * 16 : 0), o >= 0);
                     }
                 }
+                bad = __any_sync(0xffffffffu, bad);
             }
-            badmask = (badmask & ~(1u << stage)) | ((__any_sync(0xffffffffu, bad) ? 1u : 0u) << stage);
-            ++loaded;
-            L = N;
-#pragma unroll
-            for (int g = 0; g < C::NG; ++g) page[g] = npage[g];
-            if (loaded + 1 < n) {
-                advance<C>(p, N);
-                look(N, npage);
+            if (!V) badmask = (badmask & ~(1u << stage)) | ((bad ? 1u : 0u) << stage);
+            if (V && i + 1 < n) {
+                advance<C>(p, L);
+                look();
             }
         };
 
@@ -378,27 +396,44 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
         float m[C::F32 ? HB : 2 * NT], l[C::F32 ? HB : 2 * NT], fac[2 * NT];
         float O[C::F32 ? HB : C::KD][C::F32 ? (HD + 127) / 128 : NT][4];
         uint32_t qf[C::F32 ? 1 : C::SQ][NT][C::F32 ? 1 : C::KD][2];
-        const float sl2 = p.scale * LOG2E;
-        int quse = -1;
+        // the scores' factor; the sign goes to the queries, and 0 becomes a factor too small to matter,
+        // so that a masked score of -inf stays one
+        const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);
+        int quse = 0;
         int bad = 0;  // status bits of the current row
         bool fresh = true;
 
+        // where this lane's ldmatrix rows lie in a tile: chunk c of 16 keys' K, transposed V
+        uint32_t kat[4], vat[4];
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) {
-            if (loaded < n) issue(s);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int k = 0; k < 4; ++k) {
+            kat[k] = C::at(lane & 15, 2 * k + (lane >> 4));
+            vat[k] = TK * C::ROWB + C::at((lane & 7) + ((lane >> 4) & 1) * 8, 2 * k + ((lane >> 3) & 1));
         }
-        int stage = 0;
-        for (int i = 0; i < n; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        bool stuck = false;  // a wait for copies ran out: nothing more is waited for, the results are NaN
+        auto wait = [&](int which, int i) {
+            if constexpr (TMA)
+                for (uint32_t tries = 0; !stuck && !tc::mbar_try_wait(&full[warp][which], (i / STAGES) & 1); ++tries)
+                    stuck = tries >= 1u << 22;
+            else
+                asm volatile("cp.async.wait_group 3;" ::: "memory");
             __syncwarp();
-            if (loaded < n) issue(stage == 0 ? STAGES - 1 : stage - 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-
+        };
+        // Two tiles are on their way while one is worked on: the next keys come into a tile's keys as
+        // soon as its scores are done, the next values into its values at its end.
+        for (int i = -STAGES; i < n; ++i) {
+            const int stage = (i + STAGES) % STAGES;
+            const uint32_t kt = ring32 + stage * C::STAGE;
+            int klo = 0, khi = TK;  // the tile's keys that are the row's
+            float s[C::F32 ? HB : 1], S[C::F32 ? 1 : MT][NT][C::acc()][4];  // scores: of a key, or of a tile
+            if (i >= 0) {
             if (fresh) {
+                // every load of queries is in the group of its tile's keys
+                asm volatile("cp.async.wait_group 3;" ::: "memory");
+                __syncwarp();
                 fresh = false;
                 bad = w.over ? GPT2Q_STATUS_POSITION : 0;
-                quse = quse + 1 == STAGES ? 0 : quse + 1;
+                quse = quse + 1 == C::QS ? 0 : quse + 1;
                 const unsigned char* q = qring + quse * hv * qrow;
 #pragma unroll
                 for (int k = 0; k < (C::F32 ? HB : 2 * NT); ++k) m[k] = -INFINITY, l[k] = 0.f;
@@ -414,7 +449,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     for (int nt = 0; nt < NT; ++nt) {
                         const int h = nt * 8 + (lane >> 2);
                         const TI* qh = reinterpret_cast<const TI*>(q + h * qrow) + (lane & 3) * 2;
-                        float down = 1.f, up = 1.f;
+                        float down = 1.f, up = 1.f;  // of the queries, and back
                         if constexpr (C::SQ > 1 && C::HALF) {
                             // fp16 pieces of an fp32 query: scaled by a power of two so that the
                             // head's largest element lies in [1, 2), undone on the scores
@@ -435,9 +470,11 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                             for (int x = 0; x < 2; ++x) {
                                 if constexpr (C::SQ == 1) {
                                     qf[0][nt][k][x] = h < hv ? *reinterpret_cast<const uint32_t*>(qh + k * 16 + x * 8) : 0u;
+                                    if (p.scale < 0.f) qf[0][nt][k][x] ^= 0x80008000u;
                                 } else {
                                     float u = 0.f, v = 0.f;
-                                    if (h < hv) u = to_f(qh[k * 16 + x * 8]) * down, v = to_f(qh[k * 16 + x * 8 + 1]) * down;
+                                    const float sd = p.scale < 0.f ? -down : down;
+                                    if (h < hv) u = to_f(qh[k * 16 + x * 8]) * sd, v = to_f(qh[k * 16 + x * 8 + 1]) * sd;
 #pragma unroll
                                     for (int s = 0; s < C::SQ; ++s) qf[s][nt][k][x] = take_pair<TC>(u, v);
                                 }
@@ -449,31 +486,86 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                 }
             }
             if ((badmask >> stage) & 1u) bad |= GPT2Q_STATUS_PAGE;
-            const int k0 = (w.start / TK + w.j) * TK, klo = w.start - k0, khi = w.end - k0;
-            const bool cut = klo > 0 || khi < TK;  // some of the tile's keys are not the row's
-            const uint32_t kt = ring32 + stage * C::STAGE, vt = kt + TK * C::ROWB;
+            if (w.j == 0 || w.j + 1 == w.nt) {
+                const int k0 = ((unsigned)w.start / TK + w.j) * TK;
+                klo = w.start - k0;
+                khi = w.end - k0;
+            }
+            wait(2 * stage, i);
 
             if constexpr (!C::F32) {
                 // S^T = K q^T: keys are the rows of the product, heads its columns
-                float s[MT][NT][2][4];
 #pragma unroll
                 for (int x = 0; x < MT; ++x)
 #pragma unroll
                     for (int y = 0; y < NT; ++y)
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) s[x][y][0][z] = s[x][y][1][z] = 0.f;
+                        for (int z = 0; z < 4; ++z) S[x][y][0][z] = S[x][y][C::acc() - 1][z] = 0.f;
 #pragma unroll
                 for (int k = 0; k < C::KD; ++k) {
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
-                        const int r = x * 16 + (lane & 15), c = 2 * k + (lane >> 4);
                         uint32_t af[4];
-                        ldsm4(af, kt + r * C::ROWB + ((c ^ (r & 7)) * 16));
+                        ldsm4(af, kt + kat[k & 3] + (k >> 2) * (TK * 128) + x * 2048);
 #pragma unroll
                         for (int y = 0; y < NT; ++y)
 #pragma unroll
-                            for (int t = 0; t < C::SQ; ++t) mma16816<TC>(s[x][y][k & 1], af, qf[t][y][k][0], qf[t][y][k][1]);
+                            for (int t = 0; t < C::SQ; ++t) mma16816<TC>(S[x][y][k & (C::acc() - 1)], af, qf[t][y][k][0], qf[t][y][k][1]);
                     }
+                }
+            } else {
+                // CUDA cores: LPK lanes share a key and take its chunks in turn
+                const unsigned char* q = qring + quse * hv * qrow;
+                const unsigned char* kp = ring + stage * C::STAGE;
+                // eight neighbouring lanes read eight keys
+                const int key = (lane & 7) + (lane >> 3) / C::lpk() * 8, part = (lane >> 3) % C::lpk();
+#pragma unroll
+                for (int h = 0; h < HB; ++h) s[h] = 0.f;
+#pragma unroll 4
+                for (int c = part; c < nch; c += C::lpk()) {
+                    const float4 kv = *reinterpret_cast<const float4*>(kp + C::at(key, c));
+#pragma unroll
+                    for (int h = 0; h < HB; ++h)
+                        if (h < hv) {
+                            const float4 qv = *reinterpret_cast<const float4*>(q + h * qrow + c * 16);
+                            s[h] = fmaf(kv.x, qv.x, s[h]);
+                            s[h] = fmaf(kv.y, qv.y, s[h]);
+                            s[h] = fmaf(kv.z, qv.z, s[h]);
+                            s[h] = fmaf(kv.w, qv.w, s[h]);
+                        }
+                }
+            }
+            }  // i >= 0
+            __syncwarp();
+            if (i + STAGES < n && !stuck) issue(i + STAGES, std::false_type{});
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            const bool cut = klo > 0 || khi < TK;
+            // the tile's values are there
+            auto arrived = [&] {
+                if (TMA && cut) {
+                    // values that are not the row's may be anything; with weight 0 they have to be finite
+                    for (int x = lane; x < TK * p.boxes * 8; x += 32) {
+                        const int r = x / (p.boxes * 8), c = x % (p.boxes * 8);
+                        if (r < klo || r >= khi)
+                            *reinterpret_cast<uint4*>(ring + stage * C::STAGE + TK * C::ROWB + C::at(r, c)) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_proxy_async_smem();  // before the stage's next TMA write
+                    __syncwarp();
+                }
+            };
+            if (i >= 0) {
+            if constexpr (!C::F32) {
+                if (cut) {
+#pragma unroll
+                    for (int x = 0; x < MT; ++x)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const int r = x * 16 + (lane >> 2) + (z >> 1) * 8;
+                            if (r < klo || r >= khi) {
+#pragma unroll
+                                for (int y = 0; y < NT; ++y) S[x][y][0][z] = -INFINITY, S[x][y][C::acc() - 1][z] = -INFINITY;
+                            }
+                        }
                 }
                 bool moved = false;
                 float al[2 * NT];
@@ -486,19 +578,17 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         for (int x = 0; x < MT; ++x)
 #pragma unroll
                             for (int z = c; z < 4; z += 2) {
-                                float v = (s[x][y][0][z] + s[x][y][1][z]) * fac[2 * y + c];
-                                const int r = x * 16 + (lane >> 2) + (z >> 1) * 8;
-                                if (cut && (r < klo || r >= khi)) v = -INFINITY;
-                                s[x][y][0][z] = v;
-                                mx = fmaxf(mx, v);
+                                if (C::acc() == 2) S[x][y][0][z] += S[x][y][C::acc() - 1][z];
+                                mx = fmaxf(mx, S[x][y][0][z]);
                             }
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                         const int k = 2 * y + c;
+                        // m is the largest score before the factor, so that its own weight is exactly 1
                         const float mn = fmaxf(m[k], mx);
                         const float ms = mn == -INFINITY ? 0.f : mn;
-                        al[k] = ex2(m[k] - ms);
+                        al[k] = ex2((m[k] - ms) * fac[k]);
                         moved |= m[k] != mn;
                         m[k] = mn;
                         float sum = 0.f;
@@ -506,8 +596,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         for (int x = 0; x < MT; ++x)
 #pragma unroll
                             for (int z = c; z < 4; z += 2) {
-                                const float e = ex2(s[x][y][0][z] - ms + C::shift());
-                                s[x][y][0][z] = e;
+                                const float e = ex2(fmaf(S[x][y][0][z] - ms, fac[k], C::shift()));
+                                S[x][y][0][z] = e;
                                 sum += e;
                             }
                         l[k] = l[k] * al[k] + sum;
@@ -528,16 +618,17 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     for (int y = 0; y < NT; ++y)
 #pragma unroll
                         for (int t = 0; t < C::sp(); ++t) {
-                            pf[t][x][y][0] = movm(take_pair<TC>(s[x][y][0][0], s[x][y][0][1]));
-                            pf[t][x][y][1] = movm(take_pair<TC>(s[x][y][0][2], s[x][y][0][3]));
+                            pf[t][x][y][0] = movm(take_pair<TC>(S[x][y][0][0], S[x][y][0][1]));
+                            pf[t][x][y][1] = movm(take_pair<TC>(S[x][y][0][2], S[x][y][0][3]));
                         }
+                wait(2 * stage + 1, i);
+                arrived();
 #pragma unroll
                 for (int d = 0; d < C::KD; ++d) {
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
-                        const int r = x * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, c = 2 * d + ((lane >> 3) & 1);
                         uint32_t af[4];
-                        ldsm4t(af, vt + r * C::ROWB + ((c ^ (r & 7)) * 16));
+                        ldsm4t(af, kt + vat[d & 3] + (d >> 2) * (TK * 128) + x * 2048);
 #pragma unroll
                         for (int y = 0; y < NT; ++y)
 #pragma unroll
@@ -545,36 +636,18 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     }
                 }
             } else {
-                // CUDA cores: LPK lanes share a key and take its chunks in turn
-                const unsigned char* q = qring + quse * hv * qrow;
-                const unsigned char* kp = ring + stage * C::STAGE;
-                const unsigned char* vp = kp + TK * C::ROWB;
-                const int key = lane / C::LPK, part = lane % C::LPK;
-                float s[HB];
-#pragma unroll
-                for (int h = 0; h < HB; ++h) s[h] = 0.f;
-#pragma unroll 4
-                for (int c = part; c < nch; c += C::LPK) {
-                    const float4 kv = *reinterpret_cast<const float4*>(kp + key * C::ROWB + ((c ^ ((key * C::LPK) & 7)) * 16));
-#pragma unroll
-                    for (int h = 0; h < HB; ++h)
-                        if (h < hv) {
-                            const float4 qv = *reinterpret_cast<const float4*>(q + h * qrow + c * 16);
-                            s[h] = fmaf(kv.x, qv.x, s[h]);
-                            s[h] = fmaf(kv.y, qv.y, s[h]);
-                            s[h] = fmaf(kv.z, qv.z, s[h]);
-                            s[h] = fmaf(kv.w, qv.w, s[h]);
-                        }
-                }
+                const unsigned char* vp = ring + stage * C::STAGE + TK * C::ROWB;
+                const int key = (lane & 7) + (lane >> 3) / C::lpk() * 8, part = (lane >> 3) % C::lpk();
 #pragma unroll
                 for (int h = 0; h < HB; ++h) {
                     float v = s[h];
 #pragma unroll
-                    for (int o = 1; o < C::LPK; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    v = key >= klo && key < khi ? v * sl2 : -INFINITY;
+                    for (int o = 8; o < 8 * C::lpk(); o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    v = key >= klo && key < khi ? v * (p.scale * LOG2E) : -INFINITY;
                     float mx = v;
 #pragma unroll
-                    for (int o = C::LPK; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    for (int o = 1; o < 32; o <<= 1)  // the lanes of the other keys
+                        if (o < 8 || o >= 8 * C::lpk()) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                     const float mn = fmaxf(m[h], mx);
                     const float ms = mn == -INFINITY ? 0.f : mn;
                     const float al = ex2(m[h] - ms);
@@ -587,6 +660,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                         for (int z = 0; z < 4; ++z) O[h][y][z] *= al;
                     if (part == 0) pbuf[key * HB + h] = e;
                 }
+                wait(2 * stage + 1, i);
+                arrived();
                 __syncwarp();
                 constexpr int KH = HD == 64 ? 2 : 1;  // keys the warp takes at once
                 const int c0 = HD == 64 ? lane & 15 : lane, k0 = HD == 64 ? lane >> 4 : 0;
@@ -603,7 +678,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     }
 #pragma unroll
                     for (int y = 0; y < (HD + 127) / 128; ++y) {
-                        const float4 v = *reinterpret_cast<const float4*>(vp + r * C::ROWB + (((c0 + 32 * y) ^ ((r * C::LPK) & 7)) * 16));
+                        const float4 v = *reinterpret_cast<const float4*>(vp + C::at(r, c0 + 32 * y));
 #pragma unroll
                         for (int h = 0; h < HB; ++h) {
                             O[h][y][0] = fmaf(e[h], v.x, O[h][y][0]);
@@ -614,6 +689,11 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     }
                 }
             }
+            }  // i >= 0
+            __syncwarp();
+            if (i + STAGES < n && !stuck) issue(i + STAGES, std::true_type{});
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (i < 0) continue;
 
             const bool last = i == n - 1;
             if (last || w.j + 1 == w.nt) {
@@ -621,14 +701,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                 fresh = true;
                 const long long first = a + i - w.j;  // its first tile
                 const bool whole = first >= a && w.j + 1 == w.nt;
-                const int kvh = w.vh / p.blocks_per_kv, h0 = (w.vh - kvh * p.blocks_per_kv) * HB;
-                const int head0 = kvh * p.group + h0, nh = min(HB, p.group - h0);
+                const int h0 = w.hb * HB, head0 = w.kvh * p.group + h0, nh = min(HB, p.group - h0);
+                if (TMA && __any_sync(0xffffffffu, stuck)) bad |= GPT2Q_STATUS_TIMEOUT;
                 if (bad && p.status && lane == 0) atomicOr(p.status, bad);
 #pragma unroll
                 for (int k = 0; k < (C::F32 ? HB : 2 * NT); ++k) {
 #pragma unroll
                     for (int o = C::F32 ? 1 : 4; o < 32; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
                     l[k] *= C::UNSHIFT;
+                    if (!C::F32) m[k] *= fac[k % (2 * NT)];
                     if (bad) l[k] = NAN;
                 }
                 if constexpr (C::F32 && HD == 64) {
@@ -643,7 +724,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                     // in the middle of a range to memory, at its end into the drained ring
                     dst = last ? reinterpret_cast<float*>(ring)
                                : p.warp_part + ((long long)blockIdx.x * MAX_WARPS + warp) * HB * C::HS;
-                    if (lane == 0) pieces[ps] = Piece{first, w.nt, w.row, w.vh, dst};
+                    if (lane == 0) pieces[ps] = Piece{first, w.nt, w.row, w.kvh * p.blocks_per_kv + w.hb, dst};
                     __syncwarp();
                 }
                 if constexpr (!C::F32) {
@@ -703,7 +784,6 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                 }
             }
             if (!last) advance<C>(p, w);
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
     }
     __syncthreads();
@@ -724,7 +804,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) k_paged_attn(const __grid_c
                 e = j + 1;
             }
         const bool whole = P.first >= ca && P.first + P.nt <= cb;
-        if (P.first >= ca && !whole) tail_row = P.row, tail_vh = P.vh, tail_last = (P.first + P.nt - 1) / per;
+        if (P.first >= ca && !whole) tail_row = P.row, tail_vh = P.vh, tail_last = quotient(P.first + P.nt - 1, per);
         const int kvh = P.vh / p.blocks_per_kv, h0 = (P.vh - kvh * p.blocks_per_kv) * HB;
         const int nh = min(HB, p.group - h0);
         for (int h = 0; h < nh; ++h) {
@@ -832,34 +912,74 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(const __grid_constant__
     if (tid == 0 && p.lse) p.lse[(long long)meta.x * p.n_heads + head] = log_sum(M, L);
 }
 
-constexpr size_t SMEM_LIMIT = 227 * 1024 - 8 * 1024;  // dynamic; the rest for the static arrays
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder() {
+    static const EncodeTiledFn fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<EncodeTiledFn>(ptr)
+                   : nullptr;
+    }();
+    return fn;
+}
+
+constexpr size_t SMEM_LIMIT = 218 * 1024;  // dynamic; the rest for the static arrays
+
+// A pool as a tensor [page][head][slot][dim]; dims past the head's own are read as zero.
+template <class C>
+bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base) {
+    const auto encode = tensor_map_encoder();
+    if (!encode) return false;
+    using TC = typename C::TC;
+    const auto type = C::F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                             : C::HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.page, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+    // the stride of a dimension of one element does not matter, but may not be 0
+    const cuuint64_t row = ((cuuint64_t)p.dim * sizeof(TC) + 15) / 16 * 16;
+    const cuuint64_t strides[3] = {p.page == 1 ? row : p.ts16 * 16ull, p.n_kv == 1 ? row : p.hs16 * 16ull,
+                                   p.n_pages == 1 ? row : p.ps16 * 16ull};
+    const cuuint32_t box[4] = {(cuuint32_t)C::BOX, (cuuint32_t)C::GR, 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(m, type, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class C, bool TMA>
+cudaError_t launch_main(const PagedAttn& p, const CUtensorMap& km, const CUtensorMap& vm, int grid, int nw, size_t smem, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        e = cudaFuncSetAttribute(k_paged_attn<C, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready |= 1ull << dev;
+    }
+    return launch_dependent(k_paged_attn<C, TMA>, dim3(grid), dim3(nw * 32), smem, st, p, km, vm);
+}
 
 template <class C>
 cudaError_t launch(PagedAttn p, cudaStream_t st) {
     p.blocks_per_kv = (p.group + C::HB - 1) / C::HB;
     p.n_vh = p.n_kv * p.blocks_per_kv;
     p.heads_per_block = std::min(p.group, C::HB);
-    size_t wb = STAGES * C::STAGE + (size_t)STAGES * p.heads_per_block * C::HD * sizeof(typename C::TI);
+    size_t wb = STAGES * C::STAGE + (size_t)C::QS * p.heads_per_block * C::HD * sizeof(typename C::TI);
     if (C::F32) wb += (size_t)C::TK * C::HB * 4;
-    p.grouped = p.page % C::GR == 0;
-    p.warp_bytes = (int)((wb + 127) / 128 * 128);
-    const int nw = (int)std::min<size_t>(MAX_WARPS, SMEM_LIMIT / p.warp_bytes);
+    p.warp_bytes = (int)((wb + 1023) / 1024 * 1024);
+    const int nw = (int)std::min<size_t>(C::WARPS, SMEM_LIMIT / p.warp_bytes);
     // no more blocks than the longest rows the table can hold would fill
     const long long longest = p.window > 0 ? std::min(p.window, p.cap) : p.cap;
     const long long tiles = ((longest + C::TK - 1) / C::TK + (p.window > 0 ? 1 : 0)) * p.n_vh;
     const long long want = tiles > MAX_CTAS * 8LL ? MAX_CTAS : (tiles * p.n_rows + nw - 1) / nw;
     const int grid = (int)std::clamp<long long>(want, 1, MAX_CTAS);
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+    p.boxes = (p.dim * (int)sizeof(typename C::TC) + 127) / 128;
+    CUtensorMap km{}, vm{};
+    const bool tma = p.page % C::GR == 0 && make_map<C>(&km, p, p.k) && make_map<C>(&vm, p, p.v);
     const size_t smem = (size_t)nw * p.warp_bytes;
-    if (dev >= 64 || !(ready.load() >> dev & 1)) {
-        e = cudaFuncSetAttribute(k_paged_attn<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) ready |= 1ull << dev;
-    }
-    e = launch_dependent(k_paged_attn<C>, dim3(grid), dim3(nw * 32), smem, st, p);
+    cudaError_t e = tma ? launch_main<C, true>(p, km, vm, grid, nw, smem, st) : launch_main<C, false>(p, km, vm, grid, nw, smem, st);
     if (e != cudaSuccess || grid == 1) return e;
     return launch_dependent(k_paged_attn_join<typename C::TI, C::HD, C::HB>, dim3(grid, p.heads_per_block), dim3(128), 0, st, p);
 }

@@ -17,7 +17,7 @@ import math
 from . import _ffi
 from .device import DTYPES, ops
 
-STATUS_PAGE, STATUS_POSITION, STATUS_ROW = 1, 2, 4
+STATUS_PAGE, STATUS_POSITION, STATUS_ROW, STATUS_TIMEOUT = 1, 2, 4, 8
 
 
 class Rotary:
