@@ -34,7 +34,8 @@ struct PagedAttn {
     float scale;
     int* status;
     int page_shift;  // page = 1 << page_shift, or -1
-    int boxes;       // pieces of 128 bytes of a key
+    // pieces of 128 bytes of a key, TMA copies of a group of keys, and its bytes in shared memory
+    int boxes, box_loads, group_bytes;
     // a kv head's `group` query heads are taken in blocks_per_kv blocks of up to heads_per_block
     int blocks_per_kv, n_vh, heads_per_block;
     int warp_bytes;  // shared memory of a warp

@@ -162,10 +162,11 @@ __device__ __forceinline__ uint32_t take_pair(float& a, float& b) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+// coordinates: dim, slot, piece of 128 bytes (0), head, page
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int h, int page, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(h), "r"(page), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp; results under 2^-126 are 0
@@ -299,30 +300,32 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         w.j = (int)(rem - (long long)vh * w.nt);
         w.kvh = vh / p.blocks_per_kv;
         w.hb = vh - w.kvh * p.blocks_per_kv;
-        Walk L = w;  // the next tile to load; its pages are looked up when the tile before it is loaded
+        // L is the next tile to load, from key L_key on; its pages are looked up when the tile before
+        // it is loaded
+        Walk L = w;
+        int L_key = ((unsigned)L.start / TK + L.j) * TK;
+        const int* L_ids = p.table + (long long)L.row * p.ld;
         int page[C::NG];
         // page ids of a tile: of every group of GR keys (the same load in all lanes) where a page is
-        // a multiple of GR, else of the lane's own key, in element 0
-        auto look = [&]() {
-            const int k0 = ((unsigned)L.start / TK + L.j) * TK;
-            const int* ids = p.table + (long long)L.row * p.ld;
+        // a multiple of GR, else of the lane's own key, in element 0. -1 for keys the row does not have
+        auto look = [&](auto steady) {
 #pragma unroll
-            for (int g = 0; g < C::NG; ++g) {
-                const int key = TMA ? k0 + g * C::GR : k0 + (lane & (TK - 1));
-                page[g] = key < L.end && key + (TMA ? C::GR : 1) > L.start
-                              ? __ldcg(ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page))
-                              : -1;
-                if (!TMA) break;
+            for (int g = 0; g < (TMA ? C::NG : 1); ++g) {
+                const int key = TMA ? L_key + g * C::GR : L_key + (lane & (TK - 1));
+                page[g] = -1;
+                if (decltype(steady)::value || (key < L.end && key + (TMA ? C::GR : 1) > L.start))
+                    page[g] = __ldcg(L_ids + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page));
             }
         };
-        look();
+        look(std::false_type{});
         int qload = 0;         // where the last queries went
         uint32_t badmask = 0;  // stages with a page id out of range
         // Starts the copies of tile i's keys (and its row's queries) or values; values come second.
-        auto issue = [&](int i, auto values) {
-            constexpr bool V = decltype(values)::value;
+        // steady: the tile and the one after it lie inside the row that the loads are in.
+        auto issue = [&](int i, auto values, auto steady) {
+            constexpr bool V = decltype(values)::value, ST = decltype(steady)::value;
             const int stage = i % STAGES;
-            if (!V && (i == 0 || L.j == 0)) {
+            if (!V && !ST && (i == 0 || L.j == 0)) {
                 qload = qload + 1 == C::QS ? 0 : qload + 1;
                 const int h0 = L.hb * HB;
                 const char* q = static_cast<const char*>(p.q) +
@@ -334,39 +337,37 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                         cp16(q32 + qload * hv * qrow + x * 16, q + (there ? h * p.q_hs * (int)sizeof(TI) + c * 16 : 0), there);
                 }
             }
-            const int k0 = ((unsigned)L.start / TK + L.j) * TK;
             const uint32_t dst = ring32 + stage * C::STAGE + (V ? TK * C::ROWB : 0);
             bool bad = false;
             if constexpr (TMA) {
                 // groups of keys that the row has, and whose page is in the pool
-                int n_load = 0;
+                int bytes = 0;
 #pragma unroll
                 for (int g = 0; g < C::NG; ++g) {
                     const bool in = (unsigned)page[g] < (unsigned)p.n_pages;
-                    bad |= !in && k0 + g * C::GR < L.end && k0 + (g + 1) * C::GR > L.start;
-                    n_load += in;
+                    if (!V) bad |= !in && (ST || (L_key + g * C::GR < L.end && L_key + (g + 1) * C::GR > L.start));
+                    bytes += in ? p.group_bytes : 0;
                 }
                 if (lane == 0) {
-                    tc::mbar_arrive_expect_tx(&full[warp][2 * stage + V], n_load * p.boxes * C::GR * 128);
+                    tc::mbar_arrive_expect_tx(&full[warp][2 * stage + V], bytes);
                     const uint32_t bar = tc::smem_u32(&full[warp][2 * stage + V]);
 #pragma unroll
                     for (int g = 0; g < C::NG; ++g) {
                         if ((unsigned)page[g] >= (unsigned)p.n_pages) continue;
-                        const int key = k0 + g * C::GR;
+                        const int key = L_key + g * C::GR;
                         const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
-#pragma unroll
-                        for (int x = 0; x < C::ROWB / 128; ++x) {
-                            if (x >= p.boxes) break;
-                            tma_load_4d(dst + x * (TK * 128) + g * (C::GR * 128), V ? &vmap : &kmap, x * C::BOX, slot, L.kvh, page[g], bar);
-                        }
+                        const CUtensorMap* map = V ? &vmap : &kmap;
+                        tma_load(dst + g * (C::GR * 128), map, 0, slot, L.kvh, page[g], bar);
+                        for (int x = 1; x < p.box_loads; ++x)
+                            tma_load(dst + g * (C::GR * 128) + x * (TK * 128), map, x * C::BOX, slot, L.kvh, page[g], bar);
                     }
                 }
             } else {
                 const unsigned long long hoff = (unsigned long long)L.kvh * p.hs16 * 16;
                 const char* pool = static_cast<const char*>(V ? p.v : p.k);
-                const int key = k0 + (lane & (TK - 1));
+                const int key = L_key + (lane & (TK - 1));
                 long long at = -1;
-                if (key < L.end && key >= L.start) {
+                if (ST || (key < L.end && key >= L.start)) {
                     const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
                     if ((unsigned)page[0] < (unsigned)p.n_pages)
                         at = (long long)(hoff + ((unsigned long long)(unsigned)page[0] * p.ps16 +
@@ -386,9 +387,15 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 bad = __any_sync(0xffffffffu, bad);
             }
             if (!V) badmask = (badmask & ~(1u << stage)) | ((bad ? 1u : 0u) << stage);
-            if (V && i + 1 < n) {
-                advance<C>(p, L);
-                look();
+            if (V && (ST || i + 1 < n)) {
+                L_key += TK;
+                if (++L.j == L.nt && !ST) {
+                    --L.j;
+                    advance<C>(p, L);
+                    L_key = (unsigned)L.start / TK * TK;
+                    L_ids = p.table + (long long)L.row * p.ld;
+                }
+                look(steady);
             }
         };
 
@@ -421,13 +428,14 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         };
         // Two tiles are on their way while one is worked on: the next keys come into a tile's keys as
         // soon as its scores are done, the next values into its values at its end.
-        for (int i = -STAGES; i < n; ++i) {
+        auto step = [&](int i, auto steady) {
+            constexpr bool ST = decltype(steady)::value;
             const int stage = (i + STAGES) % STAGES;
             const uint32_t kt = ring32 + stage * C::STAGE;
             int klo = 0, khi = TK;  // the tile's keys that are the row's
             float s[C::F32 ? HB : 1], S[C::F32 ? 1 : MT][NT][C::acc()][4];  // scores: of a key, or of a tile
-            if (i >= 0) {
-            if (fresh) {
+            if (ST || i >= 0) {
+            if (!ST && fresh) {
                 // every load of queries is in the group of its tile's keys
                 asm volatile("cp.async.wait_group 3;" ::: "memory");
                 __syncwarp();
@@ -485,8 +493,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     }
                 }
             }
-            if ((badmask >> stage) & 1u) bad |= GPT2Q_STATUS_PAGE;
-            if (w.j == 0 || w.j + 1 == w.nt) {
+            static_assert(GPT2Q_STATUS_PAGE == 1, "the mask's bit is the status");
+            bad |= (badmask >> stage) & 1u;
+            if (!ST && (w.j == 0 || w.j + 1 == w.nt)) {
                 const int k0 = ((unsigned)w.start / TK + w.j) * TK;
                 klo = w.start - k0;
                 khi = w.end - k0;
@@ -537,7 +546,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
             }
             }  // i >= 0
             __syncwarp();
-            if (i + STAGES < n && !stuck) issue(i + STAGES, std::false_type{});
+            if (ST || (i + STAGES < n && !stuck)) issue(i + STAGES, std::false_type{}, steady);
             asm volatile("cp.async.commit_group;" ::: "memory");
             const bool cut = klo > 0 || khi < TK;
             // the tile's values are there
@@ -553,7 +562,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     __syncwarp();
                 }
             };
-            if (i >= 0) {
+            if (ST || i >= 0) {
             if constexpr (!C::F32) {
                 if (cut) {
 #pragma unroll
@@ -691,12 +700,18 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
             }
             }  // i >= 0
             __syncwarp();
-            if (i + STAGES < n && !stuck) issue(i + STAGES, std::true_type{});
+            if (ST || (i + STAGES < n && !stuck)) issue(i + STAGES, std::true_type{}, steady);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (i < 0) continue;
-
+        };
+        for (int i = -STAGES; i < n; ++i) {
+            // tiles inside a row, whose loads stay inside it too, need none of the checks at its ends
+            if (i > 0 && !fresh && w.j > 0) {
+                for (int run = min(w.nt - STAGES - 2 - w.j, n - STAGES - 1 - i); run > 0 && !stuck; --run, ++i, ++w.j)
+                    step(i, std::true_type{});
+            }
+            step(i, std::false_type{});
             const bool last = i == n - 1;
-            if (last || w.j + 1 == w.nt) {
+            if (i >= 0 && (last || w.j + 1 == w.nt)) {
                 // the segment ends, here or in this warp's range
                 fresh = true;
                 const long long first = a + i - w.j;  // its first tile
@@ -783,7 +798,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                         }
                 }
             }
-            if (!last) advance<C>(p, w);
+            if (i >= 0 && !last) advance<C>(p, w);
         }
     }
     __syncthreads();
@@ -929,7 +944,7 @@ EncodeTiledFn tensor_map_encoder() {
 
 constexpr size_t SMEM_LIMIT = 218 * 1024;  // dynamic; the rest for the static arrays
 
-// A pool as a tensor [page][head][slot][dim]; dims past the head's own are read as zero.
+// A pool as a tensor [page][head][piece][slot][dim]; dims past the head's own are read as zero.
 template <class C>
 bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base) {
     const auto encode = tensor_map_encoder();
@@ -937,13 +952,18 @@ bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base) {
     using TC = typename C::TC;
     const auto type = C::F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                              : C::HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.page, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+    // heads of whole pieces of 128 bytes are read with one box of all their pieces, others piece by
+    // piece (a tile of several groups of keys has one piece)
+    const bool merged = p.box_loads == 1;
+    const cuuint64_t pieces = merged ? p.boxes : 1;
+    const cuuint64_t dims[5] = {(cuuint64_t)(merged && p.boxes > 1 ? C::BOX : p.dim), (cuuint64_t)p.page, pieces, (cuuint64_t)p.n_kv,
+                                (cuuint64_t)p.n_pages};
     // the stride of a dimension of one element does not matter, but may not be 0
     const cuuint64_t row = ((cuuint64_t)p.dim * sizeof(TC) + 15) / 16 * 16;
-    const cuuint64_t strides[3] = {p.page == 1 ? row : p.ts16 * 16ull, p.n_kv == 1 ? row : p.hs16 * 16ull,
+    const cuuint64_t strides[4] = {p.page == 1 ? row : p.ts16 * 16ull, 128, p.n_kv == 1 ? row : p.hs16 * 16ull,
                                    p.n_pages == 1 ? row : p.ps16 * 16ull};
-    const cuuint32_t box[4] = {(cuuint32_t)C::BOX, (cuuint32_t)C::GR, 1, 1}, step[4] = {1, 1, 1, 1};
-    return encode(m, type, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint32_t box[5] = {(cuuint32_t)C::BOX, (cuuint32_t)C::GR, (cuuint32_t)pieces, 1, 1}, step[5] = {1, 1, 1, 1, 1};
+    return encode(m, type, 5, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -976,6 +996,8 @@ cudaError_t launch(PagedAttn p, cudaStream_t st) {
     const long long want = tiles > MAX_CTAS * 8LL ? MAX_CTAS : (tiles * p.n_rows + nw - 1) / nw;
     const int grid = (int)std::clamp<long long>(want, 1, MAX_CTAS);
     p.boxes = (p.dim * (int)sizeof(typename C::TC) + 127) / 128;
+    p.box_loads = p.boxes > 1 && p.dim % C::BOX == 0 && C::NG == 1 ? 1 : p.boxes;
+    p.group_bytes = p.boxes * C::GR * 128;
     CUtensorMap km{}, vm{};
     const bool tma = p.page % C::GR == 0 && make_map<C>(&km, p, p.k) && make_map<C>(&vm, p, p.v);
     const size_t smem = (size_t)nw * p.warp_bytes;
