@@ -35,6 +35,7 @@ namespace {
 
 constexpr int STAGES = 2;
 constexpr int MAX_WARPS = 12;
+constexpr int LENS = 512;     // rows whose lengths a block keeps in shared memory
 constexpr int MAX_CTAS = 148;  // one per SM of a B200
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -90,10 +91,11 @@ struct Piece {
     const float* data;
 };
 
+// Row `row` of the walk; `lens` holds the first LENS rows' lengths.
 template <class C>
-__device__ __forceinline__ void enter(const PagedAttn& p, Walk& w, int row) {
+__device__ __forceinline__ void enter(const PagedAttn& p, const int* lens, Walk& w, int row) {
     w.row = row;
-    const int len = row < p.n_rows ? __ldcg(p.lens + row) : 0;
+    const int len = row >= p.n_rows ? 0 : row < LENS ? lens[row] : __ldcg(p.lens + row);
     w.over = len > p.cap;
     w.end = w.over ? p.cap : len;
     w.start = p.window > 0 && w.end > p.window ? w.end - p.window : 0;
@@ -102,7 +104,7 @@ __device__ __forceinline__ void enter(const PagedAttn& p, Walk& w, int row) {
 }
 
 template <class C>
-__device__ __forceinline__ void advance(const PagedAttn& p, Walk& w) {
+__device__ __forceinline__ void advance(const PagedAttn& p, const int* lens, Walk& w) {
     if (++w.j < w.nt) return;
     w.j = 0;
     if (++w.hb < p.blocks_per_kv) return;
@@ -110,7 +112,7 @@ __device__ __forceinline__ void advance(const PagedAttn& p, Walk& w) {
     if (++w.kvh < p.n_kv) return;
     w.kvh = 0;
     do {
-        enter<C>(p, w, w.row + 1);
+        enter<C>(p, lens, w, w.row + 1);
     } while (w.nt == 0 && w.row < p.n_rows);
 }
 
@@ -216,6 +218,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ long long cum[MAX_WARPS * 32 + 1];
     __shared__ long long wsum[MAX_WARPS];
+    __shared__ int slen[LENS];
     __shared__ Piece pieces[2 * MAX_WARPS];
     __shared__ __align__(8) uint64_t full[MAX_WARPS][2 * STAGES];  // per stage: keys, values
     __shared__ float pm[2 * MAX_WARPS][HB], pl[2 * MAX_WARPS][HB];
@@ -254,8 +257,10 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     const int nc = (p.n_rows + nthr - 1) / nthr;  // rows a thread counts
     Walk w;
     long long mine = 0;
+    for (int r = tid; r < min(LENS, p.n_rows); r += nthr) slen[r] = __ldcg(p.lens + r);
+    if (nc > 1) __syncthreads();
     for (int r = tid * nc; r < min((tid + 1) * nc, p.n_rows); ++r) {
-        enter<C>(p, w, r);
+        enter<C>(p, slen, w, r);  // with nc == 1 the thread's own
         mine += w.nt;
     }
     mine *= p.n_vh;
@@ -291,10 +296,10 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         }
         long long rem = a - cum[lo];
         int row = lo * nc;
-        enter<C>(p, w, row);
+        enter<C>(p, slen, w, row);
         while (rem >= (long long)w.nt * p.n_vh) {
             rem -= (long long)w.nt * p.n_vh;
-            enter<C>(p, w, ++row);
+            enter<C>(p, slen, w, ++row);
         }
         const int vh = (int)quotient(rem, w.nt);
         w.j = (int)(rem - (long long)vh * w.nt);
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 L_key += TK;
                 if (++L.j == L.nt && !ST) {
                     --L.j;
-                    advance<C>(p, L);
+                    advance<C>(p, slen, L);
                     L_key = (unsigned)L.start / TK * TK;
                     L_ids = p.table + (long long)L.row * p.ld;
                 }
@@ -431,9 +436,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         auto step = [&](int i, auto steady) {
             constexpr bool ST = decltype(steady)::value;
             const int stage = (i + STAGES) % STAGES;
-            const uint32_t kt = ring32 + stage * C::STAGE;
             int klo = 0, khi = TK;  // the tile's keys that are the row's
-            float s[C::F32 ? HB : 1], S[C::F32 ? 1 : MT][NT][C::acc()][4];  // scores: of a key, or of a tile
+            [[maybe_unused]] const uint32_t kt = ring32 + stage * C::STAGE;
+            [[maybe_unused]] float s[C::F32 ? HB : 1], S[C::F32 ? 1 : MT][NT][C::acc()][4];  // scores: of a key, or of a tile
             if (ST || i >= 0) {
             if (!ST && fresh) {
                 // every load of queries is in the group of its tile's keys
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 fresh = false;
                 bad = w.over ? GPT2Q_STATUS_POSITION : 0;
                 quse = quse + 1 == C::QS ? 0 : quse + 1;
-                const unsigned char* q = qring + quse * hv * qrow;
+                [[maybe_unused]] const unsigned char* q = qring + quse * hv * qrow;
 #pragma unroll
                 for (int k = 0; k < (C::F32 ? HB : 2 * NT); ++k) m[k] = -INFINITY, l[k] = 0.f;
 #pragma unroll
@@ -457,7 +462,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     for (int nt = 0; nt < NT; ++nt) {
                         const int h = nt * 8 + (lane >> 2);
                         const TI* qh = reinterpret_cast<const TI*>(q + h * qrow) + (lane & 3) * 2;
-                        float down = 1.f, up = 1.f;  // of the queries, and back
+                        [[maybe_unused]] float down = 1.f, up = 1.f;  // of the queries, and back
                         if constexpr (C::SQ > 1 && C::HALF) {
                             // fp16 pieces of an fp32 query: scaled by a power of two so that the
                             // head's largest element lies in [1, 2), undone on the scores
@@ -798,73 +803,83 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                         }
                 }
             }
-            if (i >= 0 && !last) advance<C>(p, w);
+            if (i >= 0 && !last) advance<C>(p, slen, w);
         }
     }
     __syncthreads();
 
     // ---- the block's pieces, joined where they belong to one (row, head block) ----
-    int chain = 0, tail_row = -1, tail_vh = 0;
+    // lane i has piece i; pieces of one (row, head block) are neighbours and form a chain
+    const bool there = lane < 2 * nw && pieces[lane].nt > 0;
+    const long long of = there ? pieces[lane].first : -1 - lane;
+    const unsigned mates = __match_any_sync(0xffffffffu, of);
+    const unsigned heads = __ballot_sync(0xffffffffu, there && __ffs(mates) - 1 == lane);
+    const int chains = __popc(heads);
+    int tail_row = -1, tail_vh = 0;
     long long tail_last = 0;
-    for (int i = 0; i < 2 * nw;) {
-        if (pieces[i].nt == 0) {
-            ++i;
-            continue;
-        }
-        const Piece P = pieces[i];
-        int e = i + 1;
-        for (int j = i + 1; j < 2 * nw; ++j)
-            if (pieces[j].nt) {
-                if (pieces[j].first != P.first) break;
-                e = j + 1;
-            }
-        const bool whole = P.first >= ca && P.first + P.nt <= cb;
-        if (P.first >= ca && !whole) tail_row = P.row, tail_vh = P.vh, tail_last = quotient(P.first + P.nt - 1, per);
+    if (warp == 0 && chains) {
+        const Piece P = pieces[31 - __clz(heads)];  // only the last chain may go on behind the block
+        if (P.first >= ca && P.first + P.nt > cb)
+            tail_row = P.row, tail_vh = P.vh, tail_last = quotient(P.first + P.nt - 1, per);
+    }
+    for (int u = warp; u < chains * hv; u += nw) {
+        const int ch = u / hv, h = u - ch * hv;
+        const int i0 = __fns(heads, 0, ch + 1);
+        const Piece P = pieces[i0];
+        unsigned members = __shfl_sync(0xffffffffu, mates, i0);
         const int kvh = P.vh / p.blocks_per_kv, h0 = (P.vh - kvh * p.blocks_per_kv) * HB;
-        const int nh = min(HB, p.group - h0);
-        for (int h = 0; h < nh; ++h) {
-            if ((chain * hv + h) % nw != warp) continue;
-            float M = -INFINITY, Ls = 0.f;
-            for (int j = i; j < e; ++j)
-                if (pieces[j].nt) M = fmaxf(M, pm[j][h]);
-            const float ms = M == -INFINITY ? 0.f : M;
-            for (int j = i; j < e; ++j)
-                if (pieces[j].nt) Ls += pl[j][h] * ex2(pm[j][h] - ms);
-            const float f = whole ? inverse(Ls) : 1.f;
-            const long long ci = ((long long)blockIdx.x * 2 + (P.first < ca ? 0 : 1)) * HB + h;
-            for (int d = lane * 4; d < p.dim; d += 128) {
-                float r[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int j = i; j < e; ++j)
-                    if (pieces[j].nt) {
-                        const float4 v = *reinterpret_cast<const float4*>(pieces[j].data + h * C::HS + d);
-                        const float wt = ex2(pm[j][h] - ms);
-                        r[0] = fmaf(v.x, wt, r[0]);
-                        r[1] = fmaf(v.y, wt, r[1]);
-                        r[2] = fmaf(v.z, wt, r[2]);
-                        r[3] = fmaf(v.w, wt, r[3]);
-                    }
+        if (h0 + h >= p.group) continue;
+        const bool in = members >> lane & 1;
+        const float mm = in ? pm[lane][h] : -INFINITY, ll = in ? pl[lane][h] : 0.f;
+        float M = mm;
 #pragma unroll
-                for (int z = 0; z < 4; ++z) r[z] *= f;
-                if (whole)
-                    write4<TI>(p, P.row, kvh * p.group + h0 + h, d, r);
-                else
-                    *reinterpret_cast<float4*>(p.block_part + ci * HD + d) = make_float4(r[0], r[1], r[2], r[3]);
-            }
-            if (lane == 0) {
-                if (!whole)
-                    p.block_ml[ci] = make_float2(M, Ls);
-                else if (p.lse)
-                    p.lse[(long long)P.row * p.n_heads + kvh * p.group + h0 + h] = log_sum(M, Ls);
-            }
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float wt = ex2(mm - (M == -INFINITY ? 0.f : M));
+        float Ls = ll * wt;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
+        const bool whole = P.first >= ca && P.first + P.nt <= cb;
+        const float f = whole ? inverse(Ls) : 1.f;
+        const long long ci = ((long long)blockIdx.x * 2 + (P.first < ca ? 0 : 1)) * HB + h;
+        float r[(HD + 127) / 128][4] = {};
+        while (members) {
+            const int j = __ffs(members) - 1;
+            members &= members - 1;
+            const float wj = __shfl_sync(0xffffffffu, wt, j);
+            const float* data = pieces[j].data + h * C::HS + lane * 4;
+#pragma unroll
+            for (int y = 0; y < (HD + 127) / 128; ++y)
+                if (lane * 4 + y * 128 < p.dim) {
+                    const float4 v = *reinterpret_cast<const float4*>(data + y * 128);
+                    r[y][0] = fmaf(v.x, wj, r[y][0]);
+                    r[y][1] = fmaf(v.y, wj, r[y][1]);
+                    r[y][2] = fmaf(v.z, wj, r[y][2]);
+                    r[y][3] = fmaf(v.w, wj, r[y][3]);
+                }
         }
-        ++chain;
-        i = e;
+#pragma unroll
+        for (int y = 0; y < (HD + 127) / 128; ++y) {
+            const int d = lane * 4 + y * 128;
+            if (d >= p.dim) break;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) r[y][z] *= f;
+            if (whole)
+                write4<TI>(p, P.row, kvh * p.group + h0 + h, d, r[y]);
+            else
+                *reinterpret_cast<float4*>(p.block_part + ci * HD + d) = make_float4(r[y][0], r[y][1], r[y][2], r[y][3]);
+        }
+        if (lane == 0) {
+            if (!whole)
+                p.block_ml[ci] = make_float2(M, Ls);
+            else if (p.lse)
+                p.lse[(long long)P.row * p.n_heads + kvh * p.group + h0 + h] = log_sum(M, Ls);
+        }
     }
     if (tid == 0) p.meta[blockIdx.x] = make_int4(tail_row, tail_vh, (int)tail_last, 0);
 
     // ---- rows without a cached token ----
     for (int r = blockIdx.x; r < p.n_rows; r += gridDim.x) {
-        if (__ldcg(p.lens + r) > 0) continue;
+        if ((r < LENS ? slen[r] : __ldcg(p.lens + r)) > 0) continue;
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         for (int i = tid * 4; i < p.n_heads * p.dim; i += nthr * 4) write4<TI>(p, r, i / p.dim, i % p.dim, zero);
         if (p.lse)
@@ -878,6 +893,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
 template <class TI, int HD, int HB>
 __global__ void __launch_bounds__(128) k_paged_attn_join(const __grid_constant__ PagedAttn p) {
     __shared__ float4 part[128];
+    __shared__ float weight[MAX_CTAS];
     tc::pdl_trigger();
     tc::pdl_wait();
     const int c = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -887,30 +903,49 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(const __grid_constant__
     if (h0 + h >= p.group) return;
     const int n = meta.z - c + 1;
     auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * HB + h; };
-    float M = -INFINITY, L = 0.f;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(p.block_ml + at(i)).x);
+    constexpr int DG = HD / 4, PG = 128 / DG;  // threads over dims, and over pieces
+    const int d = tid % DG * 4, g = tid / DG;
+    // the first pieces' values are on their way while the weights are computed
+    float4 v0[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (d < p.dim && g + k * PG < n) v0[k] = __ldcg(reinterpret_cast<const float4*>(p.block_part + at(g + k * PG) * HD + d));
+    float2 ml = lane < n ? __ldcg(p.block_ml + at(lane)) : make_float2(-INFINITY, 0.f);
+    float M = ml.x, L = 0.f;
+    for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, __ldcg(p.block_ml + at(i)).x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ms = M == -INFINITY ? 0.f : M;
     for (int i = lane; i < n; i += 32) {
-        const float2 ml = __ldcg(p.block_ml + at(i));
-        L += ml.y * ex2(ml.x - ms);
+        if (i >= 32) ml = __ldcg(p.block_ml + at(i));
+        const float wt = ex2(ml.x - ms);
+        L += ml.y * wt;
+        if ((tid >> 5) == 0) weight[i] = wt;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    constexpr int DG = HD / 4, PG = 128 / DG;  // threads over dims, and over pieces
-    const int d = tid % DG * 4, g = tid / DG;
+    __syncthreads();
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < p.dim)
+    if (d < p.dim) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (g + k * PG < n) {
+                const float wt = weight[g + k * PG];
+                r.x = fmaf(v0[k].x, wt, r.x);
+                r.y = fmaf(v0[k].y, wt, r.y);
+                r.z = fmaf(v0[k].z, wt, r.z);
+                r.w = fmaf(v0[k].w, wt, r.w);
+            }
 #pragma unroll 4
-        for (int i = g; i < n; i += PG) {
-            const float wt = ex2(__ldcg(p.block_ml + at(i)).x - ms);
+        for (int i = g + 2 * PG; i < n; i += PG) {
+            const float wt = weight[i];
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p.block_part + at(i) * HD + d));
             r.x = fmaf(v.x, wt, r.x);
             r.y = fmaf(v.y, wt, r.y);
             r.z = fmaf(v.z, wt, r.z);
             r.w = fmaf(v.w, wt, r.w);
         }
+    }
     part[tid] = r;
     __syncthreads();
     const int head = kvh * p.group + h0 + h;
@@ -942,7 +977,7 @@ EncodeTiledFn tensor_map_encoder() {
     return fn;
 }
 
-constexpr size_t SMEM_LIMIT = 218 * 1024;  // dynamic; the rest for the static arrays
+constexpr size_t SMEM_LIMIT = 217 * 1024;  // dynamic; the rest for the static arrays
 
 // A pool as a tensor [page][head][piece][slot][dim]; dims past the head's own are read as zero.
 template <class C>
