@@ -373,6 +373,37 @@ int gpt2q_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int n_rows,
                         const void* d_targets, int targets_i64, const float* d_stats, const float* d_lp,
                         const float* d_ent, void* d_dlogits, int64_t ld_out, void* stream);
 
+/* ---- The model over the operators above ---- */
+
+/* Scores ids[1..n-1] under the model, as gpt2q_nll runs it (same prefill in cache slot `slot`, same limits, the
+ * published adapter applied): lp[p] is the log probability of ids[p+1] after ids[0..p], entropy[p] (may be NULL) the
+ * entropy there, top_ids / top_lp [n-1][top] the `top` likeliest tokens (0 <= top <= min(vocab, GPT2Q_TOP_MAX); NULL
+ * when top is 0). Host buffers of n - 1 rows; the logits stay on the device. */
+int gpt2q_score(gpt2q_handle* h, const uint32_t* ids, int n, int slot, int top, float* lp, float* entropy,
+                int32_t* top_ids, float* top_lp);
+
+/* gpt2q_trunk_input_grad for the loss sum_p d_lp[p] * ln p(targets[p] | ids[0..p]) + d_entropy[p] * H_p: the logits'
+ * gradient is computed on the device from the forward's own logits, so no [n][vocab] array crosses the bus. targets [n]
+ * (negative: no target at that position), d_lp and d_entropy [n] (either may be NULL) and the outputs lp, entropy [n]
+ * (may be NULL), dx and lnf_out [n][n_embd] (lnf_out may be NULL) are host buffers. */
+int gpt2q_trunk_score_grad(gpt2q_handle* h, const uint32_t* ids, int n, const int32_t* targets, const float* d_lp,
+                           const float* d_entropy, float* lp, float* entropy, float* dx, float* lnf_out);
+
+/* Copies the first n_tokens cached keys and values of arena slot `slot` (as a prefill or decode left them) into
+ * positions 0..n_tokens-1 of row `row` of `table`, in every layer's paged cache: layers[n_layer], each with the model's
+ * heads and head dim, of any cache type. Single-GPU handles only. The pools and the table are device memory of the
+ * handle's device, ready on the handle's stream. Returns when the copy is done. */
+int gpt2q_page_out(gpt2q_handle* h, int slot, int n_tokens, const gpt2q_paged_kv* layers, const gpt2q_page_table* table,
+                   int row);
+
+/* gpt2q_decode over paged caches instead of the arena: sequence i feeds tok[i] at pos[i], its keys and values go to row
+ * i of `table` (table->n_rows == n_seq), and it attends over positions 0..pos[i] of that row. n_seq is limited by the
+ * activation workspace (max(max_seqs, max_tokens)), not by the arena's slots, and sequences may share pages of a common
+ * prefix. Optional host outputs as in gpt2q_decode. A page id out of range, or a row too short for pos[i], fails with
+ * GPT2Q_EARG after the step has run (the outputs are then not meaningful). */
+int gpt2q_decode_paged(gpt2q_handle* h, const uint32_t* tok, const int32_t* pos, int n_seq, const gpt2q_paged_kv* layers,
+                       const gpt2q_page_table* table, float* logits, uint32_t* next_tok);
+
 #ifdef __cplusplus
 }
 #endif

@@ -166,4 +166,14 @@ extern "C" {
                                temperature: f32, d_targets: *const c_void, targets_i64: c_int, d_stats: *const f32,
                                d_lp: *const f32, d_ent: *const f32, d_dlogits: *mut c_void, ld_out: i64,
                                stream: *mut c_void) -> c_int;
+    pub fn gpt2q_score(h: *mut gpt2q_handle, ids: *const u32, n: c_int, slot: c_int, top: c_int, lp: *mut f32,
+                       entropy: *mut f32, top_ids: *mut i32, top_lp: *mut f32) -> c_int;
+    pub fn gpt2q_trunk_score_grad(h: *mut gpt2q_handle, ids: *const u32, n: c_int, targets: *const i32,
+                                  d_lp: *const f32, d_entropy: *const f32, lp: *mut f32, entropy: *mut f32,
+                                  dx: *mut f32, lnf_out: *mut f32) -> c_int;
+    pub fn gpt2q_page_out(h: *mut gpt2q_handle, slot: c_int, n_tokens: c_int, layers: *const gpt2q_paged_kv,
+                          table: *const gpt2q_page_table, row: c_int) -> c_int;
+    pub fn gpt2q_decode_paged(h: *mut gpt2q_handle, tok: *const u32, pos: *const i32, n_seq: c_int,
+                              layers: *const gpt2q_paged_kv, table: *const gpt2q_page_table, logits: *mut f32,
+                              next: *mut u32) -> c_int;
 }

@@ -27,6 +27,7 @@ EXPORTS = [
     "gpt2q_bwd_attn_train",
     "gpt2q_rotary_init", "gpt2q_paged_append", "gpt2q_paged_attention", "gpt2q_paged_attention_workspace",
     "gpt2q_logprobs", "gpt2q_logprobs_grad",
+    "gpt2q_score", "gpt2q_trunk_score_grad", "gpt2q_page_out", "gpt2q_decode_paged",
 ]
 
 
@@ -168,6 +169,12 @@ def load(path: str | None = None):
     lib.gpt2q_logprobs.restype = ci
     lib.gpt2q_logprobs_grad.argtypes = [vp, ci, C.c_int64, ci, ci, C.c_float, vp, ci, vp, vp, vp, vp, C.c_int64, vp]
     lib.gpt2q_logprobs_grad.restype = ci
+    lib.gpt2q_score.argtypes = [_hp, vp, ci, ci, ci, vp, vp, vp, vp]
+    lib.gpt2q_trunk_score_grad.argtypes = [_hp, vp, ci, vp, vp, vp, vp, vp, vp, vp]
+    lib.gpt2q_page_out.argtypes = [_hp, ci, ci, vp, vp, ci]
+    lib.gpt2q_decode_paged.argtypes = [_hp, vp, vp, ci, vp, vp, vp, vp]
+    for fn in (lib.gpt2q_score, lib.gpt2q_trunk_score_grad, lib.gpt2q_page_out, lib.gpt2q_decode_paged):
+        fn.restype = ci
     for fn in (lib.gpt2q_quantize_q8, lib.gpt2q_quantize_q4):
         fn.argtypes = [_f32p, C.c_size_t, C.POINTER(C.c_uint8)]
         fn.restype = C.c_int

@@ -27,7 +27,7 @@ LIB = os.path.join(LIBDIR, "libgpt2q.so")
 TORCH_LIB = os.path.join(LIBDIR, "gpt2q_torch.so")
 
 SOURCES = ["kernels.cu", "runtime.cu", "gemm.cu", "gemm_mma.cu", "attn_tc.cu", "persistent.cu", "tp.cu", "noalloc.cu", "synth.cpp", "blake3.cpp", "smt.cpp", "backward.cu", "paged.cu", "paged_attn.cu", "logprobs.cu"]
-HEADERS = ["common.cuh", "kernels.h", "gemm.h", "gemm_mma.h", "persistent.h", "tp.h", "tcgen05.cuh", "blake3.h", "backward.h", "paged.h", "device_op.cuh"]
+HEADERS = ["common.cuh", "kernels.h", "gemm.h", "gemm_mma.h", "persistent.h", "tp.h", "tcgen05.cuh", "blake3.h", "backward.h", "paged.h", "device_op.cuh", "logprobs.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -9,6 +9,7 @@
 
 #include "device_op.cuh"
 #include "gpt2q.h"
+#include "logprobs.h"
 
 namespace gpt2q {
 void set_global_error(const std::string& msg);  // runtime.cu
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
 }
 
 template <class T, int THREADS>
-cudaError_t launch_logprobs_by(LpParams p, cudaStream_t st) {
+cudaError_t launch_rows_by(LpParams p, cudaStream_t st) {
     if ((long long)p.rows * p.parts > INT32_MAX) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.rows * p.parts);
@@ -451,7 +452,7 @@ cudaError_t launch_logprobs_by(LpParams p, cudaStream_t st) {
 }
 
 template <class T>
-cudaError_t launch_logprobs(LpParams p, cudaStream_t st) {
+cudaError_t launch_rows(LpParams p, cudaStream_t st) {
     // Blocks per row: as many as still run at the same time (four of 256 threads per SM), while a
     // thread has a batch. 256 rows of 128000 bf16, 20 alternatives: 29.6, 21.4, 25.3 and 35.0 us with
     // 1, 2, 4 and 8 blocks per row; one row: 15.8, 11.1, 7.7, 6.6 us.
@@ -462,8 +463,8 @@ cudaError_t launch_logprobs(LpParams p, cudaStream_t st) {
     // other rows' loads better than four of 256 (2000 rows of 50257 bf16: 44 and 46 us, with 20
     // alternatives 62 and 66), but for many alternatives, whose ranking is shared by the threads (64 of
     // 4096 fp32 rows: 228 and 190 us).
-    if (p.rows > 148 * 4 && p.top <= 20) return launch_logprobs_by<T, 128>(p, st);
-    return launch_logprobs_by<T, 256>(p, st);
+    if (p.rows > 148 * 4 && p.top <= 20) return launch_rows_by<T, 128>(p, st);
+    return launch_rows_by<T, 256>(p, st);
 }
 
 struct GradParams {
@@ -640,6 +641,16 @@ int check(const char* who, const void* x, int dtype, int64_t ld, int n_rows, int
 
 }  // namespace
 
+cudaError_t gpt2q::launch_logprobs(const float* logits, int ld, int rows, int vocab, const int32_t* targets, int top,
+                                   float* lp, float* entropy, float* stats, int32_t* top_ids, float* top_lp, cudaStream_t st) {
+    return launch_rows<float>(LpParams{logits, ld, rows, vocab, top, 1, 1.f, targets, 0, lp, entropy, stats, top_ids, top_lp}, st);
+}
+
+cudaError_t gpt2q::launch_logprobs_grad(float* logits, int ld, int rows, int vocab, const int32_t* targets, const float* stats,
+                                        const float* d_lp, const float* d_ent, cudaStream_t st) {
+    return launch_grad<float>(GradParams{logits, logits, ld, ld, rows, vocab, 1, 1.f, targets, 0, stats, d_lp, d_ent}, st);
+}
+
 extern "C" int gpt2q_logprobs(const void* d_logits, int dtype, int64_t ld, int n_rows, int vocab, float temperature,
                               const void* d_targets, int targets_i64, int top, float* d_lp, float* d_entropy,
                               float* d_stats, int32_t* d_top_ids, float* d_top_lp, void* stream) {
@@ -655,11 +666,11 @@ extern "C" int gpt2q_logprobs(const void* d_logits, int dtype, int64_t ld, int n
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (dtype == GPT2Q_F32)
-        e = launch_logprobs<float>(p, st);
+        e = launch_rows<float>(p, st);
     else if (dtype == GPT2Q_F16)
-        e = launch_logprobs<__half>(p, st);
+        e = launch_rows<__half>(p, st);
     else
-        e = launch_logprobs<bf16>(p, st);
+        e = launch_rows<bf16>(p, st);
     if (e != cudaSuccess) {
         set_global_error(std::string(who) + ": " + cudaGetErrorString(e));
         return GPT2Q_ECUDA;

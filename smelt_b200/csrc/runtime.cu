@@ -29,6 +29,8 @@
 #include "gemm_mma.h"
 #include "backward.h"
 #include "kernels.h"
+#include "logprobs.h"
+#include "paged.h"
 #include "persistent.h"
 #include "tp.h"
 
@@ -139,6 +141,15 @@ struct gpt2q_handle {
     float* nll_logits = nullptr;
     int* nll_tgt = nullptr;
     double* nll_terms = nullptr;
+    float* score_out = nullptr;  // gpt2q_score: log probabilities, entropies and alternatives of n_ctx positions
+    // decode over a caller's paged cache (grown on demand): q|k|v rows, logits, argmax slots, the
+    // step's token ids, positions, lengths and picks, the attention's workspace, the status word
+    int pg_rows = 0;
+    std::vector<void*> pg_allocs;
+    float *pg_qkv = nullptr, *pg_logits = nullptr;
+    unsigned long long* pg_best = nullptr;
+    int *pg_ints = nullptr, *pg_status = nullptr;
+    void* pg_work = nullptr;
     int* kerr = nullptr;  // device error word of the CUDA-core kernels' bounded waits
     // trunk backward workspace (grown on demand, freed by destroy)
     float* bwd_ws = nullptr;
@@ -519,8 +530,9 @@ bool ln_fusable(const gpt2q_handle* H, const Linear& prod, const In& pin, const 
 
 // One transformer block over M activation rows (gpt2.rs:238-322). attn_fn runs the
 // attention of this layer (decode or prefill form).
+// qkv: where q|k|v rows go instead of the query buffer and the KV arena (paged decode).
 template <class AttnFn>
-int block(gpt2q_handle* H, int layer, int M, const int* slot, const int* pos, AttnFn&& attn_fn) {
+int block(gpt2q_handle* H, int layer, int M, const int* slot, const int* pos, AttnFn&& attn_fn, float* qkv = nullptr) {
     const int d = H->cfg.n_embd;
     const float eps = H->cfg.ln_eps;
     LayerW& Lw = H->layers[layer];
@@ -542,7 +554,8 @@ int block(gpt2q_handle* H, int layer, int M, const int* slot, const int* pos, At
         RUN("layernorm", (double)M * d * 8,
             launch_layernorm(H->x, d, nullptr, reads_f32(H, Lw.attn, hin, M) ? H->h : nullptr, d, H->h_hi, H->h_lo,
                              Lw.ln1_g, Lw.ln1_b, d, eps, M, H->stream));
-    int rc = linear(H, "linear_qkv", Lw.attn, hin, M, epi_qkv(H, layer, slot, pos, Lw.attn.bias), fuse1 ? &ln1 : nullptr);
+    const Epi eq = qkv ? epi_store(qkv, 3 * H->d_local, Lw.attn.bias) : epi_qkv(H, layer, slot, pos, Lw.attn.bias);
+    int rc = linear(H, "linear_qkv", Lw.attn, hin, M, eq, fuse1 ? &ln1 : nullptr);
     if (rc) return rc;
     rc = attn_fn(layer);
     if (rc) return rc;
@@ -1310,7 +1323,16 @@ int create_common(const gpt2q_config* cfg, const gpt2q_tensor_desc* tensors, int
 // input of ln_f and its output), then trunk_input_grad (gpu_backward.rs:651-790) with every op
 // batched over the T positions. Weights are read in their uploaded atoms; the dequantised
 // values are exactly Engine::vec_f32's, the f32 weights the reference's backward uses.
-int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits, float* dx_out, float* lnf_out) {
+//
+// With `score` the logits' gradient is that of the positions' log probabilities and entropies, and
+// comes from the forward's own logits on the device.
+struct TrunkScore {
+    const int32_t* targets;           // host [T]; negative: none
+    const float *d_lp, *d_entropy;    // host [T], may be null
+    float *lp, *entropy;              // host [T], may be null
+};
+int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits, float* dx_out, float* lnf_out,
+               const TrunkScore* score = nullptr) {
     // The stash feeds a backward that amplifies activation rounding (fp16 activations in the
     // forward gave 6 % relative error in dx at 128 positions): the wide tiles compute all
     // three products here, whatever GPT2Q_TC_PRODUCTS selected for inference.
@@ -1339,6 +1361,7 @@ int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits
                         + 2 * Td + TF                                      // their fp16 hi/lo splits
                         + up64((size_t)T * V)                              // dlogits
                         + 3 * Td + TF + T3                                 // G, DH, DATT, DFC, DQKV
+                        + up64((size_t)8 * T)                              // score: targets, gradients, outputs
                         + up64(part_n) + up64((size_t)3 * NH * T) + up64((size_t)2 * T) + n_ctr;
     if (H->bwd_ws_floats < need) {
         if (H->bwd_ws) {
@@ -1381,6 +1404,7 @@ int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits
     float* DATT = take(Td);
     float* DFC = take(TF);
     float* DQKV = take(T3);
+    float* SC = take(up64((size_t)8 * T));
     float* part = take(up64(part_n));
     float* stats = take(up64((size_t)3 * NH * T));
     int* d_ids = reinterpret_cast<int*>(take(up64((size_t)2 * T)));
@@ -1393,7 +1417,7 @@ int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits
         hi[T + p] = p;
     }
     CK(cudaMemcpyAsync(d_ids, hi.data(), hi.size() * 4, cudaMemcpyHostToDevice, H->stream));
-    CK(cudaMemcpyAsync(DL, dlogits, (size_t)T * V * 4, cudaMemcpyHostToDevice, H->stream));
+    if (!score) CK(cudaMemcpyAsync(DL, dlogits, (size_t)T * V * 4, cudaMemcpyHostToDevice, H->stream));
 
     // ---- forward with the stash ----
     RUN("embed", (double)T * d * 8,
@@ -1430,7 +1454,26 @@ int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits
     }
     const float* xL = xs + (size_t)L * Td;
     RUN("layernorm", (double)T * d * 8,
-        launch_layernorm(xL, d, nullptr, lnf, d, nullptr, nullptr, H->lnf_g, H->lnf_b, d, eps, T, H->stream));
+        launch_layernorm(xL, d, nullptr, lnf, d, score ? hb_hi : nullptr, score ? hb_lo : nullptr, H->lnf_g, H->lnf_b, d, eps, T,
+                         H->stream));
+    if (score) {
+        int32_t* tgt = reinterpret_cast<int32_t*>(SC);
+        float *glp = SC + T, *gen = SC + 2 * (size_t)T, *lp = SC + 3 * (size_t)T, *en = SC + 4 * (size_t)T, *st = SC + 5 * (size_t)T;
+        CK(cudaMemcpyAsync(tgt, score->targets, (size_t)T * 4, cudaMemcpyHostToDevice, H->stream));
+        if (score->d_lp) CK(cudaMemcpyAsync(glp, score->d_lp, (size_t)T * 4, cudaMemcpyHostToDevice, H->stream));
+        if (score->d_entropy) CK(cudaMemcpyAsync(gen, score->d_entropy, (size_t)T * 4, cudaMemcpyHostToDevice, H->stream));
+        for (int r0 = 0; r0 < T; r0 += 256) {
+            const size_t o = (size_t)r0 * d;
+            const int rc = linear(H, "linear_head", H->wte, In{lnf + o, hb_hi + o, hb_lo + o, d}, std::min(256, T - r0),
+                                  epi_store(DL + (size_t)r0 * V, V, nullptr));
+            if (rc) return rc;
+        }
+        RUN("logprobs", (double)T * V * 4, launch_logprobs(DL, V, T, V, tgt, 0, lp, en, st, nullptr, nullptr, H->stream));
+        RUN("logprobs_grad", (double)T * V * 8,
+            launch_logprobs_grad(DL, V, T, V, tgt, st, score->d_lp ? glp : nullptr, score->d_entropy ? gen : nullptr, H->stream));
+        if (score->lp) CK(cudaMemcpyAsync(score->lp, lp, (size_t)T * 4, cudaMemcpyDeviceToHost, H->stream));
+        if (score->entropy) CK(cudaMemcpyAsync(score->entropy, en, (size_t)T * 4, cudaMemcpyDeviceToHost, H->stream));
+    }
 
     // ---- backward: head, ln_f, then the layers in reverse ----
     // algorithmic bytes: the weights once, dY, the output (and the GELU input or the added-to output)
@@ -1475,6 +1518,104 @@ int trunk_grad(gpt2q_handle* H, const uint32_t* ids, int T, const float* dlogits
     CK(cudaStreamSynchronize(H->stream));
     return check_device_error(H);
 }
+
+// ------------------------------------------------------------------ scoring, paged decode
+// One prefill of ids in `slot`, ln_f over positions 0..n-2, and the tied head in chunks of up to 256
+// rows: rows_fn(logits, r0, rows) takes each chunk's logits; the target of row p is ids[p + 1]
+// (nll_tgt).
+template <class F>
+int score_positions(gpt2q_handle* H, const uint32_t* ids, int n, int slot, F&& rows_fn) {
+    if (n < 2 || n > H->cfg.n_ctx || n > H->Mmax) return H->fail(GPT2Q_EARG, "n out of range [2, min(n_ctx, max_tokens)]");
+    if (slot < 0 || slot >= H->cfg.max_seqs) return H->fail(GPT2Q_EARG, "slot out of range");
+    CK(cudaSetDevice(H->device));
+    int rc = check_tokens(H, ids, (size_t)n);
+    if (rc) return rc;
+    constexpr int NLL_ROWS = 256;
+    const int d = H->cfg.n_embd, V = H->cfg.vocab, R = n - 1;
+    if (!H->nll_logits) {
+        H->nll_logits = H->dalloc<float>((size_t)NLL_ROWS * V * 4);
+        H->nll_tgt = H->dalloc<int>((size_t)H->cfg.n_ctx * 4);
+        H->nll_terms = H->dalloc<double>((size_t)H->cfg.n_ctx * 8);
+        if (!H->nll_logits || !H->nll_tgt || !H->nll_terms) return H->fail(GPT2Q_EOOM, "NLL buffers");
+    }
+    const int32_t offs[2] = {0, n};
+    const int32_t slots[1] = {slot};
+    rc = prefill_chunk(H, ids, offs, slots, 0, 1, true);
+    if (rc) return rc;
+    std::vector<int> tgt(R);
+    for (int p = 0; p < R; ++p) tgt[p] = (int)ids[p + 1];
+    CK(cudaMemcpyAsync(H->nll_tgt, tgt.data(), (size_t)R * 4, cudaMemcpyHostToDevice, H->stream));
+    RUN("layernorm", (double)R * d * 8,
+        launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, R,
+                         H->stream));
+    rc = apply_adapter(H, R);
+    if (rc) return rc;
+    for (int r0 = 0; r0 < R; r0 += NLL_ROWS) {
+        const int rows = std::min(NLL_ROWS, R - r0);
+        const size_t o = (size_t)r0 * d;
+        rc = linear(H, "linear_head", H->wte, In{H->h + o, H->h_hi + o, H->h_lo + o, d}, rows,
+                    epi_store(H->nll_logits, V, nullptr));
+        if (!rc) rc = rows_fn(H->nll_logits, r0, rows);
+        if (rc) return rc;
+    }
+    return GPT2Q_OK;
+}
+
+// A paged cache per layer, of this model's heads.
+int check_paged(gpt2q_handle* H, const gpt2q_paged_kv* layers) {
+    if (H->tp_size > 1) return H->fail(GPT2Q_EUNSUP, "a paged cache needs a single-GPU handle");
+    if (!layers) return H->fail(GPT2Q_EARG, "null layers");
+    for (int l = 0; l < H->cfg.n_layer; ++l)
+        if (layers[l].n_kv_heads != H->H_local || layers[l].head_dim != H->hd)
+            return H->fail(GPT2Q_EARG, "layer " + std::to_string(l) + ": the cache must have the model's heads and head dim");
+    return GPT2Q_OK;
+}
+
+// Buffers of a paged decode of up to `rows` sequences.
+int ensure_paged(gpt2q_handle* H, int rows) {
+    if (H->pg_rows >= rows) return GPT2Q_OK;
+    CK(cudaStreamSynchronize(H->stream));
+    for (void* p : H->pg_allocs) cudaFree(p);
+    H->pg_allocs.clear();
+    H->pg_rows = 0;
+    const int R = std::min(std::max(rows, std::min(32, H->Mmax)), H->Mmax);
+    bool ok = true;
+    auto take = [&](size_t bytes) {
+        void* p = nullptr;
+        if (cudaMalloc(&p, bytes) != cudaSuccess) {
+            cudaGetLastError();
+            ok = false;
+            return p = nullptr;
+        }
+        H->pg_allocs.push_back(p);
+        return p;
+    };
+    gpt2q_paged_kv kv{};
+    kv.n_kv_heads = H->H_local;
+    kv.head_dim = H->hd;
+    H->pg_qkv = static_cast<float*>(take((size_t)R * 3 * H->d_local * 4));
+    H->pg_logits = static_cast<float*>(take((size_t)R * H->cfg.vocab * 4));
+    H->pg_best = static_cast<unsigned long long*>(take((size_t)R * 8));
+    H->pg_ints = static_cast<int*>(take((size_t)4 * R * 4));
+    H->pg_status = static_cast<int*>(take(16));
+    H->pg_work = take((size_t)gpt2q_paged_attention_workspace(&kv, H->H_local));
+    if (!ok) return H->fail(GPT2Q_EOOM, "paged decode buffers");
+    CK(cudaMemsetAsync(H->pg_best, 0, (size_t)R * 8, H->stream));
+    H->pg_rows = R;
+    return GPT2Q_OK;
+}
+
+// Waits for the handle's work and turns the paged kernels' status word into an error.
+int paged_status(gpt2q_handle* H) {
+    int status = 0;
+    CK(cudaMemcpyAsync(&status, H->pg_status, 4, cudaMemcpyDeviceToHost, H->stream));
+    CK(cudaStreamSynchronize(H->stream));
+    const int rc = check_device_error(H);
+    if (rc) return rc;
+    if (status & GPT2Q_STATUS_TIMEOUT) return H->fail(GPT2Q_ETIMEOUT, "a bounded device-side wait timed out (paged attention)");
+    if (status) return H->fail(GPT2Q_EARG, "the page table names a page out of range or is too short (status " + std::to_string(status) + ")");
+    return GPT2Q_OK;
+}
 }  // namespace
 
 // Message for gpt2q_last_error(NULL), used by calls that have no handle.
@@ -1513,6 +1654,7 @@ void gpt2q_destroy(gpt2q_handle* H) {
     mk_destroy(H->mk);
     for (auto& a : H->allocs) cudaFree(a.p);
     if (H->bwd_ws) cudaFree(H->bwd_ws);
+    for (void* p : H->pg_allocs) cudaFree(p);
     if (H->h_stage) cudaFreeHost(H->h_stage);
     if (H->h_err) cudaFreeHost(H->h_err);
     if (H->own_stream) cudaStreamDestroy(H->own_stream);
@@ -1687,41 +1829,14 @@ int gpt2q_clear_adapter(gpt2q_handle* H) {
 int gpt2q_nll(gpt2q_handle* H, const uint32_t* ids, int n, int slot, double* out) {
     if (!H) return GPT2Q_EARG;
     if (!ids || !out) return H->fail(GPT2Q_EARG, "null ids/out");
-    if (n < 2 || n > H->cfg.n_ctx || n > H->Mmax) return H->fail(GPT2Q_EARG, "n out of range [2, min(n_ctx, max_tokens)]");
-    if (slot < 0 || slot >= H->cfg.max_seqs) return H->fail(GPT2Q_EARG, "slot out of range");
-    CK(cudaSetDevice(H->device));
-    int rc = check_tokens(H, ids, (size_t)n);
-    if (rc) return rc;
-    constexpr int NLL_ROWS = 256;
-    const int d = H->cfg.n_embd, V = H->cfg.vocab, R = n - 1;
-    if (!H->nll_logits) {
-        H->nll_logits = H->dalloc<float>((size_t)NLL_ROWS * V * 4);
-        H->nll_tgt = H->dalloc<int>((size_t)H->cfg.n_ctx * 4);
-        H->nll_terms = H->dalloc<double>((size_t)H->cfg.n_ctx * 8);
-        if (!H->nll_logits || !H->nll_tgt || !H->nll_terms) return H->fail(GPT2Q_EOOM, "NLL buffers");
-    }
-    const int32_t offs[2] = {0, n};
-    const int32_t slots[1] = {slot};
-    rc = prefill_chunk(H, ids, offs, slots, 0, 1, true);
-    if (rc) return rc;
-    // positions 0..n-2 predict ids[1..n-1]: ln_f over their rows, the head in chunks, the terms
-    std::vector<int> tgt(R);
-    for (int p = 0; p < R; ++p) tgt[p] = (int)ids[p + 1];
-    CK(cudaMemcpyAsync(H->nll_tgt, tgt.data(), (size_t)R * 4, cudaMemcpyHostToDevice, H->stream));
-    RUN("layernorm", (double)R * d * 8,
-        launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, R,
-                         H->stream));
-    rc = apply_adapter(H, R);
-    if (rc) return rc;
-    for (int r0 = 0; r0 < R; r0 += NLL_ROWS) {
-        const int rows = std::min(NLL_ROWS, R - r0);
-        const size_t o = (size_t)r0 * d;
-        rc = linear(H, "linear_head", H->wte, In{H->h + o, H->h_hi + o, H->h_lo + o, d}, rows,
-                    epi_store(H->nll_logits, V, nullptr));
-        if (rc) return rc;
+    const int R = n - 1;
+    int rc = score_positions(H, ids, n, slot, [&](float* logits, int r0, int rows) {
+        const int V = H->cfg.vocab;
         RUN("nll", (double)rows * V * 4,
-            launch_nll_rows(H->nll_logits, V, V, rows, H->nll_tgt + r0, H->nll_terms + r0, H->stream));
-    }
+            launch_nll_rows(logits, V, V, rows, H->nll_tgt + r0, H->nll_terms + r0, H->stream));
+        return GPT2Q_OK;
+    });
+    if (rc) return rc;
     std::vector<double> terms(R);
     CK(cudaMemcpyAsync(terms.data(), H->nll_terms, (size_t)R * 8, cudaMemcpyDeviceToHost, H->stream));
     CK(cudaStreamSynchronize(H->stream));
@@ -1733,6 +1848,152 @@ int gpt2q_nll(gpt2q_handle* H, const uint32_t* ids, int n, int slot, double* out
     *out = total / (double)R;
     // the slot's cache now holds this sequence; its decode state is not advanced
     return GPT2Q_OK;
+}
+
+int gpt2q_score(gpt2q_handle* H, const uint32_t* ids, int n, int slot, int top, float* lp, float* entropy,
+                int32_t* top_ids, float* top_lp) {
+    if (!H) return GPT2Q_EARG;
+    if (!ids || !lp) return H->fail(GPT2Q_EARG, "null ids/lp");
+    const int V = H->cfg.vocab, R = n - 1;
+    const size_t C = H->cfg.n_ctx;
+    if (top < 0 || top > GPT2Q_TOP_MAX || top > V) return H->fail(GPT2Q_EARG, "top out of range [0, min(vocab, GPT2Q_TOP_MAX)]");
+    if (top > 0 && (!top_ids || !top_lp)) return H->fail(GPT2Q_EARG, "null top_ids/top_lp");
+    CK(cudaSetDevice(H->device));
+    if (!H->score_out) H->score_out = H->dalloc<float>(C * (2 + 2 * GPT2Q_TOP_MAX) * 4);
+    if (!H->score_out) return H->fail(GPT2Q_EOOM, "score buffers");
+    float *d_lp = H->score_out, *d_ent = d_lp + C, *d_top = d_ent + C;
+    int32_t* d_ids = reinterpret_cast<int32_t*>(d_top + C * GPT2Q_TOP_MAX);
+    int rc = score_positions(H, ids, n, slot, [&](float* logits, int r0, int rows) {
+        const size_t t0 = (size_t)r0 * top;
+        RUN("logprobs", (double)rows * V * 4,
+            launch_logprobs(logits, V, rows, V, H->nll_tgt + r0, top, d_lp + r0, d_ent + r0, nullptr, d_ids + t0, d_top + t0,
+                            H->stream));
+        return GPT2Q_OK;
+    });
+    if (rc) return rc;
+    CK(cudaMemcpyAsync(lp, d_lp, (size_t)R * 4, cudaMemcpyDeviceToHost, H->stream));
+    if (entropy) CK(cudaMemcpyAsync(entropy, d_ent, (size_t)R * 4, cudaMemcpyDeviceToHost, H->stream));
+    if (top > 0) {
+        CK(cudaMemcpyAsync(top_ids, d_ids, (size_t)R * top * 4, cudaMemcpyDeviceToHost, H->stream));
+        CK(cudaMemcpyAsync(top_lp, d_top, (size_t)R * top * 4, cudaMemcpyDeviceToHost, H->stream));
+    }
+    CK(cudaStreamSynchronize(H->stream));
+    return check_device_error(H);
+}
+
+int gpt2q_page_out(gpt2q_handle* H, int slot, int n_tokens, const gpt2q_paged_kv* layers, const gpt2q_page_table* table,
+                   int row) {
+    if (!H) return GPT2Q_EARG;
+    if (slot < 0 || slot >= H->cfg.max_seqs) return H->fail(GPT2Q_EARG, "slot out of range");
+    if (n_tokens < 1 || n_tokens > H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "n_tokens out of range [1, n_ctx]");
+    if (!table || row < 0 || row >= table->n_rows) return H->fail(GPT2Q_EARG, "null table or row out of range");
+    CK(cudaSetDevice(H->device));
+    int rc = check_paged(H, layers);
+    if (!rc) rc = ensure_paged(H, 1);
+    if (rc) return rc;
+    gpt2q_page_table t = *table;
+    t.ids += (size_t)row * t.ld;
+    t.n_rows = 1;
+    CK(cudaMemsetAsync(H->pg_status, 0, 4, H->stream));
+    for (int l = 0; l < H->cfg.n_layer; ++l) {
+        float* k = H->kv.base + (size_t)slot * H->kv.slot_stride + (size_t)l * H->kv.layer_stride;
+        const gpt2q_heads kh{k, H->hd, (int64_t)H->kv.head_stride};
+        const gpt2q_heads vh{k + H->kv.sel_stride, H->hd, (int64_t)H->kv.head_stride};
+        std::string why;
+        rc = paged_append(&layers[l], &t, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, n_tokens, nullptr, 0, nullptr, nullptr,
+                          H->pg_status, H->stream, &why);
+        if (rc) return H->fail(rc, "page_out: " + why);
+        H->launches++;
+    }
+    return paged_status(H);
+}
+
+int gpt2q_decode_paged(gpt2q_handle* H, const uint32_t* tok, const int32_t* pos, int n_seq, const gpt2q_paged_kv* layers,
+                       const gpt2q_page_table* table, float* logits, uint32_t* next_tok) {
+    if (!H) return GPT2Q_EARG;
+    if (!tok || !pos) return H->fail(GPT2Q_EARG, "null tok/pos");
+    if (n_seq < 1 || n_seq > H->Mmax) return H->fail(GPT2Q_EARG, "n_seq out of range [1, max(max_seqs, max_tokens)]");
+    if (!table || table->n_rows != n_seq) return H->fail(GPT2Q_EARG, "the table must have n_seq rows");
+    for (int i = 0; i < n_seq; ++i)
+        if (pos[i] < 0 || pos[i] >= H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "pos out of range [0, n_ctx)");
+    CK(cudaSetDevice(H->device));
+    int rc = check_tokens(H, tok, (size_t)n_seq);
+    if (!rc) rc = check_paged(H, layers);
+    if (!rc) rc = ensure_paged(H, n_seq);
+    if (!rc) rc = ensure_stage(H, (size_t)3 * n_seq);
+    if (rc) return rc;
+    const int d = H->cfg.n_embd, V = H->cfg.vocab, B = n_seq, R = H->pg_rows, NH = H->H_local, hd = H->hd;
+    // tokens | positions | lengths | picks, pg_rows each
+    uint32_t* d_tok = reinterpret_cast<uint32_t*>(H->pg_ints);
+    int *d_pos = H->pg_ints + R, *d_len = H->pg_ints + 2 * (size_t)R;
+    uint32_t* d_next = reinterpret_cast<uint32_t*>(H->pg_ints + 3 * (size_t)R);
+    for (int i = 0; i < B; ++i) {
+        H->h_stage[i] = (int)tok[i];
+        H->h_stage[B + i] = pos[i];
+        H->h_stage[2 * B + i] = pos[i] + 1;
+    }
+    CK(cudaMemcpyAsync(d_tok, H->h_stage, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
+    CK(cudaMemcpyAsync(d_pos, H->h_stage + B, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
+    CK(cudaMemcpyAsync(d_len, H->h_stage + 2 * (size_t)B, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
+    CK(cudaMemsetAsync(H->pg_status, 0, 4, H->stream));
+    const float scale = 1.0f / std::sqrt((float)hd);
+    const gpt2q_heads qh{H->pg_qkv, 3 * (int64_t)d, hd}, kh{H->pg_qkv + d, 3 * (int64_t)d, hd}, vh{H->pg_qkv + 2 * d, 3 * (int64_t)d, hd};
+    double keys = 0;
+    for (int i = 0; i < B; ++i) keys += pos[i] + 1;
+    RUN("embed", (double)B * d * 6, launch_embed(H->wte.w, H->wpe.w, d_tok, d_pos, H->x, d, B, H->stream));
+    for (int l = 0; l < H->cfg.n_layer; ++l) {
+        rc = block(H, l, B, nullptr, nullptr, [&](int layer) {
+            const In ain{H->att, H->att_hi, H->att_lo, H->d_local};
+            const bool att32 = reads_f32(H, H->layers[layer].proj, ain, B);
+            const gpt2q_heads oh{att32 ? H->att : nullptr, d, hd};
+            const gpt2q_paged_kv& kv = layers[layer];
+            std::string why;
+            int prc = GPT2Q_OK;
+            auto launched_as = [&](int code) { return prc = code, code == GPT2Q_OK ? cudaSuccess : cudaErrorInvalidValue; };
+            const int es = kv.dtype == GPT2Q_F32 ? 4 : 2;
+            int krc = run_kernel(H, "paged_append", (double)B * 2 * d * (4 + es), [&] {
+                return launched_as(paged_append(&kv, table, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, B, d_pos, 0, nullptr,
+                                                nullptr, H->pg_status, H->stream, &why));
+            });
+            if (!krc)
+                krc = run_kernel(H, "paged_attention", keys * 2 * d * es + (double)B * d * 8, [&] {
+                    return launched_as(paged_attention(&kv, table, d_len, &qh, &oh, GPT2Q_F32, NH, scale, 0, nullptr, H->pg_status,
+                                                       H->pg_work, HiLo{H->att_hi, H->att_lo, d}, H->stream, &why));
+                });
+            if (!krc) H->launches++;  // the attention and its join
+            return prc ? H->fail(prc, "decode_paged: " + why) : krc;
+        }, H->pg_qkv);
+        if (rc) return rc;
+    }
+    RUN("layernorm", (double)B * d * 8,
+        launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, B, H->stream));
+    rc = apply_adapter(H, B);
+    if (!rc) rc = head(H, B, H->pg_logits);
+    if (rc) return rc;
+    RUN("argmax", (double)B * V * 4,
+        launch_argmax(H->pg_logits, V, V, B, H->pg_best, d_next, nullptr, nullptr, 0, nullptr, nullptr, H->stream));
+    H->launches++;  // argmax is two kernels
+    if (logits) CK(cudaMemcpyAsync(logits, H->pg_logits, (size_t)B * V * 4, cudaMemcpyDeviceToHost, H->stream));
+    if (next_tok) CK(cudaMemcpyAsync(next_tok, d_next, (size_t)B * 4, cudaMemcpyDeviceToHost, H->stream));
+    rc = paged_status(H);
+    if (!rc && H->prof) rc = flush_profile(H);
+    return rc;
+}
+
+int gpt2q_trunk_score_grad(gpt2q_handle* H, const uint32_t* ids, int n, const int32_t* targets, const float* d_lp,
+                           const float* d_entropy, float* lp, float* entropy, float* dx, float* lnf_out) {
+    if (!H) return GPT2Q_EARG;
+    if (!ids || !targets || !dx) return H->fail(GPT2Q_EARG, "null ids/targets/dx");
+    if (n < 1 || n > H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "n out of range [1, n_ctx]");
+    if (H->tp_size > 1) return H->fail(GPT2Q_EUNSUP, "trunk backward needs a single-GPU handle");
+    if (H->hd > 128) return H->fail(GPT2Q_EUNSUP, "trunk backward needs head dim <= 128");
+    for (int i = 0; i < n; ++i)
+        if (targets[i] >= H->cfg.vocab) return H->fail(GPT2Q_EARG, "target id " + std::to_string(targets[i]) + " >= vocab");
+    CK(cudaSetDevice(H->device));
+    const int rc = check_tokens(H, ids, (size_t)n);
+    if (rc) return rc;
+    const TrunkScore sc{targets, d_lp, d_entropy, lp, entropy};
+    return trunk_grad(H, ids, n, nullptr, dx, lnf_out, &sc);
 }
 
 int gpt2q_trunk_input_grad(gpt2q_handle* H, const uint32_t* ids, int n, const float* dlogits, float* dx,

@@ -205,6 +205,70 @@ class Gpu:
                                                      lnf.ctypes.data_as(_ffi._f32p)))
         return dx, lnf
 
+    def score(self, ids, top: int = 0, slot: int = 0):
+        """Log probabilities of ids[1:] under the model, the entropies, and the `top` likeliest tokens at
+        every position: (lp [n-1], entropy [n-1], top_ids [n-1][top], top_lp [n-1][top]); overwrites the
+        KV cache of `slot`, as nll does."""
+        ids = np.ascontiguousarray(ids, dtype=np.uint32)
+        rows = max(0, ids.size - 1)
+        lp, ent = np.empty(rows, np.float32), np.empty(rows, np.float32)
+        top_ids, top_lp = np.empty((rows, max(0, top)), np.int32), np.empty((rows, max(0, top)), np.float32)
+        self._check(self._lib.gpt2q_score(self.h, ids.ctypes.data, int(ids.size), int(slot), int(top), lp.ctypes.data,
+                                          ent.ctypes.data, top_ids.ctypes.data, top_lp.ctypes.data))
+        return lp, ent, top_ids, top_lp
+
+    def trunk_score_grad(self, ids, targets, d_lp=None, d_entropy=None):
+        """trunk_input_grad for the loss sum(d_lp * lp + d_entropy * entropy) over the positions' log
+        probabilities of `targets` (negative: none) and entropies, all on the device. Returns (dx, lnf_out, lp,
+        entropy)."""
+        ids = np.ascontiguousarray(ids, dtype=np.uint32)
+        n, d = ids.size, self.meta.n_embd
+        tgt = np.ascontiguousarray(targets, dtype=np.int32)
+        grads = [None if g is None else np.ascontiguousarray(g, dtype=np.float32) for g in (d_lp, d_entropy)]
+        if tgt.shape != (n,) or any(g is not None and g.shape != (n,) for g in grads):
+            raise ValueError(f"targets, d_lp and d_entropy must have {n} elements")
+        dx, lnf = np.empty((n, d), np.float32), np.empty((n, d), np.float32)
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        g0, g1 = (None if g is None else g.ctypes.data for g in grads)
+        self._check(self._lib.gpt2q_trunk_score_grad(self.h, ids.ctypes.data, n, tgt.ctypes.data, g0, g1, lp.ctypes.data,
+                                                     ent.ctypes.data, dx.ctypes.data, lnf.ctypes.data))
+        return dx, lnf, lp, ent
+
+    # ---- decode over paged caches (smelt_b200.paged.PagedKV, one per layer) ----
+    def _paged(self, layers, table):
+        import torch
+
+        if len(layers) != self.meta.n_layer or any(kv.index != self.device for kv in layers):
+            raise ValueError(f"{self.meta.n_layer} paged caches on device {self.device} are needed, one per layer")
+        if (not table.is_cuda or table.get_device() != self.device or table.dtype != torch.int32 or table.dim() != 2
+                or table.stride(1) != 1):
+            raise ValueError(f"table must be int32 [rows, pages] on cuda:{self.device}")
+        # what torch has queued (the pools, the table) comes before this handle's stream
+        torch.cuda.current_stream(self.device).synchronize()
+        rows, width = table.shape
+        return ((_ffi.PagedKV * len(layers))(*(kv.c for kv in layers)),
+                _ffi.PageTable(table.data_ptr(), rows, width, max(table.stride(0), width)))
+
+    def page_out(self, slot: int, n_tokens: int, layers, table, row: int):
+        """Copies the first n_tokens cached positions of arena slot `slot` into row `row` of `table` of every
+        layer's paged cache."""
+        arr, t = self._paged(layers, table)
+        self._check(self._lib.gpt2q_page_out(self.h, int(slot), int(n_tokens), arr, C.byref(t), int(row)))
+
+    def decode_paged(self, tok, pos, layers, table, want_logits: bool = False):
+        """decode() over paged caches: sequence i is row i of `table`."""
+        tok = np.ascontiguousarray(tok, dtype=np.uint32)
+        pos = np.ascontiguousarray(pos, dtype=np.int32)
+        n = tok.size
+        if pos.size != n:
+            raise ValueError("tok and pos must have the same length")
+        nxt = np.empty(n, dtype=np.uint32)
+        lg = np.empty((n, self.meta.vocab), dtype=np.float32) if want_logits else None
+        arr, t = self._paged(layers, table)
+        self._check(self._lib.gpt2q_decode_paged(self.h, tok.ctypes.data, pos.ctypes.data, n, arr, C.byref(t),
+                                                 None if lg is None else lg.ctypes.data, nxt.ctypes.data))
+        return (nxt, lg) if want_logits else nxt
+
     def dequant(self, name: str, numel: int) -> np.ndarray:
         out = np.empty(numel, dtype=np.float32)
         self._check(self._lib.gpt2q_dequant(self.h, name.encode(), out.ctypes.data_as(_ffi._f32p), numel))
