@@ -32,14 +32,19 @@ struct AppendParams {
     double turns[128];
 };
 
-// A unit is two chunks of V consecutive elements, the (a, b) of V rotated pairs or 2 V elements that
-// are only copied; a head has dim / (2 V) of them. A thread takes one unit index of one token and
-// walks over the token's heads (queries, keys, values), `groups` threads sharing a unit index, so
-// that the sines and cosines of its V pairs are computed once per thread. The angle is the
-// fractional part of position * turns, formed in fp64 (fp32 would lose 2^-24 * position turns:
-// 0.4 rad at a position of a million), then sincospif in fp32.
+// A unit is two chunks of V consecutive elements of a head, chosen so that neighbouring threads' chunks
+// are neighbours: the (a, b) of V rotated pairs, or chunks that are rotated within themselves
+// (interleaved pairs) or only copied; a head has dim / (2 V) of them. A thread takes one unit index of one
+// token and walks over the token's heads (queries, keys, values), `groups` threads sharing a unit
+// index, so that the sines and cosines of its V pairs are computed once per thread. The angle is
+// the fractional part of position * turns, formed in fp64 (fp32 would lose 2^-24 * position turns:
+// 0.4 rad at a position of a million), then sincospif in fp32. Bound by the memory in a prompt;
+// loading four heads at a time was slower (117 against 88 us at 16 thousand tokens of 48 heads), as it
+// halved the threads an SM holds.
+constexpr int BLOCKS = 4;  // of 256 threads per SM (64 registers a thread): 80 us at 16 thousand tokens; 88, 86, 90 with 3, 5, 6
+
 template <class TI, class TC, int V>
-__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, BLOCKS) k_paged_append(const __grid_constant__ AppendParams p) {
     tc::pdl_trigger();
     tc::pdl_wait();
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -67,50 +72,60 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
         }
         if (why && p.status && u == 0 && g == 0) atomicOr(p.status, why);
     }
-    const bool turned = u * 2 * V < p.rot;
-    const bool halves = turned && !p.interleaved;
-    const int ca = halves ? u * V : u * 2 * V;
-    const int cb = halves ? p.rot / 2 + u * V : ca + V;
-    const bool turn = turned && pos >= 0;
+    // the unit's chunks in queries and keys (values: those of plain copies), and whether each is rotated
+    const int va = V == 1 ? 2 * u : u * V, vb = V == 1 ? va + 1 : va + p.dim / 2;
+    int ca = va, cb = vb;
+    if (!p.interleaved && p.rot) {
+        const int w = u - p.rot / (2 * V);  // units after the rotated pairs
+        ca = w < 0 ? u * V : p.rot + w * V;
+        cb = w < 0 ? ca + p.rot / 2 : ca + (p.dim - p.rot) / 2;
+    }
+    const bool turn_a = pos >= 0 && ca < p.rot, turn_b = pos >= 0 && cb < p.rot;
     float cs[V], sn[V];
-    if (turn) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            double t = (double)pos * p.turns[u * V + e];
+    for (int e = 0; e < V; ++e) {
+        // pair of element e: of (a[e], b[e]), or with interleaved pairs of a's V / 2 pairs, then b's
+        const int pair = !p.interleaved || V == 1 ? u * V + e : e < V / 2 ? ca / 2 + e : cb / 2 + e - V / 2;
+        const bool on = !p.interleaved || V == 1 || e < V / 2 ? turn_a : turn_b;
+        cs[e] = 1.f;
+        sn[e] = 0.f;
+        if (on) {
+            double t = (double)pos * p.turns[pair];
             t -= rint(t);
             sincospif((float)(2.0 * t), &sn[e], &cs[e]);
         }
     }
     const int heads = p.n_q + 2 * p.n_kv;
     for (int h = g; h < heads; h += p.groups) {
-        const bool is_q = h < p.n_q;
-        const bool is_v = h >= p.n_q + p.n_kv;
+        const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
         if (!is_q && at < 0) continue;
         const int hk = is_q ? h : is_v ? h - p.n_q - p.n_kv : h - p.n_q;
         const TI* src = is_q ? static_cast<const TI*>(p.q) + ti * p.q_ts + hk * p.q_hs
                              : is_v ? static_cast<const TI*>(p.v) + ti * p.v_ts + hk * p.v_hs
                                     : static_cast<const TI*>(p.k) + ti * p.k_ts + hk * p.k_hs;
-        const int oa = is_v ? u * 2 * V : ca, ob = is_v ? oa + V : cb;
+        const int oa = is_v ? va : ca, ob = is_v ? vb : cb;
         float a[V], b[V];
         load_vec<TI, V>(src + oa, a);
         load_vec<TI, V>(src + ob, b);
-        if (turn && !is_v) {
-            if (halves || V == 1) {
+        if (!is_v && (turn_a || turn_b)) {
+            if (!p.interleaved || V == 1) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float x = a[e], y = b[e];
                     a[e] = x * cs[e] - y * sn[e];
                     b[e] = y * cs[e] + x * sn[e];
                 }
-            } else {  // pairs (2i, 2i + 1): the first V / 2 in a, the rest in b
+            } else {
 #pragma unroll
                 for (int e = 0; e + 1 < V; e += 2) {
                     float x = a[e], y = a[e + 1];
                     a[e] = x * cs[e / 2] - y * sn[e / 2];
                     a[e + 1] = y * cs[e / 2] + x * sn[e / 2];
-                    x = b[e], y = b[e + 1];
-                    b[e] = x * cs[V / 2 + e / 2] - y * sn[V / 2 + e / 2];
-                    b[e + 1] = y * cs[V / 2 + e / 2] + x * sn[V / 2 + e / 2];
+                    if (turn_b) {
+                        x = b[e], y = b[e + 1];
+                        b[e] = x * cs[V / 2 + e / 2] - y * sn[V / 2 + e / 2];
+                        b[e + 1] = y * cs[V / 2 + e / 2] + x * sn[V / 2 + e / 2];
+                    }
                 }
             }
         }

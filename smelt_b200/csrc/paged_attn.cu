@@ -64,10 +64,11 @@ struct Cfg {
     static constexpr int STAGE = 2 * TK * ROWB;
     static constexpr int HS = HD + 4;  // floats of a partial result's row
     // 16-bit pieces of the query and of the weights. Queries of the cache's type are exact in one;
-    // fp32 ones take two fp16 (22 bits) or three bf16 (24 bits). Weights take as many, and two where
+    // fp32 ones take three (24 bits: two fp16 pieces left scores of 10 off by 1e-6, and the output with
+    // them). Weights take two pieces of fp16 (22 bits) and three of bf16 for fp32 outputs, and two where
     // the output has 16 bits: one piece would add an error as large as the output's own rounding.
-    static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : HALF ? 2 : 3;
-    static constexpr int sp() { return SQ == 1 ? 2 : SQ; }
+    static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : 3;
+    static constexpr int sp() { return SQ == 1 || HALF ? 2 : 3; }
     static constexpr int MT = TK / 16, NT = HB / 8, KD = HD / 16;
     static __device__ constexpr int acc() { return MT * NT == 1 ? 2 : 1; }  // independent sums of a score tile
     // fp16 weights are held times 2^10, so that small ones stay normal numbers
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                         [[maybe_unused]] float down = 1.f, up = 1.f;  // of the queries, and back
                         if constexpr (C::SQ > 1 && C::HALF) {
                             // fp16 pieces of an fp32 query: scaled by a power of two so that the
-                            // head's largest element lies in [1, 2), undone on the scores
+                            // head's largest element lies in [2^10, 2^11), undone on the scores
                             float top = 0.f;
 #pragma unroll
                             for (int k = 0; k < HD / 8; ++k)
@@ -473,9 +474,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                             int e = (int)(__float_as_uint(top) >> 23);  // biased exponent
-                            e = e == 0 || e == 255 ? 127 : min(max(e, 2), 252);
-                            down = __uint_as_float((uint32_t)(254 - e) << 23);
-                            up = __uint_as_float((uint32_t)e << 23);
+                            e = e == 0 || e == 255 ? 127 : min(max(e, 12), 252);
+                            down = __uint_as_float((uint32_t)(264 - e) << 23);
+                            up = __uint_as_float((uint32_t)(e - 10) << 23);
                         }
 #pragma unroll
                         for (int k = 0; k < C::KD; ++k)
