@@ -191,16 +191,6 @@ __device__ __forceinline__ void write4(const PagedAttn& p, int row, int head, in
         store_vec<__half, 4>(p.hl.lo + at, lo);
     }
 }
-template <class TI>
-__device__ __forceinline__ void write1(const PagedAttn& p, int row, int head, int d, float r) {
-    if (p.out) static_cast<TI*>(p.out)[row * p.o_ts + head * p.o_hs + d] = from_f<TI>(r);
-    if (p.hl.hi) {
-        const long long at = (long long)row * p.hl.ld + head * p.dim + d;
-        const __half h = __float2half_rn(r);
-        p.hl.hi[at] = h;
-        p.hl.lo[at] = __float2half_rn(r - __half2float(h));
-    }
-}
 // l of a row whose keys all have weight 0 is 0: its result is 0 and its logarithm -inf
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
@@ -749,33 +739,42 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     __syncwarp();
                 }
                 if constexpr (!C::F32) {
+                    // a lane has dims lane / 4 + {0, 8, 16, ...} of heads 2 (lane % 4) + {0, 1}; the addresses
+                    // are one base per head and constants, as this code runs too rarely to stay in the
+                    // instruction cache (a flush took 5 us with an address computed per element)
+                    const int d0 = lane >> 2;
 #pragma unroll
                     for (int y = 0; y < NT; ++y)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             const int h = y * 8 + (lane & 3) * 2 + c, k = 2 * y + c;
-                            if (h < nh) {
-                                const float f = whole ? inverse(l[k]) * C::UNSHIFT : C::UNSHIFT;
+                            if (h >= nh) continue;
+                            if (!whole) {
+                                float* at = dst + h * C::HS + d0;  // dims past the head's own are 0, and not read
 #pragma unroll
-                                for (int d = 0; d < C::KD; ++d)
-#pragma unroll
-                                    for (int z = 0; z < 2; ++z) {
-                                        const int at = d * 16 + z * 8 + (lane >> 2);
-                                        const float v = O[d][y][2 * z + c] * f;
-                                        if (at < p.dim) {
-                                            if (whole)
-                                                write1<TI>(p, w.row, head0 + h, at, v);
-                                            else
-                                                dst[h * C::HS + at] = v;
-                                        }
-                                    }
-                                if (lane < 4) {
-                                    if (!whole)
-                                        pm[ps][h] = m[k], pl[ps][h] = l[k];
-                                    else if (p.lse)
-                                        p.lse[(long long)w.row * p.n_heads + head0 + h] = log_sum(m[k], l[k]);
-                                }
+                                for (int d = 0; d < 2 * C::KD; ++d) at[d * 8] = O[d / 2][y][2 * (d & 1) + c] * C::UNSHIFT;
+                                if (lane < 4) pm[ps][h] = m[k], pl[ps][h] = l[k];
+                                continue;
                             }
+                            const float f = inverse(l[k]) * C::UNSHIFT;
+                            if (p.out) {
+                                TI* at = static_cast<TI*>(p.out) + w.row * p.o_ts + (head0 + h) * p.o_hs + d0;
+#pragma unroll
+                                for (int d = 0; d < 2 * C::KD; ++d)
+                                    if (d * 8 < p.dim) at[d * 8] = from_f<TI>(O[d / 2][y][2 * (d & 1) + c] * f);
+                            }
+                            if (std::is_same<TI, float>::value && p.hl.hi) {
+                                const long long o = (long long)w.row * p.hl.ld + (head0 + h) * p.dim + d0;
+#pragma unroll
+                                for (int d = 0; d < 2 * C::KD; ++d)
+                                    if (d * 8 < p.dim) {
+                                        const float v = O[d / 2][y][2 * (d & 1) + c] * f;
+                                        const __half hi = __float2half_rn(v);
+                                        p.hl.hi[o + d * 8] = hi;
+                                        p.hl.lo[o + d * 8] = __float2half_rn(v - __half2float(hi));
+                                    }
+                            }
+                            if (p.lse && lane < 4) p.lse[(long long)w.row * p.n_heads + head0 + h] = log_sum(m[k], l[k]);
                         }
                 } else {
 #pragma unroll
