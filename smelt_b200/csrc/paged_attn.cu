@@ -70,7 +70,9 @@ struct Cfg {
     static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : 3;
     static constexpr int sp() { return SQ == 1 || HALF ? 2 : 3; }
     static constexpr int MT = TK / 16, NT = HB / 8, KD = HD / 16;
-    static __device__ constexpr int acc() { return MT * NT == 1 ? 2 : 1; }  // independent sums of a score tile
+    // independent sums of a score tile: of even and odd steps where there is no other work to overlap
+    // with, and for fp32 queries the lower pieces' apart, as the tensor cores round a running sum down
+    static __device__ constexpr int acc() { return SQ > 1 ? 3 : MT * NT == 1 ? 2 : 1; }
     // fp16 weights are held times 2^10, so that small ones stay normal numbers
     static constexpr float shift() { return HALF ? 10.f : 0.f; }
     // rows whose queries are staged per warp: of the two tiles on their way and, where they are not held in
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
 #pragma unroll
                     for (int y = 0; y < NT; ++y)
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) S[x][y][0][z] = S[x][y][C::acc() - 1][z] = 0.f;
+                        for (int z = 0; z < 4; ++z) S[x][y][0][z] = S[x][y][C::acc() / 2][z] = S[x][y][C::acc() - 1][z] = 0.f;
 #pragma unroll
                 for (int k = 0; k < C::KD; ++k) {
 #pragma unroll
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
 #pragma unroll
                         for (int y = 0; y < NT; ++y)
 #pragma unroll
-                            for (int t = 0; t < C::SQ; ++t) mma16816<TC>(S[x][y][k & (C::acc() - 1)], af, qf[t][y][k][0], qf[t][y][k][1]);
+                            for (int t = 0; t < C::SQ; ++t) mma16816<TC>(S[x][y][t ? 2 : C::acc() > 1 ? k & 1 : 0], af, qf[t][y][k][0], qf[t][y][k][1]);
                     }
                 }
             } else {
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                             const int r = x * 16 + (lane >> 2) + (z >> 1) * 8;
                             if (r < klo || r >= khi) {
 #pragma unroll
-                                for (int y = 0; y < NT; ++y) S[x][y][0][z] = -INFINITY, S[x][y][C::acc() - 1][z] = -INFINITY;
+                                for (int y = 0; y < NT; ++y) S[x][y][0][z] = S[x][y][C::acc() / 2][z] = S[x][y][C::acc() - 1][z] = -INFINITY;
                             }
                         }
                 }
@@ -583,7 +585,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                         for (int x = 0; x < MT; ++x)
 #pragma unroll
                             for (int z = c; z < 4; z += 2) {
-                                if (C::acc() == 2) S[x][y][0][z] += S[x][y][C::acc() - 1][z];
+                                if (C::acc() == 3) S[x][y][1][z] += S[x][y][2][z];
+                                if (C::acc() > 1) S[x][y][0][z] += S[x][y][1][z];
                                 mx = fmaxf(mx, S[x][y][0][z]);
                             }
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));

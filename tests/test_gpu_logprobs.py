@@ -98,6 +98,16 @@ def test_ties_and_orders(vocab, shape):
     check(x.to(torch.bfloat16), t, 20)
 
 
+@pytest.mark.parametrize("rows,top", [(600, 20), (600, 64), (1, 20)])
+def test_alternatives_crowded_into_few_threads(rows, top):
+    """The likeliest tokens all lie in the same few strided vectors, thousands of them above the best of the rest."""
+    vocab = 50256
+    lane = (torch.arange(vocab, device="cuda") // 4) % 128
+    g = torch.Generator(device="cuda").manual_seed(14)
+    x = torch.empty(rows, vocab, device="cuda").normal_(0, 0.1, generator=g) - lane
+    check(x, torch.zeros(rows, dtype=torch.int64, device="cuda"), top)
+
+
 def test_signed_zeros_tie():
     x = torch.full((1, 3000), -1.0, device="cuda")
     x[0, 5], x[0, 2000] = -0.0, 0.0
