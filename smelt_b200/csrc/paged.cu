@@ -82,15 +82,13 @@ __global__ void __launch_bounds__(256, BLOCKS) k_paged_append(const __grid_const
     }
     const bool turn_a = pos >= 0 && ca < p.rot, turn_b = pos >= 0 && cb < p.rot;
     float cs[V], sn[V];
+    if (turn_a) {  // turn_b only where turn_a
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        // pair of element e: of (a[e], b[e]), or with interleaved pairs of a's V / 2 pairs, then b's
-        const int pair = !p.interleaved || V == 1 ? u * V + e : e < V / 2 ? ca / 2 + e : cb / 2 + e - V / 2;
-        const bool on = !p.interleaved || V == 1 || e < V / 2 ? turn_a : turn_b;
-        cs[e] = 1.f;
-        sn[e] = 0.f;
-        if (on) {
-            double t = (double)pos * p.turns[pair];
+        for (int e = 0; e < V; ++e) {
+            // pair of element e: of (a[e], b[e]), or with interleaved pairs of a's V / 2 pairs, then b's
+            const bool own = !p.interleaved || V == 1 || e < V / 2;
+            const int pair = !p.interleaved || V == 1 ? u * V + e : own ? ca / 2 + e : cb / 2 + e - V / 2;
+            double t = own || turn_b ? (double)pos * p.turns[pair] : 0.0;
             t -= rint(t);
             sincospif((float)(2.0 * t), &sn[e], &cs[e]);
         }
@@ -107,7 +105,7 @@ __global__ void __launch_bounds__(256, BLOCKS) k_paged_append(const __grid_const
         float a[V], b[V];
         load_vec<TI, V>(src + oa, a);
         load_vec<TI, V>(src + ob, b);
-        if (!is_v && (turn_a || turn_b)) {
+        if (!is_v && turn_a) {
             if (!p.interleaved || V == 1) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
@@ -172,7 +170,7 @@ int check_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, 
         return refuse(why, "cache stride past 64 GB");
     if (!aligned16(kv->k, kv->page_stride, kv->head_stride, sz) || !aligned16(kv->v, kv->token_stride, 0, sz))
         return refuse(why, "the cache's addresses and strides must be multiples of 16 bytes");
-    if (!t || !t->ids || t->n_rows < 0 || t->width < 1 || t->ld < t->width)
+    if (!t || (!t->ids && t->n_rows > 0) || t->n_rows < 0 || t->width < 1 || t->ld < t->width)
         return refuse(why, "null page table, or bad n_rows / width / ld");
     return GPT2Q_OK;
 }

@@ -13,6 +13,7 @@ import numpy as np
 import pytest
 import torch
 
+from smelt_b200._ffi import Gpt2qError
 from smelt_b200.paged import STATUS_PAGE, STATUS_POSITION, STATUS_ROW, PagedKV, Rotary
 
 pytestmark = pytest.mark.gpu
@@ -88,6 +89,8 @@ APPEND = [  # io, cache, heads, kv, dim, rot, interleaved, page, layout
     ("f32", "f16", 0, 12, 64, 0, False, 64, "hnd"),
     ("f32", "f32", 5, 5, 80, 80, False, 1, "nhd"),
     ("f32", "bf16", 4, 1, 256, 64, True, 24, "hnd"),
+    ("bf16", "bf16", 4, 2, 128, 64, False, 16, "hnd"),
+    ("f32", "f16", 2, 2, 96, 32, False, 8, "nhd"),
     ("bf16", "bf16", 3, 1, 8, 6, False, 5, "hnd"),      # element by element: the dims are no multiples of 16
     ("f16", "f16", 2, 2, 24, 24, True, 3, "nhd"),
 ]
@@ -370,6 +373,54 @@ def test_attend_offsets_past_32_bits():
     kv.append(k, v, use, torch.arange(100, dtype=torch.int32, device="cuda"), seq=torch.zeros(100, dtype=torch.int32, device="cuda"))
     assert torch.equal(k_pool[1099, 0, 5], k[69, 0]) and torch.equal(v_pool[1024, 0, 3], v[99, 0])
     check_attend(randn(g, 1, 4, dim, kind="f16"), k_pool, v_pool, use, lens)
+
+
+def test_calls_without_tokens_or_rows():
+    g = gen(19)
+    k_pool, v_pool = pools(g, 2, 2, 16, 64, "bf16")
+    kv = PagedKV(k_pool, v_pool)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    for table in (torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.empty(0, 3, dtype=torch.int32, device="cuda")):
+        z = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+        assert kv.append(z, z, table, none, q=torch.empty(0, 8, 64, dtype=torch.bfloat16, device="cuda")).shape == (0, 8, 64)
+    assert kv.attend(torch.empty(0, 8, 64, dtype=torch.bfloat16, device="cuda"), table, none).shape == (0, 8, 64)
+
+
+def test_python_refusals_on_the_device():
+    g = gen(20)
+    k_pool, v_pool = pools(g, 2, 2, 16, 64, "bf16")
+    kv = PagedKV(k_pool, v_pool)
+    table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    lens = torch.ones(3, dtype=torch.int32, device="cuda")
+    q = randn(g, 3, 8, 64, kind="bf16")
+    k = randn(g, 3, 2, 64, kind="bf16")
+    bad = [
+        lambda: kv.attend(q.half(), table, lens),                       # neither the cache's type nor fp32
+        lambda: kv.attend(q[:, :, :32], table, lens),
+        lambda: kv.attend(q.transpose(0, 1).contiguous().transpose(0, 1)[:2], table, lens),
+        lambda: kv.attend(q, table[:2], lens),
+        lambda: kv.attend(q, table.long(), lens),
+        lambda: kv.attend(q, table, lens.long()),
+        lambda: kv.attend(q, table, lens.cpu()),
+        lambda: kv.attend(q, table, lens, out=q.float()),
+        lambda: kv.attend(q, table, lens, lse=torch.empty(3, 8, dtype=torch.float64, device="cuda")),
+        lambda: kv.append(k, k[:2], table, lens),
+        lambda: kv.append(k, k, table, lens[:2]),
+        lambda: kv.append(k, k, table, lens, q_out=q),
+        lambda: kv.append(k, k, table, lens, status=lens),
+        lambda: PagedKV(k_pool, v_pool.float()),
+        lambda: PagedKV(k_pool, v_pool.transpose(1, 2).contiguous().transpose(1, 2)),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(Gpt2qError, match="n_heads"):
+        kv.attend(q[:, :7], table, lens)
+    with pytest.raises(Gpt2qError, match="window"):
+        kv.attend(q, table, lens, window=-1)
+    with pytest.raises(Gpt2qError, match="16 bytes"):
+        kv.attend(torch.zeros(3 * 8 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(3, 8, 64), table, lens)
+    assert kv.attend(q, table, lens).shape == q.shape
 
 
 def test_attend_strided_inputs_outputs_and_table():
