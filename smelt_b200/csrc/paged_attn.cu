@@ -234,12 +234,14 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 tc::prefetch_tmap(&vmap);
             }
         }
-    } else if (nch < C::CHP) {
-        // dims past the head's own are zero in the ring and are never written again (TMA fills them)
-        for (int r = lane; r < STAGES * 2 * TK; r += 32)
-            for (int c = nch; c < C::CHP; ++c)
-                *reinterpret_cast<uint4*>(ring + r / TK * TK * C::ROWB + C::at(r % TK, c)) = make_uint4(0, 0, 0, 0);
     }
+    // dims past the head's own are zero in the ring and are never written again; TMA fills its last piece
+    // of 128 bytes with zeros itself
+    const int c_own = TMA ? p.boxes * 8 : nch;
+    if (c_own < C::CHP)
+        for (int r = lane; r < STAGES * 2 * TK; r += 32)
+            for (int c = c_own; c < C::CHP; ++c)
+                *reinterpret_cast<uint4*>(ring + r / TK * TK * C::ROWB + C::at(r % TK, c)) = make_uint4(0, 0, 0, 0);
     if (nch < C::CHP)
         for (int i = lane; i < C::QS * hv * (qrow / 16); i += 32)
             if (i % (qrow / 16) >= nqch) *reinterpret_cast<uint4*>(qring + i * 16) = make_uint4(0, 0, 0, 0);
@@ -818,6 +820,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     const unsigned mates = __match_any_sync(0xffffffffu, of);
     const unsigned heads = __ballot_sync(0xffffffffu, there && __ffs(mates) - 1 == lane);
     const int chains = __popc(heads);
+    const int rank = heads >> lane & 1 ? __popc(heads & ((1u << lane) - 1)) : -1;  // which chain this lane heads
     int tail_row = -1, tail_vh = 0;
     long long tail_last = 0;
     if (warp == 0 && chains) {
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     }
     for (int u = warp; u < chains * hv; u += nw) {
         const int ch = u / hv, h = u - ch * hv;
-        const int i0 = __fns(heads, 0, ch + 1);
+        const int i0 = __ffs(__ballot_sync(0xffffffffu, rank == ch)) - 1;  // the chain's first piece
         const Piece P = pieces[i0];
         unsigned members = __shfl_sync(0xffffffffu, mates, i0);
         const int kvh = P.vh / p.blocks_per_kv, h0 = (P.vh - kvh * p.blocks_per_kv) * HB;
@@ -900,20 +903,26 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(const __grid_constant__
     tc::pdl_trigger();
     tc::pdl_wait();
     const int c = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * HB + h; };
+    constexpr int DG = HD / 4, PG = 128 / DG;  // threads over dims, and over pieces
+    const int d = tid % DG * 4, g = tid / DG;
+    // In a small grid the first pieces are loaded along with the word that says whether, and how many,
+    // there are (1001 keys, 12 heads: 12.75 to 12.55 us); in a large one most blocks only end here, and the
+    // loads of all would cost more than they save (131071 keys, 64 heads: 94 and 97 us).
     const int4 meta = __ldcg(p.meta + c);
+    if (gridDim.x * gridDim.y > 64 && meta.x < 0) return;
+    const int most = gridDim.x - c;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < most) ml = __ldcg(p.block_ml + at(lane));
+    float4 v0[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (d < p.dim && g + k * PG < most) v0[k] = __ldcg(reinterpret_cast<const float4*>(p.block_part + at(g + k * PG) * HD + d));
     if (meta.x < 0) return;
     const int kvh = meta.y / p.blocks_per_kv, h0 = (meta.y - kvh * p.blocks_per_kv) * HB;
     if (h0 + h >= p.group) return;
     const int n = meta.z - c + 1;
-    auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * HB + h; };
-    constexpr int DG = HD / 4, PG = 128 / DG;  // threads over dims, and over pieces
-    const int d = tid % DG * 4, g = tid / DG;
-    // the first pieces' values are on their way while the weights are computed
-    float4 v0[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (d < p.dim && g + k * PG < n) v0[k] = __ldcg(reinterpret_cast<const float4*>(p.block_part + at(g + k * PG) * HD + d));
-    float2 ml = lane < n ? __ldcg(p.block_ml + at(lane)) : make_float2(-INFINITY, 0.f);
+    if (lane >= n) ml = make_float2(-INFINITY, 0.f);
     float M = ml.x, L = 0.f;
     for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, __ldcg(p.block_ml + at(i)).x);
 #pragma unroll

@@ -280,6 +280,18 @@ def test_attend_head_dims(io, cache, dim):
 
 
 @pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("dim", [136, 160, 192, 80, 40])
+def test_attend_after_a_call_full_of_nan(io, cache, dim):
+    """What an earlier call left in shared memory does not reach the dims that a head does not fill."""
+    g = gen(21)
+    k_pool, v_pool = pools(g, 64, 8, 16, 256, cache, fill=math.nan)
+    table = torch.arange(64, dtype=torch.int32, device="cuda")[None].repeat(16, 1)
+    out = PagedKV(k_pool, v_pool).attend(randn(g, 16, 16, 256, kind=io), table, torch.full((16,), 1024, dtype=torch.int32, device="cuda"))
+    assert bool(torch.isnan(out).all())
+    attend_case(22, [200, 17, 900] * 8, 8, 4, dim, io, cache, 16)
+
+
+@pytest.mark.parametrize("io,cache", TYPES)
 @pytest.mark.parametrize("page", [1, 3, 16, 64, 1000])
 @pytest.mark.parametrize("window", [0, 1, 17, 250])
 def test_attend_pages_and_windows(io, cache, page, window):
