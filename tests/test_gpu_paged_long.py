@@ -162,6 +162,34 @@ def test_the_tolerance_notices_a_tile(case, io, cache):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("io,cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_of_one_sign_do_not_drift(dim, io, cache):
+    """Values of 1 everywhere: the result is 1 whatever the weights. Sums that are rounded to nearest leave a random walk:
+    over n additions to a growing sum, u sqrt(n) / 3 rms, for numerator and denominator; six of them for both, 3 u sqrt(n). A
+    tile's own matrix steps (at most six) round down by 2 u each: 12 u; pieces of a weight and the joins 12 u more."""
+    from smelt_b200.paged import PagedKV
+
+    kv, rows, page, pages = 4, 40, 64, 16
+    keys = 110_000 if cache != "f32" else 30_000
+    g = torch.Generator(device="cuda").manual_seed(6)
+    k = torch.empty(pages, kv, page, dim, dtype=T[cache], device="cuda").normal_(0, 1, generator=g)
+    v = torch.ones_like(k)
+    q = torch.empty(rows, kv, dim, dtype=T[io], device="cuda").normal_(0, 1, generator=g)
+    width = -(-keys // page)
+    table = torch.randint(0, pages, (rows, width), generator=g, device="cuda").to(torch.int32)
+    lens = [keys - 7 * r for r in range(rows)]
+    out = PagedKV(k, v).attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    n = 2 * tiles_per_warp(lens, 0, kv, cache, dim) * (tile_keys(cache, dim) if cache == "f32" else 1)
+    assert n > 500
+    off = float((out.double() - 1).abs().max())
+    lim = (3 * math.sqrt(n) + 24) * U
+    if io != "f32":
+        lim = 0.0  # 1 is a number of the type, and the sums' error is far below half a step beside it
+    assert off <= lim, (off / U, lim / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("io,cache", TYPES)
 def test_values_that_cancel_keep_the_weights_bits(io, cache):
     """The likeliest key has the value 0; two others of almost equal score have 1 and -1, so the result is the small
     difference of their weights and shows how many bits those have. Scores and the largest weight are exact; a weight is within
