@@ -230,6 +230,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
     namespace cg = cooperative_groups;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    // without alternatives nothing else tells a block that the first one of its cluster has started
+    // when it writes into that one's shared memory
+    if (!TOP && p.parts > 1) tc::cluster_arrive_relaxed();
     tc::pdl_trigger();
     tc::pdl_wait();
     const T* x = static_cast<const T*>(p.x) + (long long)r * p.ld;
@@ -371,6 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
         }
     } else {
         __syncthreads();
+        if (p.parts > 1) tc::cluster_wait();
     }
     if (warp == 0) {
         a = join(lane < THREADS / 32 ? sh.warp[lane] : none, c);

@@ -1,0 +1,41 @@
+"""Token log probabilities of a few long rows, each of which a cluster of 2 to 8 blocks shares: the form without
+alternatives against the form with one, and against 64 bits.
+
+Tolerance: test_gpu_logprobs derives it (d = (V / 256 + 64) 2^-24 + 2^-18 for the sums of V terms)."""
+import pytest
+import torch
+
+from smelt_b200.logprobs import token_logprobs
+
+pytestmark = pytest.mark.gpu
+T = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    from smelt_b200 import build
+    build.build()
+
+
+def delta(vocab):
+    return (vocab / 256 + 64) * 2.0 ** -24 + 2.0 ** -18
+
+
+@pytest.mark.parametrize("kind", list(T))
+@pytest.mark.parametrize("vocab", [8193, 50257])
+@pytest.mark.parametrize("rows", [1, 2, 74, 75, 148, 149, 296, 297])
+def test_without_alternatives(kind, vocab, rows):
+    """Calls that follow one another without a pause, so that blocks of the next cluster start while others still run."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.empty(rows, vocab, dtype=T[kind], device="cuda").normal_(0, 2.5, generator=g)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    got = [token_logprobs(x, t) for _ in range(20)]
+    one = token_logprobs(x, t, top=1)
+    for r in got:
+        assert torch.equal(r.lp, one.lp) and torch.equal(r.entropy, one.entropy) and torch.equal(r.stats, one.stats)
+    lp = torch.log_softmax(x.double(), 1)
+    h = torch.special.entr(lp.exp()).sum(1)
+    want = lp.gather(1, t[:, None])[:, 0]
+    d = delta(vocab)
+    assert bool(((one.lp.double() - want).abs() <= 2.0 ** -22 * (want.abs() + 16) + d).all())
+    assert bool(((one.entropy.double() - h).abs() <= 2 * d * (1 + 2 * h)).all())
