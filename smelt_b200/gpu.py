@@ -36,6 +36,13 @@ def _descs(pack: Pack):
     return arr, keep
 
 
+def _page_table(table) -> _ffi.PageTable:
+    """A tensor [rows, pages] as the C structure. One row may have any stride; rows that share storage (an expanded
+    table, overlapping windows) keep theirs, which is below the width and refused by the call."""
+    rows, width = table.shape
+    return _ffi.PageTable(table.data_ptr(), rows, width, table.stride(0) if rows > 1 else max(table.stride(0), width))
+
+
 class Gpu:
     def __init__(self, pack: Pack, device: int = 0, max_seqs: int = 1, max_tokens: int = 0,
                  tp_size: int = 1, tp_rank: int = 0, nccl_id: bytes | None = None):
@@ -245,9 +252,7 @@ class Gpu:
             raise ValueError(f"table must be int32 [rows, pages] on cuda:{self.device}")
         # what torch has queued (the pools, the table) comes before this handle's stream
         torch.cuda.current_stream(self.device).synchronize()
-        rows, width = table.shape
-        return ((_ffi.PagedKV * len(layers))(*(kv.c for kv in layers)),
-                _ffi.PageTable(table.data_ptr(), rows, width, max(table.stride(0), width)))
+        return (_ffi.PagedKV * len(layers))(*(kv.c for kv in layers)), _page_table(table)
 
     def page_out(self, slot: int, n_tokens: int, layers, table, row: int):
         """Copies the first n_tokens cached positions of arena slot `slot` into row `row` of `table` of every

@@ -169,3 +169,19 @@ def test_python_wrappers_refuse_host_tensors(lib):
         Rotary(8, inv_freq=[1.0])
     with pytest.raises(_ffi.Gpt2qError):
         Rotary(7)
+
+
+def test_tables_whose_rows_share_storage(lib):
+    """The handle's page tables keep the tensor's stride, so that the call refuses rows that lie in one another."""
+    from smelt_b200.gpu import _page_table
+
+    t = torch.arange(8, dtype=torch.int32).view(2, 4)
+    for x, ld in ((t, 4), (t[:, :3], 4), (t[:1], 4), (t[1:, 1:], 4), (torch.arange(4, dtype=torch.int32).expand(1, 4), 4)):
+        p = _page_table(x)
+        assert (p.ids, p.n_rows, p.width, p.ld) == (x.data_ptr(), *x.shape, ld)
+    for x in (t[:1].expand(3, -1), t.view(-1).as_strided((3, 4), (2, 1))):
+        p = _page_table(x)
+        assert (p.n_rows, p.width, p.ld) == (3, 4, x.stride(0))
+        p.ids = A  # never read
+        refused(lib, append(lib, t=p), "page table")
+        refused(lib, attend(lib, t=p), "page table")
