@@ -157,7 +157,9 @@ int refuse(std::string* why, const char* msg) {
     return GPT2Q_EARG;
 }
 
-int check_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, std::string* why) {
+}  // namespace
+
+int gpt2q::check_paged_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, std::string* why) {
     if (!kv || !kv->k || !kv->v) return refuse(why, "null cache");
     if (kv->dtype < GPT2Q_F32 || kv->dtype > GPT2Q_BF16) return refuse(why, "unknown cache dtype");
     if (dtype != kv->dtype && dtype != GPT2Q_F32) return refuse(why, "dtype must be the cache's or GPT2Q_F32");
@@ -175,13 +177,11 @@ int check_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, 
     return GPT2Q_OK;
 }
 
-}  // namespace
-
 int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
                         const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads,
                         int n_tokens, const int32_t* d_pos, int pos0, const int32_t* d_seq, const gpt2q_rotary* rot,
                         int32_t* d_status, cudaStream_t st, std::string* why) {
-    const int rc = check_cache(kv, table, dtype, why);
+    const int rc = check_paged_cache(kv, table, dtype, why);
     if (rc) return rc;
     if (n_tokens < 0) return refuse(why, "n_tokens < 0");
     if (n_tokens == 0) return GPT2Q_OK;
@@ -244,7 +244,7 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
                            const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
                            int window, float* d_lse, int32_t* d_status, void* d_work, const HiLo& hl, cudaStream_t st,
                            std::string* why) {
-    const int rc = check_cache(kv, table, dtype, why);
+    const int rc = check_paged_cache(kv, table, dtype, why);
     if (rc) return rc;
     if (table->n_rows == 0) return GPT2Q_OK;
     if (!d_lens || !q || !q->data || !out || (!out->data && !hl.hi)) return refuse(why, "null d_lens, q or out");

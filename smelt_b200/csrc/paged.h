@@ -46,6 +46,9 @@ struct PagedAttn {
 uint64_t paged_attn_workspace(int dim, int group);
 cudaError_t launch_paged_attn(PagedAttn p, int cache_dtype, int dtype, void* work, cudaStream_t st);
 
+// What both calls ask of a cache and a page table; `why` receives the message. Returns a GPT2Q_* code.
+int check_paged_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, int dtype, std::string* why);
+
 // The checks and launches behind gpt2q_paged_append / gpt2q_paged_attention; `why` receives the
 // message of a failed call. Return GPT2Q_* codes. In paged_append a null d_pos means positions
 // pos0, pos0 + 1, ... of table row 0.

@@ -1561,13 +1561,18 @@ int score_positions(gpt2q_handle* H, const uint32_t* ids, int n, int slot, F&& r
     return GPT2Q_OK;
 }
 
-// A paged cache per layer, of this model's heads.
-int check_paged(gpt2q_handle* H, const gpt2q_paged_kv* layers) {
+// A paged cache per layer, of this model's heads, and the table: before anything is launched or a row
+// of the table is taken.
+int check_paged(gpt2q_handle* H, const gpt2q_paged_kv* layers, const gpt2q_page_table* table) {
     if (H->tp_size > 1) return H->fail(GPT2Q_EUNSUP, "a paged cache needs a single-GPU handle");
     if (!layers) return H->fail(GPT2Q_EARG, "null layers");
-    for (int l = 0; l < H->cfg.n_layer; ++l)
+    for (int l = 0; l < H->cfg.n_layer; ++l) {
+        std::string why;
+        const int rc = check_paged_cache(&layers[l], table, GPT2Q_F32, &why);
+        if (rc) return H->fail(rc, "layer " + std::to_string(l) + ": " + why);
         if (layers[l].n_kv_heads != H->H_local || layers[l].head_dim != H->hd)
             return H->fail(GPT2Q_EARG, "layer " + std::to_string(l) + ": the cache must have the model's heads and head dim");
+    }
     return GPT2Q_OK;
 }
 
@@ -1888,7 +1893,7 @@ int gpt2q_page_out(gpt2q_handle* H, int slot, int n_tokens, const gpt2q_paged_kv
     if (n_tokens < 1 || n_tokens > H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "n_tokens out of range [1, n_ctx]");
     if (!table || row < 0 || row >= table->n_rows) return H->fail(GPT2Q_EARG, "null table or row out of range");
     CK(cudaSetDevice(H->device));
-    int rc = check_paged(H, layers);
+    int rc = check_paged(H, layers, table);
     if (!rc) rc = ensure_paged(H, 1);
     if (rc) return rc;
     gpt2q_page_table t = *table;
@@ -1918,7 +1923,7 @@ int gpt2q_decode_paged(gpt2q_handle* H, const uint32_t* tok, const int32_t* pos,
         if (pos[i] < 0 || pos[i] >= H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "pos out of range [0, n_ctx)");
     CK(cudaSetDevice(H->device));
     int rc = check_tokens(H, tok, (size_t)n_seq);
-    if (!rc) rc = check_paged(H, layers);
+    if (!rc) rc = check_paged(H, layers, table);
     if (!rc) rc = ensure_paged(H, n_seq);
     if (!rc) rc = ensure_stage(H, (size_t)3 * n_seq);
     if (rc) return rc;

@@ -1,8 +1,11 @@
 """Page tables that the model's paged calls refuse: before anything is written."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
+from smelt_b200 import _ffi
 from smelt_b200._ffi import Gpt2qError
 from smelt_b200.gpu import Gpu
 from smelt_b200.paged import PagedKV
@@ -46,3 +49,29 @@ def test_rows_that_share_storage_are_refused():
         g.page_out(0, 5, layers, one.expand(3, -1).contiguous(), 2)
         assert not untouched(layers)
         assert g.decode_paged([1], [5], layers, one[:, :4]).shape == (1,)
+
+
+@pytest.mark.parametrize("change", [dict(ids=None), dict(width=0), dict(ld=3), dict(ld=-4)])
+def test_bad_tables_are_refused_whatever_the_row(change):
+    with Gpu(make_pack(TINY, "auto"), max_seqs=2) as g:
+        g.prefill([np.arange(5, dtype=np.uint32)])
+        ids = torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+        layers = caches(8, 16)
+        arr = (_ffi.PagedKV * len(layers))(*(kv.c for kv in layers))
+        t = _ffi.PageTable(**(dict(ids=ids.data_ptr(), n_rows=3, width=4, ld=4) | change))
+        torch.cuda.synchronize()
+        tok, pos = np.arange(3, dtype=np.uint32), np.zeros(3, np.int32)
+        nxt = np.empty(3, np.uint32)
+        for row in (0, 1, 2):
+            with pytest.raises(Gpt2qError, match="page table"):
+                g._check(g._lib.gpt2q_page_out(g.h, 0, 5, arr, C.byref(t), row))
+        with pytest.raises(Gpt2qError, match="page table"):
+            g._check(g._lib.gpt2q_decode_paged(g.h, tok.ctypes.data, pos.ctypes.data, 3, arr, C.byref(t), None, nxt.ctypes.data))
+        # a bad cache in the last layer: the earlier ones are not written either
+        good = _ffi.PageTable(ids.data_ptr(), 3, 4, 4)
+        arr[TINY.n_layer - 1].token_stride += 1
+        with pytest.raises(Gpt2qError, match="16 bytes"):
+            g._check(g._lib.gpt2q_page_out(g.h, 0, 5, arr, C.byref(good), 1))
+        with pytest.raises(Gpt2qError, match="16 bytes"):
+            g._check(g._lib.gpt2q_decode_paged(g.h, tok.ctypes.data, pos.ctypes.data, 3, arr, C.byref(good), None, nxt.ctypes.data))
+        assert untouched(layers)
