@@ -140,6 +140,7 @@ struct gpt2q_handle {
     // the target ids and the per-position f64 terms
     float* nll_logits = nullptr;
     int* nll_tgt = nullptr;
+    std::vector<int> nll_host;  // what nll_tgt is copied from; the callers wait for the stream
     double* nll_terms = nullptr;
     float* score_out = nullptr;  // gpt2q_score: log probabilities, entropies and alternatives of n_ctx positions
     // decode over a caller's paged cache (grown on demand): q|k|v rows, logits, argmax slots, the
@@ -1542,9 +1543,8 @@ int score_positions(gpt2q_handle* H, const uint32_t* ids, int n, int slot, F&& r
     const int32_t slots[1] = {slot};
     rc = prefill_chunk(H, ids, offs, slots, 0, 1, true);
     if (rc) return rc;
-    std::vector<int> tgt(R);
-    for (int p = 0; p < R; ++p) tgt[p] = (int)ids[p + 1];
-    CK(cudaMemcpyAsync(H->nll_tgt, tgt.data(), (size_t)R * 4, cudaMemcpyHostToDevice, H->stream));
+    H->nll_host.assign(ids + 1, ids + n);
+    CK(cudaMemcpyAsync(H->nll_tgt, H->nll_host.data(), (size_t)R * 4, cudaMemcpyHostToDevice, H->stream));
     RUN("layernorm", (double)R * d * 8,
         launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, R,
                          H->stream));
