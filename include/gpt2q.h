@@ -270,7 +270,7 @@ int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float
  * (in elements): the entry of token slot o in page p for kv head h starts at
  * p * page_stride + h * head_stride + o * token_stride and holds head_dim elements. The pools' base
  * addresses and all strides are multiples of 16 bytes; head_dim is a multiple of 8, at most 256.
- * Entries must not overlap. */
+ * Entries must not overlap (an append refuses strides by which they would). */
 typedef struct gpt2q_paged_kv {
     void* k;
     void* v;
@@ -305,7 +305,8 @@ typedef struct gpt2q_rotary {
 /* turns[i] = base^(-2i/dim) / (2 pi). dim even, 2..256; a caller may write other turns afterwards. */
 int gpt2q_rotary_init(gpt2q_rotary* rot, int dim, int interleaved, double base);
 
-/* A device tensor [token][head][head_dim] with unit stride over head_dim; strides in elements. */
+/* A device tensor [token][head][head_dim] with unit stride over head_dim; strides in elements. Tensors
+ * that are written have entries that share no memory (a call refuses others). */
 typedef struct gpt2q_heads {
     void* data;
     int64_t token_stride;

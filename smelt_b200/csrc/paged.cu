@@ -2,7 +2,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <string>
+#include <utility>
 
 #include "device_op.cuh"
 #include "gpt2q.h"
@@ -152,6 +154,20 @@ bool aligned16(const void* p, int64_t a, int64_t b, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
 }
 
+// Whether two of n x m runs of dim elements, starting at i * a + j * b, share an element.
+bool overlap(int64_t n, int64_t a, int64_t m, int64_t b, int64_t dim) {
+    if (n < 1 || m < 1) return false;
+    a = std::abs(a), b = std::abs(b);
+    if (a > b) std::swap(a, b), std::swap(n, m);
+    if ((n > 1 && a < dim) || (m > 1 && b < dim)) return true;
+    if (n == 1 || m == 1 || b >= a * (n - 1) + dim) return false;
+    for (int64_t j = 1; j < m && j * b < a * (n - 1) + dim; ++j) {  // runs that lie between one another
+        const int64_t i = j * b / a;  // the nearest of the a-steps on either side
+        if ((i < n && j * b - i * a < dim) || (i + 1 < n && (i + 1) * a - j * b < dim)) return true;
+    }
+    return false;
+}
+
 int refuse(std::string* why, const char* msg) {
     *why = msg;
     return GPT2Q_EARG;
@@ -225,6 +241,10 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
     p.groups = (int)((heads + walk - 1) / walk);
     const long long blocks = ((((long long)n_tokens * p.groups) << p.unit_shift) + 255) / 256;
     if (heads > INT32_MAX / 2 || blocks > INT32_MAX) return refuse(why, "too many tokens in one call");
+    if (with_q && overlap(n_tokens, p.qo_ts, n_q_heads, p.qo_hs, p.dim)) return refuse(why, "the queries of q_out overlap");
+    if (overlap(p.n_pages, p.c_ps, p.n_kv, p.c_hs, p.dim) || overlap(p.n_pages, p.c_ps, p.page, p.c_ts, p.dim) ||
+        overlap(p.n_kv, p.c_hs, p.page, p.c_ts, p.dim))
+        return refuse(why, "the cache's entries overlap");
     cudaError_t e;
     const unsigned nb = (unsigned)blocks;
     if (kv->dtype == GPT2Q_F32)
@@ -256,6 +276,8 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     if (!aligned16(q->data, q->token_stride, q->head_stride, sz) ||
         !aligned16(out->data, out->token_stride, out->head_stride, sz))
         return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
+    if (out->data && overlap(table->n_rows, out->token_stride, n_heads, out->head_stride, kv->head_dim))
+        return refuse(why, "the results in out overlap");
     PagedAttn p{};
     p.k = kv->k, p.v = kv->v;
     const int csz = size_of(kv->dtype);

@@ -185,3 +185,47 @@ def test_tables_whose_rows_share_storage(lib):
         p.ids = A  # never read
         refused(lib, append(lib, t=p), "page table")
         refused(lib, attend(lib, t=p), "page table")
+
+
+def test_outputs_and_entries_that_overlap(lib):
+    """An expanded or self-overlapping output, and for an append a cache whose entries share memory."""
+    ok = dict(token_stride=256, head_stride=64)
+    for bad in (dict(token_stride=0, head_stride=64), dict(token_stride=256, head_stride=0), dict(token_stride=64, head_stride=64),
+                dict(token_stride=128, head_stride=64), dict(token_stride=56, head_stride=512), dict(token_stride=160, head_stride=320),
+                dict(token_stride=-192, head_stride=64)):
+        refused(lib, attend(lib, q=heads(**ok), o=heads(**bad)), "overlap")
+        refused(lib, append(lib, q=heads(**ok), qo=heads(**bad), nq=4), "overlap")
+    for bad in (dict(page_stride=0), dict(head_stride=0), dict(token_stride=0), dict(token_stride=32), dict(head_stride=512),
+                dict(page_stride=1024)):
+        refused(lib, append(lib, kv=cache(**bad)), "entries overlap")
+
+
+def test_overlap_rule_against_every_element():
+    """The rule, restated, against a count of every element: the library's is the same arithmetic."""
+    import itertools
+    import random
+
+    def rule(n, a, m, b, dim):
+        if n < 1 or m < 1:
+            return False
+        if a > b:
+            a, b, n, m = b, a, m, n
+        if (n > 1 and a < dim) or (m > 1 and b < dim):
+            return True
+        if n == 1 or m == 1 or b >= a * (n - 1) + dim:
+            return False
+        for j in range(1, m):
+            i = j * b // a
+            if (i < n and j * b - i * a < dim) or (i + 1 < n and (i + 1) * a - j * b < dim):
+                return True
+        return False
+
+    rng = random.Random(1)
+    seen = set()
+    for _ in range(4000):
+        n, m, dim = rng.randint(1, 6), rng.randint(1, 6), rng.randint(1, 5)
+        a, b = rng.randint(0, 24), rng.randint(0, 24)
+        at = [i * a + j * b + d for i, j, d in itertools.product(range(n), range(m), range(dim))]
+        assert rule(n, a, m, b, dim) == (len(set(at)) < len(at)), (n, a, m, b, dim)
+        seen.add(rule(n, a, m, b, dim))
+    assert seen == {True, False}

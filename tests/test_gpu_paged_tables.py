@@ -75,3 +75,32 @@ def test_bad_tables_are_refused_whatever_the_row(change):
         with pytest.raises(Gpt2qError, match="16 bytes"):
             g._check(g._lib.gpt2q_decode_paged(g.h, tok.ctypes.data, pos.ctypes.data, 3, arr, C.byref(good), None, nxt.ctypes.data))
         assert untouched(layers)
+
+
+def test_expanded_outputs_are_refused_and_interleaved_ones_are_not():
+    from smelt_b200.paged import Rotary
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v, q = (torch.empty(3, h, 64, dtype=torch.bfloat16, device="cuda").normal_(generator=g) for h in (2, 2, 4))
+    kv = PagedKV(*(torch.empty(8, 2, 16, 64, dtype=torch.bfloat16, device="cuda").normal_(generator=g) for _ in range(2)))
+    table = torch.arange(6, dtype=torch.int32, device="cuda").view(3, 2)
+    pos = torch.tensor([17, 3, 30], dtype=torch.int32, device="cuda")
+    rot = Rotary(64)
+    for bad in (q[:1].expand(3, -1, -1), q[:, :1].expand(-1, 4, -1)):
+        with pytest.raises(Gpt2qError, match="overlap"):
+            kv.attend(q, table, pos, out=bad)
+        with pytest.raises(Gpt2qError, match="overlap"):
+            kv.append(k, v, table, pos, rotary=rot, q=q, q_out=bad)
+    shared = PagedKV(*(x[:, :1].expand(-1, 2, -1, -1) for x in (kv.k, kv.v)))
+    with pytest.raises(Gpt2qError, match="overlap"):
+        shared.append(k, v, table, pos)
+    want = kv.attend(q, table, pos)
+    turned = kv.append(k, v, table, pos, rotary=rot, q=q)
+    # rows every 192 elements, heads every 320: entries lie between one another and share nothing
+    hold = torch.zeros(2 * 192 + 3 * 320 + 64, dtype=torch.bfloat16, device="cuda")
+    woven = hold.as_strided((3, 4, 64), (192, 320, 1))
+    assert torch.equal(kv.append(k, v, table, pos, rotary=rot, q=q, q_out=woven), turned)
+    swapped = torch.zeros(4, 3, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    kv2 = PagedKV(kv.k.clone(), kv.v.clone())
+    assert torch.equal(kv2.attend(q, table, pos, out=swapped), kv2.attend(q, table, pos, out=woven))
+    assert want.shape == q.shape
