@@ -640,8 +640,8 @@ int check(const char* who, const void* x, int dtype, int64_t ld, int n_rows, int
     if (n_rows < 0) return refuse(who, "n_rows < 0");
     if (vocab < 1 || ld < vocab) return refuse(who, "vocab must be >= 1 and ld >= vocab");
     if (dtype < GPT2Q_F32 || dtype > GPT2Q_BF16) return refuse(who, "unknown dtype");
-    if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.f / temperature))
-        return refuse(who, "temperature must be positive and finite");
+    // below about 1e-36 the kernels' factors leave fp32, and 0 times one of them would be NaN
+    if (!(temperature >= 1e-30f) || !std::isfinite(temperature)) return refuse(who, "temperature must be finite and at least 1e-30");
     if (n_rows > 0 && !x) return refuse(who, "null logits");
     if (reinterpret_cast<uintptr_t>(x) % (dtype == GPT2Q_F32 ? 4 : 2)) return refuse(who, "unaligned logits");
     return GPT2Q_OK;

@@ -229,3 +229,10 @@ def test_overlap_rule_against_every_element():
         assert rule(n, a, m, b, dim) == (len(set(at)) < len(at)), (n, a, m, b, dim)
         seen.add(rule(n, a, m, b, dim))
     assert seen == {True, False}
+
+
+def test_temperatures_too_small_to_divide_by(lib):
+    for temp in (1e-45, 3e-39, 4.2e-39, 1e-36, 0.99e-30):
+        refused(lib, logprobs(lib, temp=temp), "temperature")
+        refused(lib, grad(lib, temp=temp), "temperature")
+    assert logprobs(lib, rows=0, temp=1.01e-30) == 0 and grad(lib, rows=0, temp=1.01e-30) == 0

@@ -2,10 +2,12 @@
 alternatives against the form with one, and against 64 bits.
 
 Tolerance: test_gpu_logprobs derives it (d = (V / 256 + 64) 2^-24 + 2^-18 for the sums of V terms)."""
+import math
+
 import pytest
 import torch
 
-from smelt_b200.logprobs import token_logprobs
+from smelt_b200.logprobs import token_logprobs, token_logprobs_grad
 
 pytestmark = pytest.mark.gpu
 T = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
@@ -39,3 +41,17 @@ def test_without_alternatives(kind, vocab, rows):
     d = delta(vocab)
     assert bool(((one.lp.double() - want).abs() <= 2.0 ** -22 * (want.abs() + 16) + d).all())
     assert bool(((one.entropy.double() - h).abs() <= 2 * d * (1 + 2 * h)).all())
+
+
+@pytest.mark.parametrize("temperature", [1.01e-30, 1e-20, 1e30])
+def test_extreme_temperatures(temperature):
+    """Almost 0: all of the probability on the largest logit, nothing else. Very high: all alike."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(2, 300, device="cuda").normal_(0, 3, generator=g)
+    best = x.argmax(1)
+    r = token_logprobs(x, best, top=3, temperature=temperature)
+    assert torch.equal(r.top_ids[:, 0].long(), best)
+    want = 0.0 if temperature < 1 else -math.log(300)
+    assert bool(((r.lp - want).abs() < 1e-5).all()) and bool(((r.entropy + want).abs() < 1e-5).all())
+    d = token_logprobs_grad(x, best, r.stats, torch.ones(2, device="cuda"), torch.ones(2, device="cuda"), temperature=temperature)
+    assert bool(torch.isfinite(d).all())
