@@ -195,7 +195,8 @@ template <int THREADS>
 struct LpShared {
     Sums warp[THREADS / 32];
     Sums part[8];                          // of every block of the cluster (first block)
-    unsigned long long group[THREADS];     // best of every group of threads
+    unsigned long long key[THREADS];       // best of every thread
+    unsigned long long group[128];         // best of every group of threads
     unsigned long long every[128];         // those of the whole cluster
     unsigned long long threshold;
     unsigned long long best[THREADS / 32];
@@ -209,9 +210,9 @@ struct LpSharedSums {  // without alternatives
 };
 
 // One pass over the logits. A cluster of `parts` blocks shares a row (one where there are rows
-// enough), each block a consecutive range of vectors. A thread takes a batch of 32 elements at a
-// time: the batch's largest logit first, so that the running sums are rescaled at most once per
-// batch, then the exponentials.
+// enough); their warps take 32 vectors each in turn, so that every block sees all parts of the row. A
+// thread takes a batch of 32 elements at a time: the batch's largest logit first, so that the running
+// sums are rescaled at most once per batch, then the exponentials.
 //
 // Alternatives need no second pass. Each thread keeps its best logit, the vector that holds it and
 // the best of its other vectors. The k-th best of the bests of 64 or 128 groups of threads is
@@ -237,8 +238,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
     tc::pdl_wait();
     const T* x = static_cast<const T*>(p.x) + (long long)r * p.ld;
     const Row<T> row(x, p.vocab);
-    const int share = (row.vectors + p.parts - 1) / p.parts;
-    const int v0 = share * part, v1 = min(v0 + share, row.vectors);
+    // blocks of 128 threads have a row each, and addresses with a constant stride (1 us of 130 in 4093 rows)
+    const int stride = THREADS == 128 ? THREADS : p.parts * THREADS, v1 = row.vectors;
+    const int v0 = (warp * p.parts + part) * 32 + lane;  // this thread's vectors: v0, v0 + stride, ...
     const float c = p.inv_t * LOG2E;
     long long target = -1;
     float xt = 0.f;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
 
     float m = -INFINITY, second = -INFINITY;
     float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
-    int at = v0 + tid;  // the first vector that holds this thread's best logit
+    int at = v0;  // the first vector that holds this thread's best logit
     // a batch whose vectors all lie inside the row takes no checks of its own
     const int in0 = row.shift ? 1 : 0, in1 = min(v1, (p.vocab + row.shift) / VE);
     const uint4* vec = reinterpret_cast<const uint4*>(x - row.shift);
@@ -264,15 +266,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
             t = fma2(e, make_float2(fmaxf(z.x, -2000.f), fmaxf(z.y, -2000.f)), t);
         }
     };
-    for (int v = v0 + tid; v < v1; v += U * THREADS) {
+    for (int v = v0; v < v1; v += U * stride) {
         uint4 raw[U];
-        const bool inside = v >= in0 && v + (U - 1) * THREADS < in1;
+        const bool inside = v >= in0 && v + (U - 1) * stride < in1;
         if (inside) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = __ldcg(vec + v + u * THREADS);
+            for (int u = 0; u < U; ++u) raw[u] = __ldcg(vec + v + u * stride);
         } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = v + u * THREADS < v1 ? row.load(v + u * THREADS) : nothing<T>();
+            for (int u = 0; u < U; ++u) raw[u] = v + u * stride < v1 ? row.load(v + u * stride) : nothing<T>();
         }
         float bm = m;
 #pragma unroll
@@ -280,8 +282,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
             const float um = largest<T>(raw[u]);
             if constexpr (TOP) {
                 // the first vector counts as the best until a larger one comes
-                if (u > 0 || v != v0 + tid) second = fmaxf(second, fminf(bm, um));
-                if (um > bm) at = v + u * THREADS;
+                if (u > 0 || v != v0) second = fmaxf(second, fminf(bm, um));
+                if (um > bm) at = v + u * stride;
             }
             bm = fmaxf(bm, um);
         }
@@ -299,17 +301,24 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (v + u * THREADS < v1) sums(raw[u], nm, cc);
+                if (v + u * stride < v1) sums(raw[u], nm, cc);
         }
     }
     if constexpr (TOP) {
-        // at most the key of the thread's best element: its value, and its vector's last index
-        const int groups = (p.top <= 20 ? 64 : 128) / p.parts, g = THREADS / groups;
-        unsigned long long key = v0 + tid < v1 ? rank_key(m, row.first(at) + VE - 1) : (unsigned)blockIdx.x * THREADS + tid;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-            if (o < g) key = maxu(key, __shfl_xor_sync(0xffffffffu, key, o));
-        if (tid % g == 0) sh.group[tid / g] = key;
+        // at most the key of the thread's best element: its value, and its vector's last index. Neighbouring
+        // threads are of different groups, and neighbouring warps' vectors of different blocks, so that likely
+        // tokens that lie together count as many: with a range of 6000 allowed ids, 20 alternatives of one row
+        // took 308 us from consecutive threads and ranges (no threshold left of 13000 candidates), 6.0 so
+        unsigned long long key = v0 < v1 ? rank_key(m, row.first(at) + VE - 1) : (unsigned)blockIdx.x * THREADS + tid;
+        const int groups = (p.top <= 20 ? 64 : 128) / p.parts;
+        for (int o = 16; o >= groups; o >>= 1) key = maxu(key, __shfl_xor_sync(0xffffffffu, key, o));
+        sh.key[tid] = key;
+        __syncthreads();
+        if (tid < groups) {
+            // groups below 32 have their warps' keys in the first lanes of each
+            for (int i = tid + max(groups, 32); i < THREADS; i += max(groups, 32)) key = maxu(key, sh.key[i]);
+            sh.group[tid] = key;
+        }
         if (tid == 0) sh.n_cand = 0, sh.threshold = 0;
     }
     const Sums none{-INFINITY, 0.f, 0.f};
@@ -357,19 +366,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __gr
             }
         };
         // the best keys possible: of the best element, and of the other vectors' best
-        const int other = at == v0 + tid ? at + THREADS : v0 + tid;
+        const int other = at == v0 ? at + stride : v0;
         const bool every = other < v1 && second >= least && rank_key(second, max(0, row.first(other))) >= thr;
-        if (!every && v0 + tid < v1 && m >= least && rank_key(m, max(0, row.first(at))) >= thr) take(row.load(at), at);
+        if (!every && v0 < v1 && m >= least && rank_key(m, max(0, row.first(at))) >= thr) take(row.load(at), at);
         for (unsigned todo = __ballot_sync(0xffffffffu, every); todo; todo &= todo - 1) {
             // the warp rereads all vectors of one of its threads, four loads at a time
-            const int v2 = v0 + warp * 32 + __ffs(todo) - 1;
-            for (int v = v2 + lane * THREADS; v < v1; v += 4 * 32 * THREADS) {
+            const int v2 = v0 - lane + __ffs(todo) - 1;
+            for (int v = v2 + lane * stride; v < v1; v += 4 * 32 * stride) {
                 uint4 raw[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) raw[q] = v + q * 32 * THREADS < v1 ? row.load(v + q * 32 * THREADS) : nothing<T>();
+                for (int q = 0; q < 4; ++q) raw[q] = v + q * 32 * stride < v1 ? row.load(v + q * 32 * stride) : nothing<T>();
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (v + q * 32 * THREADS < v1) take(raw[q], v + q * 32 * THREADS);
+                    if (v + q * 32 * stride < v1) take(raw[q], v + q * 32 * stride);
             }
         }
     } else {

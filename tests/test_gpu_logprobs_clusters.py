@@ -55,3 +55,28 @@ def test_extreme_temperatures(temperature):
     assert bool(((r.lp - want).abs() < 1e-5).all()) and bool(((r.entropy + want).abs() < 1e-5).all())
     d = token_logprobs_grad(x, best, r.stats, torch.ones(2, device="cuda"), torch.ones(2, device="cuda"), temperature=temperature)
     assert bool(torch.isfinite(d).all())
+
+
+@pytest.mark.parametrize("kind", list(T))
+@pytest.mark.parametrize("rows", [1, 3, 40, 148, 300, 600])
+@pytest.mark.parametrize("top", [1, 20, 21, 64])
+def test_alternatives_that_lie_together(kind, rows, top):
+    """A contiguous range of the vocabulary is allowed, from a few tokens to thousands, at its beginning, middle or end; and a
+    vocabulary ordered by frequency."""
+    vocab = 50257
+    g = torch.Generator(device="cuda").manual_seed(rows + top)
+    base = torch.empty(rows, vocab, device="cuda").normal_(0, 2.5, generator=g)
+    for low, high in ((0, 6000), (0, 5), (31_000, 33_100), (49_000, vocab), (20_000, 20_500), (7, 9000)):
+        x = torch.full_like(base, -math.inf)
+        x[:, low:high] = base[:, low:high]
+        x = x.to(T[kind])
+        r = token_logprobs(x, top=top)
+        ids = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(r.top_ids.long(), ids), (low, high)
+    x = (base * 0.2 - 6 * torch.log1p(torch.arange(vocab, device="cuda") / 100.0)).to(T[kind])
+    r = token_logprobs(x, top=top)
+    lp = torch.log_softmax(x.double(), 1)
+    ids = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(r.top_ids.long(), ids)
+    want = lp.gather(1, ids)
+    assert bool(((r.top_lp.double() - want).abs() <= 2.0 ** -22 * (want.abs() + 16) + delta(vocab)).all())
