@@ -236,3 +236,18 @@ def test_temperatures_too_small_to_divide_by(lib):
         refused(lib, logprobs(lib, temp=temp), "temperature")
         refused(lib, grad(lib, temp=temp), "temperature")
     assert logprobs(lib, rows=0, temp=1.01e-30) == 0 and grad(lib, rows=0, temp=1.01e-30) == 0
+
+
+def test_a_copied_rotation_is_its_own(lib):
+    """deepcopy (of a model that holds one) and pickling: the address is the copy's, not the original's."""
+    import copy
+    import pickle
+
+    from smelt_b200.paged import Rotary
+
+    r = Rotary(16, 1000.0, interleaved=True)
+    turns = list(r.c.turns)
+    for other in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert other.address == C.addressof(other.c) != r.address
+        assert list(other.c.turns) == turns and (other.c.dim, other.c.interleaved) == (16, 1)
+    assert r.address == C.addressof(r.c)
