@@ -57,12 +57,20 @@ class PagedKV:
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("the pools must share their strides, unit over the head dim")
         self._append, self._attend = ops().append, ops().attend
-        self.k, self.v = k, v
+        self._pools = k, v  # `c` holds their addresses
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.index = k.dtype, k.get_device()
         self.c = _ffi.PagedKV(k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], *(k.shape[i] for i in (0, 2, 1, 3)), 0,
                               k.stride(0), k.stride(1), k.stride(2))
         self.address = C.addressof(self.c)
+
+    @property
+    def k(self):
+        return self._pools[0]
+
+    @property
+    def v(self):
+        return self._pools[1]
 
     def append(self, k, v, table, pos, seq=None, rotary: Rotary | None = None, q=None, q_out=None, status=None):
         """Writes token i's k[i] and v[i] ([tokens, kv heads, head dim]) at position pos[i] of table row

@@ -251,3 +251,14 @@ def test_a_copied_rotation_is_its_own(lib):
         assert other.address == C.addressof(other.c) != r.address
         assert list(other.c.turns) == turns and (other.c.dim, other.c.interleaved) == (16, 1)
     assert r.address == C.addressof(r.c)
+
+
+def test_pools_are_not_replaced(lib):
+    from smelt_b200.paged import PagedKV
+
+    kv = PagedKV.__new__(PagedKV)
+    kv._pools = 1, 2
+    assert (kv.k, kv.v) == (1, 2)
+    for name in ("k", "v"):
+        with pytest.raises(AttributeError):
+            setattr(kv, name, 3)
