@@ -3,7 +3,8 @@
     r = token_logprobs(logits, targets, top=5)       # r.lp, r.entropy, r.top_ids, r.top_lp, r.stats
     dlogits = token_logprobs_grad(logits, targets, r.stats, d_lp, d_entropy)
 
-torch CUDA tensors on the current torch stream; include/gpt2q.h (gpt2q_logprobs) states what masked
+torch CUDA tensors on the current torch stream. Nothing is recorded by autograd, for logits that require a
+gradient either: training code calls token_logprobs_grad. include/gpt2q.h (gpt2q_logprobs) states what masked
 logits, empty rows, ties and negative targets give.
 """
 from __future__ import annotations
