@@ -13,8 +13,8 @@
 //
 // A warp streams its tiles through a ring of two shared-memory stages of its own, so warps never
 // wait for each other while they stream. Where a page is a multiple of 16 keys (8 for the short
-// tiles of an fp32 cache), one lane starts the tile's copies as TMA boxes of up to 16 keys x 128
-// bytes, swizzled; pages are looked up a tile ahead. Other page sizes are gathered key by key
+// tiles of an fp32 cache), one lane starts the tile's copies as TMA boxes of up to 16 keys, swizzled in
+// pieces of 128 bytes (all pieces of a key in one box where they are whole); pages are looked up a tile ahead. Other page sizes are gathered key by key
 // with cp.async. Measured: 64 query heads on 8 kv heads of 128 in bf16 over 131071 keys 92.6 us
 // (5.8 TB/s; four times the keys 353 us, 6.1 TB/s), 63 rows of 17 to 9000 keys 81.5 us (4.5 TB/s), one
 // row of 1001 keys of 12 heads of 64 12.6 us, of which the joins and the first tile are most.
@@ -69,8 +69,11 @@ struct Cfg {
     static constexpr int HS = HD + 4;  // floats of a partial result's row
     // 16-bit pieces of the query and of the weights. Queries of the cache's type are exact in one;
     // fp32 ones take three (24 bits: two fp16 pieces left scores of 10 off by 1e-6, and the output with
-    // them). Weights take two pieces of fp16 (22 bits) and three of bf16 for fp32 outputs, and two where
-    // the output has 16 bits: one piece would add an error as large as the output's own rounding.
+    // them). Weights take two pieces of fp16 (22 bits; the rest is a quarter of ex2's own error), of bf16 three
+    // for fp32 outputs and two where the output has 16 bits: one would add an error as large as the output's own
+    // rounding, two leave 2^-16 of sum w |v|, which only results that cancel below 2^-8 of that show. A third
+    // took 3 to 4 % (63 ragged rows 84.5 to 87.8 us a call, one of 131071 keys 97.1 to 100.0), with the same error
+    // against 64 bits.
     static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : 3;
     static constexpr int sp() { return SQ == 1 || HALF ? 2 : 3; }
     static constexpr int MT = TK / 16, NT = HB / 8, KD = HD / 16;
@@ -190,21 +193,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(h), "r"(page), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp; results under 2^-126 are 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two fp32 operations in one instruction
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
-          "l"(reinterpret_cast<unsigned long long&>(c)));
-    return d;
-}
-
 // Four elements of one head's result to the output and, when wanted, its fp16 hi/lo copies.
 template <class TI>
 __device__ __forceinline__ void write4(const PagedAttn& p, int row, int head, int d, const float* r) {
@@ -944,8 +932,10 @@ __global__ void __launch_bounds__(128) k_paged_attn_join(const __grid_constant__
     constexpr int DG = HD / 4, PG = 128 / DG;  // threads over dims, and over pieces
     const int d = tid % DG * 4, g = tid / DG;
     // In a small grid the first pieces are loaded along with the word that says whether, and how many,
-    // there are (1001 keys, 12 heads: 12.75 to 12.55 us); in a large one most blocks only end here, and the
-    // loads of all would cost more than they save (131071 keys, 64 heads: 94 and 97 us).
+    // there are; in a large one most blocks only end here, and the loads of all would cost more than they
+    // save. One row of bf16, loading early against late: 0.1 to 0.4 us less in grids of 16 to 64 blocks
+    // (3000 keys of 4 heads, 63 x 1: 12.2 and 12.6 us), 0.3 to 0 less in 86 to 176, 0.3 more in 344, and 1.2
+    // to 1.7 more where 148 blocks had a part (20000 keys, 148 x 1: 22.7 and 21.1; x 8: 26.0 and 24.7).
     const int4 meta = __ldcg(p.meta + c);
     if (gridDim.x * gridDim.y > 64 && meta.x < 0) return;
     const int most = gridDim.x - c;
