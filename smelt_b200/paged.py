@@ -35,11 +35,12 @@ class Rotary:
                 raise ValueError(f"inv_freq must have {dim // 2} finite elements")
             for i, x in enumerate(f):
                 self.c.turns[i] = x / (2.0 * math.pi)
+        self.address = C.addressof(self.c)
 
-    @property
-    def address(self) -> int:
-        """Of this object's own structure, also where it is a copy."""
-        return C.addressof(self.c)
+    def __setstate__(self, state):
+        """Of a copy or an unpickled object: the address of its own structure."""
+        self.__dict__.update(state)
+        self.address = C.addressof(self.c)
 
 
 class PagedKV:

@@ -251,6 +251,7 @@ def test_a_copied_rotation_is_its_own(lib):
         assert other.address == C.addressof(other.c) != r.address
         assert list(other.c.turns) == turns and (other.c.dim, other.c.interleaved) == (16, 1)
     assert r.address == C.addressof(r.c)
+    assert copy.copy(r).address == r.address  # shares the structure, and keeps it
 
 
 def test_pools_are_not_replaced(lib):
