@@ -194,7 +194,7 @@ struct LpSharedSums {  // without alternatives
 // thousand cycles a row in a call of 4096 rows, as the row had left L2 by then. Rows that put more
 // than CANDIDATES elements above the threshold take one round of search per alternative.
 // Measured: 4093 rows of 50257 fp32 125 us (6.6 TB/s, the memory's rate), 256 rows of 128000 bf16 with 20
-// alternatives 21.4 us (15 without), one row of 50257 with 5 alternatives 5.8 us.
+// alternatives 21.3 us (15 without), one row of 50257 with 5 alternatives 5.8 us.
 template <class T, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_logprobs(const __grid_constant__ LpParams p) {
     constexpr int VE = Row<T>::VE, U = 32 / VE;  // vectors of a batch
@@ -490,7 +490,7 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int by)
 // cut from two aligned vectors, the second of which the neighbouring lane holds. Only warps at a
 // row's ends check where they are.
 // Measured: 4096 rows of 50257 bf16, input rows padded by 7, 142 us (5.8 TB/s; 130 us where both rows lie alike),
-// 64 rows of fp32 6.8 us.
+// 64 rows of fp32 6.6 us.
 template <class T, bool ENT>
 __global__ void __launch_bounds__(THREADS) k_logprobs_grad(const __grid_constant__ GradParams p) {
     constexpr int VE = Row<T>::VE, U = 4;

@@ -13,11 +13,12 @@
 //
 // A warp streams its tiles through a ring of two shared-memory stages of its own, so warps never
 // wait for each other while they stream. Where a page is a multiple of 16 keys (8 for the short
-// tiles of an fp32 cache), one lane starts the tile's copies as TMA boxes of up to 16 keys, swizzled in
-// pieces of 128 bytes (all pieces of a key in one box where they are whole); pages are looked up a tile ahead. Other page sizes are gathered key by key
-// with cp.async. Measured: 64 query heads on 8 kv heads of 128 in bf16 over 131071 keys 92.6 us
-// (5.8 TB/s; four times the keys 353 us, 6.1 TB/s), 63 rows of 17 to 9000 keys 81.5 us (4.5 TB/s), one
-// row of 1001 keys of 12 heads of 64 12.6 us, of which the joins and the first tile are most.
+// tiles of an fp32 cache), one lane starts the tile's copies as TMA boxes of up to 16 keys, swizzled
+// in pieces of 128 bytes (all pieces of a key in one box where they are whole); pages are looked up
+// a tile ahead. Other page sizes are gathered key by key with cp.async. Measured: 64 query heads on
+// 8 kv heads of 128 in bf16 over 131071 keys 94.0 us (5.7 TB/s; four times the keys 349 us, 6.1
+// TB/s), 63 rows of 17 to 9000 keys 83.1 us (4.5 TB/s), one row of 1001 keys of 12 heads of 64 12.3
+// us, of which the joins and the first tile are most.
 #include <cuda.h>
 
 #include <algorithm>
