@@ -348,7 +348,7 @@ int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
                           int window, float* d_lse, int32_t* d_status, void* d_work, void* stream);
 
 /* Log probabilities of given tokens under softmax(logits / temperature), temperature >= 1e-30, per row of n_rows rows of
- * `vocab` logits (type `dtype`, row stride ld >= vocab elements, any alignment of that type):
+ * `vocab` logits (at most 2^30; type `dtype`, row stride ld >= vocab elements, any alignment of that type):
  *   d_lp[r]       log probability of targets[r] (int32, or int64 when targets_i64 != 0). A negative
  *                 target gives 0, one >= vocab NaN.
  *   d_entropy[r]  -sum p ln p

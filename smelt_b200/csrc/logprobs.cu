@@ -619,6 +619,7 @@ int refuse(const char* who, const char* msg) {
 int check(const char* who, const void* x, int dtype, int64_t ld, int n_rows, int vocab, float temperature) {
     if (n_rows < 0) return refuse(who, "n_rows < 0");
     if (vocab < 1 || ld < vocab) return refuse(who, "vocab must be >= 1 and ld >= vocab");
+    if (vocab > 1 << 30) return refuse(who, "vocab must be at most 2^30");  // the kernels count a row's elements in 32 bits
     if (dtype < GPT2Q_F32 || dtype > GPT2Q_BF16) return refuse(who, "unknown dtype");
     // below about 1e-36 the kernels' factors leave fp32, and 0 times one of them would be NaN
     if (!(temperature >= 1e-30f) || !std::isfinite(temperature)) return refuse(who, "temperature must be finite and at least 1e-30");

@@ -263,3 +263,11 @@ def test_pools_are_not_replaced(lib):
     for name in ("k", "v"):
         with pytest.raises(AttributeError):
             setattr(kv, name, 3)
+
+
+def test_rows_longer_than_the_kernels_count(lib):
+    """Ends of rows near 2^31 elements would pass 32 bits: (vector + 34) * 8 <= vocab was true for them."""
+    for vocab in ((1 << 30) + 1, (1 << 31) - 1):
+        refused(lib, logprobs(lib, vocab=vocab, ld=vocab), "2^30")
+        refused(lib, grad(lib, vocab=vocab, ld=vocab, ldo=vocab), "2^30")
+    assert logprobs(lib, rows=0, vocab=1 << 30, ld=1 << 30) == 0
