@@ -679,6 +679,14 @@ extern "C" int gpt2q_logprobs_grad(const void* d_logits, int dtype, int64_t ld, 
     if (d_lp && !d_targets) return refuse(who, "null targets");
     if (reinterpret_cast<uintptr_t>(d_dlogits) % (dtype == GPT2Q_F32 ? 4 : 2)) return refuse(who, "unaligned dlogits");
     if (d_dlogits == d_logits && ld_out != ld) return refuse(who, "in place ld_out must equal ld");
+    if (d_dlogits != d_logits && ld_out == ld) {
+        // rows of the one that lie over rows of the other; those of both side by side in one buffer do not
+        const int size = dtype == GPT2Q_F32 ? 4 : 2;
+        const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(d_dlogits) - reinterpret_cast<uintptr_t>(d_logits)) / size;
+        const int64_t apart = off < 0 ? -off : off, in_row = apart % ld;
+        if (apart < (n_rows - 1) * ld + vocab && (in_row < vocab || (in_row > ld - vocab && apart / ld < n_rows - 1)))
+            return refuse(who, "dlogits overlap the logits");
+    }
     const GradParams p{d_logits, d_dlogits, ld, ld_out, n_rows, vocab, 1, 1.f / temperature, d_targets, targets_i64 != 0,
                        d_stats, d_lp, d_ent};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -271,3 +271,14 @@ def test_rows_longer_than_the_kernels_count(lib):
         refused(lib, logprobs(lib, vocab=vocab, ld=vocab), "2^30")
         refused(lib, grad(lib, vocab=vocab, ld=vocab, ldo=vocab), "2^30")
     assert logprobs(lib, rows=0, vocab=1 << 30, ld=1 << 30) == 0
+
+
+def test_gradients_over_other_logits(lib):
+    """dlogits in place are the logits themselves; one that starts elsewhere in them is refused, rows side by side are not."""
+    for d in (4, -4, 36, 40, 76, -76, 48):  # rows of 10 floats, every 10 or 12
+        refused(lib, grad(lib, dx=A + d, rows=3), "overlap")
+    for d in (4, -4, 36, 44, 48, 52, -44, 96, 100):
+        refused(lib, grad(lib, dx=A + d, rows=3, ld=12, ldo=12), "overlap")
+    # accepted by the check: nothing of the kind is refused (without a GPU the launch fails, or nothing is launched)
+    for d, ld in ((120, 10), (-120, 10), (40, 20), (-40, 20), (136, 12)):
+        assert grad(lib, dx=A + d, rows=3, ld=ld, ldo=ld) != -1 if not torch.cuda.is_available() else True

@@ -80,3 +80,26 @@ def test_alternatives_that_lie_together(kind, rows, top):
     assert torch.equal(r.top_ids.long(), ids)
     want = lp.gather(1, ids)
     assert bool(((r.top_lp.double() - want).abs() <= 2.0 ** -22 * (want.abs() + 16) + delta(vocab)).all())
+
+
+@pytest.mark.parametrize("kind", list(T))
+def test_gradient_beside_its_logits_in_one_buffer(kind):
+    """Logits and gradient side by side in the rows of one buffer; one shifted over the other is refused."""
+    from smelt_b200._ffi import Gpt2qError
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    buf = torch.empty(9, 2 * 1003, dtype=T[kind], device="cuda").normal_(0, 2, generator=g)
+    x, dx = buf[:, :1003], buf[:, 1003:]
+    t = torch.randint(0, 1003, (9,), generator=g, device="cuda")
+    d = torch.empty(9, device="cuda").normal_(generator=g)
+    r = token_logprobs(x, t)
+    want = token_logprobs_grad(x.contiguous(), t, r.stats, d, d)
+    keep = x.clone()
+    token_logprobs_grad(x, t, r.stats, d, d, out=dx)
+    assert torch.equal(dx, want) and torch.equal(x, keep)
+    for out in (buf[:, 1:1004], buf[:, 1002:2005]):
+        with pytest.raises(Gpt2qError, match="overlap"):
+            token_logprobs_grad(x, t, r.stats, d, d, out=out)
+    with pytest.raises(Gpt2qError, match="overlap"):
+        token_logprobs_grad(x[:8], t[:8], r.stats[:8], d[:8], d[:8], out=x[1:])
+    assert torch.equal(x, keep)
