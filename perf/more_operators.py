@@ -183,9 +183,9 @@ def _randn(g, *shape, kind="f32", scale=1.0):
 def _quantise(x, kind):
     """Codes and scales of entries x [..., dim]: one scale per entry, which takes its largest element to the largest code."""
     top = x.abs().amax(-1)
-    scale = top / TOP[kind]
-    code = x * torch.where(top > 0, TOP[kind] / top, 0.0)[..., None]
-    return (code.round() if kind == "i8" else code).to(TYPES[kind]), scale
+    most = torch.full_like(top, TOP[kind])  # quotients of tensors are rounded once; those of a number and a tensor go by a reciprocal
+    code = x * torch.where(top > 0, most / top, 0.0)[..., None]
+    return (code.round() if kind == "i8" else code).to(TYPES[kind]), top / most
 
 
 def _pool(g, c, pages):
