@@ -265,6 +265,9 @@ int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float
 #define GPT2Q_F32 0
 #define GPT2Q_F16 1
 #define GPT2Q_BF16 2
+/* types of a cache alone: 8-bit codes with one scale per entry (gpt2q_paged_kv8) */
+#define GPT2Q_I8 8   /* int8, -127..127 */
+#define GPT2Q_E4M3 9 /* 8-bit floating point, 4 exponent and 3 mantissa bits, largest 448 */
 
 /* One layer's paged cache. Keys and values lie in two pools of n_pages pages with the same strides
  * (in elements): the entry of token slot o in page p for kv head h starts at
@@ -274,16 +277,34 @@ int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float
 typedef struct gpt2q_paged_kv {
     void* k;
     void* v;
-    int32_t dtype; /* GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16 */
+    int32_t dtype; /* GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16; GPT2Q_I8 or GPT2Q_E4M3 in a gpt2q_paged_kv8 */
     int32_t n_pages;
     int32_t page_size; /* token slots of a page, any number >= 1 */
     int32_t n_kv_heads;
     int32_t head_dim;
-    int32_t reserved; /* 0 */
+    int32_t reserved; /* 0; GPT2Q_SCALED in a gpt2q_paged_kv8 */
     int64_t page_stride;
     int64_t head_stride;
     int64_t token_stride;
 } gpt2q_paged_kv;
+
+/* A paged cache of 8-bit codes: kv.reserved is GPT2Q_SCALED, kv.dtype GPT2Q_I8 or GPT2Q_E4M3, and head_dim a multiple of 16.
+ * An entry (the head_dim codes of one token, kv head and pool) stands for code * scale; its scale is the fp32 number at
+ * page * scale_page_stride + head * scale_head_stride + slot * scale_token_stride (elements, any strides >= 0) of k_scale or
+ * v_scale. Every call that takes a gpt2q_paged_kv takes the address of `kv`; those that take one per layer take an array of
+ * gpt2q_paged_kv8 where the first has 8 bits. q, k, v and outputs of such calls are GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16.
+ * Written entries: scale = top / T and code = round(x * (T / top)), to nearest with ties to even, where top is the entry's
+ * largest magnitude (after the rotation) and T is 127 or 448, all in fp32 (the scale at most what T times it is finite for). An entry whose top is under 2^-100 has scale and
+ * codes 0; one with a NaN or an infinity has codes 0 and scale NaN. */
+#define GPT2Q_SCALED 1
+typedef struct gpt2q_paged_kv8 {
+    gpt2q_paged_kv kv;
+    float* k_scale;
+    float* v_scale;
+    int64_t scale_page_stride;
+    int64_t scale_head_stride;
+    int64_t scale_token_stride;
+} gpt2q_paged_kv8;
 
 /* Rows of page ids: row r's token at position p lies in page table[r * ld + p / page_size], slot
  * p % page_size. Entries past a row's last used page are never read. */
@@ -332,6 +353,21 @@ int gpt2q_paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, 
                        int n_tokens, const int32_t* d_pos, const int32_t* d_seq, const gpt2q_rotary* rot,
                        int32_t* d_status, void* stream);
 
+/* gpt2q_paged_append whose tokens lie at cache positions d_slot[i] (NULL: d_pos[i]), while the rotation is that of position
+ * d_pos[i]: drafted tokens of a tree follow one another in the cache, but are as far from its root as their depth. A token with
+ * d_pos[i] < 0 is padding whatever d_slot[i] is; with d_pos[i] >= 0 a negative d_slot[i] is out of range. */
+int gpt2q_paged_append_at(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                          const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads,
+                          int n_tokens, const int32_t* d_pos, const int32_t* d_slot, const int32_t* d_seq,
+                          const gpt2q_rotary* rot, int32_t* d_status, void* stream);
+
+/* Reads n_tokens entries into k and v ([token][kv head][head_dim], type `dtype`: the cache's or GPT2Q_F32, of an 8-bit cache any
+ * of the three): token i is that of table row d_seq[i] (d_seq NULL: row i) at position d_pos[i]. Each element is rounded once from
+ * the value it stands for. d_pos[i] < 0 gives zeros; a row, position or page out of range gives NaN and sets its bit in
+ * d_status (may be NULL). */
+int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k, const gpt2q_heads* v,
+                     int dtype, int n_tokens, const int32_t* d_pos, const int32_t* d_seq, int32_t* d_status, void* stream);
+
 /* Attention of one new token per table row over that row's cached entries:
  * out[r][h] = sum_j softmax_j(scale * q[r][h] . K[j][h / (n_heads / n_kv_heads)]) V[j], j over the
  * last `window` of the positions 0..d_lens[r]-1 (window 0: all of them). q and out are of type
@@ -346,6 +382,31 @@ uint64_t gpt2q_paged_attention_workspace(const gpt2q_paged_kv* kv, int n_heads);
 int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
                           const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
                           int window, float* d_lse, int32_t* d_status, void* d_work, void* stream);
+
+/* Attention of drafted tokens over a paged cache: row r has the tokens d_first[r] .. d_first[r + 1] - 1 of q and out (d_first:
+ * n_rows + 1 numbers, rising, within 0..n_tokens), which lie in its cache behind a prefix of d_lens[r] tokens, token i of the row
+ * at position d_lens[r] + i. Every token sees the whole prefix, and of the row's drafted tokens those that its mask names: bit j & 31 of
+ * d_mask[t * mask_words + j / 32] says whether token t (of all n_tokens) sees its row's drafted token j; tokens past the words
+ * are not seen. A tree's tokens name their ancestors and themselves. d_mask NULL: a token sees itself and those before it (a
+ * chain, or a chunk of a prompt). A token that sees nothing gives zeros and an lse of -inf. What a token does not see does not
+ * reach it, infinities and NaN included; a drafted token's value with an infinity or NaN gives NaN in those that see it. Tokens that
+ * belong to no row are left as they were. Otherwise as gpt2q_paged_attention: types, alignment, d_lse [n_tokens][n_heads],
+ * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order; for
+ * 16-bit outputs the weights are rounded to 16 bits where the products run on wide tensor-core tiles. A length <= 0 is a prefix of none.
+ * d_work: gpt2q_paged_tree_attention_workspace(kv, n_heads, n_tokens) bytes, 16-byte aligned, of one call at a time. */
+uint64_t gpt2q_paged_tree_attention_workspace(const gpt2q_paged_kv* kv, int n_heads, int n_tokens);
+int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                               const int32_t* d_first, const int32_t* d_mask, int mask_words, const gpt2q_heads* q,
+                               const gpt2q_heads* out, int dtype, int n_heads, int n_tokens, float scale, float* d_lse,
+                               int32_t* d_status, void* d_work, void* stream);
+
+/* Keeps the accepted ones of each row's drafted tokens: d_accept[r * ld + i], i < width, are the row's tokens to keep, in rising
+ * order (a negative one ends the list). Entry d_lens[r] + d_accept[r * ld + i] moves to position d_lens[r] + i, codes and scales as
+ * they are (keys stay rotated by the position they had), and d_new_lens[r] = max(d_lens[r], 0) + the number kept. At a token that does
+ * not rise, or whose page or position is out of range, the row's list ends and the bit is set in d_status (may be NULL;
+ * GPT2Q_STATUS_POSITION, GPT2Q_STATUS_PAGE). Rows must not share the pages that are written. d_new_lens is not d_lens. */
+int gpt2q_paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                       const int32_t* d_accept, int width, int64_t ld, int32_t* d_new_lens, int32_t* d_status, void* stream);
 
 /* Log probabilities of given tokens under softmax(logits / temperature), temperature >= 1e-30, per row of n_rows rows of
  * `vocab` logits (at most 2^30; type `dtype`, row stride ld >= vocab elements, any alignment of that type):
@@ -404,6 +465,21 @@ int gpt2q_page_out(gpt2q_handle* h, int slot, int n_tokens, const gpt2q_paged_kv
  * GPT2Q_EARG after the step has run (the outputs are then not meaningful). */
 int gpt2q_decode_paged(gpt2q_handle* h, const uint32_t* tok, const int32_t* pos, int n_seq, const gpt2q_paged_kv* layers,
                        const gpt2q_page_table* table, float* logits, uint32_t* next_tok);
+
+/* Feeds drafted tokens of n_seq sequences over paged caches (table->n_rows == n_seq): sequence i has tok[first[i]] ..
+ * tok[first[i + 1] - 1] (first[0] = 0; n = first[n_seq] of them in all, at most max(max_seqs, max_tokens)) behind lens[i] cached
+ * tokens. parent[t] is the index of a token's parent among its sequence's earlier drafted tokens, or -1 for one that follows
+ * the cached ones; a token is at its parent's position + 1 and attends over the cached tokens, its ancestors and itself. Keys and
+ * values go to positions lens[i], lens[i] + 1, ... of the row, in the tokens' order. Optional host outputs: logits [n][vocab] and
+ * next_tok [n], the likeliest token after each drafted one. Errors as gpt2q_decode_paged's. */
+int gpt2q_verify_paged(gpt2q_handle* h, const uint32_t* tok, const int32_t* parent, const int32_t* first, const int32_t* lens,
+                       int n_seq, const gpt2q_paged_kv* layers, const gpt2q_page_table* table, float* logits,
+                       uint32_t* next_tok);
+
+/* gpt2q_paged_commit in every layer: accept[i][width] names the drafted tokens of sequence i that stay, rising, ended by a
+ * negative one. lens, accept and new_lens (may be NULL) are host arrays; table->n_rows sequences. */
+int gpt2q_commit_paged(gpt2q_handle* h, const int32_t* lens, const int32_t* accept, int width, int32_t* new_lens,
+                       const gpt2q_paged_kv* layers, const gpt2q_page_table* table);
 
 #ifdef __cplusplus
 }

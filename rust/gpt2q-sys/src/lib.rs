@@ -17,6 +17,9 @@ pub const GPT2Q_NOALLOC_MAX_ROWS: c_int = 1024;
 pub const GPT2Q_F32: c_int = 0;
 pub const GPT2Q_F16: c_int = 1;
 pub const GPT2Q_BF16: c_int = 2;
+pub const GPT2Q_I8: c_int = 8;
+pub const GPT2Q_E4M3: c_int = 9;
+pub const GPT2Q_SCALED: c_int = 1;
 pub const GPT2Q_STATUS_PAGE: c_int = 1;
 pub const GPT2Q_STATUS_POSITION: c_int = 2;
 pub const GPT2Q_STATUS_ROW: c_int = 4;
@@ -69,6 +72,18 @@ pub struct gpt2q_paged_kv {
     pub page_stride: i64,
     pub head_stride: i64,
     pub token_stride: i64,
+}
+
+/// A paged cache of 8-bit codes with a scale per entry; calls take the address of `kv`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct gpt2q_paged_kv8 {
+    pub kv: gpt2q_paged_kv,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub scale_page_stride: i64,
+    pub scale_head_stride: i64,
+    pub scale_token_stride: i64,
 }
 
 /// Rows of page ids on the device.
@@ -158,6 +173,23 @@ extern "C" {
                                  q: *const gpt2q_heads, out: *const gpt2q_heads, dtype: c_int, n_heads: c_int,
                                  scale: f32, window: c_int, d_lse: *mut f32, d_status: *mut i32, d_work: *mut c_void,
                                  stream: *mut c_void) -> c_int;
+    pub fn gpt2q_paged_append_at(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, k: *const gpt2q_heads,
+                                 v: *const gpt2q_heads, q: *const gpt2q_heads, q_out: *const gpt2q_heads, dtype: c_int,
+                                 n_q_heads: c_int, n_tokens: c_int, d_pos: *const i32, d_slot: *const i32,
+                                 d_seq: *const i32, rot: *const gpt2q_rotary, d_status: *mut i32,
+                                 stream: *mut c_void) -> c_int;
+    pub fn gpt2q_paged_read(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, k: *const gpt2q_heads,
+                            v: *const gpt2q_heads, dtype: c_int, n_tokens: c_int, d_pos: *const i32, d_seq: *const i32,
+                            d_status: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn gpt2q_paged_tree_attention_workspace(kv: *const gpt2q_paged_kv, n_heads: c_int, n_tokens: c_int) -> u64;
+    pub fn gpt2q_paged_tree_attention(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, d_lens: *const i32,
+                                      d_first: *const i32, d_mask: *const i32, mask_words: c_int,
+                                      q: *const gpt2q_heads, out: *const gpt2q_heads, dtype: c_int, n_heads: c_int,
+                                      n_tokens: c_int, scale: f32, d_lse: *mut f32, d_status: *mut i32,
+                                      d_work: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn gpt2q_paged_commit(kv: *const gpt2q_paged_kv, table: *const gpt2q_page_table, d_lens: *const i32,
+                              d_accept: *const i32, width: c_int, ld: i64, d_new_lens: *mut i32, d_status: *mut i32,
+                              stream: *mut c_void) -> c_int;
     pub fn gpt2q_logprobs(d_logits: *const c_void, dtype: c_int, ld: i64, n_rows: c_int, vocab: c_int, temperature: f32,
                           d_targets: *const c_void, targets_i64: c_int, top: c_int, d_lp: *mut f32,
                           d_entropy: *mut f32, d_stats: *mut f32, d_top_ids: *mut i32, d_top_lp: *mut f32,
@@ -176,4 +208,10 @@ extern "C" {
     pub fn gpt2q_decode_paged(h: *mut gpt2q_handle, tok: *const u32, pos: *const i32, n_seq: c_int,
                               layers: *const gpt2q_paged_kv, table: *const gpt2q_page_table, logits: *mut f32,
                               next: *mut u32) -> c_int;
+    pub fn gpt2q_verify_paged(h: *mut gpt2q_handle, tok: *const u32, parent: *const i32, first: *const i32,
+                              lens: *const i32, n_seq: c_int, layers: *const gpt2q_paged_kv,
+                              table: *const gpt2q_page_table, logits: *mut f32, next: *mut u32) -> c_int;
+    pub fn gpt2q_commit_paged(h: *mut gpt2q_handle, lens: *const i32, accept: *const i32, width: c_int,
+                              new_lens: *mut i32, layers: *const gpt2q_paged_kv,
+                              table: *const gpt2q_page_table) -> c_int;
 }

@@ -26,8 +26,11 @@ EXPORTS = [
     "gpt2q_trunk_input_grad", "gpt2q_bwd_lin_input_grad", "gpt2q_bwd_ln_backward", "gpt2q_bwd_gelu",
     "gpt2q_bwd_attn_train",
     "gpt2q_rotary_init", "gpt2q_paged_append", "gpt2q_paged_attention", "gpt2q_paged_attention_workspace",
+    "gpt2q_paged_append_at", "gpt2q_paged_read", "gpt2q_paged_tree_attention", "gpt2q_paged_tree_attention_workspace",
+    "gpt2q_paged_commit",
     "gpt2q_logprobs", "gpt2q_logprobs_grad",
     "gpt2q_score", "gpt2q_trunk_score_grad", "gpt2q_page_out", "gpt2q_decode_paged",
+    "gpt2q_verify_paged", "gpt2q_commit_paged",
 ]
 
 
@@ -46,6 +49,14 @@ class PagedKV(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32),
                 ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32),
                 ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+SCALED = 1  # GPT2Q_SCALED
+
+
+class PagedKV8(C.Structure):
+    _fields_ = [("kv", PagedKV), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_page_stride", C.c_int64),
+                ("scale_head_stride", C.c_int64), ("scale_token_stride", C.c_int64)]
 
 
 class PageTable(C.Structure):
@@ -165,6 +176,16 @@ def load(path: str | None = None):
     lib.gpt2q_paged_attention_workspace.restype = C.c_uint64
     lib.gpt2q_paged_attention.argtypes = [vp, vp, vp, vp, vp, ci, ci, C.c_float, ci, vp, vp, vp, vp]
     lib.gpt2q_paged_attention.restype = ci
+    lib.gpt2q_paged_append_at.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp]
+    lib.gpt2q_paged_append_at.restype = ci
+    lib.gpt2q_paged_read.argtypes = [vp, vp, vp, vp, ci, ci, vp, vp, vp, vp]
+    lib.gpt2q_paged_read.restype = ci
+    lib.gpt2q_paged_tree_attention_workspace.argtypes = [vp, ci, ci]
+    lib.gpt2q_paged_tree_attention_workspace.restype = C.c_uint64
+    lib.gpt2q_paged_tree_attention.argtypes = [vp, vp, vp, vp, vp, ci, vp, vp, ci, ci, ci, C.c_float, vp, vp, vp, vp]
+    lib.gpt2q_paged_tree_attention.restype = ci
+    lib.gpt2q_paged_commit.argtypes = [vp, vp, vp, vp, ci, C.c_int64, vp, vp, vp]
+    lib.gpt2q_paged_commit.restype = ci
     lib.gpt2q_logprobs.argtypes = [vp, ci, C.c_int64, ci, ci, C.c_float, vp, ci, ci, vp, vp, vp, vp, vp, vp]
     lib.gpt2q_logprobs.restype = ci
     lib.gpt2q_logprobs_grad.argtypes = [vp, ci, C.c_int64, ci, ci, C.c_float, vp, ci, vp, vp, vp, vp, C.c_int64, vp]
@@ -173,7 +194,10 @@ def load(path: str | None = None):
     lib.gpt2q_trunk_score_grad.argtypes = [_hp, vp, ci, vp, vp, vp, vp, vp, vp, vp]
     lib.gpt2q_page_out.argtypes = [_hp, ci, ci, vp, vp, ci]
     lib.gpt2q_decode_paged.argtypes = [_hp, vp, vp, ci, vp, vp, vp, vp]
-    for fn in (lib.gpt2q_score, lib.gpt2q_trunk_score_grad, lib.gpt2q_page_out, lib.gpt2q_decode_paged):
+    lib.gpt2q_verify_paged.argtypes = [_hp, vp, vp, vp, vp, ci, vp, vp, vp, vp]
+    lib.gpt2q_commit_paged.argtypes = [_hp, vp, vp, ci, vp, vp, vp]
+    for fn in (lib.gpt2q_score, lib.gpt2q_trunk_score_grad, lib.gpt2q_page_out, lib.gpt2q_decode_paged, lib.gpt2q_verify_paged,
+               lib.gpt2q_commit_paged):
         fn.restype = ci
     for fn in (lib.gpt2q_quantize_q8, lib.gpt2q_quantize_q4):
         fn.argtypes = [_f32p, C.c_size_t, C.POINTER(C.c_uint8)]

@@ -1,4 +1,4 @@
-// Paged key/value cache (gpt2q_paged_append, gpt2q_paged_attention): gpt2q.h states the layout.
+// Paged key/value cache (gpt2q_paged_*): checks and the C-ABI; gpt2q.h states the layout.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -17,138 +17,6 @@ void set_global_error(const std::string& msg);  // runtime.cu
 using namespace gpt2q;
 
 namespace {
-
-// ------------------------------------------------------------------ append
-struct AppendParams {
-    const void *k, *v, *q;
-    void* qo;
-    long long k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, qo_ts, qo_hs;  // elements
-    void *kc, *vc;
-    long long c_ps, c_hs, c_ts;
-    int page, n_pages, n_tokens, n_q, n_kv, dim, rot, interleaved;
-    const int *pos, *seq, *table;
-    int pos0, n_rows, width;
-    long long ld;
-    int* status;
-    int unit_shift, groups;  // threads of a token: groups * 2^unit_shift
-    double turns[128];
-};
-
-// A unit is two chunks of V consecutive elements of a head, chosen so that neighbouring threads' chunks
-// are neighbours: the (a, b) of V rotated pairs, or chunks that are rotated within themselves
-// (interleaved pairs) or only copied; a head has dim / (2 V) of them. A thread takes one unit index of one
-// token and walks over the token's heads (queries, keys, values), `groups` threads sharing a unit
-// index, so that the sines and cosines of its V pairs are computed once per thread. The angle is
-// the fractional part of position * turns, formed in fp64 (fp32 would lose 2^-24 * position turns:
-// 0.4 rad at a position of a million), then sincospif in fp32. Bound by the memory in a prompt;
-// loading four heads at a time was slower (117 against 88 us at 16 thousand tokens of 48 heads), as it
-// halved the threads an SM holds.
-constexpr int BLOCKS = 4;  // of 256 threads per SM (64 registers a thread): 80 us at 16 thousand tokens; 88, 86, 90 with 3, 5, 6
-
-template <class TI, class TC, int V>
-__global__ void __launch_bounds__(256, BLOCKS) k_paged_append(const __grid_constant__ AppendParams p) {
-    tc::pdl_trigger();
-    tc::pdl_wait();
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int u = (int)(id & ((1 << p.unit_shift) - 1));
-    const long long rest = id >> p.unit_shift;
-    const int g = (int)(rest % p.groups);
-    const long long ti = rest / p.groups;
-    if (ti >= p.n_tokens || u * 2 * V >= p.dim) return;
-    const int pos = p.pos ? __ldcg(p.pos + ti) : p.pos0 + (int)ti;
-    const int row = p.pos ? (p.seq ? __ldcg(p.seq + ti) : (int)ti) : 0;
-    long long at = -1;  // the token's entry in a pool, before the head
-    int why = 0;
-    if (pos >= 0) {
-        const int pg = pos / p.page;
-        if (row < 0 || row >= p.n_rows) {
-            why = GPT2Q_STATUS_ROW;
-        } else if (pg >= p.width) {
-            why = GPT2Q_STATUS_POSITION;
-        } else {
-            const int id_ = __ldcg(p.table + (long long)row * p.ld + pg);
-            if (id_ < 0 || id_ >= p.n_pages)
-                why = GPT2Q_STATUS_PAGE;
-            else
-                at = (long long)id_ * p.c_ps + (long long)(pos - pg * p.page) * p.c_ts;
-        }
-        if (why && p.status && u == 0 && g == 0) atomicOr(p.status, why);
-    }
-    // the unit's chunks in queries and keys (values: those of plain copies), and whether each is rotated
-    const int va = V == 1 ? 2 * u : u * V, vb = V == 1 ? va + 1 : va + p.dim / 2;
-    int ca = va, cb = vb;
-    if (!p.interleaved && p.rot) {
-        const int w = u - p.rot / (2 * V);  // units after the rotated pairs
-        ca = w < 0 ? u * V : p.rot + w * V;
-        cb = w < 0 ? ca + p.rot / 2 : ca + (p.dim - p.rot) / 2;
-    }
-    const bool turn_a = pos >= 0 && ca < p.rot, turn_b = pos >= 0 && cb < p.rot;
-    float cs[V], sn[V];
-    if (turn_a) {  // turn_b only where turn_a
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            // pair of element e: of (a[e], b[e]), or with interleaved pairs of a's V / 2 pairs, then b's
-            const bool own = !p.interleaved || V == 1 || e < V / 2;
-            const int pair = !p.interleaved || V == 1 ? u * V + e : own ? ca / 2 + e : cb / 2 + e - V / 2;
-            double t = own || turn_b ? (double)pos * p.turns[pair] : 0.0;
-            t -= rint(t);
-            sincospif((float)(2.0 * t), &sn[e], &cs[e]);
-        }
-    }
-    const int heads = p.n_q + 2 * p.n_kv;
-    for (int h = g; h < heads; h += p.groups) {
-        const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
-        if (!is_q && at < 0) continue;
-        const int hk = is_q ? h : is_v ? h - p.n_q - p.n_kv : h - p.n_q;
-        const TI* src = is_q ? static_cast<const TI*>(p.q) + ti * p.q_ts + hk * p.q_hs
-                             : is_v ? static_cast<const TI*>(p.v) + ti * p.v_ts + hk * p.v_hs
-                                    : static_cast<const TI*>(p.k) + ti * p.k_ts + hk * p.k_hs;
-        const int oa = is_v ? va : ca, ob = is_v ? vb : cb;
-        float a[V], b[V];
-        load_vec<TI, V>(src + oa, a);
-        load_vec<TI, V>(src + ob, b);
-        if (!is_v && turn_a) {
-            if (!p.interleaved || V == 1) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float x = a[e], y = b[e];
-                    a[e] = x * cs[e] - y * sn[e];
-                    b[e] = y * cs[e] + x * sn[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e + 1 < V; e += 2) {
-                    float x = a[e], y = a[e + 1];
-                    a[e] = x * cs[e / 2] - y * sn[e / 2];
-                    a[e + 1] = y * cs[e / 2] + x * sn[e / 2];
-                    if (turn_b) {
-                        x = b[e], y = b[e + 1];
-                        b[e] = x * cs[V / 2 + e / 2] - y * sn[V / 2 + e / 2];
-                        b[e + 1] = y * cs[V / 2 + e / 2] + x * sn[V / 2 + e / 2];
-                    }
-                }
-            }
-        }
-        if (is_q) {
-            TI* dst = static_cast<TI*>(p.qo) + ti * p.qo_ts + hk * p.qo_hs;
-            store_vec<TI, V>(dst + oa, a);
-            store_vec<TI, V>(dst + ob, b);
-        } else {
-            TC* dst = static_cast<TC*>(is_v ? p.vc : p.kc) + at + hk * p.c_hs;
-            store_vec<TC, V>(dst + oa, a);
-            store_vec<TC, V>(dst + ob, b);
-        }
-    }
-}
-
-template <class TI, class TC>
-cudaError_t launch_append(const AppendParams& p, bool vec, unsigned blocks, cudaStream_t st) {
-    return vec ? launch_dependent(k_paged_append<TI, TC, 8>, dim3(blocks), dim3(256), 0, st, p)
-               : launch_dependent(k_paged_append<TI, TC, 1>, dim3(blocks), dim3(256), 0, st, p);
-}
-
-// ------------------------------------------------------------------ checks
-int size_of(int dtype) { return dtype == GPT2Q_F32 ? 4 : 2; }
 
 bool aligned16(const void* p, int64_t a, int64_t b, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
@@ -172,22 +40,69 @@ int refuse(std::string* why, const char* msg) {
     *why = msg;
     return GPT2Q_EARG;
 }
+int launched(cudaError_t e, std::string* why) {
+    if (e == cudaSuccess) return GPT2Q_OK;
+    *why = cudaGetErrorString(e);
+    return GPT2Q_ECUDA;
+}
+
+const gpt2q_paged_kv8* scaled(const gpt2q_paged_kv* kv) { return reinterpret_cast<const gpt2q_paged_kv8*>(kv); }
+
+// The cache's part of a call's parameters.
+template <class P>
+void take_cache(P* p, const gpt2q_paged_kv* kv) {
+    p->kc = kv->k, p->vc = kv->v;
+    p->c_ps = kv->page_stride, p->c_hs = kv->head_stride, p->c_ts = kv->token_stride;
+    p->page = kv->page_size, p->n_pages = kv->n_pages, p->n_kv = kv->n_kv_heads, p->dim = kv->head_dim;
+}
+template <class P>
+void take_scales(P* p, const gpt2q_paged_kv* kv) {
+    if (!is_8bit(kv->dtype)) return;
+    const gpt2q_paged_kv8* s = scaled(kv);
+    p->k_scale = s->k_scale, p->v_scale = s->v_scale;
+    p->s_ps = s->scale_page_stride, p->s_hs = s->scale_head_stride, p->s_ts = s->scale_token_stride;
+}
+
+// Whether entries of a cache that is written, or their scales, share memory.
+bool entries_overlap(const gpt2q_paged_kv* kv) {
+    auto any = [&](int64_t ps, int64_t hs, int64_t ts, int64_t dim) {
+        return overlap(kv->n_pages, ps, kv->n_kv_heads, hs, dim) || overlap(kv->n_pages, ps, kv->page_size, ts, dim) ||
+               overlap(kv->n_kv_heads, hs, kv->page_size, ts, dim);
+    };
+    if (any(kv->page_stride, kv->head_stride, kv->token_stride, kv->head_dim)) return true;
+    if (!is_8bit(kv->dtype)) return false;
+    const gpt2q_paged_kv8* s = scaled(kv);
+    return any(s->scale_page_stride, s->scale_head_stride, s->scale_token_stride, 1);
+}
 
 }  // namespace
 
 int gpt2q::check_paged_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t, int dtype, std::string* why) {
     if (!kv || !kv->k || !kv->v) return refuse(why, "null cache");
-    if (kv->dtype < GPT2Q_F32 || kv->dtype > GPT2Q_BF16) return refuse(why, "unknown cache dtype");
-    if (dtype != kv->dtype && dtype != GPT2Q_F32) return refuse(why, "dtype must be the cache's or GPT2Q_F32");
+    const bool eight = is_8bit(kv->dtype);
+    if (!eight && (kv->dtype < GPT2Q_F32 || kv->dtype > GPT2Q_BF16)) return refuse(why, "unknown cache dtype");
+    if (!eight && dtype != kv->dtype && dtype != GPT2Q_F32) return refuse(why, "dtype must be the cache's or GPT2Q_F32");
+    if (eight && (dtype < GPT2Q_F32 || dtype > GPT2Q_BF16))
+        return refuse(why, "dtype must be GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16");
     if (kv->n_pages < 1 || kv->page_size < 1 || kv->n_kv_heads < 1) return refuse(why, "n_pages, page_size and n_kv_heads must be >= 1");
     if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8)
         return refuse(why, "head_dim must be a multiple of 8 in [8, 256]");
+    if (eight && kv->head_dim % 16) return refuse(why, "head_dim of an 8-bit cache must be a multiple of 16");
     if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0) return refuse(why, "negative cache stride");
     const int sz = size_of(kv->dtype);
     if (std::max({kv->page_stride, kv->head_stride, kv->token_stride}) > (int64_t)UINT32_MAX * 16 / sz)
         return refuse(why, "cache stride past 64 GB");
     if (!aligned16(kv->k, kv->page_stride, kv->head_stride, sz) || !aligned16(kv->v, kv->token_stride, 0, sz))
         return refuse(why, "the cache's addresses and strides must be multiples of 16 bytes");
+    if (eight) {
+        if (kv->reserved != GPT2Q_SCALED) return refuse(why, "an 8-bit cache is a gpt2q_paged_kv8, reserved GPT2Q_SCALED");
+        const gpt2q_paged_kv8* s = scaled(kv);
+        if (!s->k_scale || !s->v_scale) return refuse(why, "null scales");
+        if (reinterpret_cast<uintptr_t>(s->k_scale) % 4 || reinterpret_cast<uintptr_t>(s->v_scale) % 4)
+            return refuse(why, "unaligned scales");
+        for (int64_t x : {s->scale_page_stride, s->scale_head_stride, s->scale_token_stride})
+            if (x < 0 || x > (int64_t)UINT32_MAX * 16) return refuse(why, "negative scale stride, or one past 64 G elements");
+    }
     if (!t || (!t->ids && t->n_rows > 0) || t->n_rows < 0 || t->width < 1 || t->ld < t->width)
         return refuse(why, "null page table, or bad n_rows / width / ld");
     return GPT2Q_OK;
@@ -195,8 +110,8 @@ int gpt2q::check_paged_cache(const gpt2q_paged_kv* kv, const gpt2q_page_table* t
 
 int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
                         const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype, int n_q_heads,
-                        int n_tokens, const int32_t* d_pos, int pos0, const int32_t* d_seq, const gpt2q_rotary* rot,
-                        int32_t* d_status, cudaStream_t st, std::string* why) {
+                        int n_tokens, const int32_t* d_pos, int pos0, const int32_t* d_slot, const int32_t* d_seq,
+                        const gpt2q_rotary* rot, int32_t* d_status, cudaStream_t st, std::string* why) {
     const int rc = check_paged_cache(kv, table, dtype, why);
     if (rc) return rc;
     if (n_tokens < 0) return refuse(why, "n_tokens < 0");
@@ -205,7 +120,7 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
     if ((q && q->data) != (q_out && q_out->data)) return refuse(why, "q and q_out come together");
     const bool with_q = q && q->data;
     if (with_q && n_q_heads < 1) return refuse(why, "n_q_heads must be >= 1");
-    if (!d_pos && (d_seq || table->n_rows < 1 || pos0 < 0)) return refuse(why, "null d_pos");
+    if (!d_pos && (d_seq || d_slot || table->n_rows < 1 || pos0 < 0)) return refuse(why, "null d_pos");
     if (d_pos && !d_seq && n_tokens > table->n_rows) return refuse(why, "more tokens than table rows, and no d_seq");
     if (rot && (rot->dim < 2 || rot->dim % 2 || rot->dim > kv->head_dim))
         return refuse(why, "the rotary dim must be even and at most head_dim");
@@ -221,52 +136,54 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
         p.n_q = n_q_heads;
         vec = vec && aligned16(p.q, p.q_ts, p.q_hs, sz) && aligned16(p.qo, p.qo_ts, p.qo_hs, sz);
     }
-    p.kc = kv->k, p.vc = kv->v;
-    p.c_ps = kv->page_stride, p.c_hs = kv->head_stride, p.c_ts = kv->token_stride;
-    p.page = kv->page_size, p.n_pages = kv->n_pages, p.n_tokens = n_tokens, p.n_kv = kv->n_kv_heads, p.dim = kv->head_dim;
-    p.pos = d_pos, p.pos0 = pos0, p.seq = d_seq, p.table = table->ids, p.n_rows = table->n_rows, p.width = table->width;
+    take_cache(&p, kv);
+    take_scales(&p, kv);
+    p.n_tokens = n_tokens;
+    p.pos = d_pos, p.pos0 = pos0, p.slot = d_slot, p.seq = d_seq, p.table = table->ids, p.n_rows = table->n_rows, p.width = table->width;
     p.ld = table->ld, p.status = d_status;
     if (rot) {
         p.rot = rot->dim, p.interleaved = rot->interleaved != 0;
         for (int i = 0; i < rot->dim / 2; ++i) p.turns[i] = rot->turns[i];
     }
-    const int units = kv->head_dim / (vec ? 16 : 2);
-    while ((1 << p.unit_shift) < units) ++p.unit_shift;
-    // heads a thread walks over: one while the call has fewer threads than the GPU holds, so that a
-    // decode step is one round of loads; up to 8 in a large call, where the angles' arithmetic
-    // would otherwise be repeated for every head
-    const long long heads = (long long)p.n_q + 2LL * p.n_kv;
-    const long long threads = ((long long)n_tokens << p.unit_shift) * heads;
-    const long long walk = std::clamp<long long>(threads / (148 * 2048), 1, 8);
-    p.groups = (int)((heads + walk - 1) / walk);
-    const long long blocks = ((((long long)n_tokens * p.groups) << p.unit_shift) + 255) / 256;
-    if (heads > INT32_MAX / 2 || blocks > INT32_MAX) return refuse(why, "too many tokens in one call");
+    if ((long long)p.n_q + 2LL * p.n_kv > INT32_MAX / 2) return refuse(why, "too many heads");
     if (with_q && overlap(n_tokens, p.qo_ts, n_q_heads, p.qo_hs, p.dim)) return refuse(why, "the queries of q_out overlap");
-    if (overlap(p.n_pages, p.c_ps, p.n_kv, p.c_hs, p.dim) || overlap(p.n_pages, p.c_ps, p.page, p.c_ts, p.dim) ||
-        overlap(p.n_kv, p.c_hs, p.page, p.c_ts, p.dim))
-        return refuse(why, "the cache's entries overlap");
-    cudaError_t e;
-    const unsigned nb = (unsigned)blocks;
-    if (kv->dtype == GPT2Q_F32)
-        e = launch_append<float, float>(p, vec, nb, st);
-    else if (kv->dtype == GPT2Q_F16)
-        e = dtype == GPT2Q_F32 ? launch_append<float, __half>(p, vec, nb, st) : launch_append<__half, __half>(p, vec, nb, st);
-    else
-        e = dtype == GPT2Q_F32 ? launch_append<float, bf16>(p, vec, nb, st) : launch_append<bf16, bf16>(p, vec, nb, st);
-    if (e != cudaSuccess) {
-        *why = cudaGetErrorString(e);
-        return GPT2Q_ECUDA;
-    }
-    return GPT2Q_OK;
+    if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
+    const cudaError_t e = launch_append(p, kv->dtype, dtype, vec, st);
+    if (e == cudaErrorInvalidConfiguration) return refuse(why, "too many tokens in one call");
+    return launched(e, why);
+}
+
+int gpt2q::paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens, const int32_t* d_accept,
+                        int width, int64_t ld, int32_t* d_new_lens, int32_t* d_status, cudaStream_t st, std::string* why) {
+    const int rc = check_paged_cache(kv, table, GPT2Q_F32, why);
+    if (rc) return rc;
+    if (width < 0 || ld < width) return refuse(why, "width < 0 or ld < width");
+    if (table->n_rows == 0) return GPT2Q_OK;
+    if (!d_lens || !d_new_lens || (width > 0 && !d_accept)) return refuse(why, "null d_lens, d_accept or d_new_lens");
+    if (d_new_lens < d_lens + table->n_rows && d_lens < d_new_lens + table->n_rows)
+        return refuse(why, "d_new_lens must not be d_lens");
+    if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
+    EntryParams p{};
+    take_cache(&p, kv);
+    take_scales(&p, kv);
+    p.table = table->ids, p.n_rows = table->n_rows, p.width = table->width, p.ld = table->ld, p.status = d_status;
+    p.lens = d_lens, p.accept = d_accept, p.n_accept = width, p.accept_ld = ld, p.new_lens = d_new_lens;
+    return launched(launch_commit(p, kv->dtype, st), why);
 }
 
 int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
                            const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads, float scale,
                            int window, float* d_lse, int32_t* d_status, void* d_work, const HiLo& hl, cudaStream_t st,
-                           std::string* why) {
+                           std::string* why, const Tree* tree) {
     const int rc = check_paged_cache(kv, table, dtype, why);
     if (rc) return rc;
-    if (table->n_rows == 0) return GPT2Q_OK;
+    if (tree && tree->n_tokens < 0) return refuse(why, "n_tokens < 0");
+    if (table->n_rows == 0 || (tree && tree->n_tokens == 0)) return GPT2Q_OK;
+    if (tree) {
+        if (!tree->d_first) return refuse(why, "null d_first");
+        if (tree->d_mask && tree->mask_words < 1) return refuse(why, "mask_words must be >= 1");
+        if (n_heads > 0 && (long long)tree->n_tokens * n_heads > INT32_MAX / 2) return refuse(why, "too many tokens in one call");
+    }
     if (!d_lens || !q || !q->data || !out || (!out->data && !hl.hi)) return refuse(why, "null d_lens, q or out");
     if (n_heads < 1 || n_heads % kv->n_kv_heads) return refuse(why, "n_heads must be a multiple of n_kv_heads");
     if (!std::isfinite(scale)) return refuse(why, "scale must be finite");
@@ -276,7 +193,7 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     if (!aligned16(q->data, q->token_stride, q->head_stride, sz) ||
         !aligned16(out->data, out->token_stride, out->head_stride, sz))
         return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
-    if (out->data && overlap(table->n_rows, out->token_stride, n_heads, out->head_stride, kv->head_dim))
+    if (out->data && overlap(tree ? tree->n_tokens : table->n_rows, out->token_stride, n_heads, out->head_stride, kv->head_dim))
         return refuse(why, "the results in out overlap");
     PagedAttn p{};
     p.k = kv->k, p.v = kv->v;
@@ -290,12 +207,9 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX - 64);
     p.n_heads = n_heads, p.n_kv = kv->n_kv_heads, p.group = n_heads / kv->n_kv_heads, p.dim = kv->head_dim;
     p.window = window, p.scale = scale, p.status = d_status;
-    const cudaError_t e = launch_paged_attn(p, kv->dtype, dtype, d_work, st);
-    if (e != cudaSuccess) {
-        *why = cudaGetErrorString(e);
-        return GPT2Q_ECUDA;
-    }
-    return GPT2Q_OK;
+    take_scales(&p, kv);
+    if (tree) p.first = tree->d_first, p.mask = tree->d_mask, p.mask_words = tree->mask_words, p.n_tokens = tree->n_tokens;
+    return launched(launch_paged_attn(p, kv->dtype, dtype, d_work, st), why);
 }
 
 // =================================================================== C-ABI
@@ -320,9 +234,68 @@ extern "C" int gpt2q_paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_tab
     if (!d_pos && n_tokens > 0)
         rc = refuse(&why, "null d_pos");
     else
-        rc = paged_append(kv, table, k, v, q, q_out, dtype, n_q_heads, n_tokens, d_pos, 0, d_seq, rot, d_status,
+        rc = paged_append(kv, table, k, v, q, q_out, dtype, n_q_heads, n_tokens, d_pos, 0, nullptr, d_seq, rot, d_status,
                           static_cast<cudaStream_t>(stream), &why);
     if (rc) set_global_error("gpt2q_paged_append: " + why);
+    return rc;
+}
+
+extern "C" int gpt2q_paged_append_at(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                                     const gpt2q_heads* v, const gpt2q_heads* q, const gpt2q_heads* q_out, int dtype,
+                                     int n_q_heads, int n_tokens, const int32_t* d_pos, const int32_t* d_slot,
+                                     const int32_t* d_seq, const gpt2q_rotary* rot, int32_t* d_status, void* stream) {
+    std::string why;
+    int rc;
+    if (!d_pos && n_tokens > 0)
+        rc = refuse(&why, "null d_pos");
+    else
+        rc = paged_append(kv, table, k, v, q, q_out, dtype, n_q_heads, n_tokens, d_pos, 0, d_slot, d_seq, rot, d_status,
+                          static_cast<cudaStream_t>(stream), &why);
+    if (rc) set_global_error("gpt2q_paged_append_at: " + why);
+    return rc;
+}
+
+extern "C" int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k,
+                                const gpt2q_heads* v, int dtype, int n_tokens, const int32_t* d_pos, const int32_t* d_seq,
+                                int32_t* d_status, void* stream) {
+    std::string why;
+    auto call = [&]() -> int {
+        const int rc = check_paged_cache(kv, table, dtype, &why);
+        if (rc) return rc;
+        if (n_tokens < 0) return refuse(&why, "n_tokens < 0");
+        if (n_tokens == 0) return GPT2Q_OK;
+        if (!k || !k->data || !v || !v->data) return refuse(&why, "null k or v");
+        if (!d_pos) return refuse(&why, "null d_pos");
+        if (!d_seq && n_tokens > table->n_rows) return refuse(&why, "more tokens than table rows, and no d_seq");
+        const int sz = size_of(dtype);
+        if (reinterpret_cast<uintptr_t>(k->data) % sz || reinterpret_cast<uintptr_t>(v->data) % sz)
+            return refuse(&why, "unaligned k or v");
+        for (const gpt2q_heads* h : {k, v})
+            if (overlap(n_tokens, h->token_stride, kv->n_kv_heads, h->head_stride, kv->head_dim))
+                return refuse(&why, "the entries of k or v overlap");
+        EntryParams p{};
+        take_cache(&p, kv);
+        take_scales(&p, kv);
+        p.table = table->ids, p.n_rows = table->n_rows, p.width = table->width, p.ld = table->ld, p.status = d_status;
+        p.k = k->data, p.k_ts = k->token_stride, p.k_hs = k->head_stride;
+        p.v = v->data, p.v_ts = v->token_stride, p.v_hs = v->head_stride;
+        p.n_tokens = n_tokens, p.pos = d_pos, p.seq = d_seq;
+        const bool vec = aligned16(p.k, p.k_ts, p.k_hs, sz) && aligned16(p.v, p.v_ts, p.v_hs, sz);
+        const cudaError_t e = launch_read(p, kv->dtype, dtype, vec, static_cast<cudaStream_t>(stream));
+        if (e == cudaErrorInvalidConfiguration) return refuse(&why, "too many tokens in one call");
+        return launched(e, &why);
+    };
+    const int rc = call();
+    if (rc) set_global_error("gpt2q_paged_read: " + why);
+    return rc;
+}
+
+extern "C" int gpt2q_paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                                  const int32_t* d_accept, int width, int64_t ld, int32_t* d_new_lens, int32_t* d_status,
+                                  void* stream) {
+    std::string why;
+    const int rc = paged_commit(kv, table, d_lens, d_accept, width, ld, d_new_lens, d_status, static_cast<cudaStream_t>(stream), &why);
+    if (rc) set_global_error("gpt2q_paged_commit: " + why);
     return rc;
 }
 
@@ -338,5 +311,23 @@ extern "C" int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_
     const int rc = paged_attention(kv, table, d_lens, q, out, dtype, n_heads, scale, window, d_lse, d_status, d_work,
                                    HiLo{}, static_cast<cudaStream_t>(stream), &why);
     if (rc) set_global_error("gpt2q_paged_attention: " + why);
+    return rc;
+}
+
+extern "C" uint64_t gpt2q_paged_tree_attention_workspace(const gpt2q_paged_kv* kv, int n_heads, int n_tokens) {
+    if (!kv || n_heads < 1 || n_tokens < 0 || kv->n_kv_heads < 1 || kv->head_dim < 8 || kv->head_dim > 256) return 0;
+    return paged_attn_workspace(kv->head_dim, 16);
+}
+
+extern "C" int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
+                                          const int32_t* d_first, const int32_t* d_mask, int mask_words,
+                                          const gpt2q_heads* q, const gpt2q_heads* out, int dtype, int n_heads,
+                                          int n_tokens, float scale, float* d_lse, int32_t* d_status, void* d_work,
+                                          void* stream) {
+    std::string why;
+    const Tree tree{d_first, d_mask, mask_words, n_tokens};
+    const int rc = paged_attention(kv, table, d_lens, q, out, dtype, n_heads, scale, 0, d_lse, d_status, d_work, HiLo{},
+                                   static_cast<cudaStream_t>(stream), &why, &tree);
+    if (rc) set_global_error("gpt2q_paged_tree_attention: " + why);
     return rc;
 }

@@ -151,6 +151,8 @@ struct gpt2q_handle {
     unsigned long long* pg_best = nullptr;
     int *pg_ints = nullptr, *pg_status = nullptr;
     void* pg_work = nullptr;
+    int* pg_tree = nullptr;  // drafted tokens: ids, positions, slots, rows, picks, lengths, masks
+    size_t pg_tree_ints = 0;
     int* kerr = nullptr;  // device error word of the CUDA-core kernels' bounded waits
     // trunk backward workspace (grown on demand, freed by destroy)
     float* bwd_ws = nullptr;
@@ -1561,6 +1563,11 @@ int score_positions(gpt2q_handle* H, const uint32_t* ids, int n, int slot, F&& r
     return GPT2Q_OK;
 }
 
+// Layer l of the caller's caches: an array of gpt2q_paged_kv8 where the first has 8 bits.
+const gpt2q_paged_kv& layer_at(const gpt2q_paged_kv* layers, int l) {
+    return is_8bit(layers[0].dtype) ? reinterpret_cast<const gpt2q_paged_kv8*>(layers)[l].kv : layers[l];
+}
+
 // A paged cache per layer, of this model's heads, and the table: before anything is launched or a row
 // of the table is taken.
 int check_paged(gpt2q_handle* H, const gpt2q_paged_kv* layers, const gpt2q_page_table* table) {
@@ -1568,9 +1575,12 @@ int check_paged(gpt2q_handle* H, const gpt2q_paged_kv* layers, const gpt2q_page_
     if (!layers) return H->fail(GPT2Q_EARG, "null layers");
     for (int l = 0; l < H->cfg.n_layer; ++l) {
         std::string why;
-        const int rc = check_paged_cache(&layers[l], table, GPT2Q_F32, &why);
+        const gpt2q_paged_kv& kv = layer_at(layers, l);
+        if (is_8bit(kv.dtype) && !is_8bit(layers[0].dtype))
+            return H->fail(GPT2Q_EARG, "layer " + std::to_string(l) + ": an 8-bit cache behind a first layer of more bits");
+        const int rc = check_paged_cache(&kv, table, GPT2Q_F32, &why);
         if (rc) return H->fail(rc, "layer " + std::to_string(l) + ": " + why);
-        if (layers[l].n_kv_heads != H->H_local || layers[l].head_dim != H->hd)
+        if (kv.n_kv_heads != H->H_local || kv.head_dim != H->hd)
             return H->fail(GPT2Q_EARG, "layer " + std::to_string(l) + ": the cache must have the model's heads and head dim");
     }
     return GPT2Q_OK;
@@ -1603,10 +1613,26 @@ int ensure_paged(gpt2q_handle* H, int rows) {
     H->pg_best = static_cast<unsigned long long*>(take((size_t)R * 8));
     H->pg_ints = static_cast<int*>(take((size_t)4 * R * 4));
     H->pg_status = static_cast<int*>(take(16));
-    H->pg_work = take((size_t)gpt2q_paged_attention_workspace(&kv, H->H_local));
+    H->pg_work = take((size_t)std::max(gpt2q_paged_attention_workspace(&kv, H->H_local),
+                                       gpt2q_paged_tree_attention_workspace(&kv, H->H_local, R)));
     if (!ok) return H->fail(GPT2Q_EOOM, "paged decode buffers");
     CK(cudaMemsetAsync(H->pg_best, 0, (size_t)R * 8, H->stream));
     H->pg_rows = R;
+    return GPT2Q_OK;
+}
+
+// Device integers of a step with drafted tokens.
+int ensure_tree(gpt2q_handle* H, size_t ints) {
+    if (H->pg_tree_ints >= ints) return GPT2Q_OK;
+    CK(cudaStreamSynchronize(H->stream));
+    cudaFree(H->pg_tree);
+    H->pg_tree = nullptr;
+    H->pg_tree_ints = 0;
+    if (cudaMalloc(&H->pg_tree, ints * 4) != cudaSuccess) {
+        cudaGetLastError();
+        return H->fail(GPT2Q_EOOM, "drafted tokens' buffers");
+    }
+    H->pg_tree_ints = ints;
     return GPT2Q_OK;
 }
 
@@ -1620,6 +1646,55 @@ int paged_status(gpt2q_handle* H) {
     if (status & GPT2Q_STATUS_TIMEOUT) return H->fail(GPT2Q_ETIMEOUT, "a bounded device-side wait timed out (paged attention)");
     if (status) return H->fail(GPT2Q_EARG, "the page table names a page out of range or is too short (status " + std::to_string(status) + ")");
     return GPT2Q_OK;
+}
+// One pass of B rows through the model over paged caches: row i is token d_tok[i] at position d_pos[i], whose keys and values go to
+// slot d_slot[i] (null: its position) of table row d_row[i] (null: i). One token per sequence attends over d_len[i] cached
+// tokens; drafted ones (tree) over their sequence's prefix and what their masks name.
+int paged_step(gpt2q_handle* H, const char* name, int B, const uint32_t* d_tok, const int* d_pos, const int* d_slot, const int* d_row,
+               const int* d_len, double keys, const Tree* tree, const gpt2q_paged_kv* layers, const gpt2q_page_table* table,
+               uint32_t* d_next, float* logits, uint32_t* next_tok) {
+    const int d = H->cfg.n_embd, V = H->cfg.vocab, NH = H->H_local, hd = H->hd;
+    CK(cudaMemsetAsync(H->pg_status, 0, 4, H->stream));
+    const float scale = 1.0f / std::sqrt((float)hd);
+    const gpt2q_heads qh{H->pg_qkv, 3 * (int64_t)d, hd}, kh{H->pg_qkv + d, 3 * (int64_t)d, hd}, vh{H->pg_qkv + 2 * d, 3 * (int64_t)d, hd};
+    RUN("embed", (double)B * d * 6, launch_embed(H->wte.w, H->wpe.w, d_tok, d_pos, H->x, d, B, H->stream));
+    for (int l = 0; l < H->cfg.n_layer; ++l) {
+        const int rc = block(H, l, B, nullptr, nullptr, [&](int layer) {
+            const In ain{H->att, H->att_hi, H->att_lo, H->d_local};
+            const bool att32 = reads_f32(H, H->layers[layer].proj, ain, B);
+            const gpt2q_heads oh{att32 ? H->att : nullptr, d, hd};
+            const gpt2q_paged_kv& kv = layer_at(layers, layer);
+            std::string why;
+            int prc = GPT2Q_OK;
+            auto launched_as = [&](int code) { return prc = code, code == GPT2Q_OK ? cudaSuccess : cudaErrorInvalidValue; };
+            const int es = size_of(kv.dtype);
+            int krc = run_kernel(H, "paged_append", (double)B * 2 * d * (4 + es), [&] {
+                return launched_as(paged_append(&kv, table, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, B, d_pos, 0, d_slot, d_row,
+                                                nullptr, H->pg_status, H->stream, &why));
+            });
+            if (!krc)
+                krc = run_kernel(H, "paged_attention", keys * 2 * d * es + (double)B * d * 8, [&] {
+                    return launched_as(paged_attention(&kv, table, d_len, &qh, &oh, GPT2Q_F32, NH, scale, 0, nullptr, H->pg_status,
+                                                       H->pg_work, HiLo{H->att_hi, H->att_lo, d}, H->stream, &why, tree));
+                });
+            if (!krc) H->launches++;  // the attention and its join
+            return prc ? H->fail(prc, std::string(name) + ": " + why) : krc;
+        }, H->pg_qkv);
+        if (rc) return rc;
+    }
+    RUN("layernorm", (double)B * d * 8,
+        launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, B, H->stream));
+    int rc = apply_adapter(H, B);
+    if (!rc) rc = head(H, B, H->pg_logits);
+    if (rc) return rc;
+    RUN("argmax", (double)B * V * 4,
+        launch_argmax(H->pg_logits, V, V, B, H->pg_best, d_next, nullptr, nullptr, 0, nullptr, nullptr, H->stream));
+    H->launches++;  // argmax is two kernels
+    if (logits) CK(cudaMemcpyAsync(logits, H->pg_logits, (size_t)B * V * 4, cudaMemcpyDeviceToHost, H->stream));
+    if (next_tok) CK(cudaMemcpyAsync(next_tok, d_next, (size_t)B * 4, cudaMemcpyDeviceToHost, H->stream));
+    rc = paged_status(H);
+    if (!rc && H->prof) rc = flush_profile(H);
+    return rc;
 }
 }  // namespace
 
@@ -1659,6 +1734,7 @@ void gpt2q_destroy(gpt2q_handle* H) {
     mk_destroy(H->mk);
     for (auto& a : H->allocs) cudaFree(a.p);
     if (H->bwd_ws) cudaFree(H->bwd_ws);
+    cudaFree(H->pg_tree);
     for (void* p : H->pg_allocs) cudaFree(p);
     if (H->h_stage) cudaFreeHost(H->h_stage);
     if (H->h_err) cudaFreeHost(H->h_err);
@@ -1905,7 +1981,7 @@ int gpt2q_page_out(gpt2q_handle* H, int slot, int n_tokens, const gpt2q_paged_kv
         const gpt2q_heads kh{k, H->hd, (int64_t)H->kv.head_stride};
         const gpt2q_heads vh{k + H->kv.sel_stride, H->hd, (int64_t)H->kv.head_stride};
         std::string why;
-        rc = paged_append(&layers[l], &t, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, n_tokens, nullptr, 0, nullptr, nullptr,
+        rc = paged_append(&layer_at(layers, l), &t, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, n_tokens, nullptr, 0, nullptr, nullptr, nullptr,
                           H->pg_status, H->stream, &why);
         if (rc) return H->fail(rc, "page_out: " + why);
         H->launches++;
@@ -1927,62 +2003,108 @@ int gpt2q_decode_paged(gpt2q_handle* H, const uint32_t* tok, const int32_t* pos,
     if (!rc) rc = ensure_paged(H, n_seq);
     if (!rc) rc = ensure_stage(H, (size_t)3 * n_seq);
     if (rc) return rc;
-    const int d = H->cfg.n_embd, V = H->cfg.vocab, B = n_seq, R = H->pg_rows, NH = H->H_local, hd = H->hd;
+    const int B = n_seq, R = H->pg_rows;
     // tokens | positions | lengths | picks, pg_rows each
     uint32_t* d_tok = reinterpret_cast<uint32_t*>(H->pg_ints);
     int *d_pos = H->pg_ints + R, *d_len = H->pg_ints + 2 * (size_t)R;
     uint32_t* d_next = reinterpret_cast<uint32_t*>(H->pg_ints + 3 * (size_t)R);
+    double keys = 0;
     for (int i = 0; i < B; ++i) {
         H->h_stage[i] = (int)tok[i];
         H->h_stage[B + i] = pos[i];
         H->h_stage[2 * B + i] = pos[i] + 1;
+        keys += pos[i] + 1;
     }
     CK(cudaMemcpyAsync(d_tok, H->h_stage, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
     CK(cudaMemcpyAsync(d_pos, H->h_stage + B, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
     CK(cudaMemcpyAsync(d_len, H->h_stage + 2 * (size_t)B, (size_t)B * 4, cudaMemcpyHostToDevice, H->stream));
-    CK(cudaMemsetAsync(H->pg_status, 0, 4, H->stream));
-    const float scale = 1.0f / std::sqrt((float)hd);
-    const gpt2q_heads qh{H->pg_qkv, 3 * (int64_t)d, hd}, kh{H->pg_qkv + d, 3 * (int64_t)d, hd}, vh{H->pg_qkv + 2 * d, 3 * (int64_t)d, hd};
-    double keys = 0;
-    for (int i = 0; i < B; ++i) keys += pos[i] + 1;
-    RUN("embed", (double)B * d * 6, launch_embed(H->wte.w, H->wpe.w, d_tok, d_pos, H->x, d, B, H->stream));
-    for (int l = 0; l < H->cfg.n_layer; ++l) {
-        rc = block(H, l, B, nullptr, nullptr, [&](int layer) {
-            const In ain{H->att, H->att_hi, H->att_lo, H->d_local};
-            const bool att32 = reads_f32(H, H->layers[layer].proj, ain, B);
-            const gpt2q_heads oh{att32 ? H->att : nullptr, d, hd};
-            const gpt2q_paged_kv& kv = layers[layer];
-            std::string why;
-            int prc = GPT2Q_OK;
-            auto launched_as = [&](int code) { return prc = code, code == GPT2Q_OK ? cudaSuccess : cudaErrorInvalidValue; };
-            const int es = kv.dtype == GPT2Q_F32 ? 4 : 2;
-            int krc = run_kernel(H, "paged_append", (double)B * 2 * d * (4 + es), [&] {
-                return launched_as(paged_append(&kv, table, &kh, &vh, nullptr, nullptr, GPT2Q_F32, 0, B, d_pos, 0, nullptr,
-                                                nullptr, H->pg_status, H->stream, &why));
-            });
-            if (!krc)
-                krc = run_kernel(H, "paged_attention", keys * 2 * d * es + (double)B * d * 8, [&] {
-                    return launched_as(paged_attention(&kv, table, d_len, &qh, &oh, GPT2Q_F32, NH, scale, 0, nullptr, H->pg_status,
-                                                       H->pg_work, HiLo{H->att_hi, H->att_lo, d}, H->stream, &why));
-                });
-            if (!krc) H->launches++;  // the attention and its join
-            return prc ? H->fail(prc, "decode_paged: " + why) : krc;
-        }, H->pg_qkv);
-        if (rc) return rc;
+    return paged_step(H, "decode_paged", B, d_tok, d_pos, nullptr, nullptr, d_len, keys, nullptr, layers, table, d_next, logits, next_tok);
+}
+
+int gpt2q_verify_paged(gpt2q_handle* H, const uint32_t* tok, const int32_t* parent, const int32_t* first, const int32_t* lens,
+                       int n_seq, const gpt2q_paged_kv* layers, const gpt2q_page_table* table, float* logits,
+                       uint32_t* next_tok) {
+    if (!H) return GPT2Q_EARG;
+    if (!tok || !parent || !first || !lens) return H->fail(GPT2Q_EARG, "null tok/parent/first/lens");
+    if (n_seq < 1 || !table || table->n_rows != n_seq) return H->fail(GPT2Q_EARG, "the table must have n_seq rows");
+    if (first[0] != 0) return H->fail(GPT2Q_EARG, "first[0] must be 0");
+    int most = 1;
+    for (int r = 0; r < n_seq; ++r) {
+        if (first[r + 1] < first[r]) return H->fail(GPT2Q_EARG, "first must rise");
+        most = std::max(most, first[r + 1] - first[r]);
     }
-    RUN("layernorm", (double)B * d * 8,
-        launch_layernorm(H->x, d, nullptr, H->h, d, H->h_hi, H->h_lo, H->lnf_g, H->lnf_b, d, H->cfg.ln_eps, B, H->stream));
-    rc = apply_adapter(H, B);
-    if (!rc) rc = head(H, B, H->pg_logits);
+    const int n = first[n_seq];
+    if (n < 1 || n > H->Mmax) return H->fail(GPT2Q_EARG, "drafted tokens out of range [1, max(max_seqs, max_tokens)]");
+    const int words = (most + 31) / 32;
+    // host: tokens | positions | slots | rows | lengths | first | masks
+    const size_t ints = (size_t)4 * n + 2 * (size_t)n_seq + 1 + (size_t)n * words;
+    int rc = ensure_stage(H, ints);
     if (rc) return rc;
-    RUN("argmax", (double)B * V * 4,
-        launch_argmax(H->pg_logits, V, V, B, H->pg_best, d_next, nullptr, nullptr, 0, nullptr, nullptr, H->stream));
-    H->launches++;  // argmax is two kernels
-    if (logits) CK(cudaMemcpyAsync(logits, H->pg_logits, (size_t)B * V * 4, cudaMemcpyDeviceToHost, H->stream));
-    if (next_tok) CK(cudaMemcpyAsync(next_tok, d_next, (size_t)B * 4, cudaMemcpyDeviceToHost, H->stream));
-    rc = paged_status(H);
-    if (!rc && H->prof) rc = flush_profile(H);
-    return rc;
+    int* s_tok = H->h_stage;
+    int *s_pos = s_tok + n, *s_slot = s_pos + n, *s_row = s_slot + n, *s_len = s_row + n, *s_first = s_len + n_seq;
+    int* s_mask = s_first + n_seq + 1;
+    double keys = 0;
+    for (int r = 0; r < n_seq; ++r) {
+        if (lens[r] < 0) return H->fail(GPT2Q_EARG, "lens < 0");
+        s_len[r] = lens[r];
+        s_first[r] = first[r];
+        if (first[r + 1] > first[r]) keys += lens[r] + first[r + 1] - first[r];
+        for (int t = first[r]; t < first[r + 1]; ++t) {
+            const int i = t - first[r], up = parent[t];
+            if (up < -1 || up >= i) return H->fail(GPT2Q_EARG, "a token's parent must be an earlier token of its sequence, or -1");
+            int* m = s_mask + (size_t)t * words;
+            if (up < 0)
+                std::fill(m, m + words, 0);
+            else
+                std::copy(s_mask + (size_t)(first[r] + up) * words, s_mask + (size_t)(first[r] + up + 1) * words, m);
+            m[i / 32] |= (int)(1u << (i & 31));
+            s_tok[t] = (int)tok[t];
+            s_pos[t] = up < 0 ? lens[r] : s_pos[first[r] + up] + 1;
+            s_slot[t] = lens[r] + i;
+            s_row[t] = r;
+            if (s_pos[t] >= H->cfg.n_ctx) return H->fail(GPT2Q_EARG, "a drafted token's position is past n_ctx");
+        }
+    }
+    s_first[n_seq] = n;
+    CK(cudaSetDevice(H->device));
+    rc = check_tokens(H, tok, (size_t)n);
+    if (!rc) rc = check_paged(H, layers, table);
+    if (!rc) rc = ensure_paged(H, n);
+    if (!rc) rc = ensure_tree(H, ints + n);
+    if (rc) return rc;
+    int* dev = H->pg_tree;
+    CK(cudaMemcpyAsync(dev, H->h_stage, ints * 4, cudaMemcpyHostToDevice, H->stream));
+    const int *d_pos = dev + n, *d_slot = dev + 2 * (size_t)n, *d_row = dev + 3 * (size_t)n, *d_len = dev + 4 * (size_t)n;
+    const Tree tree{d_len + n_seq, d_len + 2 * (size_t)n_seq + 1, words, n};
+    return paged_step(H, "verify_paged", n, reinterpret_cast<uint32_t*>(dev), d_pos, d_slot, d_row, d_len, keys, &tree, layers, table,
+                      reinterpret_cast<uint32_t*>(dev + ints), logits, next_tok);
+}
+
+int gpt2q_commit_paged(gpt2q_handle* H, const int32_t* lens, const int32_t* accept, int width, int32_t* new_lens,
+                       const gpt2q_paged_kv* layers, const gpt2q_page_table* table) {
+    if (!H) return GPT2Q_EARG;
+    if (!table || table->n_rows < 1) return H->fail(GPT2Q_EARG, "null table, or one without rows");
+    if (!lens || width < 0 || (width > 0 && !accept)) return H->fail(GPT2Q_EARG, "null lens/accept, or width < 0");
+    CK(cudaSetDevice(H->device));
+    const int n = table->n_rows;
+    const size_t ints = (size_t)n * (1 + (size_t)width);
+    int rc = check_paged(H, layers, table);
+    if (!rc) rc = ensure_paged(H, 1);
+    if (!rc) rc = ensure_stage(H, ints);
+    if (!rc) rc = ensure_tree(H, ints + n);
+    if (rc) return rc;
+    std::copy(lens, lens + n, H->h_stage);
+    if (width) std::copy(accept, accept + (size_t)n * width, H->h_stage + n);
+    CK(cudaMemcpyAsync(H->pg_tree, H->h_stage, ints * 4, cudaMemcpyHostToDevice, H->stream));
+    CK(cudaMemsetAsync(H->pg_status, 0, 4, H->stream));
+    for (int l = 0; l < H->cfg.n_layer; ++l) {
+        std::string why;
+        rc = paged_commit(&layer_at(layers, l), table, H->pg_tree, H->pg_tree + n, width, width, H->pg_tree + ints, H->pg_status, H->stream, &why);
+        if (rc) return H->fail(rc, "commit_paged: " + why);
+        H->launches++;
+    }
+    if (new_lens) CK(cudaMemcpyAsync(new_lens, H->pg_tree + ints, (size_t)n * 4, cudaMemcpyDeviceToHost, H->stream));
+    return paged_status(H);
 }
 
 int gpt2q_trunk_score_grad(gpt2q_handle* H, const uint32_t* ids, int n, const int32_t* targets, const float* d_lp,

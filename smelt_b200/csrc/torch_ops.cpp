@@ -66,6 +66,7 @@ int size32(int64_t n, const char* name) {
 int type_code(at::ScalarType t) {
     return t == at::kFloat ? GPT2Q_F32 : t == at::kHalf ? GPT2Q_F16 : t == at::kBFloat16 ? GPT2Q_BF16 : -1;
 }
+constexpr bool eight(int code) { return code == GPT2Q_I8 || code == GPT2Q_E4M3; }
 const char* type_name(int code) { return code == GPT2Q_F32 ? "float32" : code == GPT2Q_F16 ? "float16" : "bfloat16"; }
 
 void on_device(const at::Tensor& t, int index, const char* name) {
@@ -97,7 +98,9 @@ gpt2q_heads heads(const at::Tensor& t, int index, const char* name, int64_t n, i
 const gpt2q_paged_kv* cache_of(PyObject* o) { return static_cast<const gpt2q_paged_kv*>(PyLong_AsVoidPtr(o)); }
 at::ScalarType io_type(const gpt2q_paged_kv* kv, const at::Tensor& t) {
     const int code = type_code(t.scalar_type());
-    if (code != kv->dtype && code != GPT2Q_F32)
+    if (eight(kv->dtype)) {
+        if (code < 0) refuse("tensors must be float32, float16 or bfloat16");
+    } else if (code != kv->dtype && code != GPT2Q_F32)
         refuse(std::string("tensors must be ") + type_name(kv->dtype) + " like the cache, or float32");
     return t.scalar_type();
 }
@@ -136,9 +139,9 @@ bool arity(Py_ssize_t n, Py_ssize_t want) {
     return false;
 }
 
-// append(cache, device, k, v, table, pos, seq, rotary, q, q_out, status) -> q_out or None
+// append(cache, device, k, v, table, pos, seq, rotary, q, q_out, status, slot) -> q_out or None
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    if (!arity(n_args, 11)) return nullptr;
+    if (!arity(n_args, 12)) return nullptr;
     return guarded([&]() -> PyObject* {
         const gpt2q_paged_kv* kv = cache_of(a[0]);
         const int index = small(a[1], "device");
@@ -151,7 +154,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const gpt2q_page_table t = page_table(tensor(a[4], "table"), index);
         const int32_t* pos = ints(tensor(a[5], "pos"), index, "pos", n);
         const at::Tensor *seq = optional(a[6], "seq"), *q = optional(a[8], "q"), *q_out = optional(a[9], "q_out");
-        const at::Tensor* status = optional(a[10], "status");
+        const at::Tensor *status = optional(a[10], "status"), *slot = optional(a[11], "slot");
+        const int32_t* lp = slot ? ints(*slot, index, "slot", n) : nullptr;
         const int32_t* sp = seq ? ints(*seq, index, "seq", n) : nullptr;
         int32_t* st = status ? ints(*status, index, "status", 1) : nullptr;
         const gpt2q_rotary* rot = a[7] == Py_None ? nullptr : static_cast<const gpt2q_rotary*>(PyLong_AsVoidPtr(a[7]));
@@ -171,31 +175,107 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             refuse("q_out without q");
         }
         Stream s(index);
-        check(gpt2q_paged_append(kv, &t, &kh, &vh, q ? &qh : nullptr, q ? &oh : nullptr, type_code(type),
-                                 size32(hq, "q"), size32(n, "k"), pos, sp, rot, st, s.handle));
+        check(gpt2q_paged_append_at(kv, &t, &kh, &vh, q ? &qh : nullptr, q ? &oh : nullptr, type_code(type),
+                                    size32(hq, "q"), size32(n, "k"), pos, lp, sp, rot, st, s.handle));
         if (!q) Py_RETURN_NONE;
         if (fresh.defined()) return THPVariable_Wrap(fresh);
         return Py_NewRef(a[9]);
     });
 }
 
+// read(cache, device, table, pos, seq, k, v, dtype, status) -> (k, v)
+PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!arity(n_args, 9)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const gpt2q_paged_kv* kv = cache_of(a[0]);
+        const int index = small(a[1], "device");
+        const gpt2q_page_table t = page_table(tensor(a[2], "table"), index);
+        const at::Tensor& p = tensor(a[3], "pos");
+        if (p.dim() != 1) refuse("pos must be a vector");
+        const int64_t n = p.size(0);
+        const int32_t* pos = ints(p, index, "pos", n);
+        const at::Tensor *seq = optional(a[4], "seq"), *k = optional(a[5], "k"), *v = optional(a[6], "v"), *status = optional(a[8], "status");
+        const int32_t* sp = seq ? ints(*seq, index, "seq", n) : nullptr;
+        int32_t* st = status ? ints(*status, index, "status", 1) : nullptr;
+        const long long code = whole(a[7]);
+        at::ScalarType type = code == GPT2Q_F32 ? at::kFloat : code == GPT2Q_F16 ? at::kHalf : at::kBFloat16;
+        if (k) type = io_type(kv, *k);
+        else if (v) type = io_type(kv, *v);
+        at::Tensor fresh_k, fresh_v;
+        const auto options = p.options().dtype(type).memory_format(at::MemoryFormat::Contiguous);
+        if (!k) k = &(fresh_k = at::empty({n, kv->n_kv_heads, kv->head_dim}, options));
+        if (!v) v = &(fresh_v = at::empty({n, kv->n_kv_heads, kv->head_dim}, options));
+        const gpt2q_heads kh = heads(*k, index, "k", n, kv->n_kv_heads, kv->head_dim, type);
+        const gpt2q_heads vh = heads(*v, index, "v", n, kv->n_kv_heads, kv->head_dim, type);
+        Stream s(index);
+        check(gpt2q_paged_read(kv, &t, &kh, &vh, type_code(type), size32(n, "pos"), pos, sp, st, s.handle));
+        PyObject* out = PyTuple_New(2);
+        PyTuple_SET_ITEM(out, 0, fresh_k.defined() ? THPVariable_Wrap(fresh_k) : Py_NewRef(a[5]));
+        PyTuple_SET_ITEM(out, 1, fresh_v.defined() ? THPVariable_Wrap(fresh_v) : Py_NewRef(a[6]));
+        return out;
+    });
+}
+
+// commit(cache, device, table, lens, accept, new_lens, status) -> new_lens
+PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!arity(n_args, 7)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const gpt2q_paged_kv* kv = cache_of(a[0]);
+        const int index = small(a[1], "device");
+        const gpt2q_page_table t = page_table(tensor(a[2], "table"), index);
+        const int32_t* lens = ints(tensor(a[3], "lens"), index, "lens", t.n_rows);
+        const at::Tensor& accept = tensor(a[4], "accept");
+        on_device(accept, index, "accept");
+        if (accept.scalar_type() != at::kInt || accept.dim() != 2 || accept.size(0) != t.n_rows || (accept.size(1) > 1 && accept.stride(1) != 1))
+            refuse("accept must be int32 [" + std::to_string(t.n_rows) + ", tokens] with unit stride over the tokens");
+        const int width = size32(accept.size(1), "accept");
+        const at::Tensor *out = optional(a[5], "new_lens"), *status = optional(a[6], "status");
+        int32_t* st = status ? ints(*status, index, "status", 1) : nullptr;
+        at::Tensor fresh;
+        if (!out) out = &(fresh = at::empty({t.n_rows}, accept.options().memory_format(at::MemoryFormat::Contiguous)));
+        int32_t* new_lens = ints(*out, index, "new_lens", t.n_rows);
+        Stream s(index);
+        check(gpt2q_paged_commit(kv, &t, lens, static_cast<const int32_t*>(accept.data_ptr()), width,
+                                 t.n_rows > 1 ? accept.stride(0) : std::max<int64_t>(accept.stride(0), width), new_lens, st, s.handle));
+        if (fresh.defined()) return THPVariable_Wrap(fresh);
+        return Py_NewRef(a[5]);
+    });
+}
+
 // attend(cache, device, q, table, lens, scale, window, out, lse, status) -> out
+// attend_tree(cache, device, q, table, lens, scale, first, mask, out, lse, status) -> out
+template <bool TREE>
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    if (!arity(n_args, 10)) return nullptr;
+    constexpr int O = TREE ? 8 : 7;  // where out is
+    if (!arity(n_args, O + 3)) return nullptr;
     return guarded([&]() -> PyObject* {
         const gpt2q_paged_kv* kv = cache_of(a[0]);
         const int index = small(a[1], "device");
         const at::Tensor& q = tensor(a[2], "q");
         const at::ScalarType type = io_type(kv, q);
-        if (q.dim() != 3) refuse("q must be [rows, heads, head dim]");
+        if (q.dim() != 3) refuse(TREE ? "q must be [tokens, heads, head dim]" : "q must be [rows, heads, head dim]");
         const int64_t n = q.size(0), hq = q.size(1);
         const gpt2q_heads qh = heads(q, index, "q", n, hq, kv->head_dim, type);
         const gpt2q_page_table t = page_table(tensor(a[3], "table"), index);
-        if (t.n_rows != n) refuse("table must have " + std::to_string(n) + " rows");
-        const int32_t* lens = ints(tensor(a[4], "lens"), index, "lens", n);
+        if (!TREE && t.n_rows != n) refuse("table must have " + std::to_string(n) + " rows");
+        const int32_t* lens = ints(tensor(a[4], "lens"), index, "lens", t.n_rows);
         const float scale = a[5] == Py_None ? 1.f / std::sqrt((float)kv->head_dim) : (float)real(a[5]);
-        const int window = small(a[6], "window");
-        const at::Tensor *out = optional(a[7], "out"), *lse = optional(a[8], "lse"), *status = optional(a[9], "status");
+        int window = 0, words = 0;
+        const int32_t *first = nullptr, *mask = nullptr;
+        if (TREE) {
+            first = ints(tensor(a[6], "first"), index, "first", (int64_t)t.n_rows + 1);
+            if (const at::Tensor* m = optional(a[7], "mask")) {
+                on_device(*m, index, "mask");
+                if (m->scalar_type() != at::kInt || m->dim() != 2 || m->size(0) != n || m->size(1) < 1 || !m->is_contiguous())
+                    refuse("mask must be a contiguous int32 tensor [" + std::to_string(n) + ", words]");
+                words = size32(m->size(1), "mask");
+                static const int32_t none = 0;  // of no tokens: a mask all the same
+                mask = n ? static_cast<const int32_t*>(m->data_ptr()) : &none;
+            }
+        } else {
+            window = small(a[6], "window");
+        }
+        const at::Tensor *out = optional(a[O], "out"), *lse = optional(a[O + 1], "lse"), *status = optional(a[O + 2], "status");
         at::Tensor fresh;
         if (!out) {
             fresh = at::empty({n, hq, kv->head_dim}, q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -208,13 +288,18 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 refuse("lse must be a contiguous float32 tensor [" + std::to_string(n) + ", " + std::to_string(hq) + "]");
         }
         int32_t* st = status ? ints(*status, index, "status", 1) : nullptr;
-        const int64_t bytes = (int64_t)gpt2q_paged_attention_workspace(kv, size32(hq, "q"));
+        float* lp = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+        const int heads32 = size32(hq, "q"), n32 = size32(n, "q");
+        const int64_t bytes = (int64_t)(TREE ? gpt2q_paged_tree_attention_workspace(kv, heads32, n32) : gpt2q_paged_attention_workspace(kv, heads32));
         const at::Tensor work = at::empty({std::max<int64_t>(16, bytes)}, q.options().dtype(at::kByte));
         Stream s(index);
-        check(gpt2q_paged_attention(kv, &t, lens, &qh, &oh, type_code(type), (int)hq, scale, window,
-                                    lse ? static_cast<float*>(lse->data_ptr()) : nullptr, st, work.data_ptr(), s.handle));
+        if (TREE)
+            check(gpt2q_paged_tree_attention(kv, &t, lens, first, mask, words, &qh, &oh, type_code(type), heads32, n32, scale, lp, st,
+                                             work.data_ptr(), s.handle));
+        else
+            check(gpt2q_paged_attention(kv, &t, lens, &qh, &oh, type_code(type), heads32, scale, window, lp, st, work.data_ptr(), s.handle));
         if (fresh.defined()) return THPVariable_Wrap(fresh);
-        return Py_NewRef(a[7]);
+        return Py_NewRef(a[O]);
     });
 }
 
@@ -322,7 +407,10 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 
 PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, nullptr},
-    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend)), METH_FASTCALL, nullptr},
+    {"read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read)), METH_FASTCALL, nullptr},
+    {"commit", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(commit)), METH_FASTCALL, nullptr},
+    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend<false>)), METH_FASTCALL, nullptr},
+    {"attend_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend<true>)), METH_FASTCALL, nullptr},
     {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(logprobs)), METH_FASTCALL, nullptr},
     {"logprobs_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(logprobs_grad)), METH_FASTCALL, nullptr},
     {"set_error", set_error, METH_O, nullptr},

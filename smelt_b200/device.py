@@ -12,6 +12,7 @@ import torch
 from . import _ffi
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CODES = {torch.int8: 8, torch.float8_e4m3fn: 9}  # types of a cache alone
 _PATH = os.path.join(_ffi.HERE, "_lib", "gpt2q_torch.so")
 _ops = None
 

@@ -252,7 +252,10 @@ class Gpu:
             raise ValueError(f"table must be int32 [rows, pages] on cuda:{self.device}")
         # what torch has queued (the pools, the table) comes before this handle's stream
         torch.cuda.current_stream(self.device).synchronize()
-        return (_ffi.PagedKV * len(layers))(*(kv.c for kv in layers)), _page_table(table)
+        kind = type(layers[0].c)
+        if any(type(kv.c) is not kind for kv in layers):
+            raise ValueError("the layers' caches must all have 8 bits, or none of them")
+        return (kind * len(layers))(*(kv.c for kv in layers)), _page_table(table)
 
     def page_out(self, slot: int, n_tokens: int, layers, table, row: int):
         """Copies the first n_tokens cached positions of arena slot `slot` into row `row` of `table` of every
@@ -273,6 +276,39 @@ class Gpu:
         self._check(self._lib.gpt2q_decode_paged(self.h, tok.ctypes.data, pos.ctypes.data, n, arr, C.byref(t),
                                                  None if lg is None else lg.ctypes.data, nxt.ctypes.data))
         return (nxt, lg) if want_logits else nxt
+
+    def verify_paged(self, drafts, parents, lens, layers, table, want_logits: bool = False):
+        """Feeds drafted tokens over paged caches: drafts[i] are those of sequence i (row i of `table`), behind its lens[i] cached
+        tokens, and parents[i] their parents among them (-1: the last cached token). Returns the likeliest token after each,
+        one array per sequence, with want_logits the logits too. commit_paged keeps the accepted ones."""
+        tok, first = self._flatten(drafts)
+        par = self._flatten([np.asarray(p, dtype=np.int64) for p in parents])
+        if not np.array_equal(first, par[1]):
+            raise ValueError("drafts and parents must have the same lengths")
+        par, lens = par[0].view(np.int32), np.ascontiguousarray(lens, dtype=np.int32)
+        if lens.size != len(drafts):
+            raise ValueError("lens must have one element per sequence")
+        nxt = np.empty(tok.size, dtype=np.uint32)
+        lg = np.empty((tok.size, self.meta.vocab), dtype=np.float32) if want_logits else None
+        arr, t = self._paged(layers, table)
+        self._check(self._lib.gpt2q_verify_paged(self.h, tok.ctypes.data, par.ctypes.data, first.ctypes.data, lens.ctypes.data,
+                                                 len(drafts), arr, C.byref(t), None if lg is None else lg.ctypes.data, nxt.ctypes.data))
+        nxt = np.split(nxt, first[1:-1])
+        return (nxt, np.split(lg, first[1:-1])) if want_logits else nxt
+
+    def commit_paged(self, lens, accept, layers, table):
+        """Keeps the drafted tokens accept[i] (rising indices) of sequence i in every layer's cache; returns the new lengths."""
+        lens = np.ascontiguousarray(lens, dtype=np.int32)
+        if len(accept) != lens.size or lens.size != table.shape[0]:
+            raise ValueError("lens and accept must have one element per row of the table")
+        width = max((len(a) for a in accept), default=0)
+        acc = np.full((lens.size, width), -1, dtype=np.int32)
+        for row, a in zip(acc, accept):
+            row[:len(a)] = a
+        out = np.empty_like(lens)
+        arr, t = self._paged(layers, table)
+        self._check(self._lib.gpt2q_commit_paged(self.h, lens.ctypes.data, acc.ctypes.data, width, out.ctypes.data, arr, C.byref(t)))
+        return out
 
     def dequant(self, name: str, numel: int) -> np.ndarray:
         out = np.empty(numel, dtype=np.float32)
