@@ -316,7 +316,7 @@ extern "C" int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_
 
 extern "C" uint64_t gpt2q_paged_tree_attention_workspace(const gpt2q_paged_kv* kv, int n_heads, int n_tokens) {
     if (!kv || n_heads < 1 || n_tokens < 0 || kv->n_kv_heads < 1 || kv->head_dim < 8 || kv->head_dim > 256) return 0;
-    return paged_attn_workspace(kv->head_dim, 16);
+    return std::max(paged_attn_workspace(kv->head_dim, 16), paged_tree_tc_workspace(kv->head_dim));
 }
 
 extern "C" int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,

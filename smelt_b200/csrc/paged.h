@@ -55,6 +55,11 @@ cudaError_t launch_paged_attn(PagedAttn p, int cache_dtype, int dtype, void* wor
 // by cache type; the workspace is laid out
 cudaError_t launch_paged_attn_i8(const PagedAttn& p, int dtype, cudaStream_t st);
 cudaError_t launch_paged_attn_e4m3(const PagedAttn& p, int dtype, cudaStream_t st);
+// drafted tokens on tcgen05 tiles (paged_tree_tc.cu): bytes of its workspace, whether it takes a call, and the call; `taken` stays
+// false where the pools cannot be described to TMA
+uint64_t paged_tree_tc_workspace(int dim);
+bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype);
+cudaError_t launch_paged_tree_tc(const PagedAttn& p, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken);
 cudaError_t launch_paged_tree(const PagedAttn& p, int cache_dtype, int dtype, cudaStream_t st);
 cudaError_t launch_paged_tree_i8(const PagedAttn& p, int dtype, cudaStream_t st);
 cudaError_t launch_paged_tree_e4m3(const PagedAttn& p, int dtype, cudaStream_t st);

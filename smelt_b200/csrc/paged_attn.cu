@@ -14,6 +14,14 @@ uint64_t gpt2q::paged_attn_workspace(int dim, int group) {
 cudaError_t gpt2q::launch_paged_attn(PagedAttn p, int cache_dtype, int dtype, void* work, cudaStream_t st) {
     const bool tree = p.first != nullptr;
     const uint64_t hd = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, hb = tree || p.group > 8 ? 16 : 8;
+    p.page_shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (p.page == 1 << s) p.page_shift = s;
+    if (tree && paged_tree_tc_serves(p, cache_dtype, dtype)) {
+        bool taken = false;
+        const cudaError_t e = launch_paged_tree_tc(p, cache_dtype, dtype, work, st, &taken);
+        if (taken || e != cudaSuccess) return e;
+    }
     char* at = static_cast<char*>(work);
     p.meta = reinterpret_cast<int4*>(at);
     at += MAX_CTAS * 16;
@@ -22,9 +30,6 @@ cudaError_t gpt2q::launch_paged_attn(PagedAttn p, int cache_dtype, int dtype, vo
     p.warp_part = reinterpret_cast<float*>(at);
     at += MAX_CTAS * MAX_WARPS * hb * (hd + 4) * 4;
     p.block_ml = reinterpret_cast<float2*>(at);
-    p.page_shift = -1;
-    for (int s = 0; s < 31; ++s)
-        if (p.page == 1 << s) p.page_shift = s;
     if (tree) return launch_paged_tree(p, cache_dtype, dtype, st);
     if (cache_dtype == GPT2Q_I8) return launch_paged_attn_i8(p, dtype, st);
     if (cache_dtype == GPT2Q_E4M3) return launch_paged_attn_e4m3(p, dtype, st);

@@ -630,8 +630,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                                 }
                             }
                         // a score's columns are heads 2 (lane % 4) + {0, 1}
-                        fac[2 * nt] = sl2 * __shfl_sync(0xffffffffu, up, (lane & 3) * 8);
-                        fac[2 * nt + 1] = sl2 * __shfl_sync(0xffffffffu, up, (lane & 3) * 8 + 4);
+                        fac[2 * nt] = fmaxf(sl2 * __shfl_sync(0xffffffffu, up, (lane & 3) * 8), 1.17549435e-38f);
+                        fac[2 * nt + 1] = fmaxf(sl2 * __shfl_sync(0xffffffffu, up, (lane & 3) * 8 + 4), 1.17549435e-38f);
                     }
                 }
             }

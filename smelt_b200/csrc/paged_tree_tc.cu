@@ -1,0 +1,1021 @@
+// Attention of drafted tokens over a paged cache on tcgen05 tiles: for 16-bit queries of which a kv head has many per row.
+//
+//   out[t][h] = sum_j softmax_j(scale q[t][h] . K[j]) V[j], j over the prefix and what t's mask names
+//
+// A kv head's queries of one row (tokens times its query heads) are the rows of the products, 128 to a tile, so that what is
+// read of the cache is used 128 times. The work is one flat list of tiles of 128 keys, ordered by row, kv head, block of 256
+// queries and position; each block takes a range of equal length, whatever the rows' lengths are, and a second kernel joins
+// what lies in several ranges. Results do not depend on the order in which blocks run.
+//
+// A block has one warp that starts the TMA copies, one that issues the MMAs, four that prepare operands, and two streams of
+// four softmax warps, a thread per query (TMEM lane), so that one stream's exponentials run beside the other's MMAs:
+//   S = Q K^T       M = 128 queries, N = 128 keys; Q and K from shared memory
+//   P = 2^(S - m)   in 16 bits over S's own TMEM columns
+//   O += P V        M = 128, N = head dim, K = 128 keys; P from TMEM, V from shared memory, O in TMEM
+// With more than 128 queries each stream has its own and both use every tile of keys; with fewer both have the same
+// queries, take tiles in turn, and are joined at the end. O is rescaled only when the maximum has risen by more than
+// 2^8 (weights stay below that, and the sum has the same reference).
+//
+// 8-bit caches: the preparing warps write the codes as fp16, in which they are exact; keys' scales multiply the scores and
+// values' scales the weights, both in fp32. The values' scales are held relative to the largest exponent so far, so that
+// weight times scale stays in fp16's range. bf16 queries are scaled per row by a power of two that brings the largest
+// element to [2^10, 2^11), and are exact in fp16 down to 2^-24 of it.
+//
+// A weight is rounded to 16 bits, once (bf16 2^-9, fp16 2^-12 of itself): as large as the output's own rounding, and of
+// random sign over the keys. fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdlib>
+#include <type_traits>
+
+#include "device_op.cuh"
+#include "gpt2q.h"
+#include "paged.h"
+
+namespace gpt2q {
+namespace {
+
+constexpr int QT = 128, KT = 128;  // queries and keys of a tile
+constexpr int SB = 2 * QT;         // queries of a block of queries
+constexpr int CTAS = 148;          // one per SM of a B200
+constexpr int WARPS = 14, THREADS = WARPS * 32;
+constexpr int W_MMA = 8, W_TMA = 9, W_PREP = 10;  // warps 0-3 and 4-7: the two streams
+constexpr int TILES = 4;           // of which scales and masks are kept: a tile's are read before its weights are handed on, and
+                                   // its slots are written again only after that
+constexpr int FLAGS = 8;           // of which page flags are kept: the copies may be four tiles ahead
+constexpr int WAIT_TRIES = 1 << 19;  // of about 1.5 us: 0.8 s
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float STALE = 8.f;  // log2 of the largest weight
+
+template <class TC_, class TI_, int HD_>
+struct Cfg {
+    using TC = TC_;
+    using TI = TI_;
+    static constexpr int HD = HD_;
+    static constexpr bool Q8 = sizeof(TC) == 1;
+    using CT = std::conditional_t<Q8, __half, TC>;
+    static constexpr bool HALF = std::is_same<CT, __half>::value;
+    static constexpr bool RANGE = HALF && !std::is_same<TI, __half>::value;
+    static constexpr int PIECES = HD / 64;               // of 128 bytes, of a 16-bit row
+    static constexpr int PIECE = KT * 128;               // bytes of a tile's piece
+    static constexpr int TILE = PIECES * PIECE;          // 16-bit tile of 128 rows
+    static constexpr int SLOTS = HD == 128 ? (Q8 ? 3 : 4) : (Q8 ? 4 : 8);  // 16-bit tiles of keys or values
+    static constexpr int RAWS = Q8 ? (HD == 128 ? 3 : 4) : 0;              // 8-bit tiles, rows of 128 bytes
+    static constexpr int OFF_KV = 2 * TILE, OFF_RAW = OFF_KV + SLOTS * TILE, SMEM = OFF_RAW + RAWS * PIECE + 1024;
+    static constexpr int LOADS = Q8 ? RAWS : SLOTS;      // slots that copies go to
+    static constexpr int BOXES = Q8 ? 1 : PIECES;        // of 128 bytes, that a row is copied in
+    // fp16 weights are held times 2^6: 2^(8 + 6) and a scale below 2 stay in range, and small ones stay normal numbers
+    static constexpr float shift() { return HALF ? 6.f : 0.f; }
+};
+
+struct Args {
+    PagedAttn p;
+    int box;           // keys of a TMA box
+    int stall;         // for the test of waits that run out
+    float* part;       // [block][2][SB][dims]
+    float2* part_ml;   // [block][2][SB]
+    int4* meta;        // per block: row (-1: none), kv head, block of queries, last block of its last segment
+};
+
+// ------------------------------------------------------------------ the list of tiles
+struct Row {
+    int row, prefix, n, token, queries, end, blocks;
+    bool over;
+};
+struct Seg {
+    Row r;
+    int kvh, sb, j0, j1, nt;  // tiles j0 .. j1 - 1 of its nt
+    __device__ __forceinline__ int queries() const { return min(SB, r.queries - sb * SB); }
+    __device__ __forceinline__ bool pair() const { return queries() > QT; }
+};
+
+__device__ __forceinline__ Row enter(const PagedAttn& p, int row) {
+    Row r{row, 0, 0, 0, 0, 0, 0, false};
+    if (row >= p.n_rows) return r;
+    const int a = __ldcg(p.first + row), b = __ldcg(p.first + row + 1);
+    r.token = min(max(a, 0), p.n_tokens);
+    r.n = max(min(b, p.n_tokens) - r.token, 0);
+    if (r.n == 0) return r;
+    r.prefix = max(__ldcg(p.lens + row), 0);
+    r.over = (long long)r.prefix + r.n > p.cap;
+    r.end = r.over ? p.cap : r.prefix + r.n;
+    r.queries = r.n * p.group;
+    r.blocks = (r.queries + SB - 1) / SB;
+    return r;
+}
+// Tiles of blocks of queries 0 .. sb - 1 of a kv head. Under a mask every block has those of all keys. A chain's block ends with its
+// last query's own key: blocks but the last have ceil((prefix + ceil(256 (x + 1) / group)) / 128) =
+// floor((2 x + c) / group) tiles, whose sum goes by whole periods of `group` blocks.
+__device__ __forceinline__ int tiles_of(const PagedAttn& p, const Row& r, int sb) {
+    int end = r.end;
+    if (!p.mask && !r.over && sb < r.blocks - 1) end = r.prefix + ((sb + 1) * SB - 1) / p.group + 1;
+    return (end + KT - 1) / KT;
+}
+__device__ __forceinline__ long long quotient(long long a, int b) { return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+__device__ __forceinline__ long long tiles_before(const PagedAttn& p, const Row& r, int sb) {
+    if (p.mask || r.over) return (long long)sb * tiles_of(p, r, 0);
+    const int G = p.group, x = min(sb, r.blocks - 1);
+    const long long c = ((long long)r.prefix * G + 2 * KT + (long long)KT * G - 1) / KT;
+    const int q = x / G, rest = x - q * G;
+    long long sum = (long long)G * q * (q - 1) + (long long)2 * q * rest;
+    for (int i = 0; i < (q ? G : rest); ++i) sum += quotient(2 * i + c, G) * (q + (i < rest ? 1 : 0));
+    return sum + (sb == r.blocks && r.blocks > 0 ? tiles_of(p, r, sb - 1) : 0);
+}
+
+struct Range {
+    long long a, b;      // this block's tiles
+    int row;             // where it begins
+    long long rem;       // tiles before it in that row
+};
+
+// The segment that lies `rem` tiles into row `row` (or behind it), cut to `left` tiles; false at the end.
+__device__ __forceinline__ bool seek(const PagedAttn& p, Seg& s, int row, long long rem, long long left) {
+    if (left <= 0) return false;
+    Row r = enter(p, row);
+    long long per = tiles_before(p, r, r.blocks);
+    while (rem >= per * p.n_kv) {
+        rem -= per * p.n_kv;
+        if (++row >= p.n_rows) return false;
+        r = enter(p, row);
+        per = tiles_before(p, r, r.blocks);
+    }
+    s.r = r;
+    s.kvh = (int)(rem >> 32 ? rem / per : per >> 32 ? 0 : (uint32_t)rem / (uint32_t)per);
+    rem -= s.kvh * per;
+    int lo = 0, hi = r.blocks - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tiles_before(p, r, mid) <= rem)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    s.sb = lo;
+    s.nt = tiles_of(p, r, lo);
+    s.j0 = (int)(rem - tiles_before(p, r, lo));
+    s.j1 = (int)min((long long)s.nt, s.j0 + left);
+    return true;
+}
+// The one after it.
+__device__ __forceinline__ bool next(const PagedAttn& p, Seg& s, long long left) {
+    if (left <= 0) return false;
+    if (++s.sb >= s.r.blocks) {
+        s.sb = 0;
+        if (++s.kvh >= p.n_kv) {
+            s.kvh = 0;
+            do {
+                if (s.r.row + 1 >= p.n_rows) return false;
+                s.r = enter(p, s.r.row + 1);
+            } while (s.r.n == 0);
+        }
+    }
+    s.nt = tiles_of(p, s.r, s.sb);
+    s.j0 = 0;
+    s.j1 = (int)min((long long)s.nt, left);
+    return true;
+}
+
+// ------------------------------------------------------------------ PTX
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void streams_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <class CT>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    if constexpr (std::is_same<CT, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+template <class CT>
+__device__ __forceinline__ float2 unpack(uint32_t v) {
+    if constexpr (std::is_same<CT, __half>::value)
+        return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+// four neighbouring codes as two pairs of fp16
+template <class TC>
+__device__ __forceinline__ void widen(uint32_t v, uint32_t& a, uint32_t& b) {
+    if constexpr (std::is_same<TC, int8_t>::value) {
+        v ^= 0x80808080u;  // 0x6400 + u is the fp16 number 1024 + u; u = code + 128
+        const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t x = __byte_perm(v, 0x64646464u, 0x4140), y = __byte_perm(v, 0x64646464u, 0x4342);
+        const __half2 hx = __hsub2(*reinterpret_cast<const __half2*>(&x), off), hy = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+        a = *reinterpret_cast<const uint32_t*>(&hx);
+        b = *reinterpret_cast<const uint32_t*>(&hy);
+    } else {
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+            : "=r"(a), "=r"(b)
+            : "r"(v));
+    }
+}
+// byte offset of 16-byte chunk c of row r in a tile of 16-bit rows: pieces of 128 bytes, chunks permuted by the row
+__device__ __forceinline__ uint32_t sw(int r, int c) { return (uint32_t)((c >> 3) * (KT * 128) + r * 128 + (((c ^ r) & 7) << 4)); }
+
+__device__ __forceinline__ uint32_t ones(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
+// Which of keys key0 .. key0 + 31 the row's token t sees.
+__device__ __forceinline__ uint32_t visible(const PagedAttn& p, const Row& r, int t, int key0) {
+    if (!p.mask) return ones(r.prefix + t + 1 - key0);
+    const int j = key0 - r.prefix;  // drafted token of the first key
+    const int* words = p.mask + (long long)(r.token + t) * p.mask_words;
+    const int w = j >> 5, sh = j & 31;
+    uint32_t v = 0;
+    if (w >= 0 && w < p.mask_words) v = (uint32_t)__ldcg(words + w) >> sh;
+    if (sh && w + 1 >= 0 && w + 1 < p.mask_words) v |= (uint32_t)__ldcg(words + w + 1) << (32 - sh);
+    return (v | ones(-j)) & ones(r.end - key0);
+}
+
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+template <class C>
+__global__ void __launch_bounds__(THREADS, 1)
+    k_paged_tree_tc(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using TC = typename C::TC;
+    using TI = typename C::TI;
+    using CT = typename C::CT;
+    constexpr int HD = C::HD;
+    constexpr bool Q8 = C::Q8;
+    const PagedAttn& p = a.p;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ long long cum[THREADS + 1];
+    __shared__ long long wsum[WARPS];
+    __shared__ __align__(8) uint64_t b_load[8], b_free[8];   // copies have landed in a slot; its tile is no longer needed
+    __shared__ __align__(8) uint64_t b_wide[8], b_reuse[8];  // 8-bit: a tile is there in fp16; its slot may be written again
+    __shared__ __align__(8) uint64_t b_prep[TILES];          // 16-bit: a tile of values with drafted tokens is looked through
+    __shared__ __align__(8) uint64_t b_q, b_s[2], b_p[2], b_o[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(16) float s_scale[Q8 ? TILES : 1][2][KT];  // of keys, of values (relative to 2^s_exp)
+    __shared__ uint32_t s_exp[TILES];
+    __shared__ uint32_t s_spoilt[TILES][4];           // drafted tokens' values that are not finite
+    __shared__ int s_bad[FLAGS];                      // a page id is out of range
+    __shared__ float s_up[SB];                        // what a row's queries were scaled by, undone
+    __shared__ float2 s_ml[QT];
+    __shared__ uint32_t s_vexp[QT];
+    __shared__ int s_stuck;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < 8; ++i) {
+            tc::mbar_init(&b_load[i], 1);
+            // 8-bit: the preparing warps; else the products and, of values (odd slots), the preparing warps too, which
+            // wait for every load of such a slot, as a parity cannot tell a phase from the one two before it
+            tc::mbar_init(&b_free[i], Q8 ? 4 : i & 1 ? 5 : 1);
+            tc::mbar_init(&b_wide[i], 4);
+            tc::mbar_init(&b_reuse[i], 1);
+        }
+        for (int i = 0; i < TILES; ++i) tc::mbar_init(&b_prep[i], 4);
+        tc::mbar_init(&b_q, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&b_s[i], 2);
+            tc::mbar_init(&b_p[i], 4);
+            tc::mbar_init(&b_o[i], 1);
+        }
+        s_stuck = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == W_MMA) {
+        tc::tmem_alloc(&tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    if (warp == W_TMA && lane == 0) {
+        tc::prefetch_tmap(&kmap);
+        tc::prefetch_tmap(&vmap);
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    tc::pdl_trigger();  // after the TMEM allocation: dependents hold no columns that this block waits for
+    tc::pdl_wait();
+
+    // ---- this block's range of tiles ----
+    const int nc = (p.n_rows + THREADS - 1) / THREADS;  // rows a thread counts
+    long long mine = 0;
+    for (int r = tid * nc; r < min((tid + 1) * nc, p.n_rows); ++r) {
+        const Row w = enter(p, r);
+        mine += tiles_before(p, w, w.blocks) * p.n_kv;
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int i = 0; i < WARPS; ++i) {
+        if (i < warp) before += wsum[i];
+        total += wsum[i];
+    }
+    cum[tid] = before + inc - mine;
+    __syncthreads();
+    const long long per = (total + gridDim.x - 1) / gridDim.x;
+    const long long t_a = per * blockIdx.x, t_b = min(t_a + per, total);
+    int row0 = 0;
+    long long rem0 = 0;
+    if (t_a < t_b) {
+        int lo = 0, hi = THREADS - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (cum[mid] <= t_a)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        row0 = lo * nc;
+        rem0 = t_a - cum[lo];
+    }
+
+    // Each thread gives up by itself and then waits for nothing more; whoever does says so to all.
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!ok) return;
+        for (int i = 0; i < WAIT_TRIES; ++i)
+            if (tc::mbar_try_wait(bar, parity)) return;
+        ok = false;
+        atomicExch(&s_stuck, 1);
+    };
+
+    Seg s;
+    long long left = t_b - t_a;
+    int g = 0;  // tiles of this block before the segment
+    if (warp == W_TMA) {
+        // ------------------------------------------------------------------ copies
+        const int groups = KT / a.box, x = lane % C::BOXES, gr = lane / C::BOXES;  // a lane per box
+        int e = 0;  // copies to slots so far
+        bool more = seek(p, s, row0, rem0, left);
+        auto look = [&](const Seg& w, int j) {  // the page of the lane's box in tile j; -1: no keys of the row, -2: out of range
+            const int key = j * KT + gr * a.box;
+            if (gr >= groups || key >= w.r.end) return -1;
+            const int id = __ldcg(p.table + (long long)w.r.row * p.ld + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page));
+            return (unsigned)id < (unsigned)p.n_pages ? id : -2;
+        };
+        int page = more ? look(s, s.j0) : -1;
+        while (more) {
+            left -= s.j1 - s.j0;
+            Seg n = s;
+            const bool after = next(p, n, left);
+            for (int j = s.j0; j < s.j1; ++j, ++g) {
+                const int key = j * KT + gr * a.box;
+                const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
+                const int id = page;
+                page = j + 1 < s.j1 ? look(s, j + 1) : after ? look(n, n.j0) : -1;
+                const unsigned there = __ballot_sync(0xffffffffu, id >= 0), bad = __ballot_sync(0xffffffffu, id == -2);
+                for (int v = 0; v < 2; ++v, ++e) {
+                    const int to = e % C::LOADS;
+                    if (e >= C::LOADS) wait(&b_free[to], (e / C::LOADS - 1) & 1);
+                    __syncwarp();
+                    const bool go = __all_sync(0xffffffffu, ok);
+                    if (lane == 0) {
+                        if (v == 0) s_bad[g % FLAGS] = bad != 0;
+                        if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * a.box * 128 + a.stall);
+                    }
+                    __syncwarp();
+                    if (go && id >= 0)
+                        tma_load_4d(tc::smem_u32(smem + (Q8 ? C::OFF_RAW : C::OFF_KV) + to * (Q8 ? C::PIECE : C::TILE) + x * C::PIECE + gr * a.box * 128),
+                                    v ? &vmap : &kmap, x * (128 / (int)sizeof(TC)), slot, s.kvh, id, tc::smem_u32(&b_load[to]));
+                    if (!go) ok = false;
+                }
+            }
+            s = n;
+            more = after;
+        }
+        // copies that nobody waited for may still be on their way when a wait has run out
+        for (int i = max(0, e - C::LOADS); i < e && lane == 0; ++i)
+            for (int k = 0; k < WAIT_TRIES / 8 && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
+    } else if (warp == W_MMA) {
+        // ------------------------------------------------------------------ products
+        constexpr uint32_t BF = C::HALF ? 0u : (1u << 7) | (1u << 10);  // operands' format: fp16 or bf16
+        constexpr uint32_t idesc_s = tc::idesc_f16_f32(QT, KT) | BF, idesc_o = tc::idesc_f16_f32_bmn(QT, HD) | BF;
+        if (lane == 0) {
+            uint64_t* there = Q8 ? b_wide : b_load;
+            uint64_t* done = Q8 ? b_reuse : b_free;
+            const uint32_t q32 = tc::smem_u32(smem), kv32 = tc::smem_u32(smem + C::OFF_KV);
+            uint32_t np[2] = {0, 0}, specials = 0;
+            bool more = seek(p, s, row0, rem0, left);
+            for (int seg = 0; more; ++seg) {
+                left -= s.j1 - s.j0;
+                const bool pair = s.pair();
+                const int T = s.j1 - s.j0, n0 = pair ? T : (T + 1) / 2, n1 = pair ? T : T / 2;
+                // tiles from here on have values that are looked through
+                const int special = max(s.r.prefix / KT, s.j0);
+                wait(&b_q, seg & 1);
+                auto tile = [&](int st, int u) { return pair ? u : 2 * u + st; };
+                auto scores = [&](int st, int u) {
+                    const int e = 2 * (g + tile(st, u)), at = e % C::SLOTS;
+                    wait(&there[at], (e / C::SLOTS) & 1);
+                    tc::tc_fence_after();
+                    const uint32_t q = q32 + (pair ? st : 0) * C::TILE, k = kv32 + at * C::TILE;
+                    if (ok) {
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            const uint32_t o = (ks >> 2) * C::PIECE + (ks & 3) * 32;
+                            tc::mma_f16(tmem + st * KT, tc::desc_sw128(q + o), tc::desc_sw128(k + o), idesc_s, ks > 0);
+                        }
+                    }
+                    tc::mma_commit(&b_s[st]);
+                    if (!pair || st == 1) tc::mma_commit(&done[at]);
+                    tc::mbar_arrive(&b_s[st]);  // what this thread has seen of the tile's flags
+                };
+                if (n0 > 0) scores(0, 0);
+                if (n1 > 0) scores(1, 0);
+                for (int u = 0; u < n0; ++u) {
+                    for (int st = 0; st < 2; ++st) {
+                        if (u >= (st ? n1 : n0)) continue;
+                        const int t = tile(st, u), e = 2 * (g + t) + 1, at = e % C::SLOTS;
+                        wait(&b_p[st], np[st]++ & 1);
+                        wait(&there[at], (e / C::SLOTS) & 1);
+                        if (!Q8 && s.j0 + t >= special) {
+                            const uint32_t k = specials + (s.j0 + t - special);
+                            wait(&b_prep[k % TILES], (k / TILES) & 1);
+                        }
+                        tc::tc_fence_after();
+                        if (ok) {
+#pragma unroll
+                            for (int ks = 0; ks < KT / 16; ++ks)
+                                mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + ks * 8,
+                                           tc::desc_sw128_mn(kv32 + at * C::TILE + ks * 2048, C::PIECE), idesc_o, u > 0 || ks > 0);
+                        }
+                        if (!pair || st == 1) tc::mma_commit(&done[at]);
+                        if (u + 1 < (st ? n1 : n0))
+                            scores(st, u + 1);
+                        else
+                            tc::mma_commit(&b_o[st]);
+                    }
+                }
+                specials += max(s.j1 - special, 0);
+                g += T;
+                more = next(p, s, left);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= W_PREP) {
+        // ------------------------------------------------------------------ operands
+        const int i = tid - W_PREP * 32;
+        bool more = seek(p, s, row0, rem0, left);
+        if constexpr (Q8) {
+            int e = 0;
+            while (more) {
+                left -= s.j1 - s.j0;
+                uint32_t vexp = 1;
+                for (int j = s.j0; j < s.j1; ++j, ++g) {
+                    const int key = j * KT + i;
+                    float sc[2] = {0.f, 0.f};
+                    if (key < s.r.end) {
+                        const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
+                        const int id = __ldcg(p.table + (long long)s.r.row * p.ld + pg);
+                        if ((unsigned)id < (unsigned)p.n_pages) {
+                            const long long at = (long long)id * p.s_ps + (long long)s.kvh * p.s_hs + (long long)(key - pg * p.page) * p.s_ts;
+                            sc[0] = __ldcg(p.k_scale + at);
+                            sc[1] = __ldcg(p.v_scale + at);
+                        }
+                    }
+                    const bool drafted = (j + 1) * KT > s.r.prefix;
+                    for (int v = 0; v < 2; ++v, ++e) {
+                        const int from = e % C::RAWS, to = e % C::SLOTS;
+                        if (e >= C::SLOTS) wait(&b_reuse[to], (e / C::SLOTS - 1) & 1);
+                        bool spoilt = false;
+                        if (v == 0) {
+                            s_scale[g % TILES][0][i] = sc[0];
+                        } else {
+                            spoilt = key >= s.r.prefix && !isfinite(sc[1]);
+                            if (drafted) {
+                                const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
+                                if (lane == 0) s_spoilt[g % TILES][warp - W_PREP] = b;
+                            }
+                            if (spoilt) sc[1] = 0.f;
+                            // the largest exponent of the tile's scales, over the four warps
+                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
+                            if (lane == 0) wsum[W_PREP + warp - W_PREP] = m;
+                            asm volatile("bar.sync 2, 128;" ::: "memory");
+                            uint32_t x = vexp;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
+                            vexp = min(x, 253u);
+                            s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
+                            if (i == 0) s_exp[g % TILES] = vexp;
+                            asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again; the masks are there
+                        }
+                        wait(&b_load[from], (e / C::RAWS) & 1);
+                        const unsigned char* src = smem + C::OFF_RAW + from * C::PIECE;
+                        unsigned char* dst = smem + C::OFF_KV + to * C::TILE;
+                        // 16 codes at a time. Eight lanes have four chunks of two rows that differ in bits 0 and 2, so that the
+                        // reads and the writes of eight lanes each meet all banks once
+#pragma unroll 4
+                        for (int it = 0; it < HD / 16; ++it) {
+                            const int x = it * 128 + i, c4 = x & 3, odd = x >> 2 & 1;
+                            int c, r;
+                            if constexpr (HD == 128) {
+                                c = (x >> 3 & 1) * 4 + c4;
+                                const int pr = x >> 4;  // pair of rows: 0..63
+                                r = (pr >> 2) * 8 + (pr & 3);
+                            } else {
+                                c = c4;
+                                const int pr = x >> 3;
+                                r = (pr >> 2) * 8 + (pr & 3);
+                            }
+                            if (odd) r ^= 5;
+                            uint4 w = *reinterpret_cast<const uint4*>(src + r * 128 + (((c ^ r) & 7) << 4));
+                            if (v && drafted) {
+                                const int k = j * KT + r;
+                                bool drop = k >= s.r.end;
+                                if (!std::is_same<TC, int8_t>::value && k >= s.r.prefix && !drop) {
+                                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                                    bool nan = false;
+#pragma unroll
+                                    for (int z = 0; z < 4; ++z) nan |= __vcmpeq4(u[z] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+                                    if (nan) {
+                                        atomicOr(&s_spoilt[g % TILES][r >> 5], 1u << (r & 31));
+                                        drop = true;
+                                    }
+                                }
+                                if (drop) w = make_uint4(0, 0, 0, 0);
+                            }
+                            uint4 lo, hi;
+                            widen<TC>(w.x, lo.x, lo.y);
+                            widen<TC>(w.y, lo.z, lo.w);
+                            widen<TC>(w.z, hi.x, hi.y);
+                            widen<TC>(w.w, hi.z, hi.w);
+                            *reinterpret_cast<uint4*>(dst + sw(r, 2 * c)) = lo;
+                            *reinterpret_cast<uint4*>(dst + sw(r, 2 * c + 1)) = hi;
+                        }
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tc::mbar_arrive(&b_free[from]);
+                            tc::mbar_arrive(&b_wide[to]);
+                        }
+                    }
+                }
+                more = next(p, s, left);
+            }
+        } else {
+            static_assert(Q8 || C::SLOTS % 2 == 0, "keys in even slots, values in odd ones");
+            uint32_t specials = 0;
+            while (more) {
+                left -= s.j1 - s.j0;
+                for (int j = s.j0; j < s.j1; ++j) {
+                    const int e = 2 * (g + j - s.j0) + 1, at = e % C::SLOTS, key = j * KT + i;
+                    wait(&b_load[at], (e / C::SLOTS) & 1);
+                    if (j < s.r.prefix / KT) {
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&b_free[at]);
+                        continue;
+                    }
+                    unsigned char* v = smem + C::OFF_KV + at * C::TILE;
+                    bool spoilt = false;
+                    if (key >= s.r.prefix && key < s.r.end) {
+#pragma unroll
+                        for (int c = 0; c < HD / 8; ++c) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(v + sw(i, c));
+                            constexpr uint32_t E = C::HALF ? 0x7c00u : 0x7f80u;
+                            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) spoilt |= (u[z] & E) == E || (u[z] >> 16 & E) == E;
+                        }
+                    }
+                    if (spoilt || key >= s.r.end)
+#pragma unroll
+                        for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(v + sw(i, c)) = make_uint4(0, 0, 0, 0);
+                    const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
+                    if (lane == 0) s_spoilt[specials % TILES][warp - W_PREP] = b;
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc::mbar_arrive(&b_prep[specials % TILES]);
+                        tc::mbar_arrive(&b_free[at]);
+                    }
+                    ++specials;
+                }
+                g += s.j1 - s.j0;
+                more = next(p, s, left);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ softmax: a thread per query
+        const int st = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t t_s = lanes + st * KT, t_o = lanes + 256 + st * HD;
+        const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);
+        uint32_t ns = 0, no = 0, specials = 0;
+        bool more = seek(p, s, row0, rem0, left);
+        while (more) {
+            left -= s.j1 - s.j0;
+            const bool pair = s.pair();
+            const int T = s.j1 - s.j0, nu = pair ? T : st ? T / 2 : (T + 1) / 2;
+            const int special = max(s.r.prefix / KT, s.j0);
+            const int qi = s.sb * SB + (pair ? st * QT : 0) + r;  // this thread's query of the kv head
+            const bool mine_q = qi < s.r.queries;
+            const int tok = (int)((unsigned)qi / (unsigned)p.group), to = s.r.token + tok, head = s.kvh * p.group + qi - tok * p.group;
+            // ---- queries ----
+            if (pair || st == 0) {
+                uint32_t w[HD / 2];
+                const char* src = static_cast<const char*>(p.q) + ((long long)to * p.q_ts + (long long)head * p.q_hs) * 2;
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c) {
+                    const uint4 v = mine_q && c * 8 < p.dim ? __ldcg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+                    w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+                }
+                float up = 1.f;
+                if constexpr (C::RANGE) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int c = 0; c < HD / 2; ++c) top = max(top, max(w[c] & 0x7fffu, w[c] >> 16 & 0x7fffu));
+                    int e = (int)(top >> 7);  // biased exponent
+                    e = e == 0 || e == 255 ? 127 : min(max(e, 12), 252);
+                    const float down = __uint_as_float((uint32_t)(264 - e) << 23);
+                    up = __uint_as_float((uint32_t)(e - 10) << 23);
+#pragma unroll
+                    for (int c = 0; c < HD / 2; ++c) {
+                        const float2 f = unpack<TI>(w[c]);
+                        w[c] = pack<CT>(f.x * down, f.y * down);
+                    }
+                }
+                if (p.scale < 0.f) {
+#pragma unroll
+                    for (int c = 0; c < HD / 2; ++c) w[c] ^= 0x80008000u;
+                }
+                unsigned char* dst = smem + st * C::TILE;
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(dst + sw(r, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                s_up[st * QT + r] = up;
+                tc::fence_proxy_async_smem();
+            }
+            tc::tc_fence_before();
+            streams_sync();
+            if (tid == 0) tc::mbar_arrive(&b_q);
+            const float fac = fmaxf(sl2 * s_up[(pair ? st * QT : 0) + r], 1.17549435e-38f);  // not 0: a masked score of -inf stays one
+            float m = -INFINITY, l = s.r.over ? NAN : 0.f;  // reference of the weights, in units before the factor; their sum
+            uint32_t vexp = 1;
+            const bool idle = s.sb * SB + (pair ? st * QT : 0) + quarter * 32 >= s.r.queries;  // no query in this warp
+            int bad = s.r.over ? GPT2Q_STATUS_POSITION : 0;
+            for (int u = 0; u < nu; ++u) {
+                const int t = pair ? u : 2 * u + st, j = s.j0 + t, gt = (g + t) % TILES;
+                wait(&b_s[st], ns++ & 1);
+                tc::tc_fence_after();
+                if (s_bad[(g + t) % FLAGS]) bad |= GPT2Q_STATUS_PAGE;
+                const bool look = j >= special;  // keys that not every query sees
+                uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                if (look && !idle) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) vis[c] = mine_q ? visible(p, s.r, tok, j * KT + c * 32) : 0u;
+                }
+                const float* ks = s_scale[Q8 ? gt : 0][0];
+                const float* vs = s_scale[Q8 ? gt : 0][1];
+                float mx = -INFINITY;
+                __syncwarp();
+                auto load = [&](int c, float* v) {
+                    tc::tmem_ld32(t_s + c * 32, v);
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(ks + c * 32 + k);
+                            const float2 x = mul2(make_float2(v[k], v[k + 1]), make_float2(f.x, f.y)), y = mul2(make_float2(v[k + 2], v[k + 3]), make_float2(f.z, f.w));
+                            v[k] = x.x, v[k + 1] = x.y, v[k + 2] = y.x, v[k + 3] = y.y;
+                        }
+                    }
+                    if (look) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = vis[c] >> k & 1 ? v[k] : -INFINITY;
+                    }
+                };
+                if (!idle) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        load(c, v);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
+                    }
+                }
+                // values' scales and what is to be known of them
+                uint32_t e = vexp;
+                if constexpr (Q8) {
+                    const int en = 2 * (g + t) + 1;
+                    wait(&b_wide[en % C::SLOTS], (en / C::SLOTS) & 1);
+                    e = s_exp[gt];
+                } else if (look) {
+                    const uint32_t k = specials + (j - special);
+                    wait(&b_prep[k % TILES], (k / TILES) & 1);
+                }
+                if (look) {
+                    const uint32_t* sp = s_spoilt[Q8 ? gt : (specials + (j - special)) % TILES];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (vis[c] & sp[c]) l = NAN;
+                }
+                // a new reference, and the results so far in it
+                const float mn = fmaxf(m, mx);
+                const bool raise = (mn - m) * fac > STALE || (m == -INFINITY && mn > -INFINITY);
+                float al = 1.f;
+                if (raise) {
+                    al = m == -INFINITY ? 0.f : ex2((m - mn) * fac);
+                    m = mn;
+                }
+                l *= al;
+                if constexpr (Q8) {
+                    if (e != vexp) {
+                        al *= e - vexp > 126 ? 0.f : __uint_as_float((127 - (e - vexp)) << 23);
+                        vexp = e;
+                    }
+                }
+                if (u > 0 && __any_sync(0xffffffffu, al != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float v[32];
+                        tc::tmem_ld32(t_o + c * 32, v);
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(v[k] * al);
+                        tmem_st16(t_o + c * 32, w);
+                        tmem_st16(t_o + c * 32 + 16, w + 16);
+                    }
+                }
+                if (!idle) {
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        load(c, v);
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            // (S - m) before the factor, where m's own score gives exactly 0
+                            const float2 d = fma2(add2(make_float2(v[k], v[k + 1]), make_float2(-ref, -ref)), make_float2(fac, fac), make_float2(C::shift(), C::shift()));
+                            float2 x = make_float2(ex2(d.x), ex2(d.y));
+                            if constexpr (Q8) {
+                                sum = add2(sum, x);
+                                const float2 f = *reinterpret_cast<const float2*>(vs + c * 32 + k);
+                                x = mul2(x, f);
+                                w[k / 2] = pack<CT>(x.x, x.y);
+                            } else {
+                                w[k / 2] = pack<CT>(x.x, x.y);
+                                sum = add2(sum, unpack<CT>(w[k / 2]));  // of the weights that the product has
+                            }
+                        }
+                        tmem_st16(t_s + c * 16, w);
+                    }
+                    l += sum.x + sum.y;
+                }
+                tmem_wait_st();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&b_p[st]);
+            }
+            if (nu > 0) wait(&b_o[st], no++ & 1);
+            tc::tc_fence_after();
+            if (!ok || *(volatile int*)&s_stuck) bad |= GPT2Q_STATUS_TIMEOUT;
+            if (bad) l = NAN;
+            if (bad && p.status && lane == 0) atomicOr(p.status, bad);
+            // ---- results ----
+            float wa = 1.f, wb = 0.f;  // weights of the streams' results
+            if (!pair) {
+                if (st == 1) {
+                    s_ml[r] = make_float2(m, l);
+                    s_vexp[r] = vexp;
+                }
+                tc::tc_fence_before();
+                streams_sync();
+                tc::tc_fence_after();
+                if (st == 0) {
+                    const float2 o = T > 1 ? s_ml[r] : make_float2(-INFINITY, s_ml[r].y);
+                    const float M = fmaxf(m, o.x), ms = M == -INFINITY ? 0.f : M;
+                    wa = ex2((m - ms) * fac), wb = ex2((o.x - ms) * fac);
+                    l = l * wa + o.y * wb;
+                    m = M;
+                    if (Q8) wa *= __uint_as_float(vexp << 23), wb *= __uint_as_float(s_vexp[r] << 23);
+                }
+            } else if (Q8) {
+                wa = __uint_as_float(vexp << 23);
+            }
+            if ((pair || st == 0) && !idle) {
+                const bool whole = s.j0 == 0 && s.j1 == s.nt;
+                const int slot = s.j0 > 0 ? 0 : 1, pr = (pair ? st * QT : 0) + r;
+                const long long part = ((long long)blockIdx.x * 2 + slot) * SB + pr;
+                const float f = whole ? inverse(l) : 1.f;
+                wa *= f, wb *= f;
+                const float mlog = m * fac;  // reference, as a power of two
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    float v[32];
+                    __syncwarp();
+                    tc::tmem_ld32(t_o + c * 32, v);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] *= wa;
+                    if (!pair && T > 1) {
+                        float x[32];
+                        tc::tmem_ld32(lanes + 256 + HD + c * 32, x);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], wb, v[k]);
+                    }
+                    if (mine_q) {
+                        if (whole) {
+                            TI* o = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + c * 32;
+#pragma unroll
+                            for (int k = 0; k < 32; k += 8)
+                                if (c * 32 + k < p.dim) store_vec<TI, 8>(o + k, v + k);
+                        } else {
+                            float* o = a.part + part * HD + c * 32;
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        }
+                    }
+                }
+                if (mine_q) {
+                    if (!whole)
+                        a.part_ml[part] = make_float2(mlog, l);
+                    else if (p.lse)
+                        p.lse[(long long)to * p.n_heads + head] = l == 0.f ? -INFINITY : (mlog + log2f(l) - C::shift()) * LN2;
+                }
+            }
+            if (tid == 0 && left <= 0) {  // the range's last segment: where it goes on behind this block
+                const bool on = s.j1 < s.nt && s.j0 == 0;
+                // a segment that also begins before this block belongs to an earlier block's list
+                a.meta[blockIdx.x] = on ? make_int4(s.r.row, s.kvh, s.sb, (int)((t_b - s.j1 + s.nt - 1) / per)) : make_int4(-1, 0, 0, 0);
+            }
+            specials += max(s.j1 - special, 0);
+            g += T;
+            more = next(p, s, left);
+            // no stream writes its queries or results before the other has read what they share
+            tc::tc_fence_before();
+            streams_sync();
+            tc::tc_fence_after();
+        }
+        if (tid == 0 && t_a >= t_b) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) tc::tmem_dealloc(tmem, 512);
+}
+
+// Joins a segment that lies in several blocks' ranges: block c of the first kernel has its beginning (slot 1), the blocks after it
+// up to `last` the rest (slot 0). A warp per query.
+template <class TI, int HD>
+__global__ void __launch_bounds__(256) k_paged_tree_join(const __grid_constant__ Args a, float shift) {
+    tc::pdl_trigger();
+    tc::pdl_wait();
+    const PagedAttn& p = a.p;
+    const int c = blockIdx.x, lane = threadIdx.x & 31, pr = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int4 meta = __ldcg(a.meta + c);
+    if (meta.x < 0) return;
+    const Row r = enter(p, meta.x);
+    const int qi = meta.z * SB + pr;
+    if (pr >= SB || qi >= r.queries) return;
+    const int tok = (int)((unsigned)qi / (unsigned)p.group), to = r.token + tok, head = meta.y * p.group + qi - tok * p.group;
+    const int n = meta.w - c + 1;
+    auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * SB + pr; };
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(a.part_ml + at(i)).x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    constexpr int V = HD / 32;
+    float o[V] = {};
+    for (int i = 0; i < n; ++i) {
+        const float2 ml = __ldcg(a.part_ml + at(i));
+        const float w = ex2(ml.x - ms);
+        L = fmaf(ml.y, w, L);
+        const float* x = a.part + at(i) * HD + lane * V;
+        float v[V];
+        if constexpr (V == 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(x));
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(x));
+            v[0] = f.x, v[1] = f.y;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = fmaf(v[k], w, o[k]);
+    }
+    const float f = inverse(L);
+    TI* out = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + lane * V;
+    if (lane * V < p.dim) {
+        *reinterpret_cast<uint32_t*>(out) = pack<TI>(o[0] * f, o[1] * f);
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + 2) = pack<TI>(o[2] * f, o[3] * f);
+    }
+    if (lane == 0 && p.lse) p.lse[(long long)to * p.n_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L) - shift) * LN2;
+}
+
+// ------------------------------------------------------------------ host
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encoder() {
+    static const EncodeTiledFn fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<EncodeTiledFn>(ptr)
+                   : nullptr;
+    }();
+    return fn;
+}
+
+// A pool as a tensor [page][head][slot][dim], in boxes of 128 bytes of `box` slots; dims past the head's own are read as zero.
+template <class C>
+bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base, int box) {
+    using TC = typename C::TC;
+    const auto encode = encoder();
+    if (!encode) return false;
+    const auto type = C::Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : C::HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.dim, (cuuint64_t)p.page, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+    // the stride of a dimension of one element does not matter, but may not be 0
+    const cuuint64_t row = ((cuuint64_t)p.dim * sizeof(TC) + 15) / 16 * 16;
+    const cuuint64_t strides[3] = {p.page == 1 ? row : p.ts16 * 16ull, p.n_kv == 1 ? row : p.hs16 * 16ull, p.n_pages == 1 ? row : p.ps16 * 16ull};
+    const cuuint32_t b[4] = {(cuuint32_t)(128 / sizeof(TC)), (cuuint32_t)box, 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(m, type, 4, const_cast<void*>(base), dims, strides, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class C>
+cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken) {
+    Args a{};
+    a.p = p;
+    a.box = std::min(KT, p.page & -p.page);
+    CUtensorMap km{}, vm{};
+    if (!make_map<C>(&km, p, p.k, a.box) || !make_map<C>(&vm, p, p.v, a.box)) return cudaSuccess;
+    *taken = true;
+    static const bool stall = std::getenv("GPT2Q_TEST_PAGED_STALL") != nullptr;
+    a.stall = stall ? 16 : 0;
+    char* at = static_cast<char*>(work);
+    a.part = reinterpret_cast<float*>(at);
+    at += (size_t)CTAS * 2 * SB * C::HD * 4;
+    a.part_ml = reinterpret_cast<float2*>(at);
+    at += (size_t)CTAS * 2 * SB * 8;
+    a.meta = reinterpret_cast<int4*>(at);
+    // no more blocks than the longest rows the table can hold would give a tile each
+    const long long rows = std::min(p.n_rows, p.n_tokens), blocks = rows + (long long)p.n_tokens * p.group / SB;
+    const long long tiles = (p.cap + (long long)KT - 1) / KT;
+    const int grid = (int)std::clamp<long long>(tiles > CTAS ? CTAS : tiles * std::min<long long>(blocks, CTAS) * p.n_kv, 1, CTAS);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        e = cudaFuncSetAttribute(k_paged_tree_tc<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready |= 1ull << dev;
+    }
+    e = launch_dependent(k_paged_tree_tc<C>, dim3(grid), dim3(THREADS), C::SMEM, st, a, km, vm);
+    if (e != cudaSuccess || grid == 1) return e;
+    const long long most = std::min<long long>(SB, (long long)p.n_tokens * p.group);
+    return launch_dependent(k_paged_tree_join<typename C::TI, C::HD>, dim3(grid, (unsigned)((most + 7) / 8)), dim3(256), 0, st, a, C::shift());
+}
+
+template <class TC, class TI>
+cudaError_t by_dim(const PagedAttn& p, void* work, cudaStream_t st, bool* taken) {
+    return p.dim <= 64 ? launch<Cfg<TC, TI, 64>>(p, work, st, taken) : launch<Cfg<TC, TI, 128>>(p, work, st, taken);
+}
+
+}  // namespace
+
+uint64_t paged_tree_tc_workspace(int dim) {
+    return dim > 128 ? 0 : (uint64_t)CTAS * (2 * SB * ((dim <= 64 ? 64 : 128) * 4 + 8) + 16);
+}
+
+bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
+    return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
+           (long long)p.n_tokens * p.group > 16LL * p.n_rows;
+}
+
+cudaError_t launch_paged_tree_tc(const PagedAttn& p, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken) {
+    if (cache_dtype == GPT2Q_F16) return by_dim<__half, __half>(p, work, st, taken);
+    if (cache_dtype == GPT2Q_BF16) return by_dim<bf16, bf16>(p, work, st, taken);
+    if (cache_dtype == GPT2Q_I8)
+        return dtype == GPT2Q_F16 ? by_dim<int8_t, __half>(p, work, st, taken) : by_dim<int8_t, bf16>(p, work, st, taken);
+    return dtype == GPT2Q_F16 ? by_dim<__nv_fp8_e4m3, __half>(p, work, st, taken) : by_dim<__nv_fp8_e4m3, bf16>(p, work, st, taken);
+}
+
+}  // namespace gpt2q
