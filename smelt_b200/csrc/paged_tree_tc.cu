@@ -10,7 +10,7 @@
 // A block has one warp that starts the TMA copies, one that issues the MMAs, four that prepare operands, and two streams of
 // four softmax warps, a thread per query (TMEM lane), so that one stream's exponentials run beside the other's MMAs:
 //   S = Q K^T       M = 128 queries, N = 128 keys; Q and K from shared memory
-//   P = 2^(S - m)   in 16 bits over S's own TMEM columns
+//   P = 2^(S - m)   in 16 bits over the later half of S's own TMEM columns
 //   O += P V        M = 128, N = head dim, K = 128 keys; P from TMEM, V from shared memory, O in TMEM
 // With more than 128 queries each stream has its own and both use every tile of keys; with fewer both have the same
 // queries, take tiles in turn, and are joined at the end. O is rescaled only when the maximum has risen by more than
@@ -42,12 +42,14 @@ namespace {
 constexpr int QT = 128, KT = 128;  // queries and keys of a tile
 constexpr int SB = 2 * QT;         // queries of a block of queries
 constexpr int CTAS = 148;          // one per SM of a B200
-constexpr int WARPS = 14, THREADS = WARPS * 32;
-constexpr int W_MMA = 8, W_TMA = 9, W_PREP = 10;  // warps 0-3 and 4-7: the two streams
+// Warps 0-3 and 4-7 are the two streams, 8-11 prepare operands. The streams take registers that the others give
+// up: 2 * 128 * (184 + 72) are the 512 * 128 of the launch.
+constexpr int WARPS = 16, THREADS = WARPS * 32, REGS_SOFTMAX = 184, REGS_OTHERS = 72;
+constexpr int W_PREP = 8, W_MMA = 12, W_TMA = 13;
 constexpr int TILES = 4;           // of which scales and masks are kept: a tile's are read before its weights are handed on, and
                                    // its slots are written again only after that
 constexpr int FLAGS = 8;           // of which page flags are kept: the copies may be four tiles ahead
-constexpr int WAIT_TRIES = 1 << 19;  // of about 1.5 us: 0.8 s
+constexpr int WAIT_TRIES = 1 << 22;  // of at least 20 ns: 0.1 s and more
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float STALE = 8.f;  // log2 of the largest weight
@@ -181,6 +183,13 @@ __device__ __forceinline__ bool next(const PagedAttn& p, Seg& s, long long left)
 }
 
 // ------------------------------------------------------------------ PTX
+// One lane of a warp; code behind it keeps its operands in uniform registers, which behind a comparison of the lane it does not
+// (a product then took 100 cycles to issue).
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -190,11 +199,43 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_de
         "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
+// 32 columns of this thread's lane, which may be used after tmem_wait32 of the same registers
+__device__ __forceinline__ void tmem_ask32(uint32_t at, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait32(float* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at)
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -220,7 +261,7 @@ __device__ __forceinline__ float2 unpack(uint32_t v) {
     if constexpr (std::is_same<CT, __half>::value)
         return __half22float2(*reinterpret_cast<const __half2*>(&v));
     else
-        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 // four neighbouring codes as two pairs of fp16
 template <class TC>
@@ -370,259 +411,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     Seg s;
     long long left = t_b - t_a;
     int g = 0;  // tiles of this block before the segment
-    if (warp == W_TMA) {
-        // ------------------------------------------------------------------ copies
-        const int groups = KT / a.box, x = lane % C::BOXES, gr = lane / C::BOXES;  // a lane per box
-        int e = 0;  // copies to slots so far
-        bool more = seek(p, s, row0, rem0, left);
-        auto look = [&](const Seg& w, int j) {  // the page of the lane's box in tile j; -1: no keys of the row, -2: out of range
-            const int key = j * KT + gr * a.box;
-            if (gr >= groups || key >= w.r.end) return -1;
-            const int id = __ldcg(p.table + (long long)w.r.row * p.ld + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page));
-            return (unsigned)id < (unsigned)p.n_pages ? id : -2;
-        };
-        int page = more ? look(s, s.j0) : -1;
-        while (more) {
-            left -= s.j1 - s.j0;
-            Seg n = s;
-            const bool after = next(p, n, left);
-            for (int j = s.j0; j < s.j1; ++j, ++g) {
-                const int key = j * KT + gr * a.box;
-                const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
-                const int id = page;
-                page = j + 1 < s.j1 ? look(s, j + 1) : after ? look(n, n.j0) : -1;
-                const unsigned there = __ballot_sync(0xffffffffu, id >= 0), bad = __ballot_sync(0xffffffffu, id == -2);
-                for (int v = 0; v < 2; ++v, ++e) {
-                    const int to = e % C::LOADS;
-                    if (e >= C::LOADS) wait(&b_free[to], (e / C::LOADS - 1) & 1);
-                    __syncwarp();
-                    const bool go = __all_sync(0xffffffffu, ok);
-                    if (lane == 0) {
-                        if (v == 0) s_bad[g % FLAGS] = bad != 0;
-                        if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * a.box * 128 + a.stall);
-                    }
-                    __syncwarp();
-                    if (go && id >= 0)
-                        tma_load_4d(tc::smem_u32(smem + (Q8 ? C::OFF_RAW : C::OFF_KV) + to * (Q8 ? C::PIECE : C::TILE) + x * C::PIECE + gr * a.box * 128),
-                                    v ? &vmap : &kmap, x * (128 / (int)sizeof(TC)), slot, s.kvh, id, tc::smem_u32(&b_load[to]));
-                    if (!go) ok = false;
-                }
-            }
-            s = n;
-            more = after;
-        }
-        // copies that nobody waited for may still be on their way when a wait has run out
-        for (int i = max(0, e - C::LOADS); i < e && lane == 0; ++i)
-            for (int k = 0; k < WAIT_TRIES / 8 && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
-    } else if (warp == W_MMA) {
-        // ------------------------------------------------------------------ products
-        constexpr uint32_t BF = C::HALF ? 0u : (1u << 7) | (1u << 10);  // operands' format: fp16 or bf16
-        constexpr uint32_t idesc_s = tc::idesc_f16_f32(QT, KT) | BF, idesc_o = tc::idesc_f16_f32_bmn(QT, HD) | BF;
-        if (lane == 0) {
-            uint64_t* there = Q8 ? b_wide : b_load;
-            uint64_t* done = Q8 ? b_reuse : b_free;
-            const uint32_t q32 = tc::smem_u32(smem), kv32 = tc::smem_u32(smem + C::OFF_KV);
-            uint32_t np[2] = {0, 0}, specials = 0;
-            bool more = seek(p, s, row0, rem0, left);
-            for (int seg = 0; more; ++seg) {
-                left -= s.j1 - s.j0;
-                const bool pair = s.pair();
-                const int T = s.j1 - s.j0, n0 = pair ? T : (T + 1) / 2, n1 = pair ? T : T / 2;
-                // tiles from here on have values that are looked through
-                const int special = max(s.r.prefix / KT, s.j0);
-                wait(&b_q, seg & 1);
-                auto tile = [&](int st, int u) { return pair ? u : 2 * u + st; };
-                auto scores = [&](int st, int u) {
-                    const int e = 2 * (g + tile(st, u)), at = e % C::SLOTS;
-                    wait(&there[at], (e / C::SLOTS) & 1);
-                    tc::tc_fence_after();
-                    const uint32_t q = q32 + (pair ? st : 0) * C::TILE, k = kv32 + at * C::TILE;
-                    if (ok) {
-#pragma unroll
-                        for (int ks = 0; ks < HD / 16; ++ks) {
-                            const uint32_t o = (ks >> 2) * C::PIECE + (ks & 3) * 32;
-                            tc::mma_f16(tmem + st * KT, tc::desc_sw128(q + o), tc::desc_sw128(k + o), idesc_s, ks > 0);
-                        }
-                    }
-                    tc::mma_commit(&b_s[st]);
-                    if (!pair || st == 1) tc::mma_commit(&done[at]);
-                    tc::mbar_arrive(&b_s[st]);  // what this thread has seen of the tile's flags
-                };
-                if (n0 > 0) scores(0, 0);
-                if (n1 > 0) scores(1, 0);
-                for (int u = 0; u < n0; ++u) {
-                    for (int st = 0; st < 2; ++st) {
-                        if (u >= (st ? n1 : n0)) continue;
-                        const int t = tile(st, u), e = 2 * (g + t) + 1, at = e % C::SLOTS;
-                        wait(&b_p[st], np[st]++ & 1);
-                        wait(&there[at], (e / C::SLOTS) & 1);
-                        if (!Q8 && s.j0 + t >= special) {
-                            const uint32_t k = specials + (s.j0 + t - special);
-                            wait(&b_prep[k % TILES], (k / TILES) & 1);
-                        }
-                        tc::tc_fence_after();
-                        if (ok) {
-#pragma unroll
-                            for (int ks = 0; ks < KT / 16; ++ks)
-                                mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + ks * 8,
-                                           tc::desc_sw128_mn(kv32 + at * C::TILE + ks * 2048, C::PIECE), idesc_o, u > 0 || ks > 0);
-                        }
-                        if (!pair || st == 1) tc::mma_commit(&done[at]);
-                        if (u + 1 < (st ? n1 : n0))
-                            scores(st, u + 1);
-                        else
-                            tc::mma_commit(&b_o[st]);
-                    }
-                }
-                specials += max(s.j1 - special, 0);
-                g += T;
-                more = next(p, s, left);
-            }
-        }
-        __syncwarp();
-    } else if (warp >= W_PREP) {
-        // ------------------------------------------------------------------ operands
-        const int i = tid - W_PREP * 32;
-        bool more = seek(p, s, row0, rem0, left);
-        if constexpr (Q8) {
-            int e = 0;
-            while (more) {
-                left -= s.j1 - s.j0;
-                uint32_t vexp = 1;
-                for (int j = s.j0; j < s.j1; ++j, ++g) {
-                    const int key = j * KT + i;
-                    float sc[2] = {0.f, 0.f};
-                    if (key < s.r.end) {
-                        const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
-                        const int id = __ldcg(p.table + (long long)s.r.row * p.ld + pg);
-                        if ((unsigned)id < (unsigned)p.n_pages) {
-                            const long long at = (long long)id * p.s_ps + (long long)s.kvh * p.s_hs + (long long)(key - pg * p.page) * p.s_ts;
-                            sc[0] = __ldcg(p.k_scale + at);
-                            sc[1] = __ldcg(p.v_scale + at);
-                        }
-                    }
-                    const bool drafted = (j + 1) * KT > s.r.prefix;
-                    for (int v = 0; v < 2; ++v, ++e) {
-                        const int from = e % C::RAWS, to = e % C::SLOTS;
-                        if (e >= C::SLOTS) wait(&b_reuse[to], (e / C::SLOTS - 1) & 1);
-                        bool spoilt = false;
-                        if (v == 0) {
-                            s_scale[g % TILES][0][i] = sc[0];
-                        } else {
-                            spoilt = key >= s.r.prefix && !isfinite(sc[1]);
-                            if (drafted) {
-                                const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
-                                if (lane == 0) s_spoilt[g % TILES][warp - W_PREP] = b;
-                            }
-                            if (spoilt) sc[1] = 0.f;
-                            // the largest exponent of the tile's scales, over the four warps
-                            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
-                            if (lane == 0) wsum[W_PREP + warp - W_PREP] = m;
-                            asm volatile("bar.sync 2, 128;" ::: "memory");
-                            uint32_t x = vexp;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
-                            vexp = min(x, 253u);
-                            s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
-                            if (i == 0) s_exp[g % TILES] = vexp;
-                            asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again; the masks are there
-                        }
-                        wait(&b_load[from], (e / C::RAWS) & 1);
-                        const unsigned char* src = smem + C::OFF_RAW + from * C::PIECE;
-                        unsigned char* dst = smem + C::OFF_KV + to * C::TILE;
-                        // 16 codes at a time. Eight lanes have four chunks of two rows that differ in bits 0 and 2, so that the
-                        // reads and the writes of eight lanes each meet all banks once
-#pragma unroll 4
-                        for (int it = 0; it < HD / 16; ++it) {
-                            const int x = it * 128 + i, c4 = x & 3, odd = x >> 2 & 1;
-                            int c, r;
-                            if constexpr (HD == 128) {
-                                c = (x >> 3 & 1) * 4 + c4;
-                                const int pr = x >> 4;  // pair of rows: 0..63
-                                r = (pr >> 2) * 8 + (pr & 3);
-                            } else {
-                                c = c4;
-                                const int pr = x >> 3;
-                                r = (pr >> 2) * 8 + (pr & 3);
-                            }
-                            if (odd) r ^= 5;
-                            uint4 w = *reinterpret_cast<const uint4*>(src + r * 128 + (((c ^ r) & 7) << 4));
-                            if (v && drafted) {
-                                const int k = j * KT + r;
-                                bool drop = k >= s.r.end;
-                                if (!std::is_same<TC, int8_t>::value && k >= s.r.prefix && !drop) {
-                                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-                                    bool nan = false;
-#pragma unroll
-                                    for (int z = 0; z < 4; ++z) nan |= __vcmpeq4(u[z] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
-                                    if (nan) {
-                                        atomicOr(&s_spoilt[g % TILES][r >> 5], 1u << (r & 31));
-                                        drop = true;
-                                    }
-                                }
-                                if (drop) w = make_uint4(0, 0, 0, 0);
-                            }
-                            uint4 lo, hi;
-                            widen<TC>(w.x, lo.x, lo.y);
-                            widen<TC>(w.y, lo.z, lo.w);
-                            widen<TC>(w.z, hi.x, hi.y);
-                            widen<TC>(w.w, hi.z, hi.w);
-                            *reinterpret_cast<uint4*>(dst + sw(r, 2 * c)) = lo;
-                            *reinterpret_cast<uint4*>(dst + sw(r, 2 * c + 1)) = hi;
-                        }
-                        tc::fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tc::mbar_arrive(&b_free[from]);
-                            tc::mbar_arrive(&b_wide[to]);
-                        }
-                    }
-                }
-                more = next(p, s, left);
-            }
-        } else {
-            static_assert(Q8 || C::SLOTS % 2 == 0, "keys in even slots, values in odd ones");
-            uint32_t specials = 0;
-            while (more) {
-                left -= s.j1 - s.j0;
-                for (int j = s.j0; j < s.j1; ++j) {
-                    const int e = 2 * (g + j - s.j0) + 1, at = e % C::SLOTS, key = j * KT + i;
-                    wait(&b_load[at], (e / C::SLOTS) & 1);
-                    if (j < s.r.prefix / KT) {
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&b_free[at]);
-                        continue;
-                    }
-                    unsigned char* v = smem + C::OFF_KV + at * C::TILE;
-                    bool spoilt = false;
-                    if (key >= s.r.prefix && key < s.r.end) {
-#pragma unroll
-                        for (int c = 0; c < HD / 8; ++c) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(v + sw(i, c));
-                            constexpr uint32_t E = C::HALF ? 0x7c00u : 0x7f80u;
-                            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) spoilt |= (u[z] & E) == E || (u[z] >> 16 & E) == E;
-                        }
-                    }
-                    if (spoilt || key >= s.r.end)
-#pragma unroll
-                        for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(v + sw(i, c)) = make_uint4(0, 0, 0, 0);
-                    const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
-                    if (lane == 0) s_spoilt[specials % TILES][warp - W_PREP] = b;
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tc::mbar_arrive(&b_prep[specials % TILES]);
-                        tc::mbar_arrive(&b_free[at]);
-                    }
-                    ++specials;
-                }
-                g += s.j1 - s.j0;
-                more = next(p, s, left);
-            }
-        }
-    } else {
+    if (warp < W_PREP) {
+        more_registers<REGS_SOFTMAX>();
         // ------------------------------------------------------------------ softmax: a thread per query
         const int st = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -691,33 +481,50 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) vis[c] = mine_q ? visible(p, s.r, tok, j * KT + c * 32) : 0u;
                 }
-                const float* ks = s_scale[Q8 ? gt : 0][0];
                 const float* vs = s_scale[Q8 ? gt : 0][1];
-                float mx = -INFINITY;
-                __syncwarp();
-                auto load = [&](int c, float* v) {
-                    tc::tmem_ld32(t_s + c * 32, v);
+                    float mx = -INFINITY;
+                // scores of a quarter of the keys; the later half stays here until its weights are formed, as the
+                // weights take the columns that it came from, the earlier half is read again
+                float v[2][32];
+                auto scores = [&](int c, float* x) {
                     if constexpr (Q8) {
+                        const float* ks = s_scale[gt][0] + c * 32;
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(ks + c * 32 + k);
-                            const float2 x = mul2(make_float2(v[k], v[k + 1]), make_float2(f.x, f.y)), y = mul2(make_float2(v[k + 2], v[k + 3]), make_float2(f.z, f.w));
-                            v[k] = x.x, v[k + 1] = x.y, v[k + 2] = y.x, v[k + 3] = y.y;
+                            const float4 f = *reinterpret_cast<const float4*>(ks + k);
+                            const float2 y = mul2(make_float2(x[k], x[k + 1]), make_float2(f.x, f.y)), z = mul2(make_float2(x[k + 2], x[k + 3]), make_float2(f.z, f.w));
+                            x[k] = y.x, x[k + 1] = y.y, x[k + 2] = z.x, x[k + 3] = z.y;
                         }
                     }
                     if (look) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = vis[c] >> k & 1 ? v[k] : -INFINITY;
+                        for (int k = 0; k < 32; ++k) x[k] = vis[c] >> k & 1 ? x[k] : -INFINITY;
                     }
                 };
+                auto largest = [&](const float* x) {
+                    float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int k = 4; k < 32; ++k) top[k & 3] = fmaxf(top[k & 3], x[k]);
+                    mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                };
+                __syncwarp();
                 if (!idle) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        load(c, v);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
-                    }
+                    tmem_ask32(t_s, v[0]);
+                    tmem_ask32(t_s + 32, v[1]);
+                    tmem_wait32(v[0]);
+                    tmem_wait32(v[1]);
+                    scores(0, v[0]);
+                    largest(v[0]);
+                    tmem_ask32(t_s + 64, v[0]);
+                    scores(1, v[1]);
+                    largest(v[1]);
+                    tmem_ask32(t_s + 96, v[1]);
+                    tmem_wait32(v[0]);
+                    scores(2, v[0]);
+                    largest(v[0]);
+                    tmem_wait32(v[1]);
+                    scores(3, v[1]);
+                    largest(v[1]);
                 }
                 // values' scales and what is to be known of them
                 uint32_t e = vexp;
@@ -751,43 +558,52 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 }
                 if (u > 0 && __any_sync(0xffffffffu, al != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; ++c) {
+                        uint32_t w[16];
+                        tmem_ld16(t_o + c * 16, w);
 #pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float v[32];
-                        tc::tmem_ld32(t_o + c * 32, v);
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(v[k] * al);
-                        tmem_st16(t_o + c * 32, w);
-                        tmem_st16(t_o + c * 32 + 16, w + 16);
+                        for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(__uint_as_float(w[k]) * al);
+                        tmem_st16(t_o + c * 16, w);
                     }
                 }
                 if (!idle) {
                     const float ref = m == -INFINITY ? 0.f : m;
-                    float2 sum = make_float2(0.f, 0.f);
+                    const float2 nref = make_float2(-ref, -ref), f2 = make_float2(fac, fac), sh = make_float2(C::shift(), C::shift());
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    auto weights = [&](int c, const float* x) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        load(c, v);
-                        uint32_t w[16];
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[8];
 #pragma unroll
-                        for (int k = 0; k < 32; k += 2) {
-                            // (S - m) before the factor, where m's own score gives exactly 0
-                            const float2 d = fma2(add2(make_float2(v[k], v[k + 1]), make_float2(-ref, -ref)), make_float2(fac, fac), make_float2(C::shift(), C::shift()));
-                            float2 x = make_float2(ex2(d.x), ex2(d.y));
-                            if constexpr (Q8) {
-                                sum = add2(sum, x);
-                                const float2 f = *reinterpret_cast<const float2*>(vs + c * 32 + k);
-                                x = mul2(x, f);
-                                w[k / 2] = pack<CT>(x.x, x.y);
-                            } else {
-                                w[k / 2] = pack<CT>(x.x, x.y);
-                                sum = add2(sum, unpack<CT>(w[k / 2]));  // of the weights that the product has
+                            for (int i = 0; i < 8; ++i) {
+                                const int k = h * 16 + i * 2;
+                                // (S - m) before the factor, where m's own score gives exactly 0
+                                const float2 d = fma2(add2(make_float2(x[k], x[k + 1]), nref), f2, sh);
+                                float2 e2 = make_float2(ex2(d.x), ex2(d.y));
+                                if constexpr (Q8) {
+                                    sum[i & 1] = add2(sum[i & 1], e2);
+                                    e2 = mul2(e2, *reinterpret_cast<const float2*>(vs + c * 32 + k));
+                                    w[i] = pack<CT>(e2.x, e2.y);
+                                } else {
+                                    w[i] = pack<CT>(e2.x, e2.y);
+                                    sum[i & 1] = add2(sum[i & 1], unpack<CT>(w[i]));  // of the weights that the product has
+                                }
                             }
+                            tmem_st8(t_s + 64 + c * 16 + h * 8, w);
                         }
-                        tmem_st16(t_s + c * 16, w);
-                    }
-                    l += sum.x + sum.y;
+                    };
+                    weights(2, v[0]);
+                    tmem_ask32(t_s, v[0]);
+                    weights(3, v[1]);
+                    tmem_ask32(t_s + 32, v[1]);
+                    tmem_wait32(v[0]);
+                    scores(0, v[0]);
+                    weights(0, v[0]);
+                    tmem_wait32(v[1]);
+                    scores(1, v[1]);
+                    weights(1, v[1]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
                 tmem_wait_st();
                 tc::tc_fence_before();
@@ -874,6 +690,261 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc::tc_fence_after();
         }
         if (tid == 0 && t_a >= t_b) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    } else {
+        fewer_registers<REGS_OTHERS>();
+        if (warp == W_TMA) {
+            // ------------------------------------------------------------------ copies
+            const int groups = KT / a.box, x = lane % C::BOXES, gr = lane / C::BOXES;  // a lane per box
+            int e = 0;  // copies to slots so far
+            bool more = seek(p, s, row0, rem0, left);
+            auto look = [&](const Seg& w, int j) {  // the page of the lane's box in tile j; -1: no keys of the row, -2: out of range
+                const int key = j * KT + gr * a.box;
+                if (gr >= groups || key >= w.r.end) return -1;
+                const int id = __ldcg(p.table + (long long)w.r.row * p.ld + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page));
+                return (unsigned)id < (unsigned)p.n_pages ? id : -2;
+            };
+            int page = more ? look(s, s.j0) : -1;
+            while (more) {
+                left -= s.j1 - s.j0;
+                Seg n = s;
+                const bool after = next(p, n, left);
+                for (int j = s.j0; j < s.j1; ++j, ++g) {
+                    const int key = j * KT + gr * a.box;
+                    const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
+                    const int id = page;
+                    page = j + 1 < s.j1 ? look(s, j + 1) : after ? look(n, n.j0) : -1;
+                    const unsigned there = __ballot_sync(0xffffffffu, id >= 0), bad = __ballot_sync(0xffffffffu, id == -2);
+                    for (int v = 0; v < 2; ++v, ++e) {
+                        const int to = e % C::LOADS;
+                        if (e >= C::LOADS) wait(&b_free[to], (e / C::LOADS - 1) & 1);
+                        __syncwarp();
+                        const bool go = __all_sync(0xffffffffu, ok);
+                        if (lane == 0) {
+                            if (v == 0) s_bad[g % FLAGS] = bad != 0;
+                            if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * a.box * 128 + a.stall);
+                        }
+                        __syncwarp();
+                        if (go && id >= 0)
+                            tma_load_4d(tc::smem_u32(smem + (Q8 ? C::OFF_RAW : C::OFF_KV) + to * (Q8 ? C::PIECE : C::TILE) + x * C::PIECE + gr * a.box * 128),
+                                        v ? &vmap : &kmap, x * (128 / (int)sizeof(TC)), slot, s.kvh, id, tc::smem_u32(&b_load[to]));
+                        if (!go) ok = false;
+                    }
+                }
+                s = n;
+                more = after;
+            }
+            // copies that nobody waited for may still be on their way when a wait has run out
+            for (int i = max(0, e - C::LOADS); i < e && lane == 0; ++i)
+                for (int k = 0; k < WAIT_TRIES / 8 && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
+        } else if (warp == W_MMA) {
+            // ------------------------------------------------------------------ products
+            constexpr uint32_t BF = C::HALF ? 0u : (1u << 7) | (1u << 10);  // operands' format: fp16 or bf16
+            constexpr uint32_t idesc_s = tc::idesc_f16_f32(QT, KT) | BF, idesc_o = tc::idesc_f16_f32_bmn(QT, HD) | BF;
+            if (elect()) {
+                uint64_t* there = Q8 ? b_wide : b_load;
+                uint64_t* done = Q8 ? b_reuse : b_free;
+                const uint32_t q32 = tc::smem_u32(smem), kv32 = tc::smem_u32(smem + C::OFF_KV);
+                uint32_t np[2] = {0, 0}, specials = 0;
+                bool more = seek(p, s, row0, rem0, left);
+                for (int seg = 0; more; ++seg) {
+                    left -= s.j1 - s.j0;
+                    const bool pair = s.pair();
+                    const int T = s.j1 - s.j0, n0 = pair ? T : (T + 1) / 2, n1 = pair ? T : T / 2;
+                    // tiles from here on have values that are looked through
+                    const int special = max(s.r.prefix / KT, s.j0);
+                    wait(&b_q, seg & 1);
+                    auto tile = [&](int st, int u) { return pair ? u : 2 * u + st; };
+                    auto scores = [&](int st, int u) {
+                        const int e = 2 * (g + tile(st, u)), at = e % C::SLOTS;
+                        wait(&there[at], (e / C::SLOTS) & 1);
+                        tc::tc_fence_after();
+                        const uint64_t q = tc::desc_sw128(q32 + (pair ? st : 0) * C::TILE), k = tc::desc_sw128(kv32 + at * C::TILE);
+                        if (ok) {
+#pragma unroll
+                            for (int ks = 0; ks < HD / 16; ++ks) {
+                                const uint32_t o = ((ks >> 2) * C::PIECE + (ks & 3) * 32) >> 4;
+                                tc::mma_f16(tmem + st * KT, q + o, k + o, idesc_s, ks > 0);
+                            }
+                        }
+                        tc::mma_commit(&b_s[st]);
+                        if (!pair || st == 1) tc::mma_commit(&done[at]);
+                        tc::mbar_arrive(&b_s[st]);  // what this thread has seen of the tile's flags
+                    };
+                    if (n0 > 0) scores(0, 0);
+                    if (n1 > 0) scores(1, 0);
+                    for (int u = 0; u < n0; ++u) {
+                        for (int st = 0; st < 2; ++st) {
+                            if (u >= (st ? n1 : n0)) continue;
+                            const int t = tile(st, u), e = 2 * (g + t) + 1, at = e % C::SLOTS;
+                            wait(&b_p[st], np[st]++ & 1);
+                            wait(&there[at], (e / C::SLOTS) & 1);
+                            if (!Q8 && s.j0 + t >= special) {
+                                const uint32_t k = specials + (s.j0 + t - special);
+                                wait(&b_prep[k % TILES], (k / TILES) & 1);
+                            }
+                            tc::tc_fence_after();
+                            const uint64_t v = tc::desc_sw128_mn(kv32 + at * C::TILE, C::PIECE);
+                            if (ok) {
+#pragma unroll
+                                for (int ks = 0; ks < KT / 16; ++ks)
+                                    mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 64 + ks * 8, v + ks * 128, idesc_o, u > 0 || ks > 0);
+                            }
+                            if (!pair || st == 1) tc::mma_commit(&done[at]);
+                            if (u + 1 < (st ? n1 : n0))
+                                scores(st, u + 1);
+                            else
+                                tc::mma_commit(&b_o[st]);
+                        }
+                    }
+                    specials += max(s.j1 - special, 0);
+                    g += T;
+                    more = next(p, s, left);
+                }
+            }
+            __syncwarp();
+        } else if (warp >= W_PREP && warp < W_PREP + 4) {
+            // ------------------------------------------------------------------ operands
+            const int i = tid - W_PREP * 32;
+            bool more = seek(p, s, row0, rem0, left);
+            if constexpr (Q8) {
+                int e = 0;
+                while (more) {
+                    left -= s.j1 - s.j0;
+                    uint32_t vexp = 1;
+                    for (int j = s.j0; j < s.j1; ++j, ++g) {
+                        const int key = j * KT + i;
+                        float sc[2] = {0.f, 0.f};
+                        if (key < s.r.end) {
+                            const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
+                            const int id = __ldcg(p.table + (long long)s.r.row * p.ld + pg);
+                            if ((unsigned)id < (unsigned)p.n_pages) {
+                                const long long at = (long long)id * p.s_ps + (long long)s.kvh * p.s_hs + (long long)(key - pg * p.page) * p.s_ts;
+                                sc[0] = __ldcg(p.k_scale + at);
+                                sc[1] = __ldcg(p.v_scale + at);
+                            }
+                        }
+                        const bool drafted = (j + 1) * KT > s.r.prefix;
+                        for (int v = 0; v < 2; ++v, ++e) {
+                            const int from = e % C::RAWS, to = e % C::SLOTS;
+                            if (e >= C::SLOTS) wait(&b_reuse[to], (e / C::SLOTS - 1) & 1);
+                            bool spoilt = false;
+                            if (v == 0) {
+                                s_scale[g % TILES][0][i] = sc[0];
+                            } else {
+                                spoilt = key >= s.r.prefix && !isfinite(sc[1]);
+                                if (drafted) {
+                                    const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
+                                    if (lane == 0) s_spoilt[g % TILES][warp - W_PREP] = b;
+                                }
+                                if (spoilt) sc[1] = 0.f;
+                                // the largest exponent of the tile's scales, over the four warps
+                                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
+                                if (lane == 0) wsum[W_PREP + warp - W_PREP] = m;
+                                asm volatile("bar.sync 2, 128;" ::: "memory");
+                                uint32_t x = vexp;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
+                                vexp = min(x, 253u);
+                                s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
+                                if (i == 0) s_exp[g % TILES] = vexp;
+                                asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again; the masks are there
+                            }
+                            wait(&b_load[from], (e / C::RAWS) & 1);
+                            const unsigned char* src = smem + C::OFF_RAW + from * C::PIECE;
+                            unsigned char* dst = smem + C::OFF_KV + to * C::TILE;
+                            // 16 codes at a time. Eight lanes have four chunks of two rows that differ in bits 0 and 2, so that the
+                            // reads and the writes of eight lanes each meet all banks once
+#pragma unroll 4
+                            for (int it = 0; it < HD / 16; ++it) {
+                                const int x = it * 128 + i, c4 = x & 3, odd = x >> 2 & 1;
+                                int c, r;
+                                if constexpr (HD == 128) {
+                                    c = (x >> 3 & 1) * 4 + c4;
+                                    const int pr = x >> 4;  // pair of rows: 0..63
+                                    r = (pr >> 2) * 8 + (pr & 3);
+                                } else {
+                                    c = c4;
+                                    const int pr = x >> 3;
+                                    r = (pr >> 2) * 8 + (pr & 3);
+                                }
+                                if (odd) r ^= 5;
+                                uint4 w = *reinterpret_cast<const uint4*>(src + r * 128 + (((c ^ r) & 7) << 4));
+                                if (v && drafted) {
+                                    const int k = j * KT + r;
+                                    bool drop = k >= s.r.end;
+                                    if (!std::is_same<TC, int8_t>::value && k >= s.r.prefix && !drop) {
+                                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                                        bool nan = false;
+#pragma unroll
+                                        for (int z = 0; z < 4; ++z) nan |= __vcmpeq4(u[z] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+                                        if (nan) {
+                                            atomicOr(&s_spoilt[g % TILES][r >> 5], 1u << (r & 31));
+                                            drop = true;
+                                        }
+                                    }
+                                    if (drop) w = make_uint4(0, 0, 0, 0);
+                                }
+                                uint4 lo, hi;
+                                widen<TC>(w.x, lo.x, lo.y);
+                                widen<TC>(w.y, lo.z, lo.w);
+                                widen<TC>(w.z, hi.x, hi.y);
+                                widen<TC>(w.w, hi.z, hi.w);
+                                *reinterpret_cast<uint4*>(dst + sw(r, 2 * c)) = lo;
+                                *reinterpret_cast<uint4*>(dst + sw(r, 2 * c + 1)) = hi;
+                            }
+                            tc::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                tc::mbar_arrive(&b_free[from]);
+                                tc::mbar_arrive(&b_wide[to]);
+                            }
+                        }
+                    }
+                    more = next(p, s, left);
+                }
+            } else {
+                static_assert(Q8 || C::SLOTS % 2 == 0, "keys in even slots, values in odd ones");
+                uint32_t specials = 0;
+                while (more) {
+                    left -= s.j1 - s.j0;
+                    for (int j = s.j0; j < s.j1; ++j) {
+                        const int e = 2 * (g + j - s.j0) + 1, at = e % C::SLOTS, key = j * KT + i;
+                        wait(&b_load[at], (e / C::SLOTS) & 1);
+                        if (j < s.r.prefix / KT) {
+                            __syncwarp();
+                            if (lane == 0) tc::mbar_arrive(&b_free[at]);
+                            continue;
+                        }
+                        unsigned char* v = smem + C::OFF_KV + at * C::TILE;
+                        bool spoilt = false;
+                        if (key >= s.r.prefix && key < s.r.end) {
+#pragma unroll
+                            for (int c = 0; c < HD / 8; ++c) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(v + sw(i, c));
+                                constexpr uint32_t E = C::HALF ? 0x7c00u : 0x7f80u;
+                                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int z = 0; z < 4; ++z) spoilt |= (u[z] & E) == E || (u[z] >> 16 & E) == E;
+                            }
+                        }
+                        if (spoilt || key >= s.r.end)
+#pragma unroll
+                            for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(v + sw(i, c)) = make_uint4(0, 0, 0, 0);
+                        const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
+                        if (lane == 0) s_spoilt[specials % TILES][warp - W_PREP] = b;
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tc::mbar_arrive(&b_prep[specials % TILES]);
+                            tc::mbar_arrive(&b_free[at]);
+                        }
+                        ++specials;
+                    }
+                    g += s.j1 - s.j0;
+                    more = next(p, s, left);
+                }
+            }
+        }
     }
     tc::tc_fence_before();
     __syncthreads();
