@@ -8,9 +8,9 @@
 // what lies in several ranges. Results do not depend on the order in which blocks run.
 //
 // A block has one warp that starts the TMA copies, one that issues the MMAs, four that prepare operands, and two streams of
-// four softmax warps, a thread per query (TMEM lane), so that one stream's exponentials run beside the other's MMAs:
+// eight softmax warps, two threads per query (TMEM lane), so that one stream's exponentials run beside the other's MMAs:
 //   S = Q K^T       M = 128 queries, N = 128 keys; Q and K from shared memory
-//   P = 2^(S - m)   in 16 bits over the later half of S's own TMEM columns
+//   P = 2^(S - m)   in 16 bits over half of S's own TMEM columns
 //   O += P V        M = 128, N = head dim, K = 128 keys; P from TMEM, V from shared memory, O in TMEM
 // With more than 128 queries each stream has its own and both use every tile of keys; with fewer both have the same
 // queries, take tiles in turn, and are joined at the end. O is rescaled only when the maximum has risen by more than
@@ -42,10 +42,9 @@ namespace {
 constexpr int QT = 128, KT = 128;  // queries and keys of a tile
 constexpr int SB = 2 * QT;         // queries of a block of queries
 constexpr int CTAS = 148;          // one per SM of a B200
-// Warps 0-3 and 4-7 are the two streams, 8-11 prepare operands. The streams take registers that the others give
-// up: 2 * 128 * (184 + 72) are the 512 * 128 of the launch.
-constexpr int WARPS = 16, THREADS = WARPS * 32, REGS_SOFTMAX = 184, REGS_OTHERS = 72;
-constexpr int W_PREP = 8, W_MMA = 12, W_TMA = 13;
+// Warps 0-7 and 8-15 are the two streams (the halves of the keys, four warps each), 16-19 prepare operands.
+constexpr int WARPS = 22, THREADS = WARPS * 32;
+constexpr int W_PREP = 16, W_MMA = 20, W_TMA = 21;
 constexpr int TILES = 4;           // of which scales and masks are kept: a tile's are read before its weights are handed on, and
                                    // its slots are written again only after that
 constexpr int FLAGS = 8;           // of which page flags are kept: the copies may be four tiles ahead
@@ -190,14 +189,16 @@ __device__ __forceinline__ bool elect() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, and A[tmem] * B[smem desc]^T, kind::f16
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a_desc),
+                 "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
-        : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
 }
 // 32 columns of this thread's lane, which may be used after tmem_wait32 of the same registers
 __device__ __forceinline__ void tmem_ask32(uint32_t at, float* v) {
@@ -213,10 +214,6 @@ __device__ __forceinline__ void tmem_wait32(float* v) {
                  :
                  : "memory");
 }
-template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
@@ -244,7 +241,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void streams_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void streams_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ void half_sync(int stream) {
+    if (stream)
+        asm volatile("bar.sync 4, 256;" ::: "memory");
+    else
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+}
 
 template <class CT>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -320,8 +323,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     __shared__ uint32_t s_spoilt[TILES][4];           // drafted tokens' values that are not finite
     __shared__ int s_bad[FLAGS];                      // a page id is out of range
     __shared__ float s_up[SB];                        // what a row's queries were scaled by, undone
-    __shared__ float2 s_ml[QT];
-    __shared__ uint32_t s_vexp[QT];
+    __shared__ float s_mx[2][2][QT], s_l[2][2][QT], s_m[2][QT];  // of the streams' halves: a tile's largest scores, the sums; references
+    __shared__ uint32_t s_vexp[2][QT];
     __shared__ int s_stuck;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc::mbar_init(&b_q, 1);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&b_s[i], 2);
-            tc::mbar_init(&b_p[i], 4);
+            tc::mbar_init(&b_p[i], 8);
             tc::mbar_init(&b_o[i], 1);
         }
         s_stuck = 0;
@@ -412,11 +415,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     long long left = t_b - t_a;
     int g = 0;  // tiles of this block before the segment
     if (warp < W_PREP) {
-        more_registers<REGS_SOFTMAX>();
-        // ------------------------------------------------------------------ softmax: a thread per query
-        const int st = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        // ------------------------------------------------------------------ softmax: two threads per query
+        const int st = warp >> 3, half = warp >> 2 & 1, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t t_s = lanes + st * KT, t_o = lanes + 256 + st * HD;
+        const uint32_t t_s = lanes + st * KT + half * (KT / 2);  // this thread's keys
         const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);
         uint32_t ns = 0, no = 0, specials = 0;
         bool more = seek(p, s, row0, rem0, left);
@@ -428,45 +430,51 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int qi = s.sb * SB + (pair ? st * QT : 0) + r;  // this thread's query of the kv head
             const bool mine_q = qi < s.r.queries;
             const int tok = (int)((unsigned)qi / (unsigned)p.group), to = s.r.token + tok, head = s.kvh * p.group + qi - tok * p.group;
-            // ---- queries ----
+            // ---- queries: a half of the dims each ----
             if (pair || st == 0) {
-                uint32_t w[HD / 2];
-                const char* src = static_cast<const char*>(p.q) + ((long long)to * p.q_ts + (long long)head * p.q_hs) * 2;
-#pragma unroll
-                for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 v = mine_q && c * 8 < p.dim ? __ldcg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-                    w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
-                }
-                float up = 1.f;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + ((long long)to * p.q_ts + (long long)head * p.q_hs) * 2);
+                auto dims = [&](int c) { return mine_q && c * 8 < p.dim ? __ldcg(src + c) : make_uint4(0, 0, 0, 0); };
+                float down = 1.f, up = 1.f;
                 if constexpr (C::RANGE) {
                     uint32_t top = 0;
+#pragma unroll 8
+                    for (int c = 0; c < HD / 8; ++c) {
+                        const uint4 v = dims(c);
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int c = 0; c < HD / 2; ++c) top = max(top, max(w[c] & 0x7fffu, w[c] >> 16 & 0x7fffu));
+                        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, w[k] >> 16 & 0x7fffu));
+                    }
                     int e = (int)(top >> 7);  // biased exponent
                     e = e == 0 || e == 255 ? 127 : min(max(e, 12), 252);
-                    const float down = __uint_as_float((uint32_t)(264 - e) << 23);
+                    down = __uint_as_float((uint32_t)(264 - e) << 23);
                     up = __uint_as_float((uint32_t)(e - 10) << 23);
-#pragma unroll
-                    for (int c = 0; c < HD / 2; ++c) {
-                        const float2 f = unpack<TI>(w[c]);
-                        w[c] = pack<CT>(f.x * down, f.y * down);
-                    }
-                }
-                if (p.scale < 0.f) {
-#pragma unroll
-                    for (int c = 0; c < HD / 2; ++c) w[c] ^= 0x80008000u;
                 }
                 unsigned char* dst = smem + st * C::TILE;
+#pragma unroll 4
+                for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
+                    const uint4 v = dims(c);
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    if constexpr (C::RANGE) {
 #pragma unroll
-                for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(dst + sw(r, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-                s_up[st * QT + r] = up;
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = unpack<TI>(w[k]);
+                            w[k] = pack<CT>(f.x * down, f.y * down);
+                        }
+                    }
+                    if (p.scale < 0.f) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] ^= 0x80008000u;
+                    }
+                    *reinterpret_cast<uint4*>(dst + sw(r, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (half == 0) s_up[st * QT + r] = up;
                 tc::fence_proxy_async_smem();
             }
             tc::tc_fence_before();
             streams_sync();
             if (tid == 0) tc::mbar_arrive(&b_q);
             const float fac = fmaxf(sl2 * s_up[(pair ? st * QT : 0) + r], 1.17549435e-38f);  // not 0: a masked score of -inf stays one
-            float m = -INFINITY, l = s.r.over ? NAN : 0.f;  // reference of the weights, in units before the factor; their sum
+            float m = -INFINITY, l = s.r.over ? NAN : 0.f;  // reference of the weights, in units before the factor; this half's sum
             uint32_t vexp = 1;
             const bool idle = s.sb * SB + (pair ? st * QT : 0) + quarter * 32 >= s.r.queries;  // no query in this warp
             int bad = s.r.over ? GPT2Q_STATUS_POSITION : 0;
@@ -476,19 +484,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::tc_fence_after();
                 if (s_bad[(g + t) % FLAGS]) bad |= GPT2Q_STATUS_PAGE;
                 const bool look = j >= special;  // keys that not every query sees
-                uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                uint32_t vis[2] = {~0u, ~0u};
                 if (look && !idle) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) vis[c] = mine_q ? visible(p, s.r, tok, j * KT + c * 32) : 0u;
+                    for (int c = 0; c < 2; ++c) vis[c] = mine_q ? visible(p, s.r, tok, j * KT + half * (KT / 2) + c * 32) : 0u;
                 }
-                const float* vs = s_scale[Q8 ? gt : 0][1];
-                    float mx = -INFINITY;
-                // scores of a quarter of the keys; the later half stays here until its weights are formed, as the
-                // weights take the columns that it came from, the earlier half is read again
-                float v[2][32];
-                auto scores = [&](int c, float* x) {
+                float mx = -INFINITY;
+                // Scores of a quarter of the keys, read once for the largest and once more for the weights: with 64 of them in
+                // registers there would be fewer warps
+                float x[32];
+                auto scores = [&](int c) {
+                    tmem_ask32(t_s + c * 32, x);
+                    tmem_wait32(x);
                     if constexpr (Q8) {
-                        const float* ks = s_scale[gt][0] + c * 32;
+                        const float* ks = s_scale[gt][0] + half * (KT / 2) + c * 32;
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) {
                             const float4 f = *reinterpret_cast<const float4*>(ks + k);
@@ -501,7 +510,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int k = 0; k < 32; ++k) x[k] = vis[c] >> k & 1 ? x[k] : -INFINITY;
                     }
                 };
-                auto largest = [&](const float* x) {
+                auto largest = [&](int c) {
+                    scores(c);
                     float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
                     for (int k = 4; k < 32; ++k) top[k & 3] = fmaxf(top[k & 3], x[k]);
@@ -509,23 +519,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 };
                 __syncwarp();
                 if (!idle) {
-                    tmem_ask32(t_s, v[0]);
-                    tmem_ask32(t_s + 32, v[1]);
-                    tmem_wait32(v[0]);
-                    tmem_wait32(v[1]);
-                    scores(0, v[0]);
-                    largest(v[0]);
-                    tmem_ask32(t_s + 64, v[0]);
-                    scores(1, v[1]);
-                    largest(v[1]);
-                    tmem_ask32(t_s + 96, v[1]);
-                    tmem_wait32(v[0]);
-                    scores(2, v[0]);
-                    largest(v[0]);
-                    tmem_wait32(v[1]);
-                    scores(3, v[1]);
-                    largest(v[1]);
+                    largest(0);
+                    largest(1);
                 }
+                s_mx[st][half][r] = mx;
+                half_sync(st);
+                mx = fmaxf(mx, s_mx[st][half ^ 1][r]);
                 // values' scales and what is to be known of them
                 uint32_t e = vexp;
                 if constexpr (Q8) {
@@ -537,10 +536,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     wait(&b_prep[k % TILES], (k / TILES) & 1);
                 }
                 if (look) {
-                    const uint32_t* sp = s_spoilt[Q8 ? gt : (specials + (j - special)) % TILES];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (vis[c] & sp[c]) l = NAN;
+                    const uint32_t* sp = s_spoilt[Q8 ? gt : (specials + (j - special)) % TILES] + half * 2;
+                    if ((vis[0] & sp[0]) | (vis[1] & sp[1])) l = NAN;
                 }
                 // a new reference, and the results so far in it
                 const float mn = fmaxf(m, mx);
@@ -557,21 +554,24 @@ __global__ void __launch_bounds__(THREADS, 1)
                         vexp = e;
                     }
                 }
+                __syncwarp();
                 if (u > 0 && __any_sync(0xffffffffu, al != 1.f)) {
 #pragma unroll 1
-                    for (int c = 0; c < HD / 16; ++c) {
+                    for (int c = half * (HD / 32); c < (half + 1) * (HD / 32); ++c) {
                         uint32_t w[16];
-                        tmem_ld16(t_o + c * 16, w);
+                        const uint32_t at = lanes + 256 + st * HD + c * 16;
+                        tmem_ld16(at, w);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(__uint_as_float(w[k]) * al);
-                        tmem_st16(t_o + c * 16, w);
+                        tmem_st16(at, w);
                     }
                 }
                 if (!idle) {
                     const float ref = m == -INFINITY ? 0.f : m;
                     const float2 nref = make_float2(-ref, -ref), f2 = make_float2(fac, fac), sh = make_float2(C::shift(), C::shift());
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    auto weights = [&](int c, const float* x) {
+                    auto weights = [&](int c) {
+                        scores(c);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             uint32_t w[8];
@@ -580,29 +580,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 const int k = h * 16 + i * 2;
                                 // (S - m) before the factor, where m's own score gives exactly 0
                                 const float2 d = fma2(add2(make_float2(x[k], x[k + 1]), nref), f2, sh);
-                                float2 e2 = make_float2(ex2(d.x), ex2(d.y));
+                                float2 y = make_float2(ex2(d.x), ex2(d.y));
                                 if constexpr (Q8) {
-                                    sum[i & 1] = add2(sum[i & 1], e2);
-                                    e2 = mul2(e2, *reinterpret_cast<const float2*>(vs + c * 32 + k));
-                                    w[i] = pack<CT>(e2.x, e2.y);
+                                    sum[i & 1] = add2(sum[i & 1], y);
+                                    y = mul2(y, *reinterpret_cast<const float2*>(s_scale[gt][1] + half * (KT / 2) + c * 32 + k));
+                                    w[i] = pack<CT>(y.x, y.y);
                                 } else {
-                                    w[i] = pack<CT>(e2.x, e2.y);
+                                    w[i] = pack<CT>(y.x, y.y);
                                     sum[i & 1] = add2(sum[i & 1], unpack<CT>(w[i]));  // of the weights that the product has
                                 }
                             }
-                            tmem_st8(t_s + 64 + c * 16 + h * 8, w);
+                            tmem_st8(t_s + 32 + c * 16 + h * 8, w);
                         }
                     };
-                    weights(2, v[0]);
-                    tmem_ask32(t_s, v[0]);
-                    weights(3, v[1]);
-                    tmem_ask32(t_s + 32, v[1]);
-                    tmem_wait32(v[0]);
-                    scores(0, v[0]);
-                    weights(0, v[0]);
-                    tmem_wait32(v[1]);
-                    scores(1, v[1]);
-                    weights(1, v[1]);
+                    // both quarters' weights take the columns of the later one
+                    weights(1);
+                    weights(0);
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
                 tmem_wait_st();
@@ -615,28 +608,28 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!ok || *(volatile int*)&s_stuck) bad |= GPT2Q_STATUS_TIMEOUT;
             if (bad) l = NAN;
             if (bad && p.status && lane == 0) atomicOr(p.status, bad);
-            // ---- results ----
-            float wa = 1.f, wb = 0.f;  // weights of the streams' results
-            if (!pair) {
-                if (st == 1) {
-                    s_ml[r] = make_float2(m, l);
-                    s_vexp[r] = vexp;
-                }
-                tc::tc_fence_before();
-                streams_sync();
-                tc::tc_fence_after();
-                if (st == 0) {
-                    const float2 o = T > 1 ? s_ml[r] : make_float2(-INFINITY, s_ml[r].y);
-                    const float M = fmaxf(m, o.x), ms = M == -INFINITY ? 0.f : M;
-                    wa = ex2((m - ms) * fac), wb = ex2((o.x - ms) * fac);
-                    l = l * wa + o.y * wb;
-                    m = M;
-                    if (Q8) wa *= __uint_as_float(vexp << 23), wb *= __uint_as_float(s_vexp[r] << 23);
-                }
-            } else if (Q8) {
-                wa = __uint_as_float(vexp << 23);
+            // ---- results: a half of the dims each ----
+            s_l[st][half][r] = l;
+            if (half == 0) {
+                s_m[st][r] = m;
+                s_vexp[st][r] = vexp;
             }
+            tc::tc_fence_before();
+            streams_sync();
+            tc::tc_fence_after();
             if ((pair || st == 0) && !idle) {
+                float wa = 1.f, wb = 0.f;  // weights of this stream's and the other's results
+                l = s_l[st][0][r] + s_l[st][1][r];
+                if (Q8) wa = __uint_as_float(vexp << 23);
+                if (!pair) {
+                    const float o = s_m[1][r], M = fmaxf(m, o), ms = M == -INFINITY ? 0.f : M;
+                    const float xa = ex2((m - ms) * fac);
+                    wb = ex2((o - ms) * fac);
+                    l = l * xa + (s_l[1][0][r] + s_l[1][1][r]) * wb;
+                    m = M;
+                    wa *= xa;
+                    if (Q8) wb *= __uint_as_float(s_vexp[1][r] << 23);
+                }
                 const bool whole = s.j0 == 0 && s.j1 == s.nt;
                 const int slot = s.j0 > 0 ? 0 : 1, pr = (pair ? st * QT : 0) + r;
                 const long long part = ((long long)blockIdx.x * 2 + slot) * SB + pr;
@@ -644,32 +637,32 @@ __global__ void __launch_bounds__(THREADS, 1)
                 wa *= f, wb *= f;
                 const float mlog = m * fac;  // reference, as a power of two
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                    float v[32];
+                for (int c = half * (HD / 32); c < (half + 1) * (HD / 32); ++c) {
+                    uint32_t w[16];
+                    float x[16];
                     __syncwarp();
-                    tc::tmem_ld32(t_o + c * 32, v);
+                    tmem_ld16(lanes + 256 + st * HD + c * 16, w);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] *= wa;
+                    for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(w[k]) * wa;
                     if (!pair && T > 1) {
-                        float x[32];
-                        tc::tmem_ld32(lanes + 256 + HD + c * 32, x);
+                        tmem_ld16(lanes + 256 + HD + c * 16, w);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], wb, v[k]);
+                        for (int k = 0; k < 16; ++k) x[k] = fmaf(__uint_as_float(w[k]), wb, x[k]);
                     }
                     if (mine_q) {
                         if (whole) {
-                            TI* o = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + c * 32;
+                            TI* o = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + c * 16;
 #pragma unroll
-                            for (int k = 0; k < 32; k += 8)
-                                if (c * 32 + k < p.dim) store_vec<TI, 8>(o + k, v + k);
+                            for (int k = 0; k < 16; k += 8)
+                                if (c * 16 + k < p.dim) store_vec<TI, 8>(o + k, x + k);
                         } else {
-                            float* o = a.part + part * HD + c * 32;
+                            float* o = a.part + part * HD + c * 16;
 #pragma unroll
-                            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                            for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
                         }
                     }
                 }
-                if (mine_q) {
+                if (mine_q && half == 0) {
                     if (!whole)
                         a.part_ml[part] = make_float2(mlog, l);
                     else if (p.lse)
@@ -684,14 +677,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             specials += max(s.j1 - special, 0);
             g += T;
             more = next(p, s, left);
-            // no stream writes its queries or results before the other has read what they share
+            // nobody writes queries, sums or results before the others have read what they share
             tc::tc_fence_before();
             streams_sync();
             tc::tc_fence_after();
         }
         if (tid == 0 && t_a >= t_b) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
     } else {
-        fewer_registers<REGS_OTHERS>();
         if (warp == W_TMA) {
             // ------------------------------------------------------------------ copies
             const int groups = KT / a.box, x = lane % C::BOXES, gr = lane / C::BOXES;  // a lane per box
@@ -754,46 +746,62 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int special = max(s.r.prefix / KT, s.j0);
                     wait(&b_q, seg & 1);
                     auto tile = [&](int st, int u) { return pair ? u : 2 * u + st; };
+                    auto keys = [&](int st, int u) {
+                        const int e = 2 * (g + tile(st, u));
+                        wait(&there[e % C::SLOTS], (e / C::SLOTS) & 1);
+                    };
                     auto scores = [&](int st, int u) {
-                        const int e = 2 * (g + tile(st, u)), at = e % C::SLOTS;
-                        wait(&there[at], (e / C::SLOTS) & 1);
-                        tc::tc_fence_after();
+                        const int at = 2 * (g + tile(st, u)) % C::SLOTS;
                         const uint64_t q = tc::desc_sw128(q32 + (pair ? st : 0) * C::TILE), k = tc::desc_sw128(kv32 + at * C::TILE);
                         if (ok) {
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ++ks) {
                                 const uint32_t o = ((ks >> 2) * C::PIECE + (ks & 3) * 32) >> 4;
-                                tc::mma_f16(tmem + st * KT, q + o, k + o, idesc_s, ks > 0);
+                                mma_f16_ss(tmem + st * KT, q + o, k + o, idesc_s, ks > 0);
                             }
                         }
                         tc::mma_commit(&b_s[st]);
-                        if (!pair || st == 1) tc::mma_commit(&done[at]);
                         tc::mbar_arrive(&b_s[st]);  // what this thread has seen of the tile's flags
+                        if (!pair || st == 1) tc::mma_commit(&done[at]);
                     };
-                    if (n0 > 0) scores(0, 0);
+                    keys(0, 0);
+                    if (n1 > 0) keys(1, 0);
+                    tc::tc_fence_after();
+                    scores(0, 0);
                     if (n1 > 0) scores(1, 0);
                     for (int u = 0; u < n0; ++u) {
                         for (int st = 0; st < 2; ++st) {
                             if (u >= (st ? n1 : n0)) continue;
                             const int t = tile(st, u), e = 2 * (g + t) + 1, at = e % C::SLOTS;
-                            wait(&b_p[st], np[st]++ & 1);
+                            // what is there already, usually: before the wait that is not over yet. (The next keys of a
+                            // stream of its own tiles come into the slot of these values where there are three)
+                            constexpr bool EARLY = C::SLOTS > 3;
+                            const bool again = u + 1 < (st ? n1 : n0);
                             wait(&there[at], (e / C::SLOTS) & 1);
                             if (!Q8 && s.j0 + t >= special) {
                                 const uint32_t k = specials + (s.j0 + t - special);
                                 wait(&b_prep[k % TILES], (k / TILES) & 1);
                             }
+                            if (EARLY && again) keys(st, u + 1);
+                            wait(&b_p[st], np[st]++ & 1);
                             tc::tc_fence_after();
                             const uint64_t v = tc::desc_sw128_mn(kv32 + at * C::TILE, C::PIECE);
                             if (ok) {
 #pragma unroll
                                 for (int ks = 0; ks < KT / 16; ++ks)
-                                    mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 64 + ks * 8, v + ks * 128, idesc_o, u > 0 || ks > 0);
+                                    mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 32 + ks * 8 + (ks >> 2) * 32, v + ks * 128, idesc_o, u > 0 || ks > 0);
                             }
-                            if (!pair || st == 1) tc::mma_commit(&done[at]);
-                            if (u + 1 < (st ? n1 : n0))
+                            if (!EARLY && (!pair || st == 1)) tc::mma_commit(&done[at]);
+                            if (again) {
+                                if (!EARLY) {
+                                    keys(st, u + 1);
+                                    tc::tc_fence_after();
+                                }
                                 scores(st, u + 1);
-                            else
+                            } else {
                                 tc::mma_commit(&b_o[st]);
+                            }
+                            if (EARLY && (!pair || st == 1)) tc::mma_commit(&done[at]);
                         }
                     }
                     specials += max(s.j1 - special, 0);
@@ -802,7 +810,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             __syncwarp();
-        } else if (warp >= W_PREP && warp < W_PREP + 4) {
+        } else {
             // ------------------------------------------------------------------ operands
             const int i = tid - W_PREP * 32;
             bool more = seek(p, s, row0, rem0, left);
