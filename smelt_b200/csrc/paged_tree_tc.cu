@@ -7,7 +7,7 @@
 // queries and position; each block takes a range of equal length, whatever the rows' lengths are, and a second kernel joins
 // what lies in several ranges. Results do not depend on the order in which blocks run.
 //
-// A block has one warp that starts the TMA copies, one that issues the MMAs, four that prepare operands, and two streams of
+// A block has two warps that start the TMA copies, one that issues the MMAs, four that prepare operands, and two streams of
 // eight softmax warps, two threads per query (TMEM lane), so that one stream's exponentials run beside the other's MMAs:
 //   S = Q K^T       M = 128 queries, N = 128 keys; Q and K from shared memory
 //   P = 2^(S - m)   in 16 bits over half of S's own TMEM columns
@@ -21,7 +21,7 @@
 // weight times scale stays in fp16's range. bf16 queries are scaled per row by a power of two that brings the largest
 // element to [2^10, 2^11), and are exact in fp16 down to 2^-24 of it.
 //
-// A weight is rounded to 16 bits, once (bf16 2^-9, fp16 2^-12 of itself): as large as the output's own rounding, and of
+// A weight is rounded to 16 bits, once (by up to 2^-8 of itself in bf16, 2^-11 in fp16): as the output is, and with
 // random sign over the keys. fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -43,14 +43,18 @@ constexpr int QT = 128, KT = 128;  // queries and keys of a tile
 constexpr int SB = 2 * QT;         // queries of a block of queries
 constexpr int CTAS = 148;          // one per SM of a B200
 // Warps 0-7 and 8-15 are the two streams (the halves of the keys, four warps each), 16-19 prepare operands.
-constexpr int WARPS = 22, THREADS = WARPS * 32;
-constexpr int W_PREP = 16, W_MMA = 20, W_TMA = 21;
+constexpr int WARPS = 23, THREADS = WARPS * 32;
+constexpr int W_PREP = 16, W_MMA = 20, W_TMA = 21;  // 21 and 22: copies of keys and of values
 constexpr int TILES = 4;           // of which scales and masks are kept: a tile's are read before its weights are handed on, and
                                    // its slots are written again only after that
 constexpr int FLAGS = 8;           // of which page flags are kept: the copies may be four tiles ahead
 constexpr int WAIT_TRIES = 1 << 22;  // of at least 20 ns: 0.1 s and more
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+// What a segment costs beside its tiles (queries, first copies, results: 22 thousand cycles against 5 thousand a tile), in tiles
+// of the list, where it comes first. Without it blocks with many short rows took twice as long as the others (tree of 31 short
+// drafts 218 us)
+constexpr int EXTRA = 4;
 constexpr float STALE = 8.f;  // log2 of the largest weight
 
 template <class TC_, class TI_, int HD_>
@@ -65,7 +69,7 @@ struct Cfg {
     static constexpr int PIECES = HD / 64;               // of 128 bytes, of a 16-bit row
     static constexpr int PIECE = KT * 128;               // bytes of a tile's piece
     static constexpr int TILE = PIECES * PIECE;          // 16-bit tile of 128 rows
-    static constexpr int SLOTS = HD == 128 ? (Q8 ? 3 : 4) : (Q8 ? 4 : 8);  // 16-bit tiles of keys or values
+    static constexpr int SLOTS = HD == 128 && Q8 ? 3 : 4;  // 16-bit tiles of keys or values
     static constexpr int RAWS = Q8 ? (HD == 128 ? 3 : 4) : 0;              // 8-bit tiles, rows of 128 bytes
     static constexpr int OFF_KV = 2 * TILE, OFF_RAW = OFF_KV + SLOTS * TILE, SMEM = OFF_RAW + RAWS * PIECE + 1024;
     static constexpr int LOADS = Q8 ? RAWS : SLOTS;      // slots that copies go to
@@ -78,7 +82,7 @@ struct Args {
     PagedAttn p;
     int box;           // keys of a TMA box
     int stall;         // for the test of waits that run out
-    float* part;       // [block][2][SB][dims]
+    float4* part;      // [block][2][dims / 4][SB]
     float2* part_ml;   // [block][2][SB]
     int4* meta;        // per block: row (-1: none), kv head, block of queries, last block of its last segment
 };
@@ -111,74 +115,72 @@ __device__ __forceinline__ Row enter(const PagedAttn& p, int row) {
 }
 // Tiles of blocks of queries 0 .. sb - 1 of a kv head. Under a mask every block has those of all keys. A chain's block ends with its
 // last query's own key: blocks but the last have ceil((prefix + ceil(256 (x + 1) / group)) / 128) =
-// floor((2 x + c) / group) tiles, whose sum goes by whole periods of `group` blocks.
+// floor((2 x + c) / group) tiles, whose sum goes by whole periods of `group` blocks. (A call has fewer than 2^31 tiles.)
 __device__ __forceinline__ int tiles_of(const PagedAttn& p, const Row& r, int sb) {
     int end = r.end;
     if (!p.mask && !r.over && sb < r.blocks - 1) end = r.prefix + ((sb + 1) * SB - 1) / p.group + 1;
     return (end + KT - 1) / KT;
 }
-__device__ __forceinline__ long long quotient(long long a, int b) { return a >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
-__device__ __forceinline__ long long tiles_before(const PagedAttn& p, const Row& r, int sb) {
-    if (p.mask || r.over) return (long long)sb * tiles_of(p, r, 0);
-    const int G = p.group, x = min(sb, r.blocks - 1);
-    const long long c = ((long long)r.prefix * G + 2 * KT + (long long)KT * G - 1) / KT;
-    const int q = x / G, rest = x - q * G;
-    long long sum = (long long)G * q * (q - 1) + (long long)2 * q * rest;
-    for (int i = 0; i < (q ? G : rest); ++i) sum += quotient(2 * i + c, G) * (q + (i < rest ? 1 : 0));
-    return sum + (sb == r.blocks && r.blocks > 0 ? tiles_of(p, r, sb - 1) : 0);
+// Places in the list: those tiles and EXTRA for each block.
+__device__ __forceinline__ int places_before(const PagedAttn& p, const Row& r, int sb) {
+    if (p.mask || r.over) return sb * (tiles_of(p, r, 0) + EXTRA);
+    const unsigned G = p.group, x = max(min(sb, r.blocks - 1), 0);
+    const unsigned c = (unsigned)(((unsigned long long)r.prefix * G + 2 * KT + (unsigned long long)KT * G - 1) / KT);
+    const unsigned q = x / G, rest = x - q * G;
+    unsigned sum = G * q * (q - 1) + 2 * q * rest + sb * EXTRA;
+    for (unsigned i = 0; i < (q ? G : rest); ++i) sum += (2 * i + c) / G * (q + (i < rest ? 1 : 0));
+    return (int)sum + (sb == r.blocks && r.blocks > 0 ? tiles_of(p, r, sb - 1) : 0);
 }
 
-struct Range {
-    long long a, b;      // this block's tiles
-    int row;             // where it begins
-    long long rem;       // tiles before it in that row
-};
-
-// The segment that lies `rem` tiles into row `row` (or behind it), cut to `left` tiles; false at the end.
-__device__ __forceinline__ bool seek(const PagedAttn& p, Seg& s, int row, long long rem, long long left) {
+// Takes the places `from` .. of the block at hand that `left` covers, which it takes them from; false if they have no tile.
+__device__ __forceinline__ bool cut(const PagedAttn& p, Seg& s, int from, int& left) {
+    s.nt = tiles_of(p, s.r, s.sb);
+    const int to = min(s.nt + EXTRA, from + left);
+    left -= to - from;
+    s.j0 = max(from - EXTRA, 0);
+    s.j1 = max(to - EXTRA, 0);
+    return s.j1 > s.j0;
+}
+// The next segment, taken from `left`; false at the end.
+__device__ __forceinline__ bool next(const PagedAttn& p, Seg& s, int& left) {
+    while (left > 0) {
+        if (++s.sb >= s.r.blocks) {
+            s.sb = 0;
+            if (++s.kvh >= p.n_kv) {
+                s.kvh = 0;
+                do {
+                    if (s.r.row + 1 >= p.n_rows) return false;
+                    s.r = enter(p, s.r.row + 1);
+                } while (s.r.n == 0);
+            }
+        }
+        if (cut(p, s, 0, left)) return true;
+    }
+    return false;
+}
+// The segment that lies `rem` places into row `row`, or behind it. By a whole warp.
+__device__ __forceinline__ bool seek(const PagedAttn& p, Seg& s, int row, int rem, int& left) {
     if (left <= 0) return false;
     Row r = enter(p, row);
-    long long per = tiles_before(p, r, r.blocks);
+    int per = places_before(p, r, r.blocks);
     while (rem >= per * p.n_kv) {
         rem -= per * p.n_kv;
         if (++row >= p.n_rows) return false;
         r = enter(p, row);
-        per = tiles_before(p, r, r.blocks);
+        per = places_before(p, r, r.blocks);
     }
     s.r = r;
-    s.kvh = (int)(rem >> 32 ? rem / per : per >> 32 ? 0 : (uint32_t)rem / (uint32_t)per);
+    s.kvh = (unsigned)rem / (unsigned)per;
     rem -= s.kvh * per;
-    int lo = 0, hi = r.blocks - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tiles_before(p, r, mid) <= rem)
-            lo = mid;
-        else
-            hi = mid - 1;
+    int lo = 0;
+    for (int n = r.blocks; n > 1;) {  // the last block that begins at or before it, 32 candidates at once
+        const int step = (n + 31) / 32, x = lo + (threadIdx.x & 31) * step;
+        const int k = __popc(__ballot_sync(0xffffffffu, x < lo + n && places_before(p, r, x) <= rem)) - 1;
+        n = min(step, n - k * step);
+        lo += k * step;
     }
     s.sb = lo;
-    s.nt = tiles_of(p, r, lo);
-    s.j0 = (int)(rem - tiles_before(p, r, lo));
-    s.j1 = (int)min((long long)s.nt, s.j0 + left);
-    return true;
-}
-// The one after it.
-__device__ __forceinline__ bool next(const PagedAttn& p, Seg& s, long long left) {
-    if (left <= 0) return false;
-    if (++s.sb >= s.r.blocks) {
-        s.sb = 0;
-        if (++s.kvh >= p.n_kv) {
-            s.kvh = 0;
-            do {
-                if (s.r.row + 1 >= p.n_rows) return false;
-                s.r = enter(p, s.r.row + 1);
-            } while (s.r.n == 0);
-        }
-    }
-    s.nt = tiles_of(p, s.r, s.sb);
-    s.j0 = 0;
-    s.j1 = (int)min((long long)s.nt, left);
-    return true;
+    return cut(p, s, rem - places_before(p, r, lo), left) || next(p, s, left);
 }
 
 // ------------------------------------------------------------------ PTX
@@ -311,8 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const PagedAttn& p = a.p;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ long long cum[THREADS + 1];
-    __shared__ long long wsum[WARPS];
+    __shared__ int cum[THREADS], wsum[WARPS];
     __shared__ __align__(8) uint64_t b_load[8], b_free[8];   // copies have landed in a slot; its tile is no longer needed
     __shared__ __align__(8) uint64_t b_wide[8], b_reuse[8];  // 8-bit: a tile is there in fp16; its slot may be written again
     __shared__ __align__(8) uint64_t b_prep[TILES];          // 16-bit: a tile of values with drafted tokens is looked through
@@ -331,8 +332,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (tid == 0) {
         for (int i = 0; i < 8; ++i) {
             tc::mbar_init(&b_load[i], 1);
-            // 8-bit: the preparing warps; else the products and, of values (odd slots), the preparing warps too, which
-            // wait for every load of such a slot, as a parity cannot tell a phase from the one two before it
+            // 8-bit copies are used by the preparing warps, as are, else, those of values (odd slots): they wait for every load
+            // of such a slot, as a parity cannot tell a phase from the one two before it
             tc::mbar_init(&b_free[i], Q8 ? 4 : i & 1 ? 5 : 1);
             tc::mbar_init(&b_wide[i], 4);
             tc::mbar_init(&b_reuse[i], 1);
@@ -364,38 +365,36 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     // ---- this block's range of tiles ----
     const int nc = (p.n_rows + THREADS - 1) / THREADS;  // rows a thread counts
-    long long mine = 0;
+    int mine = 0;
     for (int r = tid * nc; r < min((tid + 1) * nc, p.n_rows); ++r) {
         const Row w = enter(p, r);
-        mine += tiles_before(p, w, w.blocks) * p.n_kv;
+        mine += places_before(p, w, w.blocks) * p.n_kv;
     }
-    long long inc = mine;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
     for (int i = 0; i < WARPS; ++i) {
         if (i < warp) before += wsum[i];
         total += wsum[i];
     }
     cum[tid] = before + inc - mine;
     __syncthreads();
-    const long long per = (total + gridDim.x - 1) / gridDim.x;
-    const long long t_a = per * blockIdx.x, t_b = min(t_a + per, total);
-    int row0 = 0;
-    long long rem0 = 0;
+    const int per = (total - 1) / (int)gridDim.x + 1;
+    const int t_a = (int)min((long long)per * blockIdx.x, (long long)total), t_b = (int)min((long long)t_a + per, (long long)total);
+    int row0 = 0, rem0 = 0;
     if (t_a < t_b) {
-        int lo = 0, hi = THREADS - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= t_a)
-                lo = mid;
-            else
-                hi = mid - 1;
+        int lo = 0;
+        for (int n = THREADS; n > 1;) {  // the last thread whose rows begin at or before it
+            const int step = (n + 31) / 32, x = lo + lane * step;
+            const int k = __popc(__ballot_sync(0xffffffffu, x < lo + n && cum[x] <= t_a)) - 1;
+            n = min(step, n - k * step);
+            lo += k * step;
         }
         row0 = lo * nc;
         rem0 = t_a - cum[lo];
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
 
     Seg s;
-    long long left = t_b - t_a;
+    int left = t_b - t_a;
     int g = 0;  // tiles of this block before the segment
     if (warp < W_PREP) {
         // ------------------------------------------------------------------ softmax: two threads per query
@@ -421,40 +420,38 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t t_s = lanes + st * KT + half * (KT / 2);  // this thread's keys
         const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);
         uint32_t ns = 0, no = 0, specials = 0;
+        if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
         bool more = seek(p, s, row0, rem0, left);
         while (more) {
-            left -= s.j1 - s.j0;
             const bool pair = s.pair();
             const int T = s.j1 - s.j0, nu = pair ? T : st ? T / 2 : (T + 1) / 2;
             const int special = max(s.r.prefix / KT, s.j0);
             const int qi = s.sb * SB + (pair ? st * QT : 0) + r;  // this thread's query of the kv head
             const bool mine_q = qi < s.r.queries;
             const int tok = (int)((unsigned)qi / (unsigned)p.group), to = s.r.token + tok, head = s.kvh * p.group + qi - tok * p.group;
-            // ---- queries: a half of the dims each ----
-            if (pair || st == 0) {
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + ((long long)to * p.q_ts + (long long)head * p.q_hs) * 2);
-                auto dims = [&](int c) { return mine_q && c * 8 < p.dim ? __ldcg(src + c) : make_uint4(0, 0, 0, 0); };
-                float down = 1.f, up = 1.f;
-                if constexpr (C::RANGE) {
-                    uint32_t top = 0;
-#pragma unroll 8
-                    for (int c = 0; c < HD / 8; ++c) {
-                        const uint4 v = dims(c);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            // ---- queries: neighbouring threads have neighbouring dims; the streams share one tile's ----
+            {
+                unsigned char* dst = smem + (pair ? st : 0) * C::TILE;
+                constexpr int CPR = HD / 8;  // of 16 bytes, of a row
+#pragma unroll 2
+                for (int x = pair ? tid & 255 : tid; x < QT * CPR; x += pair ? 256 : 512) {
+                    const int row = x / CPR, c = x % CPR, i = s.sb * SB + (pair ? st * QT : 0) + row;
+                    const int tk = (int)((unsigned)i / (unsigned)p.group), hd = s.kvh * p.group + i - tk * p.group;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (i < s.r.queries && c * 8 < p.dim)
+                        v = __ldcg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + ((s.r.token + tk) * p.q_ts + hd * p.q_hs) * 2) + c);
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    float up = 1.f;
+                    if constexpr (C::RANGE) {
+                        uint32_t top = 0;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, w[k] >> 16 & 0x7fffu));
-                    }
-                    int e = (int)(top >> 7);  // biased exponent
-                    e = e == 0 || e == 255 ? 127 : min(max(e, 12), 252);
-                    down = __uint_as_float((uint32_t)(264 - e) << 23);
-                    up = __uint_as_float((uint32_t)(e - 10) << 23);
-                }
-                unsigned char* dst = smem + st * C::TILE;
-#pragma unroll 4
-                for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
-                    const uint4 v = dims(c);
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    if constexpr (C::RANGE) {
+#pragma unroll
+                        for (int o = 1; o < CPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        int e = (int)(top >> 7);  // biased exponent
+                        e = e == 0 || e == 255 ? 127 : min(max(e, 12), 252);
+                        const float down = __uint_as_float((uint32_t)(264 - e) << 23);
+                        up = __uint_as_float((uint32_t)(e - 10) << 23);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const float2 f = unpack<TI>(w[k]);
@@ -465,9 +462,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) w[k] ^= 0x80008000u;
                     }
-                    *reinterpret_cast<uint4*>(dst + sw(r, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(dst + sw(row, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (c == 0) s_up[(pair ? st * QT : 0) + row] = up;
                 }
-                if (half == 0) s_up[st * QT + r] = up;
                 tc::fence_proxy_async_smem();
             }
             tc::tc_fence_before();
@@ -617,63 +614,73 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc::tc_fence_before();
             streams_sync();
             tc::tc_fence_after();
-            if ((pair || st == 0) && !idle) {
-                float wa = 1.f, wb = 0.f;  // weights of this stream's and the other's results
-                l = s_l[st][0][r] + s_l[st][1][r];
-                if (Q8) wa = __uint_as_float(vexp << 23);
-                if (!pair) {
-                    const float o = s_m[1][r], M = fmaxf(m, o), ms = M == -INFINITY ? 0.f : M;
-                    const float xa = ex2((m - ms) * fac);
-                    wb = ex2((o - ms) * fac);
-                    l = l * xa + (s_l[1][0][r] + s_l[1][1][r]) * wb;
-                    m = M;
-                    wa *= xa;
-                    if (Q8) wb *= __uint_as_float(s_vexp[1][r] << 23);
-                }
+            if (pair || st == 0) {
                 const bool whole = s.j0 == 0 && s.j1 == s.nt;
-                const int slot = s.j0 > 0 ? 0 : 1, pr = (pair ? st * QT : 0) + r;
-                const long long part = ((long long)blockIdx.x * 2 + slot) * SB + pr;
-                const float f = whole ? inverse(l) : 1.f;
-                wa *= f, wb *= f;
-                const float mlog = m * fac;  // reference, as a power of two
-#pragma unroll 1
-                for (int c = half * (HD / 32); c < (half + 1) * (HD / 32); ++c) {
-                    uint32_t w[16];
-                    float x[16];
-                    __syncwarp();
-                    tmem_ld16(lanes + 256 + st * HD + c * 16, w);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(w[k]) * wa;
-                    if (!pair && T > 1) {
-                        tmem_ld16(lanes + 256 + HD + c * 16, w);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) x[k] = fmaf(__uint_as_float(w[k]), wb, x[k]);
+                unsigned char* stage = smem + st * C::TILE;  // the queries' place: their products are done
+                if (!idle) {
+                    float wa = 1.f, wb = 0.f;  // weights of this stream's and the other's results
+                    l = s_l[st][0][r] + s_l[st][1][r];
+                    if (Q8) wa = __uint_as_float(vexp << 23);
+                    if (!pair) {
+                        const float o = s_m[1][r], M = fmaxf(m, o), ms = M == -INFINITY ? 0.f : M;
+                        const float xa = ex2((m - ms) * fac);
+                        wb = ex2((o - ms) * fac);
+                        l = l * xa + (s_l[1][0][r] + s_l[1][1][r]) * wb;
+                        m = M;
+                        wa *= xa;
+                        if (Q8) wb *= __uint_as_float(s_vexp[1][r] << 23);
                     }
-                    if (mine_q) {
+                    const int pr = (pair ? st * QT : 0) + r;
+                    const long long part = (long long)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1);
+                    const float f = whole ? inverse(l) : 1.f;
+                    wa *= f, wb *= f;
+                    const float mlog = m * fac;  // reference, as a power of two
+#pragma unroll 1
+                    for (int c = half * (HD / 32); c < (half + 1) * (HD / 32); ++c) {
+                        uint32_t w[16];
+                        float x[16];
+                        tmem_ld16(lanes + 256 + st * HD + c * 16, w);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(w[k]) * wa;
+                        if (!pair && T > 1) {
+                            tmem_ld16(lanes + 256 + HD + c * 16, w);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) x[k] = fmaf(__uint_as_float(w[k]), wb, x[k]);
+                        }
                         if (whole) {
-                            TI* o = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + c * 16;
 #pragma unroll
-                            for (int k = 0; k < 16; k += 8)
-                                if (c * 16 + k < p.dim) store_vec<TI, 8>(o + k, x + k);
+                            for (int k = 0; k < 2; ++k)
+                                *reinterpret_cast<uint4*>(stage + sw(r, 2 * c + k)) =
+                                    make_uint4(pack<TI>(x[8 * k], x[8 * k + 1]), pack<TI>(x[8 * k + 2], x[8 * k + 3]), pack<TI>(x[8 * k + 4], x[8 * k + 5]),
+                                               pack<TI>(x[8 * k + 6], x[8 * k + 7]));
                         } else {
-                            float* o = a.part + part * HD + c * 16;
 #pragma unroll
-                            for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                            for (int k = 0; k < 4; ++k)
+                                a.part[(part * (HD / 4) + c * 4 + k) * SB + pr] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
                         }
                     }
+                    if (mine_q && half == 0) {
+                        if (!whole)
+                            a.part_ml[part * SB + pr] = make_float2(mlog, l);
+                        else if (p.lse)
+                            p.lse[(long long)to * p.n_heads + head] = l == 0.f ? -INFINITY : (mlog + log2f(l) - C::shift()) * LN2;
+                    }
                 }
-                if (mine_q && half == 0) {
-                    if (!whole)
-                        a.part_ml[part] = make_float2(mlog, l);
-                    else if (p.lse)
-                        p.lse[(long long)to * p.n_heads + head] = l == 0.f ? -INFINITY : (mlog + log2f(l) - C::shift()) * LN2;
+                if (whole) {  // rows to memory, neighbouring threads neighbouring dims
+                    half_sync(st);
+                    constexpr int CPR = HD / 8;
+#pragma unroll 2
+                    for (int x = tid & 255; x < QT * CPR; x += 256) {
+                        const int row = x / CPR, c = x % CPR, i = s.sb * SB + (pair ? st * QT : 0) + row;
+                        if (i >= s.r.queries || c * 8 >= p.dim) continue;
+                        const int tk = (int)((unsigned)i / (unsigned)p.group), hd = s.kvh * p.group + i - tk * p.group;
+                        *reinterpret_cast<uint4*>(static_cast<TI*>(p.out) + (s.r.token + tk) * p.o_ts + hd * p.o_hs + c * 8) =
+                            *reinterpret_cast<const uint4*>(stage + sw(row, c));
+                    }
                 }
             }
-            if (tid == 0 && left <= 0) {  // the range's last segment: where it goes on behind this block
-                const bool on = s.j1 < s.nt && s.j0 == 0;
-                // a segment that also begins before this block belongs to an earlier block's list
-                a.meta[blockIdx.x] = on ? make_int4(s.r.row, s.kvh, s.sb, (int)((t_b - s.j1 + s.nt - 1) / per)) : make_int4(-1, 0, 0, 0);
-            }
+            // a segment that goes on behind this block and begins in it (one that begins before is on an earlier block's list)
+            if (tid == 0 && s.j1 < s.nt && s.j0 == 0) a.meta[blockIdx.x] = make_int4(s.r.row, s.kvh, s.sb, (t_b - s.j1 + s.nt - 1) / per);
             specials += max(s.j1 - special, 0);
             g += T;
             more = next(p, s, left);
@@ -682,76 +689,85 @@ __global__ void __launch_bounds__(THREADS, 1)
             streams_sync();
             tc::tc_fence_after();
         }
-        if (tid == 0 && t_a >= t_b) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
     } else {
-        if (warp == W_TMA) {
-            // ------------------------------------------------------------------ copies
-            const int groups = KT / a.box, x = lane % C::BOXES, gr = lane / C::BOXES;  // a lane per box
-            int e = 0;  // copies to slots so far
+        if (warp >= W_TMA) {
+    // ------------------------------------------------------------------ copies
+            // Keys and values have a warp each, as their slots are separate (even and odd ones): the next keys do not wait
+            // for the place of values that come before them. 8-bit copies have three slots, in turn.
+            const int groups = KT / a.box, kind = warp - W_TMA;
             bool more = seek(p, s, row0, rem0, left);
-            auto look = [&](const Seg& w, int j) {  // the page of the lane's box in tile j; -1: no keys of the row, -2: out of range
-                const int key = j * KT + gr * a.box;
-                if (gr >= groups || key >= w.r.end) return -1;
+            auto look = [&](const Seg& w, int j) {  // the page of the lane's group of keys in tile j; -1: no keys of the row, -2: out of range
+                const int key = j * KT + lane * a.box;
+                if (lane >= groups || key >= w.r.end) return -1;
                 const int id = __ldcg(p.table + (long long)w.r.row * p.ld + (p.page_shift >= 0 ? key >> p.page_shift : key / p.page));
                 return (unsigned)id < (unsigned)p.n_pages ? id : -2;
             };
             int page = more ? look(s, s.j0) : -1;
             while (more) {
-                left -= s.j1 - s.j0;
                 Seg n = s;
                 const bool after = next(p, n, left);
                 for (int j = s.j0; j < s.j1; ++j, ++g) {
-                    const int key = j * KT + gr * a.box;
+                    const int key = j * KT + lane * a.box;
                     const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
                     const int id = page;
                     page = j + 1 < s.j1 ? look(s, j + 1) : after ? look(n, n.j0) : -1;
                     const unsigned there = __ballot_sync(0xffffffffu, id >= 0), bad = __ballot_sync(0xffffffffu, id == -2);
-                    for (int v = 0; v < 2; ++v, ++e) {
-                        const int to = e % C::LOADS;
+                    for (int v = 0; v < 2; ++v) {
+                        if (Q8 ? kind == 1 : v != kind) continue;
+                        const int e = 2 * g + v, to = e % C::LOADS;
                         if (e >= C::LOADS) wait(&b_free[to], (e / C::LOADS - 1) & 1);
                         __syncwarp();
                         const bool go = __all_sync(0xffffffffu, ok);
                         if (lane == 0) {
                             if (v == 0) s_bad[g % FLAGS] = bad != 0;
-                            if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * a.box * 128 + a.stall);
+                            if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * C::BOXES * a.box * 128 + a.stall);
                         }
                         __syncwarp();
-                        if (go && id >= 0)
-                            tma_load_4d(tc::smem_u32(smem + (Q8 ? C::OFF_RAW : C::OFF_KV) + to * (Q8 ? C::PIECE : C::TILE) + x * C::PIECE + gr * a.box * 128),
-                                        v ? &vmap : &kmap, x * (128 / (int)sizeof(TC)), slot, s.kvh, id, tc::smem_u32(&b_load[to]));
                         if (!go) ok = false;
+                        const uint32_t dst = tc::smem_u32(smem + (Q8 ? C::OFF_RAW : C::OFF_KV) + to * (Q8 ? C::PIECE : C::TILE)), bar = tc::smem_u32(&b_load[to]);
+                        // one group after the other, by an elected lane: lanes that each started a box went one by one, at 100 cycles
+#pragma unroll 4
+                        for (int gr = 0; gr < groups; ++gr) {
+                            const int pg = __shfl_sync(0xffffffffu, id, gr), sl = __shfl_sync(0xffffffffu, slot, gr);
+                            if (go && pg >= 0 && elect()) {
+#pragma unroll
+                                for (int x = 0; x < C::BOXES; ++x)
+                                    tma_load_4d(dst + x * C::PIECE + gr * a.box * 128, v ? &vmap : &kmap, x * (128 / (int)sizeof(TC)), sl, s.kvh, pg, bar);
+                            }
+                            __syncwarp();
+                        }
                     }
                 }
                 s = n;
                 more = after;
             }
             // copies that nobody waited for may still be on their way when a wait has run out
-            for (int i = max(0, e - C::LOADS); i < e && lane == 0; ++i)
+            for (int i = max(0, 2 * g - C::LOADS); i < 2 * g && lane == 0; ++i)
                 for (int k = 0; k < WAIT_TRIES / 8 && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
         } else if (warp == W_MMA) {
             // ------------------------------------------------------------------ products
             constexpr uint32_t BF = C::HALF ? 0u : (1u << 7) | (1u << 10);  // operands' format: fp16 or bf16
             constexpr uint32_t idesc_s = tc::idesc_f16_f32(QT, KT) | BF, idesc_o = tc::idesc_f16_f32_bmn(QT, HD) | BF;
+            bool more = seek(p, s, row0, rem0, left);
             if (elect()) {
                 uint64_t* there = Q8 ? b_wide : b_load;
-                uint64_t* done = Q8 ? b_reuse : b_free;
                 const uint32_t q32 = tc::smem_u32(smem), kv32 = tc::smem_u32(smem + C::OFF_KV);
                 uint32_t np[2] = {0, 0}, specials = 0;
-                bool more = seek(p, s, row0, rem0, left);
                 for (int seg = 0; more; ++seg) {
-                    left -= s.j1 - s.j0;
                     const bool pair = s.pair();
                     const int T = s.j1 - s.j0, n0 = pair ? T : (T + 1) / 2, n1 = pair ? T : T / 2;
                     // tiles from here on have values that are looked through
                     const int special = max(s.r.prefix / KT, s.j0);
-                    wait(&b_q, seg & 1);
-                    auto tile = [&](int st, int u) { return pair ? u : 2 * u + st; };
+                    auto tile = [&](int st, int u) { return g + (pair ? u : 2 * u + st); };
                     auto keys = [&](int st, int u) {
-                        const int e = 2 * (g + tile(st, u));
+                        const int e = 2 * tile(st, u);
                         wait(&there[e % C::SLOTS], (e / C::SLOTS) & 1);
                     };
+                    auto hand_back = [&](int st, int at) {
+                        if (!pair || st == 1) tc::mma_commit(Q8 ? &b_reuse[at] : &b_free[at]);
+                    };
                     auto scores = [&](int st, int u) {
-                        const int at = 2 * (g + tile(st, u)) % C::SLOTS;
+                        const int at = 2 * tile(st, u) % C::SLOTS;
                         const uint64_t q = tc::desc_sw128(q32 + (pair ? st : 0) * C::TILE), k = tc::desc_sw128(kv32 + at * C::TILE);
                         if (ok) {
 #pragma unroll
@@ -762,27 +778,32 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
                         tc::mma_commit(&b_s[st]);
                         tc::mbar_arrive(&b_s[st]);  // what this thread has seen of the tile's flags
-                        if (!pair || st == 1) tc::mma_commit(&done[at]);
+                        hand_back(st, at);
                     };
+                    wait(&b_q, seg & 1);
                     keys(0, 0);
                     if (n1 > 0) keys(1, 0);
                     tc::tc_fence_after();
                     scores(0, 0);
                     if (n1 > 0) scores(1, 0);
+                    // strictly in turn: where each stream's products came when its weights did, the streams got into step, each
+                    // waiting while the other waited and working while it worked (1.3 times the time)
                     for (int u = 0; u < n0; ++u) {
                         for (int st = 0; st < 2; ++st) {
                             if (u >= (st ? n1 : n0)) continue;
-                            const int t = tile(st, u), e = 2 * (g + t) + 1, at = e % C::SLOTS;
-                            // what is there already, usually: before the wait that is not over yet. (The next keys of a
-                            // stream of its own tiles come into the slot of these values where there are three)
+                            const int e = 2 * tile(st, u) + 1, at = e % C::SLOTS, j = s.j0 + tile(st, u) - g;
+                            // what is there already, usually: before the wait that is not over yet. (The next keys of a stream of
+                            // its own tiles come into the slot of these values where there are three)
                             constexpr bool EARLY = C::SLOTS > 3;
                             const bool again = u + 1 < (st ? n1 : n0);
-                            wait(&there[at], (e / C::SLOTS) & 1);
-                            if (!Q8 && s.j0 + t >= special) {
-                                const uint32_t k = specials + (s.j0 + t - special);
-                                wait(&b_prep[k % TILES], (k / TILES) & 1);
+                            if (!pair || st == 0) {
+                                wait(&there[at], (e / C::SLOTS) & 1);
+                                if (!Q8 && j >= special) {
+                                    const uint32_t k = specials + (j - special);
+                                    wait(&b_prep[k % TILES], (k / TILES) & 1);
+                                }
+                                if (EARLY && again) keys(st, u + 1);
                             }
-                            if (EARLY && again) keys(st, u + 1);
                             wait(&b_p[st], np[st]++ & 1);
                             tc::tc_fence_after();
                             const uint64_t v = tc::desc_sw128_mn(kv32 + at * C::TILE, C::PIECE);
@@ -791,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 for (int ks = 0; ks < KT / 16; ++ks)
                                     mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 32 + ks * 8 + (ks >> 2) * 32, v + ks * 128, idesc_o, u > 0 || ks > 0);
                             }
-                            if (!EARLY && (!pair || st == 1)) tc::mma_commit(&done[at]);
+                            hand_back(st, at);
                             if (again) {
                                 if (!EARLY) {
                                     keys(st, u + 1);
@@ -801,7 +822,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                             } else {
                                 tc::mma_commit(&b_o[st]);
                             }
-                            if (EARLY && (!pair || st == 1)) tc::mma_commit(&done[at]);
                         }
                     }
                     specials += max(s.j1 - special, 0);
@@ -817,7 +837,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             if constexpr (Q8) {
                 int e = 0;
                 while (more) {
-                    left -= s.j1 - s.j0;
                     uint32_t vexp = 1;
                     for (int j = s.j0; j < s.j1; ++j, ++g) {
                         const int key = j * KT + i;
@@ -914,7 +933,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 static_assert(Q8 || C::SLOTS % 2 == 0, "keys in even slots, values in odd ones");
                 uint32_t specials = 0;
                 while (more) {
-                    left -= s.j1 - s.j0;
                     for (int j = s.j0; j < s.j1; ++j) {
                         const int e = 2 * (g + j - s.j0) + 1, at = e % C::SLOTS, key = j * KT + i;
                         wait(&b_load[at], (e / C::SLOTS) & 1);
@@ -960,13 +978,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // Joins a segment that lies in several blocks' ranges: block c of the first kernel has its beginning (slot 1), the blocks after it
-// up to `last` the rest (slot 0). A warp per query.
+// up to `last` the rest (slot 0). A block takes 8 queries, whose four dims at a place lie side by side.
 template <class TI, int HD>
-__global__ void __launch_bounds__(256) k_paged_tree_join(const __grid_constant__ Args a, float shift) {
+__global__ void __launch_bounds__(HD * 2) k_paged_tree_join(const __grid_constant__ Args a, float shift) {
     tc::pdl_trigger();
     tc::pdl_wait();
     const PagedAttn& p = a.p;
-    const int c = blockIdx.x, lane = threadIdx.x & 31, pr = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int c = blockIdx.x, pr = blockIdx.y * 8 + (threadIdx.x & 7), d = threadIdx.x >> 3;  // d: of four dims
     const int4 meta = __ldcg(a.meta + c);
     if (meta.x < 0) return;
     const Row r = enter(p, meta.x);
@@ -974,38 +992,26 @@ __global__ void __launch_bounds__(256) k_paged_tree_join(const __grid_constant__
     if (pr >= SB || qi >= r.queries) return;
     const int tok = (int)((unsigned)qi / (unsigned)p.group), to = r.token + tok, head = meta.y * p.group + qi - tok * p.group;
     const int n = meta.w - c + 1;
-    auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * SB + pr; };
+    auto at = [&](int i) { return (long long)(c + i) * 2 + (i == 0 ? 1 : 0); };
     float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(a.part_ml + at(i)).x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) M = fmaxf(M, __ldcg(a.part_ml + at(i) * SB + pr).x);
     const float ms = M == -INFINITY ? 0.f : M;
     float L = 0.f;
-    constexpr int V = HD / 32;
-    float o[V] = {};
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
-        const float2 ml = __ldcg(a.part_ml + at(i));
+        const float2 ml = __ldcg(a.part_ml + at(i) * SB + pr);
+        const float4 v = __ldcg(a.part + (at(i) * (HD / 4) + d) * SB + pr);
         const float w = ex2(ml.x - ms);
         L = fmaf(ml.y, w, L);
-        const float* x = a.part + at(i) * HD + lane * V;
-        float v[V];
-        if constexpr (V == 4) {
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(x));
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
-            const float2 f = __ldcg(reinterpret_cast<const float2*>(x));
-            v[0] = f.x, v[1] = f.y;
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = fmaf(v[k], w, o[k]);
+        o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
     }
     const float f = inverse(L);
-    TI* out = static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + lane * V;
-    if (lane * V < p.dim) {
-        *reinterpret_cast<uint32_t*>(out) = pack<TI>(o[0] * f, o[1] * f);
-        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + 2) = pack<TI>(o[2] * f, o[3] * f);
-    }
-    if (lane == 0 && p.lse) p.lse[(long long)to * p.n_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L) - shift) * LN2;
+    if (d * 4 < p.dim)
+        *reinterpret_cast<uint2*>(static_cast<TI*>(p.out) + to * p.o_ts + head * p.o_hs + d * 4) =
+            make_uint2(pack<TI>(o.x * f, o.y * f), pack<TI>(o.z * f, o.w * f));
+    if (d == 0 && p.lse) p.lse[(long long)to * p.n_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L) - shift) * LN2;
 }
 
 // ------------------------------------------------------------------ host
@@ -1049,7 +1055,7 @@ cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken)
     static const bool stall = std::getenv("GPT2Q_TEST_PAGED_STALL") != nullptr;
     a.stall = stall ? 16 : 0;
     char* at = static_cast<char*>(work);
-    a.part = reinterpret_cast<float*>(at);
+    a.part = reinterpret_cast<float4*>(at);
     at += (size_t)CTAS * 2 * SB * C::HD * 4;
     a.part_ml = reinterpret_cast<float2*>(at);
     at += (size_t)CTAS * 2 * SB * 8;
@@ -1070,7 +1076,7 @@ cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken)
     e = launch_dependent(k_paged_tree_tc<C>, dim3(grid), dim3(THREADS), C::SMEM, st, a, km, vm);
     if (e != cudaSuccess || grid == 1) return e;
     const long long most = std::min<long long>(SB, (long long)p.n_tokens * p.group);
-    return launch_dependent(k_paged_tree_join<typename C::TI, C::HD>, dim3(grid, (unsigned)((most + 7) / 8)), dim3(256), 0, st, a, C::shift());
+    return launch_dependent(k_paged_tree_join<typename C::TI, C::HD>, dim3(grid, (unsigned)((most + 7) / 8)), dim3(C::HD * 2), 0, st, a, C::shift());
 }
 
 template <class TC, class TI>
@@ -1086,7 +1092,8 @@ uint64_t paged_tree_tc_workspace(int dim) {
 
 bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
     return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
-           (long long)p.n_tokens * p.group > 16LL * p.n_rows;
+           (long long)p.n_tokens * p.group > 16LL * p.n_rows &&
+           ((double)p.n_tokens * p.group / SB + p.n_rows) * ((double)p.cap / KT + 1 + EXTRA) * p.n_kv < 2147483648.0;  // tiles
 }
 
 cudaError_t launch_paged_tree_tc(const PagedAttn& p, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken) {

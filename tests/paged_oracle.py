@@ -7,7 +7,8 @@ Weights are held in 16-bit pieces: of fp16 caches and 8-bit ones 2^-20 covers tw
 weight times value scale (2^-35 of it, once for each of n keys); of bf16 caches 2^-20 covers three pieces (fp32 outputs) and 2^-16
 two. A cache's q in fp32 or bf16 is exact to 2^-22 of the head's largest element in fp16 pieces, which D u S covers too as D >= 8. All of it times
 the largest |v|; then the output's own rounding, e |o|. Drafted tokens' attention on wide tiles rounds each weight to one 16-bit
-number, with sum and product rounded alike: e_w = 2^-9 (bf16) or 2^-12 (fp16) of sum w |v|, and as much for scores' products."""
+number: half a step, e_w = 2^-8 (bf16, 8 significant bits: spacing 2^-7 from 1 on) or 2^-11 (fp16) of itself. The product is off by e_w
+of sum w |v|, the sum of the rounded weights (8-bit caches: of those before) by e_w of itself, and the logarithm by e_w."""
 import math
 
 import numpy as np
@@ -16,6 +17,7 @@ import torch
 T = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i8": torch.int8, "e4m3": torch.float8_e4m3fn}
 TOP = {"i8": 127.0, "e4m3": 448.0}
 U = 2.0 ** -24
+WEIGHT = (2.0 ** -11, 2.0 ** -8)  # half a step of a weight on wide tiles, of fp16 and of bf16
 
 
 def gen(seed):
@@ -119,7 +121,7 @@ def bound_of(tol, size, vmax, want, io, cache, wide=False):
     pieces = 2.0 ** -20 if io == "f32" or cache != "bf16" else 2.0 ** -16
     t = tol + pieces * vmax + want.abs() * e * 1.01 + (2.0 ** -25 if io == "f16" else 0)
     if wide and io != "f32":
-        t = t + 2 * (2.0 ** -9 if cache == "bf16" else 2.0 ** -12) * size
+        t = t + 2 * WEIGHT[cache == "bf16"] * size
     return t
 
 

@@ -9,7 +9,7 @@ import torch
 from smelt_b200._ffi import Gpt2qError
 from smelt_b200.paged import STATUS_PAGE, STATUS_POSITION, PagedKV, Rotary, tree_mask
 
-from .paged_oracle import T, U, Cache, attention64, bound_of, close, gen, randn, tables
+from .paged_oracle import T, U, WEIGHT, Cache, attention64, bound_of, close, gen, randn, tables
 
 pytestmark = pytest.mark.gpu
 TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16"), ("f32", "i8"), ("bf16", "i8"), ("f16", "i8"),
@@ -84,7 +84,7 @@ def tree_case(seed, prefixes, nodes, heads, kv, dim, io, cache, page, layout="hn
         fin = torch.isfinite(wl)
         assert torch.equal(fin, torch.isfinite(lse[a:b])) and bool((lse[a:b][~fin] == -math.inf).all())
         assert bool((out[a:b][~fin] == 0).all())
-        close(lse[a:b][fin], wl[fin], (rel + (wl.abs() + 1) * 4 * U + 2.0 ** -20)[fin] + (0 if io == "f32" else 2.0 ** -9 if cache == "bf16" else 2.0 ** -12), ("lse", k))
+        close(lse[a:b][fin], wl[fin], (rel + (wl.abs() + 1) * 4 * U + 2.0 ** -20)[fin] + (0 if io == "f32" else 1.01 * WEIGHT[cache == "bf16"]), ("lse", k))
     inside = torch.zeros(total, dtype=torch.bool, device="cuda")
     inside[gap:int(first[-1])] = True
     assert bool((out[~inside] == 9.0).all()) and bool((lse[~inside] == 7.0).all())
