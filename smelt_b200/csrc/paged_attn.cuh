@@ -39,7 +39,7 @@ namespace gpt2q {
 namespace {
 
 constexpr int STAGES = 2;
-constexpr int MAX_WARPS = 12;
+constexpr int MAX_WARPS = 16;
 constexpr int LENS = 512;     // rows whose lengths a block keeps in shared memory
 constexpr int MAX_CTAS = 148;  // one per SM of a B200
 constexpr int WAIT_TRIES = 1 << 19;  // of about 1.5 us: 0.8 s
@@ -60,9 +60,11 @@ struct Cfg {
     static constexpr bool HALF = std::is_same<CT, __half>::value;
     static constexpr int ROWB = Q8 && HD < 128 ? 128 : HD * (int)sizeof(TC);
     static constexpr int CHP = ROWB / 16;  // 16-byte chunks of a row
-    // keys of a tile: 8 KB of keys and values (16 KB at 256 dims)
-    static constexpr int TK = F32 ? (HD == 256 ? 8 : 4096 / ROWB) : (HD == 256 ? 16 : 4096 / ROWB);
+    // keys of a tile: 8 KB of keys and values (16 KB at 256 dims); of an 8-bit cache 16, half of that, as its tiles are bound
+    // by their instructions and 16 warps hold more of them than 12 (ragged rows 109 to 91 us, a long row 84 to 77)
+    static constexpr int TK = F32 ? (HD == 256 ? 8 : 4096 / ROWB) : (HD == 256 || Q8 ? 16 : 4096 / ROWB);
     static __device__ constexpr int lpk() { return 32 / TK; }  // lanes per key (fp32 cache)
+    static_assert(!Q8 || TK == 16, "a lane's scale goes by the tile's one page lookup");
     static constexpr int GR = TK < 16 ? TK : 16, NG = TK / GR;  // keys of one page lookup where pages allow it
     static constexpr int BOX = 128 / (int)sizeof(TC);  // dims of a TMA box
     // a tile's rows are cut into pieces of 128 bytes, piece by piece one after the other; the 16-byte
@@ -81,6 +83,8 @@ struct Cfg {
     // took 3 to 4 % (63 ragged rows 84.5 to 87.8 us a call, one of 131071 keys 97.1 to 100.0), with the same error
     // against 64 bits.
     static constexpr int SQ = F32 || !std::is_same<TI, float>::value ? 1 : 3;
+    // (One piece of fp16 for bf16 outputs of an 8-bit cache would be 6 % faster on a long row, but 2^-11 of the result off: a row
+    // of one key would not give its value.)
     static constexpr int sp() { return SQ == 1 || HALF ? 2 : 3; }
     // queries whose range the products' type does not have: scaled by a power of two per head. bf16 ones are then exact in
     // one piece of fp16 down to 2^-24 of the head's largest element
@@ -99,7 +103,7 @@ struct Cfg {
     // registers, of the one worked on
     static constexpr int QS = F32 ? 3 : 2;
     // warps of a block, by the registers that queries and results take
-    static constexpr int WARPS = !F32 && SQ * NT * KD * 2 + NT * KD * 4 > 100 ? 8 : MAX_WARPS;
+    static constexpr int WARPS = !F32 && SQ * NT * KD * 2 + NT * KD * 4 > 100 ? 8 : Q8 && NT == 1 && SQ == 1 && HD <= 128 ? 16 : 12;
     static constexpr float UNSHIFT = HALF ? 1.f / 1024.f : 1.f;
 };
 
@@ -315,12 +319,12 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     using TI = typename C::TI;
     constexpr int HB = C::HB, HD = C::HD, TK = C::TK, NT = C::NT > 0 ? C::NT : 1, MT = C::MT > 0 ? C::MT : 1;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ long long cum[MAX_WARPS * 32 + 1];
-    __shared__ long long wsum[MAX_WARPS];
+    __shared__ long long cum[C::WARPS * 32 + 1];
+    __shared__ long long wsum[C::WARPS];
     __shared__ int slen[LENS];
-    __shared__ Piece pieces[2 * MAX_WARPS];
-    __shared__ __align__(8) uint64_t full[MAX_WARPS][2 * STAGES];  // per stage: keys, values
-    __shared__ float pm[2 * MAX_WARPS][HB], pl[2 * MAX_WARPS][HB];
+    __shared__ Piece pieces[2 * C::WARPS];
+    __shared__ __align__(8) uint64_t full[C::WARPS][2 * STAGES];  // per stage: keys, values
+    __shared__ float pm[2 * C::WARPS][HB], pl[2 * C::WARPS][HB];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nthr = blockDim.x, nw = nthr >> 5;
     const int hv = p.heads_per_block;                    // heads a block's partial results hold
     const int qrow = HD * (int)sizeof(TI);               // bytes of a staged query
@@ -429,6 +433,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         bool stuck = false;    // a wait of this lane ran out
         // 8-bit cache: scales of key lane % TK, of the tile worked on and of the next one
         [[maybe_unused]] float ks[2] = {}, vs[2] = {};
+        [[maybe_unused]] long long s_at = -1;  // where the newest one lies
         // ... and the biased exponent that the results are held relative to, the largest of the values' scales so far: their
         // weights times scale / 2^exponent stay in the range of fp16
         [[maybe_unused]] uint32_t vexp = 1;
@@ -513,13 +518,15 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
             }
             if constexpr (C::Q8) {
                 // the scale of the lane's key; used two tiles later
-                const int key = L_key + (lane & (TK - 1));
-                const int id = TMA && C::NG > 1 && (lane & C::GR) ? page[C::NG - 1] : page[0];
-                float f = 0.f;
-                if ((ST || (key < L.end && key >= L.start)) && (unsigned)id < (unsigned)p.n_pages) {
-                    const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
-                    f = __ldcg((V ? p.v_scale : p.k_scale) + (long long)id * p.s_ps + (long long)L.kvh * p.s_hs + (long long)slot * p.s_ts);
+                if (!V) {
+                    const int key = L_key + (lane & (TK - 1));
+                    s_at = -1;
+                    if ((ST || (key < L.end && key >= L.start)) && (unsigned)page[0] < (unsigned)p.n_pages) {
+                        const int slot = p.page_shift >= 0 ? key & (p.page - 1) : key % p.page;
+                        s_at = (long long)page[0] * p.s_ps + (long long)L.kvh * p.s_hs + (long long)slot * p.s_ts;
+                    }
                 }
+                const float f = s_at >= 0 ? __ldcg((V ? p.v_scale : p.k_scale) + s_at) : 0.f;
                 if (V)
                     vs[0] = vs[1], vs[1] = f;
                 else

@@ -280,89 +280,81 @@ cudaError_t append(AppendParams p, bool vec, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ read
-// A thread takes 16 bytes of codes (of a float cache 8 elements) of READ tokens, `step` tokens apart, whose loads are all on
-// their way before the first is used. Neighbouring threads have neighbouring chunks of an entry, then the heads, keys before
-// values. Bound by the memory.
-constexpr int READ = 4;
+// A warp per token, whose place is looked up once: its lanes take the token's heads' elements, 16 bytes of output each and
+// neighbours side by side, READ of them at a time with all loads on their way before the first is used. (Threads that each
+// looked up their own token took 188 us for 100 thousand tokens with 16 codes each, 232 with 8.) Bound by the memory.
+constexpr int READ = 8;
 
 template <class TC, class TO, bool VEC>
-__global__ void __launch_bounds__(256) k_paged_read(const __grid_constant__ EntryParams p, int chunks, long long step) {
-    constexpr int N = sizeof(TC) == 1 ? 16 : 8, W = N * sizeof(TC) / 16;
+__global__ void __launch_bounds__(256) k_paged_read(const __grid_constant__ EntryParams p, int chunks) {
+    constexpr int N = 16 / sizeof(TO), B = N * sizeof(TC);  // elements, and their bytes in the cache: 4, 8 or 16
+    using Raw = std::conditional_t<B == 16, uint4, std::conditional_t<B == 8, uint2, unsigned>>;
     tc::pdl_trigger();
     tc::pdl_wait();
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int per = chunks * 2 * p.n_kv;  // threads of a token
-    const long long t0 = id / per;
-    const int rest = (int)(id - t0 * per), hh = rest / chunks, c = rest - hh * chunks;
-    if (t0 >= step) return;
-    const bool is_v = hh >= p.n_kv;
-    const int h = is_v ? hh - p.n_kv : hh;
-    uint4 raw[READ][W];
-    float scale[READ];
-    int what[READ];  // 1: an entry, 0: padding, -1: out of range
+    const int ti = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (ti >= p.n_tokens) return;
+    const int pos = __ldcg(p.pos + ti);
+    const Place at = pos < 0 ? Place{-1, 0} : place(p, p.seq ? __ldcg(p.seq + ti) : ti, pos);
+    const bool there = at.page >= 0;
+    if (pos >= 0 && !there && p.status && lane == 0) atomicOr(p.status, at.slot);
+    const float none = pos < 0 ? 0.f : __uint_as_float(0x7fffffffu);  // padding, or out of range
+    const long long off = (long long)at.page * p.c_ps + (long long)at.slot * p.c_ts, s_off = (long long)at.page * p.s_ps + (long long)at.slot * p.s_ts;
+    const unsigned units = 2u * p.n_kv * chunks;
+    for (unsigned u0 = lane; u0 < units; u0 += 32 * READ) {
+        Raw raw[READ];
+        float scale[READ];
 #pragma unroll
-    for (int i = 0; i < READ; ++i) {
-        const long long ti = t0 + i * step;
-        what[i] = 0;
-        if (ti >= p.n_tokens) continue;
-        const int pos = __ldcg(p.pos + ti);
-        if (pos < 0) continue;
-        const Place at = place(p, p.seq ? __ldcg(p.seq + ti) : (int)ti, pos);
-        what[i] = at.page < 0 ? -1 : 1;
-        if (at.page < 0) {
-            if (p.status && rest == 0) atomicOr(p.status, at.slot);
-            continue;
+        for (int i = 0; i < READ; ++i) {
+            const unsigned u = u0 + i * 32;
+            if (u >= units || !there) continue;
+            const int hh = u / (unsigned)chunks, c = u - hh * chunks, h = hh < p.n_kv ? hh : hh - p.n_kv;
+            raw[i] = __ldcg(reinterpret_cast<const Raw*>(static_cast<const TC*>(hh < p.n_kv ? p.kc : p.vc) + off + h * p.c_hs + c * N));
+            if constexpr (sizeof(TC) == 1) scale[i] = __ldcg((hh < p.n_kv ? p.k_scale : p.v_scale) + s_off + h * p.s_hs);
         }
-        const TC* src = static_cast<const TC*>(is_v ? p.vc : p.kc) + (long long)at.page * p.c_ps + (long long)at.slot * p.c_ts + h * p.c_hs + c * N;
 #pragma unroll
-        for (int w = 0; w < W; ++w) raw[i][w] = __ldcg(reinterpret_cast<const uint4*>(src) + w);
-        if constexpr (sizeof(TC) == 1)
-            scale[i] = __ldcg((is_v ? p.v_scale : p.k_scale) + (long long)at.page * p.s_ps + h * p.s_hs + (long long)at.slot * p.s_ts);
-    }
+        for (int i = 0; i < READ; ++i) {
+            const unsigned u = u0 + i * 32;
+            if (u >= units) continue;
+            const int hh = u / (unsigned)chunks, c = u - hh * chunks, h = hh < p.n_kv ? hh : hh - p.n_kv;
+            TO* dst = (hh < p.n_kv ? static_cast<TO*>(p.k) + ti * p.k_ts + h * p.k_hs : static_cast<TO*>(p.v) + ti * p.v_ts + h * p.v_hs) + c * N;
+            union {
+                uint4 u4;
+                TO t[N];
+            } r;
+            if (there) {
+                if constexpr (sizeof(TC) == 1) {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
-    for (int i = 0; i < READ; ++i) {
-        const long long ti = t0 + i * step;
-        if (ti >= p.n_tokens) continue;
-        TO* dst = is_v ? static_cast<TO*>(p.v) + ti * p.v_ts + h * p.v_hs : static_cast<TO*>(p.k) + ti * p.k_ts + h * p.k_hs;
-        dst += c * N;
-        float x[N];
-        if (what[i] == 1) {
-            if constexpr (sizeof(TC) == 1) {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(raw[i]);
+                    for (int e = 0; e < N; e += 2) {
+                        const float2 v = decode2<TC>(w[e / 4] >> (e & 2) * 8);
+                        r.t[e] = from_f<TO>(v.x * scale[i]), r.t[e + 1] = from_f<TO>(v.y * scale[i]);
+                    }
+                } else {
+                    const TC* v = reinterpret_cast<const TC*>(&raw[i]);
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const float2 v = decode2<TC>(w[e / 4] >> (e & 2) * 8);
-                    x[e] = v.x * scale[i], x[e + 1] = v.y * scale[i];
+                    for (int e = 0; e < N; ++e) r.t[e] = from_f<TO>(to_f(v[e]));
                 }
             } else {
-                const TC* v = reinterpret_cast<const TC*>(raw[i]);
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = to_f(v[e]);
+                for (int e = 0; e < N; ++e) r.t[e] = from_f<TO>(none);
             }
-        } else {
+            if constexpr (VEC) {
+                *reinterpret_cast<uint4*>(dst) = r.u4;
+            } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = what[i] ? __uint_as_float(0x7fffffffu) : 0.f;
-        }
-        if constexpr (VEC) {
-#pragma unroll
-            for (int e = 0; e < N; e += 8) store_vec<TO, 8>(dst + e, x + e);
-        } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) dst[e] = from_f<TO>(x[e]);
+                for (int e = 0; e < N; ++e) dst[e] = r.t[e];
+            }
         }
     }
 }
 
 template <class TC, class TO>
 cudaError_t read(const EntryParams& p, bool vec, cudaStream_t st) {
-    const int chunks = p.dim / (sizeof(TC) == 1 ? 16 : 8);
-    const long long per = (long long)chunks * 2 * p.n_kv;
-    // one token a thread while the call does not fill the GPU
-    const long long step = (long long)p.n_tokens * per <= 148 * 2048 ? p.n_tokens : ((long long)p.n_tokens + READ - 1) / READ;
-    const long long blocks = (step * per + 255) / 256;
-    if (per > INT32_MAX || blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-    return vec ? launch_dependent(k_paged_read<TC, TO, true>, dim3((unsigned)blocks), dim3(256), 0, st, p, chunks, step)
-               : launch_dependent(k_paged_read<TC, TO, false>, dim3((unsigned)blocks), dim3(256), 0, st, p, chunks, step);
+    const int chunks = p.dim * (int)sizeof(TO) / 16;
+    if (2LL * p.n_kv * chunks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    const dim3 grid((unsigned)(((long long)p.n_tokens + 7) / 8));
+    return vec ? launch_dependent(k_paged_read<TC, TO, true>, grid, dim3(256), 0, st, p, chunks)
+               : launch_dependent(k_paged_read<TC, TO, false>, grid, dim3(256), 0, st, p, chunks);
 }
 
 // ------------------------------------------------------------------ commit
@@ -388,31 +380,37 @@ __global__ void __launch_bounds__(256) k_paged_commit(const __grid_constant__ En
     const int* accept = p.accept + row * p.accept_ld;
     int last = -1, kept = 0, why = 0;
     for (bool more = true; more && kept < p.n_accept;) {
+        // everything is asked for before it is known whether the list goes on so far: one round of loads after the other, not
+        // one for each token (256 rows of up to 14 tokens 12.9 us)
+        int a[MOVES];
+        Place x[MOVES], y[MOVES];
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i) a[i] = kept + i < p.n_accept ? __ldcg(accept + kept + i) : -1;
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i) {
+            x[i] = y[i] = Place{-1, GPT2Q_STATUS_POSITION};
+            if (a[i] >= 0 && a[i] <= INT32_MAX - len) x[i] = place(p, row, len + a[i]);
+            if (a[i] >= 0 && kept + i <= INT32_MAX - len) y[i] = place(p, row, len + kept + i);
+        }
         char *from[MOVES], *to[MOVES];
         uint4 v[MOVES];
         int n = 0;
 #pragma unroll
         for (int i = 0; i < MOVES; ++i) {
             from[i] = to[i] = nullptr;
-            if (!more || kept + i >= p.n_accept) continue;
-            const int a = __ldcg(accept + kept + i);
-            more = a >= 0;
+            more = more && a[i] >= 0;
             if (!more) continue;
-            Place x{-1, GPT2Q_STATUS_POSITION}, y = x;
-            if (a > last && a <= INT32_MAX - len) {
-                x = place(p, row, len + a);
-                y = place(p, row, len + kept + i);
-            }
-            if (x.page < 0 || y.page < 0) {
-                why |= x.page < 0 ? x.slot : y.slot;
+            const bool rises = a[i] > last;
+            if (!rises || x[i].page < 0 || y[i].page < 0) {
+                why |= !rises ? GPT2Q_STATUS_POSITION : x[i].page < 0 ? x[i].slot : y[i].slot;
                 more = false;
                 continue;
             }
-            last = a;
+            last = a[i];
             ++n;
-            if (a == kept + i || !here) continue;
-            from[i] = base + x.page * ps + x.slot * ts;
-            to[i] = base + y.page * ps + y.slot * ts;
+            if (a[i] == kept + i || !here) continue;
+            from[i] = base + x[i].page * ps + x[i].slot * ts;
+            to[i] = base + y[i].page * ps + y[i].slot * ts;
             if (Q8 && scales)
                 v[i].x = __ldcg(reinterpret_cast<const unsigned*>(from[i]));
             else
