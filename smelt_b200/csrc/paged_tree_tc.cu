@@ -48,7 +48,8 @@ constexpr int W_PREP = 16, W_MMA = 20, W_TMA = 21;  // 21 and 22: copies of keys
 constexpr int TILES = 4;           // of which scales and masks are kept: a tile's are read before its weights are handed on, and
                                    // its slots are written again only after that
 constexpr int FLAGS = 8;           // of which page flags are kept: the copies may be four tiles ahead
-constexpr int WAIT_TRIES = 1 << 22;  // of at least 20 ns: 0.1 s and more
+constexpr int WAIT_TRIES = 1 << 26;  // of a wait that has no end in WAIT_NS either (a try takes from 20 ns to microseconds)
+constexpr unsigned long long WAIT_NS = 1000000000ull;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 // What a segment costs beside its tiles (queries, first copies, results: 22 thousand cycles against 5 thousand a tile), in tiles
@@ -300,6 +301,11 @@ __device__ __forceinline__ uint32_t visible(const PagedAttn& p, const Row& r, in
     return (v | ones(-j)) & ones(r.end - key0);
 }
 
+__device__ __forceinline__ unsigned long long globaltimer() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 template <class C>
@@ -400,12 +406,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         rem0 = t_a - cum[lo];
     }
 
-    // Each thread gives up by itself and then waits for nothing more; whoever does says so to all.
+    // Each thread gives up by itself and then waits for nothing more; whoever does says so to all, and results from then on are
+    // NaN. The copying warps start nothing after that: a barrier that still expects bytes must not be armed again.
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!ok) return;
-        for (int i = 0; i < WAIT_TRIES; ++i)
+        if (!ok || tc::mbar_try_wait(bar, parity)) return;
+        unsigned long long began = 0;
+        for (int i = 1; i < WAIT_TRIES; ++i) {
             if (tc::mbar_try_wait(bar, parity)) return;
+            if (i % 256) continue;
+            const unsigned long long now = globaltimer();
+            if (!began) began = now;
+            if (now - began > WAIT_NS) break;
+        }
         ok = false;
         atomicExch(&s_stuck, 1);
     };
@@ -717,7 +730,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const int e = 2 * g + v, to = e % C::LOADS;
                         if (e >= C::LOADS) wait(&b_free[to], (e / C::LOADS - 1) & 1);
                         __syncwarp();
-                        const bool go = __all_sync(0xffffffffu, ok);
+                        const bool go = __all_sync(0xffffffffu, ok && !*(volatile int*)&s_stuck);
                         if (lane == 0) {
                             if (v == 0) s_bad[g % FLAGS] = bad != 0;
                             if (go) tc::mbar_arrive_expect_tx(&b_load[to], __popc(there) * C::BOXES * a.box * 128 + a.stall);
@@ -741,9 +754,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 s = n;
                 more = after;
             }
-            // copies that nobody waited for may still be on their way when a wait has run out
-            for (int i = max(0, 2 * g - C::LOADS); i < 2 * g && lane == 0; ++i)
-                for (int k = 0; k < WAIT_TRIES / 8 && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
+            // copies that nobody waited for may still be on their way when a wait has run out: about as long again
+            if (lane == 0 && *(volatile int*)&s_stuck) {
+                const unsigned long long began = globaltimer();
+                for (int i = max(0, 2 * g - C::LOADS); i < 2 * g; ++i)
+                    for (int k = 0; k < WAIT_TRIES && globaltimer() - began < WAIT_NS && !tc::mbar_try_wait(&b_load[i % C::LOADS], (i / C::LOADS) & 1); ++k) {}
+            }
         } else if (warp == W_MMA) {
             // ------------------------------------------------------------------ products
             constexpr uint32_t BF = C::HALF ? 0u : (1u << 7) | (1u << 10);  // operands' format: fp16 or bf16
@@ -1090,9 +1106,12 @@ uint64_t paged_tree_tc_workspace(int dim) {
     return dim > 128 ? 0 : (uint64_t)CTAS * (2 * SB * ((dim <= 64 ? 64 : 128) * 4 + 8) + 16);
 }
 
+// From more than eight queries of a kv head per row on, on average, where the warp-level kernel reads the keys with a second set of
+// columns or more than once. Measured (32 heads on 8 of 128, bf16; here against there) with 8 queries: 32 rows of 1000 keys 78 to 46 us,
+// one of 30000 58 to 40; with 16: 78 to 74, 57 to 63; with 32: 79 to 106, 57 to 86; with 128: 89 to 326, 61 to 223.
 bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
     return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
-           (long long)p.n_tokens * p.group > 16LL * p.n_rows &&
+           (long long)p.n_tokens * p.group > 8LL * p.n_rows &&
            ((double)p.n_tokens * p.group / SB + p.n_rows) * ((double)p.cap / KT + 1 + EXTRA) * p.n_kv < 2147483648.0;  // tiles
 }
 
