@@ -358,16 +358,20 @@ cudaError_t read(const EntryParams& p, bool vec, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ commit
-// A thread owns 16 bytes of one (pool, head) - or its scale - and carries them through the row's list in order, eight
-// entries at a time: loads, then stores. Tokens rise, so an entry is never behind the place that it goes to, and the eight
-// places that are written lie before every entry that is still to be read.
-constexpr int MOVES = 8;
+// A block looks up 256 tokens of a row's list at once, a thread each, and finds where the list ends. Then every thread owns
+// 16 bytes of one (pool, head) - or its scale - and carries them through the list in order, eight entries at a time: loads, then
+// stores. Tokens rise, so an entry is never behind the place that it goes to, and a place that is written lies before every
+// entry that is still to be read. Bound by latency: the list, the table, then a round of loads for eight tokens (looked up eight at a time
+// in turn, 256 rows of up to 14 tokens took 12.9 us a call).
+constexpr int MOVES = 8, LIST = 256;
 
 template <bool Q8>
-__global__ void __launch_bounds__(256) k_paged_commit(const __grid_constant__ EntryParams p, int chunks, int size) {
+__global__ void __launch_bounds__(LIST) k_paged_commit(const __grid_constant__ EntryParams p, int chunks, int size) {
+    __shared__ int2 s_from[LIST], s_to[LIST];  // page, slot
+    __shared__ int s_a[LIST + 1], s_end;
     tc::pdl_trigger();
     tc::pdl_wait();
-    const int row = blockIdx.x, id = blockIdx.y * 256 + threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x, id = blockIdx.y * LIST + tid;
     const int pools = 2 * p.n_kv * chunks;  // threads of codes; then, of an 8-bit cache, those of scales
     const bool scales = Q8 && id >= pools, here = id < pools + (Q8 ? 2 * p.n_kv : 0);
     const int hh = scales ? id - pools : id / chunks, c = scales ? 0 : id - hh * chunks;
@@ -378,58 +382,55 @@ __global__ void __launch_bounds__(256) k_paged_commit(const __grid_constant__ En
     const long long ps = scales ? p.s_ps * 4 : p.c_ps * size, ts = scales ? p.s_ts * 4 : p.c_ts * size;
     const int len = max(__ldcg(p.lens + row), 0);
     const int* accept = p.accept + row * p.accept_ld;
-    int last = -1, kept = 0, why = 0;
+    int kept = 0;
     for (bool more = true; more && kept < p.n_accept;) {
-        // everything is asked for before it is known whether the list goes on so far: one round of loads after the other, not
-        // one for each token (256 rows of up to 14 tokens 12.9 us)
-        int a[MOVES];
-        Place x[MOVES], y[MOVES];
-#pragma unroll
-        for (int i = 0; i < MOVES; ++i) a[i] = kept + i < p.n_accept ? __ldcg(accept + kept + i) : -1;
-#pragma unroll
-        for (int i = 0; i < MOVES; ++i) {
-            x[i] = y[i] = Place{-1, GPT2Q_STATUS_POSITION};
-            if (a[i] >= 0 && a[i] <= INT32_MAX - len) x[i] = place(p, row, len + a[i]);
-            if (a[i] >= 0 && kept + i <= INT32_MAX - len) y[i] = place(p, row, len + kept + i);
+        const int i = kept + tid, a = i < p.n_accept ? __ldcg(accept + i) : -1;
+        if (tid == 0) {
+            s_end = LIST;
+            s_a[0] = kept ? s_a[LIST] : -1;  // the token before
         }
-        char *from[MOVES], *to[MOVES];
-        uint4 v[MOVES];
-        int n = 0;
+        __syncthreads();
+        s_a[tid + 1] = a;
+        Place x{-1, GPT2Q_STATUS_POSITION}, y = x;
+        if (a >= 0 && a <= INT32_MAX - len) x = place(p, row, len + a);
+        if (a >= 0 && i <= INT32_MAX - len) y = place(p, row, len + i);
+        s_from[tid] = make_int2(x.page, x.slot);
+        s_to[tid] = make_int2(y.page, y.slot);
+        __syncthreads();
+        const bool rises = a > s_a[tid];
+        if (a < 0 || !rises || x.page < 0 || y.page < 0) atomicMin(&s_end, tid);
+        __syncthreads();
+        const int n = s_end;
+        more = n == LIST;
+        if (tid == n && a >= 0 && blockIdx.y == 0 && p.status)
+            atomicOr(p.status, !rises ? GPT2Q_STATUS_POSITION : x.page < 0 ? x.slot : y.slot);
+        for (int j = 0; j < n && here; j += MOVES) {
+            uint4 v[MOVES];
 #pragma unroll
-        for (int i = 0; i < MOVES; ++i) {
-            from[i] = to[i] = nullptr;
-            more = more && a[i] >= 0;
-            if (!more) continue;
-            const bool rises = a[i] > last;
-            if (!rises || x[i].page < 0 || y[i].page < 0) {
-                why |= !rises ? GPT2Q_STATUS_POSITION : x[i].page < 0 ? x[i].slot : y[i].slot;
-                more = false;
-                continue;
+            for (int k = 0; k < MOVES; ++k) {
+                if (j + k >= n || s_a[j + k + 1] == kept + j + k) continue;
+                const int2 at = s_from[j + k];
+                const char* from = base + at.x * ps + at.y * ts;
+                if (Q8 && scales)
+                    v[k].x = __ldcg(reinterpret_cast<const unsigned*>(from));
+                else
+                    v[k] = __ldcg(reinterpret_cast<const uint4*>(from));
             }
-            last = a[i];
-            ++n;
-            if (a[i] == kept + i || !here) continue;
-            from[i] = base + x[i].page * ps + x[i].slot * ts;
-            to[i] = base + y[i].page * ps + y[i].slot * ts;
-            if (Q8 && scales)
-                v[i].x = __ldcg(reinterpret_cast<const unsigned*>(from[i]));
-            else
-                v[i] = __ldcg(reinterpret_cast<const uint4*>(from[i]));
-        }
 #pragma unroll
-        for (int i = 0; i < MOVES; ++i) {
-            if (!from[i]) continue;
-            if (Q8 && scales)
-                *reinterpret_cast<unsigned*>(to[i]) = v[i].x;
-            else
-                *reinterpret_cast<uint4*>(to[i]) = v[i];
+            for (int k = 0; k < MOVES; ++k) {
+                if (j + k >= n || s_a[j + k + 1] == kept + j + k) continue;
+                const int2 at = s_to[j + k];
+                char* to = base + at.x * ps + at.y * ts;
+                if (Q8 && scales)
+                    *reinterpret_cast<unsigned*>(to) = v[k].x;
+                else
+                    *reinterpret_cast<uint4*>(to) = v[k];
+            }
         }
         kept += n;
+        __syncthreads();  // before the list's next part
     }
-    if (id == 0) {
-        p.new_lens[row] = len + kept;
-        if (why && p.status) atomicOr(p.status, why);
-    }
+    if (id == 0) p.new_lens[row] = len + kept;
 }
 
 }  // namespace

@@ -426,3 +426,32 @@ def test_steps_with_drafts_equal_steps_without(io, cache):
         s = torch.full((n,), r, dtype=torch.int32, device="cuda")
         x, y = a.kv.read(table, at, seq=s, dtype=torch.float32), b.kv.read(table, at, seq=s, dtype=torch.float32)
         assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_commit_of_long_lists(cache):
+    """Lists of several hundred tokens, that end at and around a block's 256, at the width and at a token that does not rise."""
+    g, rng = gen(32), np.random.default_rng(32)
+    nodes, page = 700, 16
+    ends = [255, 256, 257, 511, 512, 513, 600, 300]
+    c = Cache(g, 420, 2, page, 32, cache)
+    table = tables(rng, [nodes + 100] * 8, page, 420)
+    accept = np.full((8, 600), -1, np.int32)
+    for r, n in enumerate(ends):
+        accept[r, :n] = np.sort(rng.permutation(nodes)[:n])
+    accept[7, 290] = accept[7, 289]  # ends there
+    ends[7] = 290
+    want = [bits(p).clone() for p in c.pools]
+    t = table.cpu().numpy()
+    for r, n in enumerate(ends):
+        src = 50 + accept[r, :n]
+        dst = 50 + np.arange(n)
+        at = torch.as_tensor(t[r, src // page]).long().cuda(), torch.as_tensor(src % page).cuda()
+        to = torch.as_tensor(t[r, dst // page]).long().cuda(), torch.as_tensor(dst % page).cuda()
+        for p, w in zip(c.pools, want):
+            w[to[0], :, to[1]] = bits(p)[at[0], :, at[1]].clone()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    new = c.kv.commit(table, torch.full((8,), 50, dtype=torch.int32, device="cuda"), i32(accept), status=status)
+    assert new.tolist() == [50 + n for n in ends] and int(status) == STATUS_POSITION
+    for p, w in zip(c.pools, want):
+        assert torch.equal(bits(p), w)
