@@ -52,10 +52,11 @@ constexpr int WAIT_TRIES = 1 << 26;  // of a wait that has no end in WAIT_NS eit
 constexpr unsigned long long WAIT_NS = 1000000000ull;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-// What a segment costs beside its tiles (queries, first copies, results: 22 thousand cycles against 5 thousand a tile), in tiles
-// of the list, where it comes first. Without it blocks with many short rows took twice as long as the others (tree of 31 short
-// drafts 218 us)
-constexpr int EXTRA = 4;
+// Places in the list: a tile of a block of at most 128 queries has one, of a block of more has two, and what a segment costs
+// beside its tiles (queries, first copies, results) has EXTRA, before them. Fitted over the blocks of a call with 31 short drafts: a
+// tile 2.0 us, a tile of two streams 4.1, a segment 9.0. With a place for every tile alone the blocks of many short rows took
+// three times as long as the others (218 us in all, with EXTRA = 4 130).
+constexpr int EXTRA = 5;
 constexpr float STALE = 8.f;  // log2 of the largest weight
 
 template <class TC_, class TI_, int HD_>
@@ -96,6 +97,7 @@ struct Row {
 struct Seg {
     Row r;
     int kvh, sb, j0, j1, nt;  // tiles j0 .. j1 - 1 of its nt
+    int behind;               // places that the block has behind them
     __device__ __forceinline__ int queries() const { return min(SB, r.queries - sb * SB); }
     __device__ __forceinline__ bool pair() const { return queries() > QT; }
 };
@@ -116,30 +118,38 @@ __device__ __forceinline__ Row enter(const PagedAttn& p, int row) {
 }
 // Tiles of blocks of queries 0 .. sb - 1 of a kv head. Under a mask every block has those of all keys. A chain's block ends with its
 // last query's own key: blocks but the last have ceil((prefix + ceil(256 (x + 1) / group)) / 128) =
-// floor((2 x + c) / group) tiles, whose sum goes by whole periods of `group` blocks. (A call has fewer than 2^31 tiles.)
+// floor((2 x + c) / group) tiles, whose sum goes by whole periods of `group` blocks. (A call has fewer than 2^31 places.)
 __device__ __forceinline__ int tiles_of(const PagedAttn& p, const Row& r, int sb) {
     int end = r.end;
     if (!p.mask && !r.over && sb < r.blocks - 1) end = r.prefix + ((sb + 1) * SB - 1) / p.group + 1;
     return (end + KT - 1) / KT;
 }
-// Places in the list: those tiles and EXTRA for each block.
+// Places of blocks 0 .. sb - 1: all but the last have more than 128 queries.
 __device__ __forceinline__ int places_before(const PagedAttn& p, const Row& r, int sb) {
-    if (p.mask || r.over) return sb * (tiles_of(p, r, 0) + EXTRA);
-    const unsigned G = p.group, x = max(min(sb, r.blocks - 1), 0);
-    const unsigned c = (unsigned)(((unsigned long long)r.prefix * G + 2 * KT + (unsigned long long)KT * G - 1) / KT);
-    const unsigned q = x / G, rest = x - q * G;
-    unsigned sum = G * q * (q - 1) + 2 * q * rest + sb * EXTRA;
-    for (unsigned i = 0; i < (q ? G : rest); ++i) sum += (2 * i + c) / G * (q + (i < rest ? 1 : 0));
-    return (int)sum + (sb == r.blocks && r.blocks > 0 ? tiles_of(p, r, sb - 1) : 0);
+    const unsigned x = max(min(sb, r.blocks - 1), 0);
+    unsigned sum;
+    if (p.mask || r.over) {
+        sum = x * tiles_of(p, r, 0);
+    } else {
+        const unsigned G = p.group;
+        const unsigned c = (unsigned)(((unsigned long long)r.prefix * G + 2 * KT + (unsigned long long)KT * G - 1) / KT);
+        const unsigned q = x / G, rest = x - q * G;
+        sum = G * q * (q - 1) + 2 * q * rest;
+        for (unsigned i = 0; i < (q ? G : rest); ++i) sum += (2 * i + c) / G * (q + (i < rest ? 1 : 0));
+    }
+    sum = 2 * sum + sb * EXTRA;
+    if (sb == r.blocks && sb > 0) sum += tiles_of(p, r, sb - 1) * (r.queries - (sb - 1) * SB > QT ? 2 : 1);
+    return (int)sum;
 }
 
 // Takes the places `from` .. of the block at hand that `left` covers, which it takes them from; false if they have no tile.
 __device__ __forceinline__ bool cut(const PagedAttn& p, Seg& s, int from, int& left) {
     s.nt = tiles_of(p, s.r, s.sb);
-    const int to = min(s.nt + EXTRA, from + left);
+    const int two = s.pair() ? 1 : 0, all = (s.nt << two) + EXTRA, to = min(all, from + left);
     left -= to - from;
-    s.j0 = max(from - EXTRA, 0);
-    s.j1 = max(to - EXTRA, 0);
+    s.j0 = max(from - EXTRA, 0) >> two;
+    s.j1 = max(to - EXTRA, 0) >> two;
+    s.behind = all - to;
     return s.j1 > s.j0;
 }
 // The next segment, taken from `left`; false at the end.
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     cum[tid] = before + inc - mine;
     __syncthreads();
-    const int per = (total - 1) / (int)gridDim.x + 1;
+    const int per = max((total - 1) / (int)gridDim.x + 1, 2);  // a block inside a segment has a tile of it
     const int t_a = (int)min((long long)per * blockIdx.x, (long long)total), t_b = (int)min((long long)t_a + per, (long long)total);
     int row0 = 0, rem0 = 0;
     if (t_a < t_b) {
@@ -693,7 +703,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             // a segment that goes on behind this block and begins in it (one that begins before is on an earlier block's list)
-            if (tid == 0 && s.j1 < s.nt && s.j0 == 0) a.meta[blockIdx.x] = make_int4(s.r.row, s.kvh, s.sb, (t_b - s.j1 + s.nt - 1) / per);
+            if (tid == 0 && s.j1 < s.nt && s.j0 == 0) a.meta[blockIdx.x] = make_int4(s.r.row, s.kvh, s.sb, (t_b + s.behind - 1) / per);
             specials += max(s.j1 - special, 0);
             g += T;
             more = next(p, s, left);
@@ -1112,7 +1122,7 @@ uint64_t paged_tree_tc_workspace(int dim) {
 bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
     return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
            (long long)p.n_tokens * p.group > 8LL * p.n_rows &&
-           ((double)p.n_tokens * p.group / SB + p.n_rows) * ((double)p.cap / KT + 1 + EXTRA) * p.n_kv < 2147483648.0;  // tiles
+           ((double)p.n_tokens * p.group / SB + p.n_rows) * (2 * ((double)p.cap / KT + 1) + EXTRA) * p.n_kv < 2147483648.0;  // places in the list
 }
 
 cudaError_t launch_paged_tree_tc(const PagedAttn& p, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken) {
