@@ -92,7 +92,8 @@ __device__ __forceinline__ float2 decode2(uint32_t v) {  // the lower 16 bits
 // halved the threads an SM holds.
 //
 // Into an 8-bit cache the threads of a unit row, neighbouring lanes, hold an entry between them: its largest magnitude
-// goes round by shuffles, and each writes 16 codes.
+// goes round by shuffles, and each writes 16 codes. 24 prompts of 60 to 2600 tokens, 48 heads of 128, bf16 to e4m3: 94 us (59 at the
+// memory rate).
 constexpr int BLOCKS = 4;  // of 256 threads per SM (64 registers a thread): 80 us at 16 thousand tokens; 88, 86, 90 with 3, 5, 6
 
 template <class TI, class TC, int V>
