@@ -24,7 +24,7 @@
 // 8-bit caches: an entry is code * scale, so codes are widened to fp16, in which they are exact, on their way from shared memory
 // to registers; a key's scale multiplies its scores and a value's scale its weight, relative to the largest exponent so far, so
 // that the product stays in fp16's range. Half the bytes leave the instructions as the bound: one row of 131071 keys in e4m3, 64
-// heads on 8 of 128, 77 us (43 at the memory rate), 63 rows of 17 to 9000 in int8 89 us (30), with the issue slots 48 % busy.
+// heads on 8 of 128, 77 us (43 at the memory rate), 63 rows of 17 to 9000 in int8 67 us (30).
 //
 // Drafted tokens: a row's queries are its tokens times the query heads of a kv head, in blocks of HB columns; a mask or the
 // position says which of the drafted keys a column sees. 8 drafted tokens behind 501, 12 heads of 64, fp32 on fp16: 17.8 us.
@@ -54,6 +54,12 @@ constexpr int MAX_CTAS = 148;  // one per SM of a B200
 constexpr int WAIT_TRIES = 1 << 19;  // of about 1.5 us: 0.8 s
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+
+// Places of a segment of an 8-bit cache beside its tiles. Its queries, first copies and results cost as much as several tiles of 16
+// keys, and blocks of many short rows ended last: SMs were active for 68 % of a call with 63 ragged rows, 92 us; with 2, 4 or 8 places
+// 70. 16 rows of 17 to 9000 keys 34.7 to 31.3 us, 32 of 400 to 500 27.5 to 26.5, 8 of those 17.6 to 20.8, as finding tiles in
+// such ranges takes 2 us. One row's segments are all alike and have none (1001 keys 13.2 us without, 15.7 with).
+constexpr int PADS = 4;
 
 // TC: cache type, TI: type of q and out, HD: head dim rounded up, HB: queries a tile is used for.
 // TREE: a row has any number of queries (drafted tokens) instead of one.
@@ -114,6 +120,9 @@ struct Cfg {
     // warps of a block, by the registers that queries and results take
     static constexpr int WARPS = !F32 && SQ * NT * KD * 2 + NT * KD * 4 > 100 ? 8 : Q8 && NT == 1 && SQ == 1 && HD <= 128 ? 16 : 12;
     static constexpr float UNSHIFT = HALF ? 1.f / 1024.f : 1.f;
+    // places that a segment (a row's keys for one block of queries) has in the list beside its tiles, before them
+    static constexpr int PAD = Q8 ? PADS : 0;
+    static constexpr size_t SMEM_LIMIT = (PAD ? 212 : 217) * 1024;  // dynamic; the rest for the static arrays
 };
 
 struct Walk {
@@ -330,6 +339,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ long long cum[C::WARPS * 32 + 1];
     __shared__ long long wsum[C::WARPS];
+    __shared__ long long segs[C::PAD ? C::WARPS * 32 : 1], sum_segs[C::PAD ? C::WARPS : 1], s_range[C::PAD ? 2 : 1];  // as cum and wsum, of segments
     __shared__ int slen[LENS];
     __shared__ Piece pieces[2 * C::WARPS];
     __shared__ __align__(8) uint64_t full[C::WARPS][2 * STAGES];  // per stage: keys, values
@@ -368,57 +378,97 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     tc::pdl_wait();
 
     // ---- this block's and this warp's range of tiles ----
+    const int pad = C::PAD && p.n_rows > 1 ? C::PAD : 0;  // one row's segments are all alike
     const int nc = (p.n_rows + nthr - 1) / nthr;  // rows a thread counts
     Walk w;
-    long long mine = 0;
+    long long mine = 0, mine_segs = 0;
     for (int r = tid; r < min(LENS, p.n_rows); r += nthr) slen[r] = __ldcg(p.lens + r);
     if (nc > 1) __syncthreads();
+    auto row_segs = [&](const Walk& x) { return C::TREE ? p.n_kv * x.blocks : p.n_vh; };
     for (int r = tid * nc; r < min((tid + 1) * nc, p.n_rows); ++r) {
         enter<C>(p, slen, w, r);  // with nc == 1 the thread's own
         mine += C::TREE ? (long long)w.nt * (p.n_kv * w.blocks) : w.nt;
+        if (pad && w.nt) mine_segs += row_segs(w);
     }
     if (!C::TREE) mine *= p.n_vh;
-    long long inc = mine;
+    if (C::PAD) mine += mine_segs * pad;
+    long long inc = mine, inc_segs = mine_segs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
+        if (pad) {
+            const long long u = __shfl_up_sync(0xffffffffu, inc_segs, o);
+            if (lane >= o) inc_segs += u;
+        }
     }
-    if (lane == 31) wsum[warp] = inc;
+    if (lane == 31) {
+        wsum[warp] = inc;
+        if (pad) sum_segs[warp] = inc_segs;
+    }
     __syncthreads();
-    long long before = 0, total = 0;
+    long long before = 0, total = 0, before_segs = 0, all_segs = 0;
     for (int i = 0; i < nw; ++i) {
         if (i < warp) before += wsum[i];
         total += wsum[i];
+        if (pad) {
+            if (i < warp) before_segs += sum_segs[i];
+            all_segs += sum_segs[i];
+        }
     }
     cum[tid] = before + inc - mine;
+    if (pad) segs[tid] = before_segs + inc_segs - mine_segs;
     __syncthreads();
     const long long wper = quotient(quotient(total + gridDim.x - 1, gridDim.x) + nw - 1, nw), per = wper * nw;
-    const long long ca = per * blockIdx.x, cb = min(ca + per, total);
-    const long long a = ca + wper * warp, b = min(a + wper, cb);
-    const int n = (int)max(0LL, b - a);
-
-    if (n > 0) {
-        // the row, head and tile that index a lies in
+    // Ranges of places are equal, of tiles they are what lies in them. `find`: w is the first tile at or behind a place of the list,
+    // the result its number.
+    auto find = [&](long long at) -> long long {
         int lo = 0, hi = nthr - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= a)
+            if (cum[mid] <= at)
                 lo = mid;
             else
                 hi = mid - 1;
         }
-        long long rem = a - cum[lo];
+        long long rem = at - cum[lo], skipped = pad ? segs[lo] : 0;
         int row = lo * nc;
         enter<C>(p, slen, w, row);
-        while (rem >= (long long)w.nt * (C::TREE ? p.n_kv * w.blocks : p.n_vh)) {
-            rem -= (long long)w.nt * (C::TREE ? p.n_kv * w.blocks : p.n_vh);
+        auto places = [&] { return w.nt ? w.nt + pad : 0; };
+        while (rem >= (long long)places() * row_segs(w)) {
+            rem -= (long long)places() * row_segs(w);
+            if (pad && w.nt) skipped += row_segs(w);
             enter<C>(p, slen, w, ++row);
         }
-        const int vh = (int)quotient(rem, w.nt);
-        w.j = (int)(rem - (long long)vh * w.nt);
+        const int vh = (int)quotient(rem, places());
+        w.j = (int)(rem - (long long)vh * places());
         w.kvh = vh / (C::TREE ? w.blocks : p.blocks_per_kv);
         w.hb = vh - w.kvh * (C::TREE ? w.blocks : p.blocks_per_kv);
+        if (!pad) return at;
+        const int pads = min(w.j, pad);
+        w.j -= pads;
+        return at - (skipped + vh) * pad - pads;
+    };
+    const long long end_place = min(per * (blockIdx.x + 1), total);
+    long long a = per * blockIdx.x + wper * warp, b = min(a + wper, end_place);
+    if (pad) {
+        // two lanes: where the warp's range begins and ends
+        const long long at = lane == 0 ? a : b;
+        long long tile = total - all_segs * pad;
+        if (lane < 2 && at < total) tile = find(at);
+        __syncwarp();
+        if (lane < 2 && warp == (lane ? nw - 1 : 0)) s_range[lane] = tile;  // the block's; read behind the next barrier
+        a = __shfl_sync(0xffffffffu, tile, 0), b = __shfl_sync(0xffffffffu, tile, 1);
+        w.row = __shfl_sync(0xffffffffu, w.row, 0), w.kvh = __shfl_sync(0xffffffffu, w.kvh, 0), w.hb = __shfl_sync(0xffffffffu, w.hb, 0);
+        w.j = __shfl_sync(0xffffffffu, w.j, 0);
+    }
+    const int n = (int)max(0LL, b - a);
+
+    if (n > 0) {
+        if (pad)
+            enter<C>(p, slen, w, w.row);
+        else
+            find(a);
         // L is the next tile to load, from key L_key on; its pages are looked up when the tile before
         // it is loaded
         Walk L = w;
@@ -1120,6 +1170,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     __syncthreads();
 
     // ---- the block's pieces, joined where they belong to one (row, head block) ----
+    const long long ca = pad ? s_range[0] : per * blockIdx.x, cb = pad ? s_range[C::PAD ? 1 : 0] : end_place;
     // lane i has piece i; pieces of one (row, head block) are neighbours and form a chain
     const bool there = lane < 2 * nw && pieces[lane].nt > 0;
     const long long of = there ? pieces[lane].first : -1 - lane;
@@ -1132,7 +1183,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
     if (warp == 0 && chains) {
         const Piece P = pieces[31 - __clz(heads)];  // only the last chain may go on behind the block
         if (P.first >= ca && P.first + P.nt > cb)
-            tail_row = P.row, tail_vh = P.vh, tail_blocks = P.blocks, tail_last = quotient(P.first + P.nt - 1, per);
+            tail_row = P.row, tail_vh = P.vh, tail_blocks = P.blocks, tail_last = quotient(end_place - cb + P.first + P.nt - 1, per);
     }
     for (int u = warp; u < chains * hv; u += nw) {
         const int ch = u / hv, h = u - ch * hv;
@@ -1309,8 +1360,6 @@ EncodeTiledFn tensor_map_encoder() {
     return fn;
 }
 
-constexpr size_t SMEM_LIMIT = 217 * 1024;  // dynamic; the rest for the static arrays
-
 // A pool as a tensor [page][head][piece][slot][dim]; dims past the head's own are read as zero.
 template <class C>
 bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base) {
@@ -1341,7 +1390,7 @@ cudaError_t launch_main(const PagedAttn& p, const CUtensorMap& km, const CUtenso
     if (e != cudaSuccess) return e;
     static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
     if (dev >= 64 || !(ready.load() >> dev & 1)) {
-        e = cudaFuncSetAttribute(k_paged_attn<C, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
+        e = cudaFuncSetAttribute(k_paged_attn<C, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM_LIMIT);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready |= 1ull << dev;
     }
@@ -1356,7 +1405,7 @@ cudaError_t launch(PagedAttn p, cudaStream_t st) {
     size_t wb = STAGES * C::STAGE + (size_t)C::QS * p.heads_per_block * C::HD * sizeof(typename C::TI);
     if (C::F32) wb += (size_t)C::TK * C::HB * 4;
     p.warp_bytes = (int)((wb + 1023) / 1024 * 1024);
-    const int nw = (int)std::min<size_t>(C::WARPS, SMEM_LIMIT / p.warp_bytes);
+    const int nw = (int)std::min<size_t>(C::WARPS, C::SMEM_LIMIT / p.warp_bytes);
     // no more blocks than the longest rows the table can hold would fill
     const long long longest = p.window > 0 ? std::min(p.window, p.cap) : p.cap;
     const long long tiles = ((longest + C::TK - 1) / C::TK + (p.window > 0 ? 1 : 0)) * p.n_vh;
