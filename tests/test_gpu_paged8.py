@@ -257,6 +257,13 @@ def test_attend_long_and_many_rows(cache, io, lens):
 
 
 @pytest.mark.parametrize("cache", CODES)
+@pytest.mark.parametrize("lens", [[0, 5, 0, 0, 40] * 110 + [3000, 0, 1, 2500] + [2] * 40, [2100, 1], [0, 17, 0] * 171 + [600]])
+def test_attend_short_rows_between_empty_and_long_ones(cache, lens):
+    """More rows than threads, ranges that begin before a row's first key or end there, long rows at the list's end."""
+    attend_case(13, lens, 6, 3, 64, "bf16", cache, 16, scale=1.0)
+
+
+@pytest.mark.parametrize("cache", CODES)
 @pytest.mark.parametrize("io", IO)
 def test_attend_scales_of_very_different_sizes(cache, io):
     """Entries' sizes over ten powers of ten: the bound is in units of the largest value, whatever comes first."""
