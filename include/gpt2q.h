@@ -295,7 +295,10 @@ typedef struct gpt2q_paged_kv {
  * gpt2q_paged_kv8 where the first has 8 bits. q, k, v and outputs of such calls are GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16.
  * Written entries: scale = top / T and code = round(x * (T / top)), to nearest with ties to even, where top is the entry's
  * largest magnitude (after the rotation) and T is 127 or 448, all in fp32 (the scale at most what T times it is finite for). An entry whose top is under 2^-100 has scale and
- * codes 0; one with a NaN or an infinity has codes 0 and scale NaN. */
+ * codes 0; one with a NaN or an infinity has codes 0 and scale NaN.
+ * Attention holds a weight times its value's scale in 16-bit numbers relative to the largest value scale among the keys that the query sees.
+ * Beside its roundings each key may add an error of 2^-35 of the largest |v| seen (2^-31 where products run on wide tensor-core
+ * tiles): a result that is much smaller than values of next to no weight has fewer digits for it. */
 #define GPT2Q_SCALED 1
 typedef struct gpt2q_paged_kv8 {
     gpt2q_paged_kv kv;

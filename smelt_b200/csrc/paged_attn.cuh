@@ -22,8 +22,8 @@
 // us, of which the joins and the first tile are most.
 //
 // 8-bit caches: an entry is code * scale, so codes are widened to fp16, in which they are exact, on their way from shared memory
-// to registers; a key's scale multiplies its scores and a value's scale its weight, relative to the largest exponent so far, so
-// that the product stays in fp16's range. Half the bytes leave the instructions as the bound: one row of 131071 keys in e4m3, 64
+// to registers; a key's scale multiplies its scores and a value's scale its weight, relative to the largest exponent so far (in tiles
+// with drafted tokens, for each query that of the keys it has a weight for), so that the product stays in fp16's range. Half the bytes leave the instructions as the bound: one row of 131071 keys in e4m3, 64
 // heads on 8 of 128, 77 us (43 at the memory rate), 63 rows of 17 to 9000 in int8 67 us (30).
 //
 // Drafted tokens: a row's queries are its tokens times the query heads of a kv head, in blocks of HB columns; a mask or the
@@ -494,8 +494,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
         [[maybe_unused]] float ks[2] = {}, vs[2] = {};
         [[maybe_unused]] long long s_at = -1;  // where the newest one lies
         // ... and the biased exponent that the results are held relative to, the largest of the values' scales so far: their
-        // weights times scale / 2^exponent stay in the range of fp16
-        [[maybe_unused]] uint32_t vexp = 1;
+        // weights times scale / 2^exponent stay in the range of fp16. Of a tree one per column, as columns do not see the same
+        constexpr int NE = C::TREE ? 2 * NT : 1;
+        [[maybe_unused]] uint32_t vexp[NE];
         // Starts the copies of tile i's keys (and its row's queries) or values; values come second.
         // steady: the tile and the one after it lie inside the row that the loads are in.
         auto issue = [&](int i, auto values, auto steady) {
@@ -649,7 +650,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 [[maybe_unused]] const unsigned char* q = qring + quse * hv * qrow;
 #pragma unroll
                 for (int k = 0; k < (C::F32 ? HB : 2 * NT); ++k) m[k] = -INFINITY, l[k] = 0.f;
-                vexp = 1;
+#pragma unroll
+                for (int k = 0; k < NE; ++k) vexp[k] = 1;
 #pragma unroll
                 for (int x = 0; x < (C::F32 ? HB : C::KD); ++x)
 #pragma unroll
@@ -896,28 +898,54 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 // to 6e-5 too small (now 1e-6). It costs 0.4 % of the time on the long row, 0.9 % on ragged ones
                 if constexpr (C::Q8) {
                     // weights times their values' scales, relative to the largest exponent of those so far
+                    auto lower = [&](int k, uint32_t e) {  // column k's results so far, relative to exponent e
+                        const uint32_t by = e - vexp[k % NE];
+                        al[k] *= by > 126 ? 0.f : __uint_as_float((127 - by) << 23);
+                    };
                     if (masked) {
                         const uint32_t rows = __ballot_sync(0xffffffffu, !isfinite(vs[0]));
                         if (rows) spoil(rows);
                         if (!isfinite(vs[0])) vs[0] = 0.f;
-                    }
-                    uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vs[0]))) >> 23;
-                    e = min(max(e, vexp), 253u);
-                    if (e != vexp) {
-                        const float r = e - vexp > 126 ? 0.f : __uint_as_float((127 - (e - vexp)) << 23);
+                        float f[2];  // of this lane's two keys
 #pragma unroll
-                        for (int k = 0; k < 2 * NT; ++k) al[k] *= r;
-                        vexp = e;
-                    }
-                    const float scaled = vs[0] * __uint_as_float((254 - e) << 23);
+                        for (int u = 0; u < 2; ++u) f[u] = __shfl_sync(0xffffffffu, vs[0], u * 8 + (lane >> 2));
 #pragma unroll
-                    for (int x = 0; x < MT; ++x)
+                        for (int k = 0; k < 2 * NT; ++k) {
+                            uint32_t top = 0;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const float f = __shfl_sync(0xffffffffu, scaled, x * 16 + u * 8 + (lane >> 2));
+                            for (int u = 0; u < 2; ++u) top = max(top, S[0][k / 2][0][2 * u + (k & 1)] != 0.f ? __float_as_uint(fabsf(f[u])) : 0u);
 #pragma unroll
-                            for (int y = 0; y < NT; ++y) S[x][y][0][2 * u] *= f, S[x][y][0][2 * u + 1] *= f;
+                            for (int o = 4; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            const uint32_t e = min(max(top >> 23, vexp[k % NE]), 253u);
+                            lower(k, e);
+                            vexp[k % NE] = e;
+                            const float down = __uint_as_float((254 - e) << 23);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                float& w = S[0][k / 2][0][2 * u + (k & 1)];
+                                w = w != 0.f ? w * (f[u] * down) : 0.f;  // (a scale without a weight may be past the range)
+                            }
                         }
+                    } else {
+                        // (of a tree, columns differ only behind the first tile with drafted tokens, which are the row's last)
+                        uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vs[0]))) >> 23;
+                        e = min(max(e, vexp[0]), 253u);
+                        if (e != vexp[0]) {
+#pragma unroll
+                            for (int k = 0; k < 2 * NT; ++k) lower(k, e);
+#pragma unroll
+                            for (int k = 0; k < NE; ++k) vexp[k] = e;
+                        }
+                        const float scaled = vs[0] * __uint_as_float((254 - e) << 23);
+#pragma unroll
+                        for (int x = 0; x < MT; ++x)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const float f = __shfl_sync(0xffffffffu, scaled, x * 16 + u * 8 + (lane >> 2));
+#pragma unroll
+                                for (int y = 0; y < NT; ++y) S[x][y][0][2 * u] *= f, S[x][y][0][2 * u + 1] *= f;
+                            }
+                    }
                 }
                 uint32_t pf[C::sp()][MT][NT][2];
 #pragma unroll
@@ -1058,7 +1086,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 const long long first = a + i - w.j;  // its first tile
                 const bool whole = first >= a && w.j + 1 == w.nt;
                 const int h0 = w.hb * HB, nh = min(HB, (C::TREE ? w.queries : p.group) - h0);
-                const float up = C::Q8 ? C::UNSHIFT * __uint_as_float(vexp << 23) : C::UNSHIFT;
+                auto up = [&](int k) { return C::Q8 ? C::UNSHIFT * __uint_as_float(vexp[k % NE] << 23) : C::UNSHIFT; };  // of column k
                 if (TMA && __any_sync(0xffffffffu, stuck)) bad |= GPT2Q_STATUS_TIMEOUT;
                 if (bad && p.status && lane == 0) atomicOr(p.status, bad);
 #pragma unroll
@@ -1103,11 +1131,11 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                             if (!whole) {
                                 float* at = dst + h * C::HS + d0;  // dims past the head's own are 0, and not read
 #pragma unroll
-                                for (int d = 0; d < 2 * C::KD; ++d) at[off(d)] = O[d / 2][y][2 * (d & 1) + c] * up;
+                                for (int d = 0; d < 2 * C::KD; ++d) at[off(d)] = O[d / 2][y][2 * (d & 1) + c] * up(k);
                                 if (lane < 4) pm[ps][h] = m[k], pl[ps][h] = l[k];
                                 continue;
                             }
-                            const float f = inverse(l[k]) * up;
+                            const float f = inverse(l[k]) * up(k);
                             int to, head;
                             query_at<C>(p, w.row, w.token, w.kvh, h0 + h, to, head);
                             if (p.out) {

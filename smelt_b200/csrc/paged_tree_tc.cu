@@ -17,8 +17,9 @@
 // 2^8 (weights stay below that, and the sum has the same reference).
 //
 // 8-bit caches: the preparing warps write the codes as fp16, in which they are exact; keys' scales multiply the scores and
-// values' scales the weights, both in fp32. The values' scales are held relative to the largest exponent so far, so that
-// weight times scale stays in fp16's range. bf16 queries are scaled per row by a power of two that brings the largest
+// values' scales the weights, both in fp32. The values' scales are held relative to the largest exponent so far of those that a query
+// sees, so that weight times scale stays in fp16's range: in tiles of the prefix alone it is the same for all queries and the preparing
+// warps have it, in those with drafted tokens each query finds its own. bf16 queries are scaled per row by a power of two that brings the largest
 // element to [2^10, 2^11), and are exact in fp16 down to 2^-24 of it.
 //
 // A weight is rounded to 16 bits, once (by up to 2^-8 of itself in bf16, 2^-11 in fp16): as the output is, and with
@@ -341,7 +342,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     __shared__ __align__(8) uint64_t b_prep[TILES];          // 16-bit: a tile of values with drafted tokens is looked through
     __shared__ __align__(8) uint64_t b_q, b_s[2], b_p[2], b_o[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float s_scale[Q8 ? TILES : 1][2][KT];  // of keys, of values (relative to 2^s_exp)
+    // of keys, of values (relative to 2^s_exp; as they are in tiles with drafted tokens)
+    __shared__ __align__(16) float s_scale[Q8 ? TILES : 1][2][KT];
+    __shared__ unsigned char s_seen[Q8 ? 2 : 1][2][Q8 ? QT : 1];  // of the streams' halves: the largest exponent of the scales that a query sees
     __shared__ uint32_t s_exp[TILES];
     __shared__ uint32_t s_spoilt[TILES][4];           // drafted tokens' values that are not finite
     __shared__ int s_bad[FLAGS];                      // a page id is out of range
@@ -556,7 +559,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if constexpr (Q8) {
                     const int en = 2 * (g + t) + 1;
                     wait(&b_wide[en % C::SLOTS], (en / C::SLOTS) & 1);
-                    e = s_exp[gt];
+                    if (look) {
+                        // what this query does not see must not count, however large it is
+                        uint32_t top = 0;
+                        if (!idle) {
+                            const float* vs = s_scale[gt][1] + half * (KT / 2);
+#pragma unroll 1
+                            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) top = max(top, vis[c] >> k & 1 ? __float_as_uint(fabsf(vs[c * 32 + k])) : 0u);
+                        }
+                        s_seen[st][half][r] = (unsigned char)(top >> 23);
+                        half_sync(st);
+                        e = min(max(max(top >> 23, (uint32_t)s_seen[st][half ^ 1][r]), vexp), 253u);
+                    } else {
+                        e = s_exp[gt];
+                    }
                 } else if (look) {
                     const uint32_t k = specials + (j - special);
                     wait(&b_prep[k % TILES], (k / TILES) & 1);
@@ -596,7 +614,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const float ref = m == -INFINITY ? 0.f : m;
                     const float2 nref = make_float2(-ref, -ref), f2 = make_float2(fac, fac), sh = make_float2(C::shift(), C::shift());
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    auto weights = [&](int c) {
+                    [[maybe_unused]] const float down = __uint_as_float((254 - vexp) << 23);
+                    auto weights = [&](int c, auto own) {  // own: the scales are as they are, and count where they are seen
                         scores(c);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -609,7 +628,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 float2 y = make_float2(ex2(d.x), ex2(d.y));
                                 if constexpr (Q8) {
                                     sum[i & 1] = add2(sum[i & 1], y);
-                                    y = mul2(y, *reinterpret_cast<const float2*>(s_scale[gt][1] + half * (KT / 2) + c * 32 + k));
+                                    float2 f = *reinterpret_cast<const float2*>(s_scale[gt][1] + half * (KT / 2) + c * 32 + k);
+                                    if constexpr (decltype(own)::value) {
+                                        f = mul2(f, make_float2(down, down));
+                                        f.x = vis[c] >> k & 1 ? f.x : 0.f, f.y = vis[c] >> (k + 1) & 1 ? f.y : 0.f;
+                                    }
+                                    y = mul2(y, f);
                                     w[i] = pack<CT>(y.x, y.y);
                                 } else {
                                     w[i] = pack<CT>(y.x, y.y);
@@ -620,8 +644,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
                     };
                     // both quarters' weights take the columns of the later one
-                    weights(1);
-                    weights(0);
+                    if (Q8 && look) {
+                        weights(1, std::bool_constant<Q8>{});
+                        weights(0, std::bool_constant<Q8>{});
+                    } else {
+                        weights(1, std::false_type{});
+                        weights(0, std::false_type{});
+                    }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
                 tmem_wait_st();
@@ -894,19 +923,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 if (drafted) {
                                     const uint32_t b = __ballot_sync(0xffffffffu, spoilt);
                                     if (lane == 0) s_spoilt[g % TILES][warp - W_PREP] = b;
-                                }
-                                if (spoilt) sc[1] = 0.f;
-                                // the largest exponent of the tile's scales, over the four warps
-                                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
-                                if (lane == 0) wsum[W_PREP + warp - W_PREP] = m;
-                                asm volatile("bar.sync 2, 128;" ::: "memory");
-                                uint32_t x = vexp;
+                                    s_scale[g % TILES][1][i] = spoilt ? 0.f : sc[1];
+                                    asm volatile("bar.sync 2, 128;" ::: "memory");  // the masks are there
+                                } else {
+                                    // the largest exponent of the tile's scales, over the four warps
+                                    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
+                                    if (lane == 0) wsum[warp] = m;
+                                    asm volatile("bar.sync 2, 128;" ::: "memory");
+                                    uint32_t x = vexp;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
-                                vexp = min(x, 253u);
-                                s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
-                                if (i == 0) s_exp[g % TILES] = vexp;
-                                asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again; the masks are there
+                                    for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
+                                    vexp = min(x, 253u);
+                                    s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
+                                    if (i == 0) s_exp[g % TILES] = vexp;
+                                    asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again
+                                }
                             }
                             wait(&b_load[from], (e / C::RAWS) & 1);
                             const unsigned char* src = smem + C::OFF_RAW + from * C::PIECE;
