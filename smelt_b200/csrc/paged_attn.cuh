@@ -798,13 +798,13 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     __syncwarp();
                 }
             };
-            // Of a tile with drafted tokens' keys: the values that are not finite, as a mask of keys. They are cleared, so that
-            // a query that does not see one is not reached by it (its weight is 0, but 0 times infinity is NaN).
-            auto unclean = [&]() -> uint32_t {
+            // Of a tile with drafted tokens' keys, from key `from` on: those values that are not finite, as a mask of keys. They are
+            // cleared, so that a query that does not see one is not reached by it (its weight is 0, but 0 times infinity is NaN).
+            auto unclean = [&](int from) -> uint32_t {
                 uint32_t rows = 0;
                 if constexpr (!std::is_same<TC, int8_t>::value) {
                     unsigned char* v = ring + stage * C::STAGE + TK * C::ROWB;
-                    for (int x = lane; x < TK * nch; x += 32)
+                    for (int x = max(from, 0) * nch + lane; x < TK * nch; x += 32)
                         if (not_finite<TC>(*reinterpret_cast<const uint4*>(v + C::at(x / nch, x % nch)))) rows |= 1u << (x / nch);
                     rows = __reduce_or_sync(0xffffffffu, rows);
                     if (rows) {
@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 wait(2 * stage + 1, i);
                 arrived();
                 if (masked) {
-                    const uint32_t rows = unclean();
+                    const uint32_t rows = unclean(drafted0 - tile0);
                     if (rows) spoil(rows);
                 }
                 constexpr int DS = C::Q8 ? 2 : 1;  // steps of 16 dims that a load has (of 8-bit codes 32 dims)
@@ -1032,7 +1032,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                 wait(2 * stage + 1, i);
                 arrived();
                 if (masked) {
-                    const uint32_t rows = unclean();
+                    const uint32_t rows = unclean(drafted0 - tile0);
 #pragma unroll
                     for (int h = 0; h < HB; ++h)
                         if (part == 0 && rows >> key & 1 && pbuf[key * HB + h] != 0.f) l[h] = NAN;
