@@ -204,7 +204,8 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     p.q = q->data, p.q_ts = q->token_stride, p.q_hs = q->head_stride;
     p.out = out->data, p.o_ts = out->token_stride, p.o_hs = out->head_stride, p.hl = hl, p.lse = d_lse;
     p.table = table->ids, p.lens = d_lens, p.ld = table->ld, p.n_rows = table->n_rows;
-    p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX - 64);
+    // (positions of a tile, and of a warp's 32 boxes of up to 128 keys, past a row's last stay below 2^31)
+    p.cap = (int)std::min<long long>((long long)table->width * kv->page_size, INT32_MAX - (tree ? 32 * 128 : 64));
     p.n_heads = n_heads, p.n_kv = kv->n_kv_heads, p.group = n_heads / kv->n_kv_heads, p.dim = kv->head_dim;
     p.window = window, p.scale = scale, p.status = d_status;
     take_scales(&p, kv);

@@ -117,7 +117,7 @@ __device__ __forceinline__ Row enter(const PagedAttn& p, int row) {
     r.n = max(min(b, p.n_tokens) - r.token, 0);
     if (r.n == 0) return r;
     r.prefix = max(__ldcg(p.lens + row), 0);
-    r.over = (long long)r.prefix + r.n > p.cap;
+    r.over = (long long)r.prefix + r.n > p.cap;  // cap + 32 * KT stays below 2^31
     r.end = r.over ? p.cap : r.prefix + r.n;
     r.queries = r.n * p.group;
     r.blocks = (r.queries + SB - 1) / SB;
