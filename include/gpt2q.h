@@ -396,7 +396,8 @@ int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
  * belong to no row are left as they were. Otherwise as gpt2q_paged_attention: types, alignment, d_lse [n_tokens][n_heads],
  * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order; for
  * 16-bit outputs the weights are rounded to 16 bits where the products run on wide tensor-core tiles. A length <= 0 is a prefix of none. A
- * prefix and its drafted tokens are at most 2^31 - 4097 together, whatever the table's width (more give NaN and the status bit).
+ * d_first that does not rise gives numbers without a meaning; where it asks for more work than one that rises could, nothing is
+ * written but GPT2Q_STATUS_POSITION. A prefix and its drafted tokens are at most 2^31 - 4097 together, whatever the table's width (more give NaN and the status bit).
  * d_work: gpt2q_paged_tree_attention_workspace(kv, n_heads, n_tokens) bytes, 16-byte aligned, of one call at a time. */
 uint64_t gpt2q_paged_tree_attention_workspace(const gpt2q_paged_kv* kv, int n_heads, int n_tokens);
 int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,

@@ -36,6 +36,7 @@ struct PagedAttn {
     // a tree of drafted tokens per row (first != null): row r has tokens first[r] .. first[r + 1] - 1; lens are those of the prefixes
     const int *first, *mask;
     int mask_words, n_tokens;
+    long long most;  // places in the list of tiles that a `first` that rises can ask for
     int n_rows, n_heads, n_kv, group, dim, window;
     int cap;  // the longest length a row of the table can hold
     float scale;

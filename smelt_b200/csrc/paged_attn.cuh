@@ -416,6 +416,10 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
             all_segs += sum_segs[i];
         }
     }
+    if (C::TREE && total > p.most) {  // a `first` that names tokens again and again: no work rather than any amount of it
+        total = all_segs = 0;
+        if (tid == 0 && blockIdx.x == 0 && p.status) atomicOr(p.status, GPT2Q_STATUS_POSITION);
+    }
     cum[tid] = before + inc - mine;
     if (pad) segs[tid] = before_segs + inc_segs - mine_segs;
     __syncthreads();
@@ -1441,6 +1445,7 @@ cudaError_t launch(PagedAttn p, cudaStream_t st) {
     const long long rows = C::TREE ? std::min<long long>(p.n_rows, p.n_tokens) + (long long)p.n_tokens * p.group / C::HB : p.n_rows;
     const long long want = tiles > MAX_CTAS * 8LL ? MAX_CTAS : (tiles * rows + nw - 1) / nw;
     const int grid = (int)std::clamp<long long>(want, 1, MAX_CTAS);
+    if (C::TREE) p.most = ((long long)p.n_tokens * p.group / C::HB + p.n_rows) * p.n_kv * (((long long)p.cap + C::TK - 1) / C::TK + C::PAD);
     p.boxes = (p.dim * (int)sizeof(typename C::TC) + 127) / 128;
     p.box_loads = p.boxes > 1 && p.dim % C::BOX == 0 && C::NG == 1 ? 1 : p.boxes;
     p.group_bytes = p.boxes * C::GR * 128;

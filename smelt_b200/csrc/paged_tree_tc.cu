@@ -336,7 +336,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const PagedAttn& p = a.p;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ int cum[THREADS], wsum[WARPS];
+    __shared__ int cum[THREADS];
+    __shared__ long long sums[WARPS];
+    __shared__ uint32_t s_top[4];  // of the preparing warps
     __shared__ __align__(8) uint64_t b_load[8], b_free[8];   // copies have landed in a slot; its tile is no longer needed
     __shared__ __align__(8) uint64_t b_wide[8], b_reuse[8];  // 8-bit: a tile is there in fp16; its slot may be written again
     __shared__ __align__(8) uint64_t b_prep[TILES];          // 16-bit: a tile of values with drafted tokens is looked through
@@ -390,25 +392,30 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     // ---- this block's range of tiles ----
     const int nc = (p.n_rows + THREADS - 1) / THREADS;  // rows a thread counts
-    int mine = 0;
+    long long mine = 0;
     for (int r = tid * nc; r < min((tid + 1) * nc, p.n_rows); ++r) {
         const Row w = enter(p, r);
-        mine += places_before(p, w, w.blocks) * p.n_kv;
+        mine += (long long)places_before(p, w, w.blocks) * p.n_kv;
     }
-    int inc = mine;
+    long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
     }
-    if (lane == 31) wsum[warp] = inc;
+    if (lane == 31) sums[warp] = inc;
     __syncthreads();
-    int before = 0, total = 0;
+    long long before = 0, all = 0;
     for (int i = 0; i < WARPS; ++i) {
-        if (i < warp) before += wsum[i];
-        total += wsum[i];
+        if (i < warp) before += sums[i];
+        all += sums[i];
     }
-    cum[tid] = before + inc - mine;
+    if (all > p.most) {  // a `first` that names tokens again and again: no work rather than any amount of it
+        all = 0;
+        if (tid == 0 && blockIdx.x == 0 && p.status) atomicOr(p.status, GPT2Q_STATUS_POSITION);
+    }
+    const int total = (int)all;
+    cum[tid] = (int)(before + inc - mine);
     __syncthreads();
     const int per = max((total - 1) / (int)gridDim.x + 1, 2);  // a block inside a segment has a tile of it
     const int t_a = (int)min((long long)per * blockIdx.x, (long long)total), t_b = (int)min((long long)t_a + per, (long long)total);
@@ -928,15 +935,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 } else {
                                     // the largest exponent of the tile's scales, over the four warps
                                     const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc[1])));
-                                    if (lane == 0) wsum[warp] = m;
+                                    if (lane == 0) s_top[warp - W_PREP] = m;
                                     asm volatile("bar.sync 2, 128;" ::: "memory");
                                     uint32_t x = vexp;
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) x = max(x, (uint32_t)wsum[W_PREP + k] >> 23);
+                                    for (int k = 0; k < 4; ++k) x = max(x, s_top[k] >> 23);
                                     vexp = min(x, 253u);
                                     s_scale[g % TILES][1][i] = sc[1] * __uint_as_float((254 - vexp) << 23);
                                     if (i == 0) s_exp[g % TILES] = vexp;
-                                    asm volatile("bar.sync 2, 128;" ::: "memory");  // wsum is used again
+                                    asm volatile("bar.sync 2, 128;" ::: "memory");  // s_top is used again
                                 }
                             }
                             wait(&b_load[from], (e / C::RAWS) & 1);
@@ -1153,17 +1160,25 @@ uint64_t paged_tree_tc_workspace(int dim) {
     return dim > 128 ? 0 : (uint64_t)CTAS * (2 * SB * ((dim <= 64 ? 64 : 128) * 4 + 8) + 16);
 }
 
+namespace {
+// At most the places in the list (tiles_of and places_before) of a `first` that rises.
+double most_places(const PagedAttn& p) {
+    return ((double)p.n_tokens * p.group / SB + p.n_rows) * (2 * ((double)p.cap / KT + 1) + EXTRA) * p.n_kv;
+}
+}  // namespace
+
 // From more than eight queries of a kv head per row on, on average, where the warp-level kernel reads the keys with a second set of
 // columns or more than once. Measured (32 heads on 8 of 128, bf16; here against there), 32 rows of 1000 keys and one of 30000: with 16
 // queries 71 to 74 us and 52 to 63, with 32 72 to 106 and 52 to 86, with 128 81 to 326 and 56 to 223. With 12 it is 71 and 52 here, with
 // 8 44 and 37 there.
 bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
     return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
-           (long long)p.n_tokens * p.group > 8LL * p.n_rows &&
-           ((double)p.n_tokens * p.group / SB + p.n_rows) * (2 * ((double)p.cap / KT + 1) + EXTRA) * p.n_kv < 2147483648.0;  // places in the list
+           (long long)p.n_tokens * p.group > 8LL * p.n_rows && most_places(p) < 2147483648.0;
 }
 
-cudaError_t launch_paged_tree_tc(const PagedAttn& p, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken) {
+cudaError_t launch_paged_tree_tc(const PagedAttn& call, int cache_dtype, int dtype, void* work, cudaStream_t st, bool* taken) {
+    PagedAttn p = call;
+    p.most = (long long)most_places(p);
     if (cache_dtype == GPT2Q_F16) return by_dim<__half, __half>(p, work, st, taken);
     if (cache_dtype == GPT2Q_BF16) return by_dim<bf16, bf16>(p, work, st, taken);
     if (cache_dtype == GPT2Q_I8)
