@@ -273,7 +273,7 @@ int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float
  * (in elements): the entry of token slot o in page p for kv head h starts at
  * p * page_stride + h * head_stride + o * token_stride and holds head_dim elements. The pools' base
  * addresses and all strides are multiples of 16 bytes; head_dim is a multiple of 8, at most 256.
- * Entries must not overlap (an append refuses strides by which they would). */
+ * Entries must not overlap, keys' and values' ones neither (an append refuses a cache in which they would). */
 typedef struct gpt2q_paged_kv {
     void* k;
     void* v;
@@ -346,7 +346,8 @@ typedef struct gpt2q_heads {
 /* Appends n_tokens keys and values (both or neither of k->data and v->data) to the cache. Token i
  * belongs to table row d_seq[i] (d_seq NULL: row i) and position d_pos[i]. Keys are rotated when
  * `rot` is given, rounded once to the cache's type; with `q` and `q_out` the token's n_q_heads
- * queries are rotated into q_out too (q_out may be q). k, v, q and q_out are of type `dtype`, the
+ * queries are rotated into q_out too (q_out may be q; it shares no other memory with q, k, v or the
+ * cache). k, v, q and q_out are of type `dtype`, the
  * cache's or GPT2Q_F32. A token with d_pos[i] < 0 is padding: nothing of it is written to the
  * cache and its queries are copied unrotated. A token whose page, position or row is out of range
  * is not written either and sets its bit in d_status (may be NULL). No two tokens of a call may
@@ -365,8 +366,8 @@ int gpt2q_paged_append_at(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
                           const gpt2q_rotary* rot, int32_t* d_status, void* stream);
 
 /* Reads n_tokens entries into k and v ([token][kv head][head_dim], type `dtype`: the cache's or GPT2Q_F32, of an 8-bit cache any
- * of the three): token i is that of table row d_seq[i] (d_seq NULL: row i) at position d_pos[i]. Each element is rounded once from
- * the value it stands for. d_pos[i] < 0 gives zeros; a row, position or page out of range gives NaN and sets its bit in
+ * of the three): token i is that of table row d_seq[i] (d_seq NULL: row i) at position d_pos[i]. k and v share no memory with one
+ * another or the cache (a call refuses those that do). Each element is rounded once from the value it stands for. d_pos[i] < 0 gives zeros; a row, position or page out of range gives NaN and sets its bit in
  * d_status (may be NULL). */
 int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k, const gpt2q_heads* v,
                      int dtype, int n_tokens, const int32_t* d_pos, const int32_t* d_seq, int32_t* d_status, void* stream);
@@ -409,7 +410,7 @@ int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table*
  * order (a negative one ends the list). Entry d_lens[r] + d_accept[r * ld + i] moves to position d_lens[r] + i, codes and scales as
  * they are (keys stay rotated by the position they had), and d_new_lens[r] = max(d_lens[r], 0) + the number kept. At a token that does
  * not rise, or whose page or position is out of range, the row's list ends and the bit is set in d_status (may be NULL;
- * GPT2Q_STATUS_POSITION, GPT2Q_STATUS_PAGE). Rows must not share the pages that are written. d_new_lens is not d_lens. */
+ * GPT2Q_STATUS_POSITION, GPT2Q_STATUS_PAGE). Rows must not share the pages that are written. d_new_lens shares no memory with d_lens or d_accept. */
 int gpt2q_paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
                        const int32_t* d_accept, int width, int64_t ld, int32_t* d_new_lens, int32_t* d_status, void* stream);
 

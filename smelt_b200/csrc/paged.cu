@@ -4,7 +4,6 @@
 #include <cstdint>
 #include <cstdlib>
 #include <string>
-#include <utility>
 
 #include "device_op.cuh"
 #include "gpt2q.h"
@@ -22,18 +21,93 @@ bool aligned16(const void* p, int64_t a, int64_t b, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
 }
 
-// Whether two of n x m runs of dim elements, starting at i * a + j * b, share an element.
-bool overlap(int64_t n, int64_t a, int64_t m, int64_t b, int64_t dim) {
-    if (n < 1 || m < 1) return false;
-    a = std::abs(a), b = std::abs(b);
-    if (a > b) std::swap(a, b), std::swap(n, m);
-    if ((n > 1 && a < dim) || (m > 1 && b < dim)) return true;
-    if (n == 1 || m == 1 || b >= a * (n - 1) + dim) return false;
-    for (int64_t j = 1; j < m && j * b < a * (n - 1) + dim; ++j) {  // runs that lie between one another
-        const int64_t i = j * b / a;  // the nearest of the a-steps on either side
-        if ((i < n && j * b - i * a < dim) || (i + 1 < n && (i + 1) * a - j * b < dim)) return true;
+// n[0] x n[1] x n[2] runs of `bytes` bytes: run (i, j, k) begins at at + i * step[0] + j * step[1] + k * step[2].
+struct Runs {
+    const void* at;
+    int64_t n[3], step[3], bytes;
+};
+// A term x * step of a sum, lo <= x <= hi, step >= 0.
+struct Term {
+    int64_t lo, hi, step;
+};
+// Of addresses up to 2^58: what lies beyond is no memory, and sums of six stay in 64 bits.
+int64_t reach(int64_t n, int64_t step) { return step >> 27 ? std::min<int64_t>(n - 1, ((int64_t)1 << 58) / step) : n - 1; }
+
+// Whether a sum of terms, ordered by falling steps, lies in [low, high]. Steps that are larger than all that follows them, as
+// those of nearly all tensors are, leave one or two values of each x to look at.
+bool hits(const Term* t, int n, int64_t low, int64_t high) {
+    if (n == 0) return low <= 0 && 0 <= high;
+    int64_t least = 0, most = 0;  // of the terms that follow
+    for (int i = 1; i < n; ++i) least += t[i].lo * t[i].step, most += t[i].hi * t[i].step;
+    if (t->step == 0) return hits(t + 1, n - 1, low, high);
+    auto below = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };  // a / b rounded down
+    const int64_t from = std::max(t->lo, -below(most - low, t->step)), to = std::min(t->hi, below(high - least, t->step));
+    for (int64_t x = from; x <= to; ++x)
+        if (hits(t + 1, n - 1, low - x * t->step, high - x * t->step)) return true;
+    return false;
+}
+// Orders terms by falling steps, those of one step as one (whose x is their sum or difference); returns how many there are.
+int by_step(Term* t, int n) {
+    std::sort(t, t + n, [](const Term& a, const Term& b) { return a.step > b.step; });
+    int m = 1;
+    for (int i = 1; i < n; ++i)
+        if (t[i].step == t[m - 1].step)
+            t[m - 1].lo += t[i].lo, t[m - 1].hi += t[i].hi;
+        else
+            t[m++] = t[i];
+    return m;
+}
+
+// Whether two runs share a byte.
+bool overlap(const Runs& r) {
+    for (int i = 0; i < 3; ++i)
+        if (r.n[i] < 1) return false;
+    // nested, as nearly all are: each step past what the smaller ones reach
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int x, int y) { return std::abs(r.step[x]) < std::abs(r.step[y]); });
+    int64_t extent = r.bytes;
+    bool nested = true;
+    for (int i : order)
+        if (r.n[i] > 1) {
+            const int64_t step = std::abs(r.step[i]);
+            nested = nested && step >= extent;
+            extent += reach(r.n[i], step) * step;
+        }
+    if (nested) return false;
+    for (int i = 0; i < 3; ++i) {  // two runs whose first index that differs is i, by 1 or more
+        if (r.n[i] == 1) continue;
+        Term t[3];
+        int n = 0;
+        for (int j = i; j < 3; ++j) {
+            const int64_t step = std::abs(r.step[j]), most = reach(r.n[j], step);
+            t[n++] = Term{j == i ? 1 : -most, most, step};
+        }
+        // (the later indices take either sign, so a step's sign matters for none)
+        if (hits(t, by_step(t, n), 1 - r.bytes, r.bytes - 1)) return true;
     }
     return false;
+}
+
+// Whether a run of one shares a byte with a run of the other.
+bool overlap(const Runs& a, const Runs& b) {
+    if (!a.at || !b.at) return false;
+    const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at));
+    int64_t low = 0, high = 0;  // of b's address less a's, less off
+    Term t[6];
+    for (int i = 0; i < 3; ++i) {
+        if (a.n[i] < 1 || b.n[i] < 1) return false;
+        for (int k = 0; k < 2; ++k) {
+            const int64_t by = k ? b.step[i] : -a.step[i], step = std::abs(by), most = reach(k ? b.n[i] : a.n[i], step);
+            t[2 * i + k] = by < 0 ? Term{-most, 0, step} : Term{0, most, step};
+            (by < 0 ? low : high) += most * by;
+        }
+    }
+    if (off + high <= -b.bytes || off + low >= a.bytes) return false;
+    return hits(t, by_step(t, 6), 1 - b.bytes - off, a.bytes - 1 - off);
+}
+
+Runs runs(const gpt2q_heads* h, int64_t tokens, int64_t heads, int64_t dim, int size) {
+    return Runs{h->data, {tokens, heads, 1}, {h->token_stride * size, h->head_stride * size, 0}, dim * size};
 }
 
 int refuse(std::string* why, const char* msg) {
@@ -63,16 +137,39 @@ void take_scales(P* p, const gpt2q_paged_kv* kv) {
     p->s_ps = s->scale_page_stride, p->s_hs = s->scale_head_stride, p->s_ts = s->scale_token_stride;
 }
 
+// What a cache lies in: keys, values and, of 8 bits, their scales; `n` of them.
+struct Parts {
+    Runs part[4];
+    int n;
+};
+Parts parts(const gpt2q_paged_kv* kv) {
+    const int size = size_of(kv->dtype);
+    Parts p{};
+    auto add = [&](const void* at, int64_t ps, int64_t hs, int64_t ts, int64_t bytes) {
+        p.part[p.n++] = Runs{at, {kv->n_pages, kv->n_kv_heads, kv->page_size}, {ps, hs, ts}, bytes};
+    };
+    for (const void* at : {kv->k, kv->v}) add(at, kv->page_stride * size, kv->head_stride * size, kv->token_stride * size, (int64_t)kv->head_dim * size);
+    if (is_8bit(kv->dtype)) {
+        const gpt2q_paged_kv8* s = scaled(kv);
+        for (const void* at : {s->k_scale, s->v_scale}) add(at, s->scale_page_stride * 4, s->scale_head_stride * 4, s->scale_token_stride * 4, 4);
+    }
+    return p;
+}
 // Whether entries of a cache that is written, or their scales, share memory.
 bool entries_overlap(const gpt2q_paged_kv* kv) {
-    auto any = [&](int64_t ps, int64_t hs, int64_t ts, int64_t dim) {
-        return overlap(kv->n_pages, ps, kv->n_kv_heads, hs, dim) || overlap(kv->n_pages, ps, kv->page_size, ts, dim) ||
-               overlap(kv->n_kv_heads, hs, kv->page_size, ts, dim);
-    };
-    if (any(kv->page_stride, kv->head_stride, kv->token_stride, kv->head_dim)) return true;
-    if (!is_8bit(kv->dtype)) return false;
-    const gpt2q_paged_kv8* s = scaled(kv);
-    return any(s->scale_page_stride, s->scale_head_stride, s->scale_token_stride, 1);
+    const Parts p = parts(kv);
+    for (int i = 0; i < p.n; ++i) {
+        if (i % 2 == 0 && overlap(p.part[i])) return true;  // (values as keys, which have the same strides)
+        for (int j = 0; j < i; ++j)
+            if (overlap(p.part[j], p.part[i])) return true;
+    }
+    return false;
+}
+bool in_cache(const gpt2q_paged_kv* kv, const Runs& r) {
+    const Parts p = parts(kv);
+    for (int i = 0; i < p.n; ++i)
+        if (overlap(p.part[i], r)) return true;
+    return false;
 }
 
 }  // namespace
@@ -146,7 +243,15 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
         for (int i = 0; i < rot->dim / 2; ++i) p.turns[i] = rot->turns[i];
     }
     if ((long long)p.n_q + 2LL * p.n_kv > INT32_MAX / 2) return refuse(why, "too many heads");
-    if (with_q && overlap(n_tokens, p.qo_ts, n_q_heads, p.qo_hs, p.dim)) return refuse(why, "the queries of q_out overlap");
+    if (with_q) {
+        const Runs o = runs(q_out, n_tokens, n_q_heads, p.dim, sz);
+        if (overlap(o)) return refuse(why, "the queries of q_out overlap");
+        const bool same = p.qo == p.q && (n_tokens == 1 || p.qo_ts == p.q_ts) && (n_q_heads == 1 || p.qo_hs == p.q_hs);
+        if ((!same && overlap(o, runs(q, n_tokens, n_q_heads, p.dim, sz))) || overlap(o, runs(k, n_tokens, p.n_kv, p.dim, sz)) ||
+            overlap(o, runs(v, n_tokens, p.n_kv, p.dim, sz)))
+            return refuse(why, "q_out overlaps k or v, or q in another order");
+        if (in_cache(kv, o)) return refuse(why, "q_out overlaps the cache");
+    }
     if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
     const cudaError_t e = launch_append(p, kv->dtype, dtype, vec, st);
     if (e == cudaErrorInvalidConfiguration) return refuse(why, "too many tokens in one call");
@@ -163,6 +268,8 @@ int gpt2q::paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
     if (d_new_lens < d_lens + table->n_rows && d_lens < d_new_lens + table->n_rows)
         return refuse(why, "d_new_lens must not be d_lens");
     if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
+    const Runs list{d_accept, {table->n_rows, 1, 1}, {ld * 4, 0, 0}, (int64_t)width * 4}, lengths{d_new_lens, {1, 1, 1}, {}, (int64_t)table->n_rows * 4};
+    if (width > 0 && overlap(list, lengths)) return refuse(why, "d_new_lens overlaps d_accept");
     EntryParams p{};
     take_cache(&p, kv);
     take_scales(&p, kv);
@@ -193,7 +300,7 @@ int gpt2q::paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tab
     if (!aligned16(q->data, q->token_stride, q->head_stride, sz) ||
         !aligned16(out->data, out->token_stride, out->head_stride, sz))
         return refuse(why, "addresses and strides of q and out must be multiples of 16 bytes");
-    if (out->data && overlap(tree ? tree->n_tokens : table->n_rows, out->token_stride, n_heads, out->head_stride, kv->head_dim))
+    if (out->data && overlap(runs(out, tree ? tree->n_tokens : table->n_rows, n_heads, kv->head_dim, sz)))
         return refuse(why, "the results in out overlap");
     PagedAttn p{};
     p.k = kv->k, p.v = kv->v;
@@ -271,9 +378,10 @@ extern "C" int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table
         const int sz = size_of(dtype);
         if (reinterpret_cast<uintptr_t>(k->data) % sz || reinterpret_cast<uintptr_t>(v->data) % sz)
             return refuse(&why, "unaligned k or v");
-        for (const gpt2q_heads* h : {k, v})
-            if (overlap(n_tokens, h->token_stride, kv->n_kv_heads, h->head_stride, kv->head_dim))
-                return refuse(&why, "the entries of k or v overlap");
+        const Runs ko = runs(k, n_tokens, kv->n_kv_heads, kv->head_dim, sz), vo = runs(v, n_tokens, kv->n_kv_heads, kv->head_dim, sz);
+        if (overlap(ko) || overlap(vo)) return refuse(&why, "the entries of k or v overlap");
+        if (overlap(ko, vo)) return refuse(&why, "k and v overlap");
+        if (in_cache(kv, ko) || in_cache(kv, vo)) return refuse(&why, "k or v overlaps the cache");
         EntryParams p{};
         take_cache(&p, kv);
         take_scales(&p, kv);
