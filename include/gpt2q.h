@@ -367,7 +367,8 @@ int gpt2q_paged_append_at(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
 
 /* Reads n_tokens entries into k and v ([token][kv head][head_dim], type `dtype`: the cache's or GPT2Q_F32, of an 8-bit cache any
  * of the three): token i is that of table row d_seq[i] (d_seq NULL: row i) at position d_pos[i]. k and v share no memory with one
- * another or the cache (a call refuses those that do). Each element is rounded once from the value it stands for. d_pos[i] < 0 gives zeros; a row, position or page out of range gives NaN and sets its bit in
+ * another or the cache (a call refuses those that do). An element is rounded to `dtype` from its value, of an 8-bit cache from the
+ * product code * scale in fp32, which is rounded itself. d_pos[i] < 0 gives zeros; a row, position or page out of range gives NaN and sets its bit in
  * d_status (may be NULL). */
 int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const gpt2q_heads* k, const gpt2q_heads* v,
                      int dtype, int n_tokens, const int32_t* d_pos, const int32_t* d_seq, int32_t* d_status, void* stream);
