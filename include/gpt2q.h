@@ -484,7 +484,8 @@ int gpt2q_verify_paged(gpt2q_handle* h, const uint32_t* tok, const int32_t* pare
                        uint32_t* next_tok);
 
 /* gpt2q_paged_commit in every layer: accept[i][width] names the drafted tokens of sequence i that stay, rising, ended by a
- * negative one. lens, accept and new_lens (may be NULL) are host arrays; table->n_rows sequences. */
+ * negative one. lens, accept and new_lens (may be NULL) are host arrays; table->n_rows sequences. A list that does not rise or
+ * names a token past the table's width is refused before anything is moved. */
 int gpt2q_commit_paged(gpt2q_handle* h, const int32_t* lens, const int32_t* accept, int width, int32_t* new_lens,
                        const gpt2q_paged_kv* layers, const gpt2q_page_table* table);
 

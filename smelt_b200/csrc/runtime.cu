@@ -2089,7 +2089,18 @@ int gpt2q_commit_paged(gpt2q_handle* H, const int32_t* lens, const int32_t* acce
     const int n = table->n_rows;
     const size_t ints = (size_t)n * (1 + (size_t)width);
     int rc = check_paged(H, layers, table);
-    if (!rc) rc = ensure_paged(H, 1);
+    if (rc) return rc;
+    // before anything is moved: the device would stop in the middle of a list
+    long long places = INT32_MAX;
+    for (int l = 0; l < H->cfg.n_layer; ++l) places = std::min(places, (long long)table->width * layer_at(layers, l).page_size);
+    for (int r = 0; r < n; ++r) {
+        const int32_t* a = accept + (size_t)r * width;
+        for (int i = 0; i < width && a[i] >= 0; ++i) {
+            if (i && a[i] <= a[i - 1]) return H->fail(GPT2Q_EARG, "accept must rise along a sequence");
+            if ((long long)std::max(lens[r], 0) + a[i] >= places) return H->fail(GPT2Q_EARG, "an accepted token lies past the table");
+        }
+    }
+    rc = ensure_paged(H, 1);
     if (!rc) rc = ensure_stage(H, ints);
     if (!rc) rc = ensure_tree(H, ints + n);
     if (rc) return rc;
