@@ -43,6 +43,14 @@ def _page_table(table) -> _ffi.PageTable:
     return _ffi.PageTable(table.data_ptr(), rows, width, table.stride(0) if rows > 1 else max(table.stride(0), width))
 
 
+def _int32(x, name):
+    """A contiguous int32 vector; numbers that do not fit are refused, not cut."""
+    a = np.asarray(x, dtype=np.int64).reshape(-1)
+    if a.size and not -2 ** 31 <= a.min() <= a.max() < 2 ** 31:
+        raise ValueError(f"{name} out of the range of 32-bit integers")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 class Gpu:
     def __init__(self, pack: Pack, device: int = 0, max_seqs: int = 1, max_tokens: int = 0,
                  tp_size: int = 1, tp_rank: int = 0, nccl_id: bytes | None = None):
@@ -282,10 +290,10 @@ class Gpu:
         tokens, and parents[i] their parents among them (-1: the last cached token). Returns the likeliest token after each,
         one array per sequence, with want_logits the logits too. commit_paged keeps the accepted ones."""
         tok, first = self._flatten(drafts)
-        par = self._flatten([np.asarray(p, dtype=np.int64) for p in parents])
-        if not np.array_equal(first, par[1]):
+        parents = [_int32(p, "parents") for p in parents]
+        if [p.size for p in parents] != np.diff(first).tolist():
             raise ValueError("drafts and parents must have the same lengths")
-        par, lens = par[0].view(np.int32), np.ascontiguousarray(lens, dtype=np.int32)
+        par, lens = np.concatenate([*parents, np.zeros(0, np.int32)]), _int32(lens, "lens")
         if lens.size != len(drafts):
             raise ValueError("lens must have one element per sequence")
         nxt = np.empty(tok.size, dtype=np.uint32)
@@ -298,13 +306,13 @@ class Gpu:
 
     def commit_paged(self, lens, accept, layers, table):
         """Keeps the drafted tokens accept[i] (rising indices) of sequence i in every layer's cache; returns the new lengths."""
-        lens = np.ascontiguousarray(lens, dtype=np.int32)
+        lens = _int32(lens, "lens")
         if len(accept) != lens.size or lens.size != table.shape[0]:
             raise ValueError("lens and accept must have one element per row of the table")
         width = max((len(a) for a in accept), default=0)
         acc = np.full((lens.size, width), -1, dtype=np.int32)
         for row, a in zip(acc, accept):
-            row[:len(a)] = a
+            row[:len(a)] = _int32(a, "accept")
         out = np.empty_like(lens)
         arr, t = self._paged(layers, table)
         self._check(self._lib.gpt2q_commit_paged(self.h, lens.ctypes.data, acc.ctypes.data, width, out.ctypes.data, arr, C.byref(t)))
