@@ -396,8 +396,9 @@ int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
  * chain, or a chunk of a prompt). A token that sees nothing gives zeros and an lse of -inf. What a token does not see does not
  * reach it, infinities and NaN included; a drafted token's value with an infinity or NaN gives NaN in those that see it. Tokens that
  * belong to no row are left as they were. Otherwise as gpt2q_paged_attention: types, alignment, d_lse [n_tokens][n_heads],
- * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order; for
- * 16-bit outputs the weights are rounded to 16 bits where the products run on wide tensor-core tiles. A length <= 0 is a prefix of none. A
+ * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order; where
+ * products run on wide tensor-core tiles (16-bit outputs only) each weight is rounded once, to bf16 for bf16 caches and to fp16 otherwise, and
+ * the sum of weights is that of the rounded ones: a result is off by up to 2^-8 or 2^-11 of sum w |v|, a single key gives its value. A length <= 0 is a prefix of none. A
  * d_first that does not rise gives numbers without a meaning; where it asks for more work than one that rises could, nothing is
  * written but GPT2Q_STATUS_POSITION. A prefix and its drafted tokens are at most 2^31 - 4097 together, whatever the table's width (more give NaN and the status bit).
  * d_work: gpt2q_paged_tree_attention_workspace(kv, n_heads, n_tokens) bytes, 16-byte aligned, of one call at a time. */

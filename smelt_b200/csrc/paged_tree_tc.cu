@@ -22,8 +22,10 @@
 // warps have it, in those with drafted tokens each query finds its own. bf16 queries are scaled per row by a power of two that brings the largest
 // element to [2^10, 2^11), and are exact in fp16 down to 2^-24 of it.
 //
-// A weight is rounded to 16 bits, once (by up to 2^-8 of itself in bf16, 2^-11 in fp16): as the output is, and with
-// random sign over the keys. fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
+// A weight is rounded to 16 bits, once (by up to 2^-8 of itself in bf16, 2^-11 in fp16), as the output is. The sum of the weights is
+// that of the rounded ones, so that a single key gives its value. Of 8-bit caches it is the product with the scale that is
+// rounded: its sums before and after give a factor that returns what the rounding took on the whole (equal scales were off by
+// the same 2^-12 in every key, and so was the result; 7 % of the time of wide drafts over int8, 341 to 366 us). fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
 //
 // Measured (one B200): 31 drafts of 5 to 60 tokens behind 100 to 8000, 32 heads on 8 of 128 in bf16, 106 us, of 38 that the cache
 // takes to read; 3 drafts of 64 tokens behind 20 to 40 thousand in int8, 64 heads on 8, 337 us (537 TFLOP/s); 2 chunks of 1100 to 2047
@@ -286,6 +288,10 @@ __device__ __forceinline__ float2 unpack(uint32_t v) {
     else
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
+// a += the two fp16 numbers of v
+__device__ __forceinline__ void add_halves(float2& a, uint32_t v) {
+    asm("{\n\t.reg .f16 x, y;\n\tmov.b32 {x, y}, %2;\n\tadd.rn.f32.f16 %0, x, %0;\n\tadd.rn.f32.f16 %1, y, %1;\n\t}" : "+f"(a.x), "+f"(a.y) : "r"(v));
+}
 // four neighbouring codes as two pairs of fp16
 template <class TC>
 __device__ __forceinline__ void widen(uint32_t v, uint32_t& a, uint32_t& b) {
@@ -512,6 +518,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float fac = fmaxf(sl2 * s_up[(pair ? st * QT : 0) + r], 1.17549435e-38f);  // not 0: a masked score of -inf stays one
             float m = -INFINITY, l = s.r.over ? NAN : 0.f;  // reference of the weights, in units before the factor; this half's sum
             uint32_t vexp = 1;
+            // 8-bit: sums of weights times scales, before and after their rounding
+            [[maybe_unused]] float exact = 0.f, rounded = 0.f;
             const bool idle = s.sb * SB + (pair ? st * QT : 0) + quarter * 32 >= s.r.queries;  // no query in this warp
             int bad = s.r.over ? GPT2Q_STATUS_POSITION : 0;
             for (int u = 0; u < nu; ++u) {
@@ -604,6 +612,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         al *= e - vexp > 126 ? 0.f : __uint_as_float((127 - (e - vexp)) << 23);
                         vexp = e;
                     }
+                    exact *= al, rounded *= al;
                 }
                 __syncwarp();
                 if (u > 0 && __any_sync(0xffffffffu, al != 1.f)) {
@@ -621,6 +630,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const float ref = m == -INFINITY ? 0.f : m;
                     const float2 nref = make_float2(-ref, -ref), f2 = make_float2(fac, fac), sh = make_float2(C::shift(), C::shift());
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    [[maybe_unused]] float2 before = make_float2(0.f, 0.f), after = make_float2(0.f, 0.f);
                     [[maybe_unused]] const float down = __uint_as_float((254 - vexp) << 23);
                     auto weights = [&](int c, auto own) {  // own: the scales are as they are, and count where they are seen
                         scores(c);
@@ -642,6 +652,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                                     }
                                     y = mul2(y, f);
                                     w[i] = pack<CT>(y.x, y.y);
+                                    before = add2(before, y);
+                                    add_halves(after, w[i]);
                                 } else {
                                     w[i] = pack<CT>(y.x, y.y);
                                     sum[i & 1] = add2(sum[i & 1], unpack<CT>(w[i]));  // of the weights that the product has
@@ -659,6 +671,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         weights(0, std::false_type{});
                     }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    if (Q8) exact += before.x + before.y, rounded += after.x + after.y;
                 }
                 tmem_wait_st();
                 tc::tc_fence_before();
@@ -672,6 +685,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (bad && p.status && lane == 0) atomicOr(p.status, bad);
             // ---- results: a half of the dims each ----
             s_l[st][half][r] = l;
+            if (Q8) s_mx[st][half][r] = __uint_as_float(pack<bf16>(exact, exact - rounded));  // (no thread reads a tile's maximum any more)
             if (half == 0) {
                 s_m[st][r] = m;
                 s_vexp[st][r] = vexp;
@@ -685,7 +699,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!idle) {
                     float wa = 1.f, wb = 0.f;  // weights of this stream's and the other's results
                     l = s_l[st][0][r] + s_l[st][1][r];
-                    if (Q8) wa = __uint_as_float(vexp << 23);
+                    // 8-bit: what the rounding of all weights together took from the product is given back, so that equal scales, or a
+                    // single key, do not leave their rounding in the result
+                    auto back = [&](int x) {
+                        const float2 a = unpack<bf16>(__float_as_uint(s_mx[x][0][r])), b = unpack<bf16>(__float_as_uint(s_mx[x][1][r]));
+                        const float all = a.x + b.x;
+                        return all != 0.f ? 1.f + fminf(fmaxf((a.y + b.y) / all, -0x1p-10f), 0x1p-10f) : 1.f;
+                    };
+                    if (Q8) wa = __uint_as_float(vexp << 23) * back(st);
                     if (!pair) {
                         const float o = s_m[1][r], M = fmaxf(m, o), ms = M == -INFINITY ? 0.f : M;
                         const float xa = ex2((m - ms) * fac);
@@ -693,7 +714,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         l = l * xa + (s_l[1][0][r] + s_l[1][1][r]) * wb;
                         m = M;
                         wa *= xa;
-                        if (Q8) wb *= __uint_as_float(s_vexp[1][r] << 23);
+                        if (Q8) wb *= __uint_as_float(s_vexp[1][r] << 23) * back(1);
                     }
                     const int pr = (pair ? st * QT : 0) + r;
                     const long long part = (long long)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1);
