@@ -67,6 +67,10 @@ constexpr float LN2 = 0.6931471805599453f;
 // three times as long as the others (218 us in all, with EXTRA = 4 130).
 constexpr int EXTRA = 5;
 constexpr float STALE = 8.f;  // log2 of the largest weight
+// Tiles of a stream whose products are summed in TMEM, before the sums go to memory and are added up there, rounded to nearest (a power of
+// two). The tensor cores round a running sum towards zero, by 2^-24 of it on average for each 16 keys: a block with 131072 keys of a row
+// left values of one sign 4.8e-4 too small, which is as much as an fp16 output's rounding; now 8e-5. 128 KB to and from L2 each time.
+constexpr int FLUSH = 256;
 
 template <class TC_, class TI_, int HD_>
 struct Cfg {
@@ -331,7 +335,30 @@ __device__ __forceinline__ unsigned long long globaltimer() {
 }
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-template <class C>
+// Adds `n` times 16 columns of this lane's sums in TMEM to keep times those in memory (SB float4 apart), if any are there; the result goes to memory, or
+// with `back` to TMEM. Apart from the loop over tiles, which it would cost registers.
+__device__ __noinline__ void carry(float4* mem, uint32_t at, int n, bool there, float keep, bool back) {
+#pragma unroll 1
+    for (int c = 0; c < n; ++c, at += 16) {
+        uint32_t w[16];
+        tmem_ld16(at, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k, mem += SB) {
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there) o = *mem;
+            o = make_float4(fmaf(o.x, keep, __uint_as_float(w[4 * k])), fmaf(o.y, keep, __uint_as_float(w[4 * k + 1])),
+                            fmaf(o.z, keep, __uint_as_float(w[4 * k + 2])), fmaf(o.w, keep, __uint_as_float(w[4 * k + 3])));
+            if (!back) *mem = o;
+            w[4 * k] = __float_as_uint(o.x), w[4 * k + 1] = __float_as_uint(o.y), w[4 * k + 2] = __float_as_uint(o.z), w[4 * k + 3] = __float_as_uint(o.w);
+        }
+        if (back) tmem_st16(at, w);
+    }
+    tmem_wait_st();
+}
+
+// LONG: a stream may have more than FLUSH tiles of a segment. A kernel of its own, as the code for it costs the others 2 to 4 %
+// (31 short drafts 106 to 110 us, chunks 423 to 433), though it is behind one comparison.
+template <class C, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1)
     k_paged_tree_tc(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using TC = typename C::TC;
@@ -615,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     exact *= al, rounded *= al;
                 }
                 __syncwarp();
-                if (u > 0 && __any_sync(0xffffffffu, al != 1.f)) {
+                if ((LONG ? u & (FLUSH - 1) : u) > 0 && __any_sync(0xffffffffu, al != 1.f)) {
 #pragma unroll 1
                     for (int c = half * (HD / 32); c < (half + 1) * (HD / 32); ++c) {
                         uint32_t w[16];
@@ -677,8 +704,29 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&b_p[st]);
+                if constexpr (!LONG) continue;
+                const bool last = u + 1 == nu;
+                if (nu <= FLUSH || (!last && ((u + 1) & (FLUSH - 1)))) continue;
+                wait(&b_o[st], no++ & 1);
+                tc::tc_fence_after();
+                // sums in memory have the place of this segment's partial results, which come later; half 0 keeps their reference there
+                const long long at = ((long long)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1)) * SB;
+                float2* ref = a.part_ml + at + st * QT + r;
+                float keep = 0.f;
+                if (u >= FLUSH) {
+                    const float2 of = *ref;
+                    keep = of.x == -INFINITY ? 0.f : ex2((of.x - m) * fac);
+                    if constexpr (Q8) {
+                        const uint32_t by = vexp - __float_as_uint(of.y);
+                        keep *= by > 126 ? 0.f : __uint_as_float((127 - by) << 23);
+                    }
+                }
+                half_sync(st);  // both halves have the reference
+                if (half == 0 && !last) *ref = make_float2(m, __uint_as_float(vexp));
+                carry(a.part + (at * (HD / 4) + (long long)half * (HD / 8) * SB) + st * QT + r, lanes + 256 + st * HD + half * (HD / 2), HD / 32, u >= FLUSH, keep, last);
+                tc::tc_fence_before();  // the next products take their place
             }
-            if (nu > 0) wait(&b_o[st], no++ & 1);
+            if (LONG ? nu > 0 && nu <= FLUSH : nu > 0) wait(&b_o[st], no++ & 1);
             tc::tc_fence_after();
             if (!ok || *(volatile int*)&s_stuck) bad |= GPT2Q_STATUS_TIMEOUT;
             if (bad) l = NAN;
@@ -899,9 +947,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                             if (ok) {
 #pragma unroll
                                 for (int ks = 0; ks < KT / 16; ++ks)
-                                    mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 32 + ks * 8 + (ks >> 2) * 32, v + ks * 128, idesc_o, u > 0 || ks > 0);
+                                    mma_f16_ts(tmem + 256 + st * HD, tmem + st * KT + 32 + ks * 8 + (ks >> 2) * 32, v + ks * 128, idesc_o, (LONG ? u & (FLUSH - 1) : u) > 0 || ks > 0);
                             }
                             hand_back(st, at);
+                            if (LONG && again && ((u + 1) & (FLUSH - 1)) == 0) tc::mma_commit(&b_o[st]);
                             if (again) {
                                 if (!EARLY) {
                                     keys(st, u + 1);
@@ -1135,6 +1184,20 @@ bool make_map(CUtensorMap* m, const PagedAttn& p, const void* base, int box) {
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <class C, bool LONG>
+cudaError_t launch_main(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int grid, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        e = cudaFuncSetAttribute(k_paged_tree_tc<C, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready |= 1ull << dev;
+    }
+    return launch_dependent(k_paged_tree_tc<C, LONG>, dim3(grid), dim3(THREADS), C::SMEM, st, a, km, vm);
+}
+
 template <class C>
 cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken) {
     Args a{};
@@ -1155,16 +1218,10 @@ cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken)
     const long long rows = std::min(p.n_rows, p.n_tokens), blocks = rows + (long long)p.n_tokens * p.group / SB;
     const long long tiles = (p.cap + (long long)KT - 1) / KT;
     const int grid = (int)std::clamp<long long>(tiles > CTAS ? CTAS : tiles * std::min<long long>(blocks, CTAS) * p.n_kv, 1, CTAS);
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
-    if (dev >= 64 || !(ready.load() >> dev & 1)) {
-        e = cudaFuncSetAttribute(k_paged_tree_tc<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) ready |= 1ull << dev;
-    }
-    e = launch_dependent(k_paged_tree_tc<C>, dim3(grid), dim3(THREADS), C::SMEM, st, a, km, vm);
+    // a stream's tiles of a segment: at most half of a block's places, and those of the longest row (half of them where both streams
+    // have the same queries, which is not known here)
+    const long long here = std::min<long long>((p.most / grid + 2) / 2, tiles);
+    const cudaError_t e = here > FLUSH ? launch_main<C, true>(a, km, vm, grid, st) : launch_main<C, false>(a, km, vm, grid, st);
     if (e != cudaSuccess || grid == 1) return e;
     const long long most = std::min<long long>(SB, (long long)p.n_tokens * p.group);
     return launch_dependent(k_paged_tree_join<typename C::TI, C::HD>, dim3(grid, (unsigned)((most + 7) / 8)), dim3(C::HD * 2), 0, st, a, C::shift());
