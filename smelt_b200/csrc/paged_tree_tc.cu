@@ -69,8 +69,9 @@ constexpr int EXTRA = 5;
 constexpr float STALE = 8.f;  // log2 of the largest weight
 // Tiles of a stream whose products are summed in TMEM, before the sums go to memory and are added up there, rounded to nearest (a power of
 // two). The tensor cores round a running sum towards zero, by 2^-24 of it on average for each 16 keys: a block with 131072 keys of a row
-// left values of one sign 4.8e-4 too small, which is as much as an fp16 output's rounding; now 8e-5. 128 KB to and from L2 each time.
-constexpr int FLUSH = 256;
+// left values of one sign 4.8e-4 too small, which is as much as an fp16 output's rounding; now 4e-5 (256 tiles 1.6e-4). 128 KB to and
+// from L2 each time. Calls that cannot have more than UNFLUSHED tiles of a stream and segment in a block do without.
+constexpr int FLUSH = 128, UNFLUSHED = 192;
 
 template <class TC_, class TI_, int HD_>
 struct Cfg {
@@ -356,7 +357,7 @@ __device__ __noinline__ void carry(float4* mem, uint32_t at, int n, bool there, 
     tmem_wait_st();
 }
 
-// LONG: a stream may have more than FLUSH tiles of a segment. A kernel of its own, as the code for it costs the others 2 to 4 %
+// LONG: a stream may have more than UNFLUSHED tiles of a segment. A kernel of its own, as the code for it costs the others 2 to 4 %
 // (31 short drafts 106 to 110 us, chunks 423 to 433), though it is behind one comparison.
 template <class C, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -1221,7 +1222,7 @@ cudaError_t launch(const PagedAttn& p, void* work, cudaStream_t st, bool* taken)
     // a stream's tiles of a segment: at most half of a block's places, and those of the longest row (half of them where both streams
     // have the same queries, which is not known here)
     const long long here = std::min<long long>((p.most / grid + 2) / 2, tiles);
-    const cudaError_t e = here > FLUSH ? launch_main<C, true>(a, km, vm, grid, st) : launch_main<C, false>(a, km, vm, grid, st);
+    const cudaError_t e = here > UNFLUSHED ? launch_main<C, true>(a, km, vm, grid, st) : launch_main<C, false>(a, km, vm, grid, st);
     if (e != cudaSuccess || grid == 1) return e;
     const long long most = std::min<long long>(SB, (long long)p.n_tokens * p.group);
     return launch_dependent(k_paged_tree_join<typename C::TI, C::HD>, dim3(grid, (unsigned)((most + 7) / 8)), dim3(C::HD * 2), 0, st, a, C::shift());

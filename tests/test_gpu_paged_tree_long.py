@@ -1,9 +1,9 @@
 """Drafted tokens behind so many keys that a block has more of a row than its products are summed over in TMEM: rows that share
 their pages, one block or more each.
 
-Where all weights are equal and the values of one sign, what is left is the sums' own error. 256 tiles of 128 keys, 16 keys at a time,
-are 2048 additions that each round a running sum towards zero, by half a unit of its last place on average: 2^-24 of the final sum
-at the most, 2^-13 in all. The outputs' own rounding averages out over 128 dims whose means are evenly spread over one step of the type
+Where all weights are equal and the values of one sign, what is left is the sums' own error. 128 tiles of 128 keys, 16 keys at a time,
+are 1024 additions that each round a running sum towards zero, by half a unit of its last place on average: 2^-24 of the final sum
+at the most, 2^-14 in all. The outputs' own rounding averages out over 128 dims whose means are evenly spread over one step of the type
 to half a step over the number of dims, 2^-10 / 2 / 128, and not worse than 2^-14 with uneven spreading."""
 import numpy as np
 import pytest
@@ -48,7 +48,7 @@ def test_a_running_sum_of_one_sign(cache, n, tokens):
     mask = torch.full((rows * tokens, words), -1, dtype=torch.int32, device="cuda")
     out = kv.attend_tree(q, table, torch.full((rows,), n - tokens, dtype=torch.int32, device="cuda"), i32(np.arange(rows + 1) * tokens), mask)
     rel = (out[:, 0].double() / want - 1).view(rows, tokens, dim).mean((1, 2))
-    assert float(rel.abs().max()) <= 2.0 ** -13 + 2.0 ** -14, float(rel.abs().max())
+    assert float(rel.abs().max()) <= 2.0 ** -14 + 2.0 ** -14, float(rel.abs().max())
 
 
 @pytest.mark.parametrize("io,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "i8"), ("bf16", "e4m3")])
@@ -87,6 +87,6 @@ def test_sums_in_memory(io, cache, tokens, heads, dim, rise):
         want, wl, tol, size, rel, vmax = attention64(q[a], values, table[r], keys, seen, sm)
         e = bound_of(tol, size, vmax, want, io, cache, wide=True)
         close(out[a], want, e, r)
-        # sums in TMEM: 2048 additions of up to 2^-23 of a sum of magnitudes, and those in memory
-        e = want.abs() * (torch.finfo(T[io]).eps / 2) + size * (2.0 ** -12 + 2 * (2.0 ** -8 if cache == "bf16" else 2.0 ** -11)) + vmax * 2.0 ** -16
+        # sums in TMEM: 1024 additions of up to 2^-23 of a sum of magnitudes, and those in memory
+        e = want.abs() * (torch.finfo(T[io]).eps / 2) + size * (2.0 ** -13 + 2 * (2.0 ** -8 if cache == "bf16" else 2.0 ** -11)) + vmax * 2.0 ** -16
         close(out[a], want, e, ("tight", r))
