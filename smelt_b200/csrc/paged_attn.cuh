@@ -885,16 +885,14 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                             }
                         l[k] = l[k] * al[k] + sum;
                     }
-                // queries that have a weight for one of these keys give NaN; `live`: which weights are not 0
-                [[maybe_unused]] uint32_t live = 0;
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < MT * NT * 4; ++i) live |= (S[i / (NT * 4)][i / 4 % NT][0][i % 4] != 0.f ? 1u : 0u) << i;
-                }
+                // queries that see one of these keys give NaN, whatever its weight
                 [[maybe_unused]] auto spoil = [&](uint32_t rows) {
 #pragma unroll
-                    for (int i = 0; i < MT * NT * 4; ++i)
-                        if (live >> i & 1 && rows >> (i / (NT * 4) * 16 + (lane >> 2) + (i % 4 >> 1) * 8) & 1) l[i / 4 % NT * 2 + (i & 1)] = NAN;
+                    for (int i = 0; i < MT * NT * 4; ++i) {
+                        const int r = i / (NT * 4) * 16 + (lane >> 2) + (i % 4 >> 1) * 8, y = i / 4 % NT;
+                        if (rows >> r & 1 && r >= klo && r < khi && sees<C>(p, w, w.hb * HB + y * 8 + (lane & 3) * 2 + (i & 1), tile0 + r - drafted0))
+                            l[y * 2 + (i & 1)] = NAN;
+                    }
                 };
                 // O^T += V^T P^T: the weights, transposed 8 x 8 in registers, are the B operand. A tile's product
                 // is summed by itself and then added to O with rounding to nearest: the tensor cores round a
@@ -1039,7 +1037,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1)
                     const uint32_t rows = unclean(drafted0 - tile0);
 #pragma unroll
                     for (int h = 0; h < HB; ++h)
-                        if (part == 0 && rows >> key & 1 && pbuf[key * HB + h] != 0.f) l[h] = NAN;
+                        if (part == 0 && rows >> key & 1 && key >= klo && key < khi && sees<C>(p, w, w.hb * HB + h, tile0 + key - drafted0)) l[h] = NAN;
                 }
                 __syncwarp();
                 constexpr int KH = HD == 64 ? 2 : 1;  // keys the warp takes at once
