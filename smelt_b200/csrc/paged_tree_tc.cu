@@ -25,11 +25,13 @@
 // A weight is rounded to 16 bits, once (by up to 2^-8 of itself in bf16, 2^-11 in fp16), as the output is. The sum of the weights is
 // that of the rounded ones, so that a single key gives its value. Of 8-bit caches it is the product with the scale that is
 // rounded: its sums before and after give a factor that returns what the rounding took on the whole (equal scales were off by
-// the same 2^-12 in every key, and so was the result; 7 % of the time of wide drafts over int8, 341 to 366 us). fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
+// the same 2^-12 in every key, and so was the result; 7 % of the time of wide drafts over int8, 341 to 366 us). Weights in two pieces of 16
+// bits, as the warp-level kernel has them, would leave the output's own rounding (error against 64 bits on the cases below 1.7e-3 and
+// not 1.9e-3 to 2.0e-3), at 114, 435 and 504 us for the three. fp32 queries and outputs, other pages and heads over 128 dims take the kernel in paged_attn.cuh.
 //
 // Measured (one B200): 31 drafts of 5 to 60 tokens behind 100 to 8000, 32 heads on 8 of 128 in bf16, 106 us, of 38 that the cache
-// takes to read; 3 drafts of 64 tokens behind 20 to 40 thousand in int8, 64 heads on 8, 337 us (537 TFLOP/s); 2 chunks of 1100 to 2047
-// tokens behind 4 to 6 thousand, 32 heads on 8 in bf16, 425 us (658 TFLOP/s). The bound of the last two is a stream's chain: read the scores, exponentials,
+// takes to read; 3 drafts of 64 tokens behind 20 to 40 thousand in int8, 64 heads on 8, 368 us (492 TFLOP/s); 2 chunks of 1100 to 2047
+// tokens behind 4 to 6 thousand, 32 heads on 8 in bf16, 423 us (662 TFLOP/s). The bound of the last two is a stream's chain: read the scores, exponentials,
 // weights to TMEM, product. Measured and not kept: an MMA warp per stream (the streams fall into step: chunks 489 us, of 472 then), slots
 // freed by a warp of their own (607), registers moved to the softmax warps, each holding its 128 scores at once (spills).
 #include <cuda.h>
@@ -1249,7 +1251,8 @@ double most_places(const PagedAttn& p) {
 // From more than eight queries of a kv head per row on, on average, where the warp-level kernel reads the keys with a second set of
 // columns or more than once. Measured (32 heads on 8 of 128, bf16; here against there), 32 rows of 1000 keys and one of 30000: with 16
 // queries 71 to 74 us and 52 to 63, with 32 72 to 106 and 52 to 86, with 128 81 to 326 and 56 to 223. With 12 it is 71 and 52 here, with
-// 8 44 and 37 there.
+// 8 44 and 37 there. All of equal rows: which rows have many is known on the device alone, so rows without a draft count too, and a row of 100
+// tokens among 63 of none takes 125 us there, which alone takes 39 here.
 bool paged_tree_tc_serves(const PagedAttn& p, int cache_dtype, int dtype) {
     return dtype != GPT2Q_F32 && cache_dtype != GPT2Q_F32 && p.dim <= 128 && p.page % 8 == 0 && p.out &&
            (long long)p.n_tokens * p.group > 8LL * p.n_rows && most_places(p) < 2147483648.0;
