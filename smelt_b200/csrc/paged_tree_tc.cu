@@ -754,8 +754,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     // single key, do not leave their rounding in the result
                     auto back = [&](int x) {
                         const float2 a = unpack<bf16>(__float_as_uint(s_mx[x][0][r])), b = unpack<bf16>(__float_as_uint(s_mx[x][1][r]));
-                        const float all = a.x + b.x;
-                        return all != 0.f ? 1.f + fminf(fmaxf((a.y + b.y) / all, -0x1p-10f), 0x1p-10f) : 1.f;
+                        const float took = (a.y + b.y) / (a.x + b.x);
+                        // (more than a rounding: sums of no sign, of weights below fp16's range, or none)
+                        return fabsf(took) <= 0x1.04p-11f ? 1.f + took : 1.f;
                     };
                     if (Q8) wa = __uint_as_float(vexp << 23) * back(st);
                     if (!pair) {

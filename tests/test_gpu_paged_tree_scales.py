@@ -112,3 +112,16 @@ def test_a_chain_whose_scales_rise(io, page, prefix):
         x.scale_at(i).fill_(2.0 ** (9 * i - 30))
     # (2^6 * 127 is the largest that fp16 has)
     x.check(range(n if io != "f16" else 5), *x.attend())
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scales_of_either_sign_and_of_zero(shape, io, cache):
+    """(append writes none that are negative, but a scale is any number)"""
+    x = Tree(4, *shape, io, cache)
+    g = gen(5)
+    for s in x.c.scales:
+        sign = torch.randint(-1, 2, s.shape, device="cuda", generator=g).float()
+        s.mul_(sign)
+    x.check(range(x.n), *x.attend())
