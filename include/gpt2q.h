@@ -273,7 +273,8 @@ int gpt2q_bwd_attn_train(int device, const float* q, const float* k, const float
  * (in elements): the entry of token slot o in page p for kv head h starts at
  * p * page_stride + h * head_stride + o * token_stride and holds head_dim elements. The pools' base
  * addresses and all strides are multiples of 16 bytes; head_dim is a multiple of 8, at most 256.
- * Entries must not overlap, keys' and values' ones neither (an append refuses a cache in which they would). */
+ * Entries must not overlap (an append refuses a cache in which they would), nor keys lie over values, but that an append of
+ * the same k and v without a rotation takes a cache whose k and v are the same. */
 typedef struct gpt2q_paged_kv {
     void* k;
     void* v;

@@ -155,13 +155,13 @@ Parts parts(const gpt2q_paged_kv* kv) {
     }
     return p;
 }
-// Whether entries of a cache that is written, or their scales, share memory.
-bool entries_overlap(const gpt2q_paged_kv* kv) {
+// Whether entries of a cache that is written, or their scales, share memory. `one`: keys and values may be the same pool.
+bool entries_overlap(const gpt2q_paged_kv* kv, bool one) {
     const Parts p = parts(kv);
     for (int i = 0; i < p.n; ++i) {
         if (i % 2 == 0 && overlap(p.part[i])) return true;  // (values as keys, which have the same strides)
         for (int j = 0; j < i; ++j)
-            if (overlap(p.part[j], p.part[i])) return true;
+            if (!(one && i == j + 1 && i % 2 && p.part[i].at == p.part[j].at) && overlap(p.part[j], p.part[i])) return true;
     }
     return false;
 }
@@ -252,7 +252,9 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
             return refuse(why, "q_out overlaps k or v, or q in another order");
         if (in_cache(kv, o)) return refuse(why, "q_out overlaps the cache");
     }
-    if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
+    // (a pool that holds keys and values at once is written twice with the same bytes)
+    const bool one = p.k == p.v && p.k_ts == p.v_ts && p.k_hs == p.v_hs && !rot;
+    if (entries_overlap(kv, one)) return refuse(why, "the cache's entries overlap");
     const cudaError_t e = launch_append(p, kv->dtype, dtype, vec, st);
     if (e == cudaErrorInvalidConfiguration) return refuse(why, "too many tokens in one call");
     return launched(e, why);
@@ -267,7 +269,7 @@ int gpt2q::paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
     if (!d_lens || !d_new_lens || (width > 0 && !d_accept)) return refuse(why, "null d_lens, d_accept or d_new_lens");
     if (d_new_lens < d_lens + table->n_rows && d_lens < d_new_lens + table->n_rows)
         return refuse(why, "d_new_lens must not be d_lens");
-    if (entries_overlap(kv)) return refuse(why, "the cache's entries overlap");
+    if (entries_overlap(kv, false)) return refuse(why, "the cache's entries overlap");
     const Runs list{d_accept, {table->n_rows, 1, 1}, {ld * 4, 0, 0}, (int64_t)width * 4}, lengths{d_new_lens, {1, 1, 1}, {}, (int64_t)table->n_rows * 4};
     if (width > 0 && overlap(list, lengths)) return refuse(why, "d_new_lens overlaps d_accept");
     EntryParams p{};

@@ -128,6 +128,20 @@ def test_outputs_over_other_tensors(lib):
     assert read(lib, heads(A + 256, 32, 16), far, kv, n=1) is None
 
 
+def test_keys_and_values_in_one_pool(lib):
+    """Taken where the same data go there twice."""
+    kv, x = cache(A, A, 4, 2, 2, 16, (64, 32, 16)), heads(A << 13, 32, 16)
+    assert append(lib, kv, k=x, v=x) is None
+    assert "entries overlap" in append(lib, kv, k=x, v=heads(A << 14, 32, 16)) and "entries overlap" in append(lib, kv, k=x, v=heads(A << 13, 48, 16))
+    assert "entries overlap" in append(lib, cache(A, A + 32, 4, 2, 2, 16, (64, 32, 16)), k=x, v=x)
+    rot = _ffi.Rotary(dim=16)
+    assert "entries overlap" in answer(lib, lib.gpt2q_paged_append(C.byref(kv), C.byref(table()), C.byref(x), C.byref(x), None, None, 1, 0, 3, A, None, C.byref(rot), None, None))
+    assert "entries overlap" in answer(lib, lib.gpt2q_paged_commit(C.byref(kv), C.byref(table(5)), A << 11, A << 12, 3, 3, A << 13, None, None))
+    for scales in ((A << 3, A << 3), (A << 3, A << 4)):
+        kv8 = cache(A, A, 4, 2, 2, 16, (64, 32, 16), 8, (*scales, 8, 4, 2))
+        assert append(lib, kv8, k=x, v=x) is None
+
+
 def test_new_lengths_over_the_list_of_a_commit(lib):
     t = table(5)
 
