@@ -21,17 +21,29 @@ bool aligned16(const void* p, int64_t a, int64_t b, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
 }
 
-// n[0] x n[1] x n[2] runs of `bytes` bytes: run (i, j, k) begins at at + i * step[0] + j * step[1] + k * step[2].
-struct Runs {
-    const void* at;
-    int64_t n[3], step[3], bytes;
-};
 // A term x * step of a sum, lo <= x <= hi, step >= 0.
 struct Term {
     int64_t lo, hi, step;
 };
 // Of addresses up to 2^58: what lies beyond is no memory, and sums of six stay in 64 bits.
-int64_t reach(int64_t n, int64_t step) { return step >> 27 ? std::min<int64_t>(n - 1, ((int64_t)1 << 58) / step) : n - 1; }
+inline int64_t reach(int64_t n, int64_t step) { return step >> 27 ? std::min<int64_t>(n - 1, ((int64_t)1 << 58) / step) : n - 1; }
+
+// n[0] x n[1] x n[2] runs of `bytes` bytes: run (i, j, k) begins at at + i * step[0] + j * step[1] + k * step[2].
+struct Runs {
+    const void* at;
+    int64_t n[3], step[3], bytes;
+    int64_t from, to;  // the bytes between, as addresses
+    Runs() = default;
+    Runs(const void* at_, int64_t n0, int64_t n1, int64_t n2, int64_t s0, int64_t s1, int64_t s2, int64_t bytes_)
+        : at(at_), n{n0, n1, n2}, step{s0, s1, s2}, bytes(bytes_) {
+        from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(at)), to = from + bytes;
+        for (int i = 0; i < 3; ++i) {
+            const int64_t most = reach(n[i], std::abs(step[i])) * step[i];
+            (most < 0 ? from : to) += most;
+        }
+    }
+    bool none() const { return !at || n[0] < 1 || n[1] < 1 || n[2] < 1; }
+};
 
 // Whether a sum of terms, ordered by falling steps, lies in [low, high]. Steps that are larger than all that follows them, as
 // those of nearly all tensors are, leave one or two values of each x to look at.
@@ -60,8 +72,7 @@ int by_step(Term* t, int n) {
 
 // Whether two runs share a byte.
 bool overlap(const Runs& r) {
-    for (int i = 0; i < 3; ++i)
-        if (r.n[i] < 1) return false;
+    if (r.none()) return false;
     // nested, as nearly all are: each step past what the smaller ones reach
     int order[3] = {0, 1, 2};
     std::sort(order, order + 3, [&](int x, int y) { return std::abs(r.step[x]) < std::abs(r.step[y]); });
@@ -90,24 +101,19 @@ bool overlap(const Runs& r) {
 
 // Whether a run of one shares a byte with a run of the other.
 bool overlap(const Runs& a, const Runs& b) {
-    if (!a.at || !b.at) return false;
+    if (a.to <= b.from || b.to <= a.from || a.none() || b.none()) return false;
     const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at));
-    int64_t low = 0, high = 0;  // of b's address less a's, less off
     Term t[6];
-    for (int i = 0; i < 3; ++i) {
-        if (a.n[i] < 1 || b.n[i] < 1) return false;
+    for (int i = 0; i < 3; ++i)
         for (int k = 0; k < 2; ++k) {
             const int64_t by = k ? b.step[i] : -a.step[i], step = std::abs(by), most = reach(k ? b.n[i] : a.n[i], step);
             t[2 * i + k] = by < 0 ? Term{-most, 0, step} : Term{0, most, step};
-            (by < 0 ? low : high) += most * by;
         }
-    }
-    if (off + high <= -b.bytes || off + low >= a.bytes) return false;
     return hits(t, by_step(t, 6), 1 - b.bytes - off, a.bytes - 1 - off);
 }
 
 Runs runs(const gpt2q_heads* h, int64_t tokens, int64_t heads, int64_t dim, int size) {
-    return Runs{h->data, {tokens, heads, 1}, {h->token_stride * size, h->head_stride * size, 0}, dim * size};
+    return Runs(h->data, tokens, heads, 1, h->token_stride * size, h->head_stride * size, 0, dim * size);
 }
 
 int refuse(std::string* why, const char* msg) {
@@ -144,9 +150,10 @@ struct Parts {
 };
 Parts parts(const gpt2q_paged_kv* kv) {
     const int size = size_of(kv->dtype);
-    Parts p{};
+    Parts p;
+    p.n = 0;
     auto add = [&](const void* at, int64_t ps, int64_t hs, int64_t ts, int64_t bytes) {
-        p.part[p.n++] = Runs{at, {kv->n_pages, kv->n_kv_heads, kv->page_size}, {ps, hs, ts}, bytes};
+        p.part[p.n++] = Runs(at, kv->n_pages, kv->n_kv_heads, kv->page_size, ps, hs, ts, bytes);
     };
     for (const void* at : {kv->k, kv->v}) add(at, kv->page_stride * size, kv->head_stride * size, kv->token_stride * size, (int64_t)kv->head_dim * size);
     if (is_8bit(kv->dtype)) {
@@ -156,8 +163,7 @@ Parts parts(const gpt2q_paged_kv* kv) {
     return p;
 }
 // Whether entries of a cache that is written, or their scales, share memory. `one`: keys and values may be the same pool.
-bool entries_overlap(const gpt2q_paged_kv* kv, bool one) {
-    const Parts p = parts(kv);
+bool entries_overlap(const Parts& p, bool one) {
     for (int i = 0; i < p.n; ++i) {
         if (i % 2 == 0 && overlap(p.part[i])) return true;  // (values as keys, which have the same strides)
         for (int j = 0; j < i; ++j)
@@ -165,8 +171,7 @@ bool entries_overlap(const gpt2q_paged_kv* kv, bool one) {
     }
     return false;
 }
-bool in_cache(const gpt2q_paged_kv* kv, const Runs& r) {
-    const Parts p = parts(kv);
+bool in_cache(const Parts& p, const Runs& r) {
     for (int i = 0; i < p.n; ++i)
         if (overlap(p.part[i], r)) return true;
     return false;
@@ -243,6 +248,7 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
         for (int i = 0; i < rot->dim / 2; ++i) p.turns[i] = rot->turns[i];
     }
     if ((long long)p.n_q + 2LL * p.n_kv > INT32_MAX / 2) return refuse(why, "too many heads");
+    const Parts cache = parts(kv);
     if (with_q) {
         const Runs o = runs(q_out, n_tokens, n_q_heads, p.dim, sz);
         if (overlap(o)) return refuse(why, "the queries of q_out overlap");
@@ -250,11 +256,11 @@ int gpt2q::paged_append(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
         if ((!same && overlap(o, runs(q, n_tokens, n_q_heads, p.dim, sz))) || overlap(o, runs(k, n_tokens, p.n_kv, p.dim, sz)) ||
             overlap(o, runs(v, n_tokens, p.n_kv, p.dim, sz)))
             return refuse(why, "q_out overlaps k or v, or q in another order");
-        if (in_cache(kv, o)) return refuse(why, "q_out overlaps the cache");
+        if (in_cache(cache, o)) return refuse(why, "q_out overlaps the cache");
     }
     // (a pool that holds keys and values at once is written twice with the same bytes)
     const bool one = p.k == p.v && p.k_ts == p.v_ts && p.k_hs == p.v_hs && !rot;
-    if (entries_overlap(kv, one)) return refuse(why, "the cache's entries overlap");
+    if (entries_overlap(cache, one)) return refuse(why, "the cache's entries overlap");
     const cudaError_t e = launch_append(p, kv->dtype, dtype, vec, st);
     if (e == cudaErrorInvalidConfiguration) return refuse(why, "too many tokens in one call");
     return launched(e, why);
@@ -269,8 +275,8 @@ int gpt2q::paged_commit(const gpt2q_paged_kv* kv, const gpt2q_page_table* table,
     if (!d_lens || !d_new_lens || (width > 0 && !d_accept)) return refuse(why, "null d_lens, d_accept or d_new_lens");
     if (d_new_lens < d_lens + table->n_rows && d_lens < d_new_lens + table->n_rows)
         return refuse(why, "d_new_lens must not be d_lens");
-    if (entries_overlap(kv, false)) return refuse(why, "the cache's entries overlap");
-    const Runs list{d_accept, {table->n_rows, 1, 1}, {ld * 4, 0, 0}, (int64_t)width * 4}, lengths{d_new_lens, {1, 1, 1}, {}, (int64_t)table->n_rows * 4};
+    if (entries_overlap(parts(kv), false)) return refuse(why, "the cache's entries overlap");
+    const Runs list(d_accept, table->n_rows, 1, 1, ld * 4, 0, 0, (int64_t)width * 4), lengths(d_new_lens, 1, 1, 1, 0, 0, 0, (int64_t)table->n_rows * 4);
     if (width > 0 && overlap(list, lengths)) return refuse(why, "d_new_lens overlaps d_accept");
     EntryParams p{};
     take_cache(&p, kv);
@@ -383,7 +389,8 @@ extern "C" int gpt2q_paged_read(const gpt2q_paged_kv* kv, const gpt2q_page_table
         const Runs ko = runs(k, n_tokens, kv->n_kv_heads, kv->head_dim, sz), vo = runs(v, n_tokens, kv->n_kv_heads, kv->head_dim, sz);
         if (overlap(ko) || overlap(vo)) return refuse(&why, "the entries of k or v overlap");
         if (overlap(ko, vo)) return refuse(&why, "k and v overlap");
-        if (in_cache(kv, ko) || in_cache(kv, vo)) return refuse(&why, "k or v overlaps the cache");
+        const Parts cache = parts(kv);
+        if (in_cache(cache, ko) || in_cache(cache, vo)) return refuse(&why, "k or v overlaps the cache");
         EntryParams p{};
         take_cache(&p, kv);
         take_scales(&p, kv);
