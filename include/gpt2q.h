@@ -295,10 +295,10 @@ typedef struct gpt2q_paged_kv {
  * v_scale. Every call that takes a gpt2q_paged_kv takes the address of `kv`; those that take one per layer take an array of
  * gpt2q_paged_kv8 where the first has 8 bits. q, k, v and outputs of such calls are GPT2Q_F32, GPT2Q_F16 or GPT2Q_BF16.
  * Written entries: scale = top / T and code = round(x * (T / top)), to nearest with ties to even, where top is the entry's
- * largest magnitude (after the rotation) and T is 127 or 448, all in fp32 (the scale at most what T times it is finite for). An entry whose top is under 2^-100 has scale and
- * codes 0; one with a NaN or an infinity has codes 0 and scale NaN.
- * Attention holds a weight times its value's scale in 16-bit numbers relative to the largest value scale among the keys that the query sees.
- * Beside its roundings each key may add an error of 2^-35 of the largest |v| seen (2^-31 where products run on wide tensor-core
+ * largest magnitude (after the rotation) and T is 127 or 448, all in fp32 (the scale at most what T times it is finite for). An
+ * entry whose top is under 2^-100 has scale and codes 0; one with a NaN or an infinity has codes 0 and scale NaN.
+ * Attention holds a weight times its value's scale in 16-bit numbers relative to the largest value scale among the keys that the query
+ * sees. Beside its roundings each key may add an error of 2^-35 of the largest |v| seen (2^-31 where products run on wide tensor-core
  * tiles): a result that is much smaller than values of next to no weight has fewer digits for it. */
 #define GPT2Q_SCALED 1
 typedef struct gpt2q_paged_kv8 {
@@ -397,11 +397,13 @@ int gpt2q_paged_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* tabl
  * chain, or a chunk of a prompt). A token that sees nothing gives zeros and an lse of -inf. What a token does not see does not
  * reach it, infinities and NaN included; a drafted token's value with an infinity or NaN gives NaN in those that see it. Tokens that
  * belong to no row are left as they were. Otherwise as gpt2q_paged_attention: types, alignment, d_lse [n_tokens][n_heads],
- * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order; where
- * products run on wide tensor-core tiles (16-bit outputs only) each weight is rounded once, to bf16 for bf16 caches and to fp16 otherwise, and
- * the sum of weights is that of the rounded ones: a result is off by up to 2^-8 or 2^-11 of sum w |v|, a single key gives its value. A length <= 0 is a prefix of none. A
- * d_first that does not rise gives numbers without a meaning; where it asks for more work than one that rises could, nothing is
- * written but GPT2Q_STATUS_POSITION. A prefix and its drafted tokens are at most 2^31 - 4097 together, whatever the table's width (more give NaN and the status bit).
+ * status bits and NaN for a row that needs a page id out of range or is longer than the table, fp32 sums in a fixed order. Where
+ * products run on wide tensor-core tiles (16-bit outputs only) each weight, of an 8-bit cache times its value's scale, is rounded once, to
+ * bf16 for bf16 caches (by up to 2^-8 of itself) and to fp16 otherwise (2^-11). Sums of weights are those of the rounded ones: a result is
+ * off by up to twice that part of sum w |v|, and a single key gives its value. A length <= 0 is a prefix of none. A d_first that does not
+ * rise gives numbers without a meaning; where it asks for more work than one that rises could, nothing is written but
+ * GPT2Q_STATUS_POSITION. A prefix and its drafted tokens are at most 2^31 - 4097 together, whatever the table's width (more give NaN
+ * and the status bit).
  * d_work: gpt2q_paged_tree_attention_workspace(kv, n_heads, n_tokens) bytes, 16-byte aligned, of one call at a time. */
 uint64_t gpt2q_paged_tree_attention_workspace(const gpt2q_paged_kv* kv, int n_heads, int n_tokens);
 int gpt2q_paged_tree_attention(const gpt2q_paged_kv* kv, const gpt2q_page_table* table, const int32_t* d_lens,
