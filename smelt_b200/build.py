@@ -26,7 +26,8 @@ LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "libgpt2q.so")
 TORCH_LIB = os.path.join(LIBDIR, "gpt2q_torch.so")
 
-SOURCES = ["kernels.cu", "runtime.cu", "gemm.cu", "gemm_mma.cu", "attn_tc.cu", "persistent.cu", "tp.cu", "noalloc.cu", "synth.cpp", "blake3.cpp", "smt.cpp", "backward.cu", "paged.cu", "paged_entries.cu", "paged_attn.cu", "paged_attn_i8.cu", "paged_attn_e4m3.cu", "paged_tree.cu", "paged_tree_i8.cu", "paged_tree_e4m3.cu", "paged_tree_tc.cu", "logprobs.cu"]
+# (those that take longest come first, as they are compiled side by side)
+SOURCES = ["paged_tree_tc.cu", "paged_tree_i8.cu", "paged_tree_e4m3.cu", "paged_tree.cu", "paged_attn_i8.cu", "paged_attn_e4m3.cu", "paged_attn.cu", "gemm.cu", "gemm_mma.cu", "logprobs.cu", "kernels.cu", "runtime.cu", "attn_tc.cu", "persistent.cu", "tp.cu", "noalloc.cu", "synth.cpp", "blake3.cpp", "smt.cpp", "backward.cu", "paged.cu", "paged_entries.cu"]
 HEADERS = ["common.cuh", "kernels.h", "gemm.h", "gemm_mma.h", "persistent.h", "tp.h", "tcgen05.cuh", "blake3.h", "backward.h", "paged.h", "paged_attn.cuh", "device_op.cuh", "logprobs.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
